@@ -45,6 +45,39 @@ pub struct hipc_conv_geom {
     pub group: i64,
 }
 
+/// the alternatives `hipc_token_logprobs` names at most
+pub const HIPC_TOP_MAX: c_int = 32;
+
+/// the heads of an attention call
+#[repr(C)]
+#[derive(Clone, Copy, Debug, Default, PartialEq)]
+pub struct hipc_attention_heads {
+    pub n_q_heads: i32,
+    pub n_kv_heads: i32,
+    pub head_dim: i32,
+    pub causal: i32,
+    pub window: i32,
+    pub scale: f32,
+}
+
+/// a paged cache of keys and values in 4 bits, and whose pages are whose
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct hipc_kv4_cache {
+    pub k_codes: *mut c_void,
+    pub k_params: *mut c_void,
+    pub v_codes: *mut c_void,
+    pub v_params: *mut c_void,
+    pub n_pages: i64,
+    pub page_size: i32,
+    pub n_kv_heads: i32,
+    pub head_dim: i32,
+    pub n_seqs: i32,
+    pub lengths: *const c_void,
+    pub table: *const c_void,
+    pub table_width: i64,
+}
+
 #[repr(C)]
 #[derive(Clone, Copy, Debug, Default, PartialEq)]
 pub struct hipc_decoder_config {
@@ -209,6 +242,31 @@ unsafe extern "C" {
     ) -> c_int;
     pub fn hipc_host_error() -> *const c_char;
 
+    // ---- attention over prompts and a cache in 4 bits
+    pub fn hipc_prompt_attention(
+        ctx: *mut hipc_ctx, heads: *const hipc_attention_heads, dtype: c_int, q: *const c_void, q_stride: i64, k: *const c_void,
+        k_stride: i64, v: *const c_void, v_stride: i64, q_starts: *const c_void, k_starts: *const c_void, n_seqs: i64,
+        total_q: i64, total_k: i64, y: *mut c_void, y_stride: i64,
+    ) -> c_int;
+    pub fn hipc_kv4_append(
+        ctx: *mut hipc_ctx, cache: *const hipc_kv4_cache, dtype: c_int, starts: *const c_void, total: i64, k: *const c_void,
+        k_stride: i64, v: *const c_void, v_stride: i64,
+    ) -> c_int;
+    pub fn hipc_kv4_read(
+        ctx: *mut hipc_ctx, cache: *const hipc_kv4_cache, dtype: c_int, starts: *const c_void, total: i64, k: *mut c_void,
+        k_stride: i64, v: *mut c_void, v_stride: i64,
+    ) -> c_int;
+    pub fn hipc_kv4_attention(
+        ctx: *mut hipc_ctx, cache: *const hipc_kv4_cache, heads: *const hipc_attention_heads, dtype: c_int, tokens: i64,
+        q: *const c_void, q_stride: i64, y: *mut c_void, y_stride: i64,
+    ) -> c_int;
+
+    // ---- probabilities of the answers
+    pub fn hipc_token_logprobs(
+        ctx: *mut hipc_ctx, dtype: c_int, logits: *const c_void, row_stride: i64, rows: i64, vocab: i64, tokens: *const c_void,
+        logprob: *mut c_void, entropy: *mut c_void, top: c_int, top_ids: *mut c_void, top_logprobs: *mut c_void,
+    ) -> c_int;
+
     // ---- decode step
     pub fn hipc_decoder_create(ctx: *mut hipc_ctx, cfg: *const hipc_decoder_config, out: *mut *mut hipc_decoder) -> c_int;
     pub fn hipc_decoder_destroy(ctx: *mut hipc_ctx, dec: *mut hipc_decoder);
@@ -224,6 +282,7 @@ unsafe extern "C" {
     pub fn hipc_decoder_set_layer_attention(ctx: *mut hipc_ctx, dec: *mut hipc_decoder, layer: c_int, window: i32, rope_theta: f32) -> c_int;
     pub fn hipc_decoder_reset(ctx: *mut hipc_ctx, dec: *mut hipc_decoder, token: i32, pos: i32) -> c_int;
     pub fn hipc_decoder_kv_cache(ctx: *mut hipc_ctx, dec: *mut hipc_decoder, layer: c_int, k_cache: *mut *mut c_void, v_cache: *mut *mut c_void) -> c_int;
+    pub fn hipc_decoder_logits(ctx: *mut hipc_ctx, dec: *mut hipc_decoder, logits: *mut *mut c_void) -> c_int;
     pub fn hipc_decoder_step(ctx: *mut hipc_ctx, dec: *mut hipc_decoder) -> c_int;
     pub fn hipc_decoder_read(
         ctx: *mut hipc_ctx, dec: *mut hipc_decoder, token: *mut i32, pos: *mut i32, logits: *mut f32, history: *mut i32,

@@ -395,6 +395,105 @@ int hipc_model_initializers(const void *model, size_t len, size_t *offsets, size
 /* message of the last failed host-only call (the two above) on the calling thread */
 const char *hipc_host_error(void);
 
+/* ------------------------------------------ attention over prompts and a cache in 4 bits */
+
+/*
+ * What the decode step below leaves to its caller: the prompt in front of it, and many sequences or long contexts at a
+ * time. It stands beside GroupQueryAttention's prompt form and the flash-attention kernel of the reference
+ * (crates/onnx-vulkan-core/src/interp.rs:7514-7949); a cache in 4 bits has no counterpart there.
+ *
+ * The heads of an attention call: query head h reads kv head h / (n_q_heads / n_kv_heads).
+ */
+typedef struct {
+    int32_t n_q_heads, n_kv_heads, head_dim;
+    int32_t causal;  /* != 0: a query sees the keys up to its own position; 0: all keys of its sequence (hipc_prompt_attention only) */
+    int32_t window;  /* > 0: ... and of those only the last `window`, its own position included (causal calls; as in hipc_decoder_set_layer_attention) */
+    float scale;     /* of the scores; 0 => 1 / sqrt(head_dim) */
+} hipc_attention_heads;
+
+/*
+ * Attention over whole prompts: y_i = sum_j softmax_j(scale q_i . k_j) v_j for sequences of different lengths packed one
+ * behind the other.
+ *   Q [total_q, n_q_heads, head_dim], K / V [total_k, n_kv_heads, head_dim], Y like Q; all f16 or all f32 (dtype). A row's heads
+ *   lie side by side; rows are *_stride elements apart (so q|k|v may be parts of one projection's rows).
+ *   q_starts / k_starts [n_seqs + 1] i32 on the device: sequence s has the query rows q_starts[s] .. q_starts[s + 1] - 1 and
+ *   the keys k_starts[s] .. k_starts[s + 1] - 1. With len_q and len_k of them, query row i stands at position
+ *   len_k - len_q + i among the keys, so a prompt that comes in pieces passes the earlier keys along with the new ones.
+ * A row that sees no key (a position below 0) is zero. Rows of Q and Y in front of the first and behind the last sequence are
+ * neither read nor written. Starts are held to [0, total]; a sequence that would end before it starts has no rows.
+ * Keys and values that a row does not see do not enter its result, whatever they hold (infinities and NaN too).
+ * f16: products of the f16 values as they are, sums in f32, softmax in f32, its weights rounded to f16 for the second
+ * product. f32: every factor as three bf16 terms (24 bits), sums in f32. head_dim is at most 512; one that is a multiple
+ * of 8, up to 256, with rows and strides on 16 bytes runs on the matrix cores, any other on a kernel that computes in f32 on
+ * the vector units. n_seqs <= 2^20; totals <= 2^31 - 1. Q, K and V may not overlap Y.
+ */
+int hipc_prompt_attention(hipc_ctx *ctx, const hipc_attention_heads *heads, int dtype, const void *Q, int64_t q_stride,
+                          const void *K, int64_t k_stride, const void *V, int64_t v_stride, const void *q_starts,
+                          const void *k_starts, int64_t n_seqs, int64_t total_q, int64_t total_k, void *Y, int64_t y_stride);
+
+/*
+ * A cache of keys and values in 4 bits, in pages, for many sequences. The memory is the caller's; every pointer is a
+ * device pointer on 16 bytes.
+ *   k_codes, v_codes    [n_pages, n_kv_heads, page_size, head_dim / 2] u8, channel 2i in the low nibble of byte i
+ *   k_params, v_params  [n_pages, n_kv_heads, page_size, head_dim / 32, 2] f16: scale and lowest value of 32 channels
+ * A code c stands for the f16 value lowest + c * scale, rounded once. head_dim is a multiple of 32, up to 256; page_size is a
+ * power of two, 16 or more (one page per sequence is a plain cache). Position t of sequence s lies in page
+ * table[s * table_width + t / page_size], at place t % page_size; table [n_seqs, table_width] and lengths [n_seqs] are i32 on the
+ * device, so a recorded call follows what is written there between its replays. A page number outside [0, n_pages) is no page:
+ * what would be stored there is not, what would be read there is zero, and attention does not see its positions (pages
+ * behind every window may so be given back). Lengths are held to [0, table_width * page_size].
+ */
+typedef struct {
+    void *k_codes, *k_params, *v_codes, *v_params;
+    int64_t n_pages;
+    int32_t page_size, n_kv_heads, head_dim, n_seqs;
+    const void *lengths, *table;
+    int64_t table_width;
+} hipc_kv4_cache;
+
+/*
+ * Store new rows: starts [n_seqs + 1] i32 on the device says which rows of K / V [total, n_kv_heads, head_dim] (f16 or f32, rows
+ * *_stride elements apart) are whose; they become the LAST positions of their sequence: row i of n goes to position
+ * lengths[s] - n + i, so lengths count the new rows already (rows at positions below 0 are not stored). Each group of 32
+ * channels is quantized by itself, values held to +-65408 first, as if with unlimited precision up to the roundings named:
+ *   lowest = f16(min), scale = f16(f32((max - min) / 15)), code = the nearest whole number to (x - lowest) / scale, ties to even, in 0..15
+ * (scale 0: code 0). A group with a NaN reads back as NaN. Two rows that go to one position (two sequences that share a page there)
+ * have to be equal.
+ */
+int hipc_kv4_append(hipc_ctx *ctx, const hipc_kv4_cache *cache, int dtype, const void *starts, int64_t total, const void *K,
+                    int64_t k_stride, const void *V, int64_t v_stride);
+/* Read the rows back as the values they stand for (exact in f16, widened in f32): the same arguments, K / V are written.
+ * A row at a position below 0, or on no page, is zero; rows outside every sequence are left as they are. */
+int hipc_kv4_read(hipc_ctx *ctx, const hipc_kv4_cache *cache, int dtype, const void *starts, int64_t total, void *K,
+                  int64_t k_stride, void *V, int64_t v_stride);
+/*
+ * Attention of the newest `tokens` (1 or more) positions of every sequence over its cache, its own positions included:
+ * Q, Y [n_seqs * tokens, n_q_heads, head_dim] f16 or f32, sequence s's token i in row s * tokens + i at position
+ * lengths[s] - tokens + i. heads->causal has to be set; heads->n_kv_heads and head_dim are the cache's. A row that sees
+ * nothing (an empty sequence, a position below 0) is zero. The cache's values enter exactly, f16 queries too, f32 queries
+ * with 22 bits of a row's largest value; weights with 22 bits; sums in f32. tokens * n_q_heads / n_kv_heads <= 1024.
+ * The order of the sums is fixed by the shapes, the lengths and the device: results repeat bit for bit.
+ */
+int hipc_kv4_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_attention_heads *heads, int dtype, int64_t tokens,
+                       const void *Q, int64_t q_stride, void *Y, int64_t y_stride);
+
+/* ----------------------------------------------- probabilities of the answers */
+
+/*
+ * Beside the greedy pick of the decode step (ArgMax, shaders/reduction.rs:76-191): for every row of logits
+ * [rows, vocab] (f16 or f32, rows row_stride elements apart), with lse = log sum_v exp(x_v) in f32,
+ *   logprob [rows] f32       x_t - lse for the row's given token t = tokens[row] (i32): -1 gives 0 (padding), any other number
+ *                            outside [0, vocab) gives NaN; tokens and logprob are given together or not at all (NULL)
+ *   entropy [rows] f32       lse - sum_v p_v x_v (a logit of -inf adds nothing), or NULL
+ *   top_ids [rows, top] i32, top_logprobs [rows, top] f32: the `top` (0 to HIPC_TOP_MAX) largest logits, largest first, the lower id
+ *                            first among equals; NaN never counts; where fewer than `top` logits compare the rest is -1 and NaN
+ * A row without a finite largest logit (all -inf, a +inf or a NaN in it) has no distribution: its logprob, entropy and
+ * top_logprobs are NaN. The logits are read once. vocab <= 2^30.
+ */
+#define HIPC_TOP_MAX 32
+int hipc_token_logprobs(hipc_ctx *ctx, int dtype, const void *logits, int64_t row_stride, int64_t rows, int64_t vocab,
+                        const void *tokens, void *logprob, void *entropy, int top, void *top_ids, void *top_logprobs);
+
 /* ------------------------------------------------------------ decode step */
 
 /*
@@ -477,6 +576,9 @@ int hipc_decoder_reset(hipc_ctx *ctx, hipc_decoder *dec, int32_t token, int32_t 
  * one 16-byte load). A caller that fills the cache itself (a prefill) writes position t of channel c of
  * kv head h at v_cache[(h * head_dim + c) * v_stride + t]. */
 int hipc_decoder_kv_cache(hipc_ctx *ctx, hipc_decoder *dec, int layer, void **k_cache, void **v_cache);
+/* Device pointer of the last step's logits, [vocab] f32 (hipc_token_logprobs reads them where they are; the next step overwrites
+ * them). The address stays while the decoder does. */
+int hipc_decoder_logits(hipc_ctx *ctx, hipc_decoder *dec, void **logits);
 /* enqueue one decode step (capturable; record it after a reset or a step has run, so that the recorded launches do
  * not include an embedding launch of their own) */
 int hipc_decoder_step(hipc_ctx *ctx, hipc_decoder *dec);

@@ -14,6 +14,8 @@ from .runtime import (  # noqa: F401
     HipComputeError,
     ConvGeom,
     DecoderConfig,
+    AttentionHeads,
+    Kv4Cache,
     library_path,
     load_library,
     F32, F16, U8, I8, I32,

@@ -1432,6 +1432,14 @@ int hipc_decoder_step(hipc_ctx *ctx, hipc_decoder *d) {
     });
 }
 
+int hipc_decoder_logits(hipc_ctx *ctx, hipc_decoder *d, void **logits) {
+    if (!d || !logits) return HIPC_ERR_INVALID;
+    return entry(ctx, [&]() -> int {
+        *logits = d->logits;
+        return HIPC_OK;
+    });
+}
+
 int hipc_decoder_read(hipc_ctx *ctx, hipc_decoder *d, int32_t *token, int32_t *pos, float *logits, int32_t *history, int32_t n_history) {
     if (!d) return HIPC_ERR_INVALID;
     return entry(ctx, [&]() -> int {

@@ -147,7 +147,8 @@ const Entry kEntries[] = {
     BIND(hipc_dynamic_quantize_linear), BIND(hipc_dynamic_quantize_linear_static), BIND(hipc_decomposed_gelu),
     BIND(hipc_dynamic_quantize_linear_gelu), BIND(hipc_matmul_integer), BIND(hipc_matmul_integer_raw),
     BIND(hipc_matmul_integer_scale_bias), BIND(hipc_requantize), BIND(hipc_qlinear_matmul), BIND(hipc_conv_integer),
-    BIND(hipc_qlinear_conv), BIND(hipc_decoder_reset), BIND(hipc_decoder_step),
+    BIND(hipc_qlinear_conv), BIND(hipc_decoder_reset), BIND(hipc_decoder_step), BIND(hipc_prompt_attention),
+    BIND(hipc_kv4_append), BIND(hipc_kv4_read), BIND(hipc_kv4_attention), BIND(hipc_token_logprobs),
 };
 #undef BIND
 

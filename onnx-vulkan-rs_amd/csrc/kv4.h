@@ -1,0 +1,72 @@
+// The 4-bit key/value cache on the device: where a position's codes and parameters lie, which sequence a packed row
+// belongs to, and what eight codes stand for. Shared by what stores, reads and attends to it (kv4_cache.hip,
+// kv4_attention.hip) and, for the packed rows, by prompt_attention.hip.
+#pragma once
+
+#include <hip/hip_fp16.h>
+
+#include "internal.h"
+
+namespace hipc {
+
+constexpr int kKv4Group = 32;      // channels that share a scale and a lowest value
+constexpr int kKv4MaxHead = 256;
+
+typedef _Float16 kvh2 __attribute__((ext_vector_type(2)));
+
+// Wave-wide: the sequence that packed row `row` belongs to, and its rows [first, end). The starts are counted 64 at a time;
+// false where no sequence has the row (in front of the first, behind the last, or starts that do not ascend).
+__device__ __forceinline__ bool packed_sequence(const int *starts, int n_seqs, int total, int row, int *seq, int *first, int *end) {
+    const int lane = threadIdx.x & 63;
+    int s = 0;
+    for (int base = 1; base <= n_seqs; base += 64) {
+        const int at = base + lane;
+        const bool before = at <= n_seqs && starts[at < n_seqs ? at : n_seqs] <= row;
+        const int c = __popcll(__ballot(before));
+        s += c;
+        if (c < 64) break;   // ascending starts: none behind this one is at or before the row
+    }
+    if (s >= n_seqs) return false;
+    const int a = starts[s], b = starts[s + 1];
+    *seq = s, *first = a < 0 ? 0 : a, *end = b > total ? total : b;
+    return *first <= row && row < *end;
+}
+
+struct Kv4Place {
+    int64_t slot;   // (page, kv head 0, place) as a row of heads: head h's row is slot + h * page_size
+    bool there;
+};
+// position t of sequence s
+__device__ __forceinline__ Kv4Place kv4_place(const hipc_kv4_cache &c, int s, int t) {
+    const int shift = 31 - __builtin_clz((unsigned)c.page_size);
+    if (t < 0 || (t >> shift) >= c.table_width) return {0, false};
+    const int page = static_cast<const int *>(c.table)[(int64_t)s * c.table_width + (t >> shift)];
+    if (page < 0 || page >= c.n_pages) return {0, false};
+    return {((int64_t)page * c.n_kv_heads << shift) + (t & (c.page_size - 1)), true};
+}
+// lengths are held to what the table can name
+__device__ __forceinline__ int kv4_length(const hipc_kv4_cache &c, int s) {
+    const int64_t most = c.table_width * c.page_size;
+    const int n = static_cast<const int *>(c.lengths)[s];
+    return n < 0 ? 0 : n > most ? (int)most : n;
+}
+
+// Eight codes as f16 values, each lowest + code * scale rounded once: the code's bits under the exponent of 1024 (or, four
+// bits further up, of 64) are that number plus the code; the subtraction is exact, and so is the product inside the fma.
+__device__ __forceinline__ void kv4_values(uint32_t w, kvh2 scale, kvh2 lowest, kvh2 (&v)[4]) {
+    auto part = [](uint32_t bits, uint32_t magic) { return __builtin_bit_cast(kvh2, bits | magic); };
+    const kvh2 k1024 = {(_Float16)1024.f, (_Float16)1024.f}, k64 = {(_Float16)64.f, (_Float16)64.f};
+    // nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7
+    v[0] = __builtin_elementwise_fma(part(w & 0x000f000fu, 0x64006400u) - k1024, scale, lowest);
+    v[1] = __builtin_elementwise_fma(part(w & 0x00f000f0u, 0x54005400u) - k64, scale, lowest);
+    w >>= 8;
+    v[2] = __builtin_elementwise_fma(part(w & 0x000f000fu, 0x64006400u) - k1024, scale, lowest);
+    v[3] = __builtin_elementwise_fma(part(w & 0x00f000f0u, 0x54005400u) - k64, scale, lowest);
+}
+
+// host side: what every call of the cache checks
+int kv4_check(hipc_ctx *ctx, const char *who, const hipc_kv4_cache *c);
+// the heads of an attention call, and the scale it uses
+int attention_check(hipc_ctx *ctx, const char *who, const hipc_attention_heads *h, int dtype, float *scale);
+
+}  // namespace hipc

@@ -129,6 +129,12 @@ class Decoder:
     def step(self):
         self.ctx._check(self.ctx.lib.hipc_decoder_step(self.ctx.handle, self.handle))
 
+    def logits(self) -> int:
+        """Device address of the last step's logits, ``[vocab]`` float32 (for ``ops.token_logprobs_device``)."""
+        p = C.c_void_p()
+        self.ctx._check(self.ctx.lib.hipc_decoder_logits(self.ctx.handle, self.handle, C.byref(p)))
+        return p.value
+
     def read(self, want_logits: bool = False, n_history: int = 0):
         tok, pos = C.c_int32(), C.c_int32()
         logits = np.empty(self.cfg["vocab"], np.float32) if want_logits else None

@@ -10,7 +10,7 @@ import ctypes as C
 
 import numpy as np
 
-from .runtime import Buffer, Context, ConvGeom, F16, F32, I8, U8, _ptr, hipc_dtype
+from .runtime import AttentionHeads, Buffer, Context, ConvGeom, F16, F32, I8, Kv4Cache, U8, _ptr, hipc_dtype
 
 _vp = C.c_void_p
 
@@ -385,3 +385,131 @@ def qlinear_conv(ctx: Context, X, x_scale, x_zp, W, w_scale, w_zp, y_scale, y_zp
     if own:
         own.destroy()
     return Y
+
+
+# ------------------------------------------ attention over prompts and a cache in 4 bits
+
+KV4_GROUP = 32   # channels that share a scale and a lowest value
+
+
+def prompt_attention_device(ctx, heads: AttentionHeads, dtype, Q, q_stride, K, k_stride, V, v_stride, q_starts, k_starts, n_seqs,
+                            total_q, total_k, Y, y_stride):
+    ctx._check(ctx.lib.hipc_prompt_attention(ctx.handle, heads, dtype, _ptr(Q), q_stride, _ptr(K), k_stride, _ptr(V), v_stride,
+                                             _ptr(q_starts), _ptr(k_starts), n_seqs, total_q, total_k, _ptr(Y), y_stride))
+
+
+def kv4_append_device(ctx, cache: Kv4Cache, dtype, starts, total, K, k_stride, V, v_stride):
+    ctx._check(ctx.lib.hipc_kv4_append(ctx.handle, cache, dtype, _ptr(starts), total, _ptr(K), k_stride, _ptr(V), v_stride))
+
+
+def kv4_read_device(ctx, cache: Kv4Cache, dtype, starts, total, K, k_stride, V, v_stride):
+    ctx._check(ctx.lib.hipc_kv4_read(ctx.handle, cache, dtype, _ptr(starts), total, _ptr(K), k_stride, _ptr(V), v_stride))
+
+
+def kv4_attention_device(ctx, cache: Kv4Cache, heads: AttentionHeads, dtype, tokens, Q, q_stride, Y, y_stride):
+    ctx._check(ctx.lib.hipc_kv4_attention(ctx.handle, cache, heads, dtype, tokens, _ptr(Q), q_stride, _ptr(Y), y_stride))
+
+
+def prompt_attention(ctx: Context, q, k, v, q_lengths, k_lengths=None, causal=True, window=0, scale=0.0):
+    """Attention over packed prompts on numpy operands: ``q [rows, heads, dim]``, ``k`` / ``v [keys, kv heads, dim]``, float16 or
+    float32; the lengths of the sequences in rows and in keys (by default the same)."""
+    q, k, v = (np.ascontiguousarray(x) for x in (q, k, v))
+    if k_lengths is None:
+        k_lengths = q_lengths
+    heads = AttentionHeads(q.shape[1], k.shape[1], q.shape[2], int(causal), window, scale)
+    starts = [np.concatenate([[0], np.cumsum(n)]).astype(np.int32) for n in (q_lengths, k_lengths)]
+    dQ, dK, dV, dqs, dks = (ctx.upload(x) for x in (q, k, v, *starts))
+    dY = ctx.upload(np.zeros_like(q))
+    row = [x.shape[1] * x.shape[2] for x in (q, k, v)]
+    prompt_attention_device(ctx, heads, hipc_dtype(q.dtype), dQ, row[0], dK, row[1], dV, row[2], dqs, dks, len(q_lengths),
+                            q.shape[0], k.shape[0], dY, row[0])
+    y = ctx.download(dY, q.dtype, q.shape)
+    for b in (dQ, dK, dV, dqs, dks, dY):
+        b.free()
+    return y
+
+
+class Kv4Pages:
+    """The memory of a paged 4-bit cache, its page table and its lengths, kept by a context (``hipc_kv4_cache``)."""
+
+    def __init__(self, ctx: Context, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, table):
+        """``table [sequences, width]``: the page numbers of every sequence."""
+        self.ctx, self.n_kv_heads, self.head_dim = ctx, n_kv_heads, head_dim
+        table = np.ascontiguousarray(table, np.int32)
+        rows = n_pages * n_kv_heads * page_size
+        codes, params = np.zeros(rows * head_dim // 2, np.uint8), np.zeros(rows * (head_dim // KV4_GROUP) * 2, np.float16)
+        self.buffers = [ctx.upload(x) for x in (codes, params, codes, params)]
+        self.table, self.lengths = ctx.upload(table), ctx.upload(np.zeros(table.shape[0], np.int32))
+        p = [b.ptr for b in self.buffers]
+        self.cache = Kv4Cache(p[0], p[1], p[2], p[3], n_pages, page_size, n_kv_heads, head_dim, table.shape[0], self.lengths.ptr,
+                              self.table.ptr, table.shape[1])
+
+    def set_lengths(self, lengths):
+        self.ctx.upload(np.ascontiguousarray(lengths, np.int32), self.lengths)
+
+    def set_table(self, table):
+        self.ctx.upload(np.ascontiguousarray(table, np.int32), self.table)
+
+    def append(self, k, v, new):
+        """Packed rows ``[sum(new), kv heads, dim]`` become the last ``new[s]`` positions of sequence s (lengths count them already)."""
+        k, v = np.ascontiguousarray(k), np.ascontiguousarray(v)
+        dK, dV, ds = self.ctx.upload(k), self.ctx.upload(v), self.ctx.upload(np.concatenate([[0], np.cumsum(new)]).astype(np.int32))
+        row = self.n_kv_heads * self.head_dim
+        kv4_append_device(self.ctx, self.cache, hipc_dtype(k.dtype), ds, k.shape[0], dK, row, dV, row)
+        for b in (dK, dV, ds):
+            b.free()
+
+    def read(self, count, dtype=np.float16):
+        """The last ``count[s]`` positions of every sequence, packed: (keys, values)."""
+        shape = (int(np.sum(count)), self.n_kv_heads, self.head_dim)
+        zero = np.zeros(shape, dtype)
+        dK, dV, ds = self.ctx.upload(zero), self.ctx.upload(zero), self.ctx.upload(np.concatenate([[0], np.cumsum(count)]).astype(np.int32))
+        row = self.n_kv_heads * self.head_dim
+        kv4_read_device(self.ctx, self.cache, hipc_dtype(np.dtype(dtype)), ds, shape[0], dK, row, dV, row)
+        out = self.ctx.download(dK, dtype, shape), self.ctx.download(dV, dtype, shape)
+        for b in (dK, dV, ds):
+            b.free()
+        return out
+
+    def attention(self, q, tokens=1, window=0, scale=0.0):
+        """``q [sequences * tokens, heads, dim]``: the newest tokens of every sequence over its cache."""
+        q = np.ascontiguousarray(q)
+        heads = AttentionHeads(q.shape[1], self.n_kv_heads, self.head_dim, 1, window, scale)
+        dQ, dY = self.ctx.upload(q), self.ctx.upload(np.zeros_like(q))
+        row = q.shape[1] * q.shape[2]
+        kv4_attention_device(self.ctx, self.cache, heads, hipc_dtype(q.dtype), tokens, dQ, row, dY, row)
+        y = self.ctx.download(dY, q.dtype, q.shape)
+        dQ.free(), dY.free()
+        return y
+
+    def free(self):
+        for b in self.buffers + [self.table, self.lengths]:
+            b.free()
+
+
+# ----------------------------------------------------- probabilities of the answers
+
+TOP_MAX = 32
+
+
+def token_logprobs_device(ctx, dtype, logits, row_stride, rows, vocab, tokens, logprob, entropy, top, top_ids, top_logprobs):
+    ctx._check(ctx.lib.hipc_token_logprobs(ctx.handle, dtype, _ptr(logits), row_stride, rows, vocab, _ptr(tokens), _ptr(logprob),
+                                           _ptr(entropy), top, _ptr(top_ids), _ptr(top_logprobs)))
+
+
+def token_logprobs(ctx: Context, logits, tokens, top=0):
+    """``logits [rows, vocab]`` float16 or float32, ``tokens [rows]``: (logprob, entropy, ids and log probabilities of the ``top``
+    best)."""
+    logits = np.ascontiguousarray(logits)
+    rows, vocab = logits.shape
+    dX, dT = ctx.upload(logits), ctx.upload(np.ascontiguousarray(tokens, np.int32))
+    dL, dE = ctx.alloc(max(4 * rows, 4)), ctx.alloc(max(4 * rows, 4))
+    dI, dP = (ctx.alloc(4 * rows * top), ctx.alloc(4 * rows * top)) if rows * top else (None, None)
+    token_logprobs_device(ctx, hipc_dtype(logits.dtype), dX, vocab, rows, vocab, dT, dL, dE, top, dI, dP)
+    out = [ctx.download(dL, np.float32, (rows,)), ctx.download(dE, np.float32, (rows,))]
+    out += [ctx.download(dI, np.int32, (rows, top)), ctx.download(dP, np.float32, (rows, top))] if dI else \
+        [np.zeros((rows, top), np.int32), np.zeros((rows, top), np.float32)]
+    for b in (dX, dT, dL, dE, dI, dP):
+        if b is not None:
+            b.free()
+    return tuple(out)

@@ -58,6 +58,18 @@ class DecoderConfig(C.Structure):
                [(n, C.c_float) for n in ("rms_eps", "rope_theta", "attn_scale", "embed_scale")]
 
 
+class AttentionHeads(C.Structure):
+    """``hipc_attention_heads``."""
+    _fields_ = [(n, C.c_int32) for n in ("n_q_heads", "n_kv_heads", "head_dim", "causal", "window")] + [("scale", C.c_float)]
+
+
+class Kv4Cache(C.Structure):
+    """``hipc_kv4_cache``: where a paged 4-bit cache lies and whose pages are whose (device addresses)."""
+    _fields_ = [(n, C.c_void_p) for n in ("k_codes", "k_params", "v_codes", "v_params")] + [("n_pages", C.c_int64)] + \
+               [(n, C.c_int32) for n in ("page_size", "n_kv_heads", "head_dim", "n_seqs")] + \
+               [("lengths", C.c_void_p), ("table", C.c_void_p), ("table_width", C.c_int64)]
+
+
 class InitializerInfo(C.Structure):
     """``hipc_initializer_info``."""
     _fields_ = [("data_type", C.c_int32), ("n_dims", C.c_int32), ("dims", C.c_int64 * 8), ("bytes", C.c_size_t),
@@ -135,6 +147,12 @@ SIGNATURES = {
     "hipc_conv_integer": (_int, [_vp, _vp, _int, _vp, _vp, _vp, C.POINTER(ConvGeom), _vp]),
     "hipc_qlinear_conv": (_int, [_vp, _vp, _int, _f, C.c_int32, _vp, _FloatArray, _i64, C.c_int32, _f,
                                  C.c_int32, _int, _vp, C.POINTER(ConvGeom), _vp]),
+    "hipc_prompt_attention": (_int, [_vp, C.POINTER(AttentionHeads), _int, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64,
+                                     _i64, _vp, _i64]),
+    "hipc_kv4_append": (_int, [_vp, C.POINTER(Kv4Cache), _int, _vp, _i64, _vp, _i64, _vp, _i64]),
+    "hipc_kv4_read": (_int, [_vp, C.POINTER(Kv4Cache), _int, _vp, _i64, _vp, _i64, _vp, _i64]),
+    "hipc_kv4_attention": (_int, [_vp, C.POINTER(Kv4Cache), C.POINTER(AttentionHeads), _int, _i64, _vp, _i64, _vp, _i64]),
+    "hipc_token_logprobs": (_int, [_vp, _int, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _int, _vp, _vp]),
     "hipc_decoder_create": (_int, [_vp, C.POINTER(DecoderConfig), C.POINTER(_vp)]),
     "hipc_decoder_destroy": (None, [_vp, _vp]),
     "hipc_decoder_set_linear": (_int, [_vp, _vp, _int, _int, _vp, _sz, _vp, _sz, _vp, _sz]),
@@ -143,6 +161,7 @@ SIGNATURES = {
     "hipc_decoder_reset": (_int, [_vp, _vp, C.c_int32, C.c_int32]),
     "hipc_decoder_set_layer_attention": (_int, [_vp, _vp, _int, C.c_int32, _f]),
     "hipc_decoder_kv_cache": (_int, [_vp, _vp, _int, C.POINTER(_vp), C.POINTER(_vp)]),
+    "hipc_decoder_logits": (_int, [_vp, _vp, C.POINTER(_vp)]),
     "hipc_decoder_step": (_int, [_vp, _vp]),
     "hipc_decoder_read": (_int, [_vp, _vp, C.POINTER(C.c_int32), C.POINTER(C.c_int32), _vp, _vp, C.c_int32]),
 }

@@ -120,6 +120,8 @@ const OptionName kOptions[] = {
     {"HIPC_DEC_WAIT", &Tuning::dec_wait},
     {"HIPC_DEC_WIDE", &Tuning::dec_wide},
     {"HIPC_DEC_POLLS", &Tuning::dec_polls},
+    {"HIPC_PROMPT_WAVES", &Tuning::prompt_waves},
+    {"HIPC_PROMPT_SPLIT", &Tuning::prompt_split},
     {"HIPC_DQL_WAIT", &Tuning::dql_wait},
     {"HIPC_DEC_PREFETCH", &Tuning::dec_prefetch},
 };

@@ -1,4 +1,6 @@
 // Attention over packed prompts (hipc_prompt_attention).
+#include <algorithm>
+
 #include "kv4.h"
 #include "lanes.h"
 
@@ -139,8 +141,75 @@ __device__ __forceinline__ pu4 descriptor(const void *p, uint32_t bytes) {
 // what one key range of a row left for the join: sums not divided yet
 __device__ __forceinline__ size_t prompt_part(const PromptArgs &a, int z, int row, int head) { return ((size_t)z * a.total_q + row) * a.n_q_heads + head; }
 
+// the key tiles of a workgroup of `rows` query rows: what its rows see together, or one of a.splits parts of it
+struct PromptSpan {
+    int t0, t1;
+    __device__ __forceinline__ PromptSpan(const PromptArgs &a, const PromptTile &pt, int rows, int key_tile) {
+        const int past = pt.keys - pt.len_q, last = (min(pt.r0 + rows, pt.rows) - 1) / a.group;
+        const int end = a.causal ? min(max(past + last + 1, 0), pt.keys) : pt.keys;
+        const int begin = a.window > 0 ? max(past + pt.r0 / a.group - a.window + 1, 0) : 0;
+        t0 = begin / key_tile, t1 = end > begin ? (end + key_tile - 1) / key_tile : t0;
+        if (a.splits > 1) {
+            const int per = (t1 - t0 + a.splits - 1) / a.splits;
+            t0 += (int)blockIdx.y * per, t1 = min(t1, t0 + per);
+        }
+    }
+};
+// a lane's query row and the keys it sees; those some and those all of its wavefront's 32 rows see
+struct PromptRow {
+    bool mine, any;
+    int token, head, lane_begin, lane_end, begin, end, all_begin, all_end;
+    __device__ __forceinline__ PromptRow(const PromptArgs &a, const PromptTile &pt, int first, int n, int kvh) {
+        const int past = pt.keys - pt.len_q, row = first + n;
+        any = first < pt.rows, mine = row < pt.rows;
+        token = row / a.group, head = kvh * a.group + (row - token * a.group);
+        const int p0 = past + first / a.group, p1 = past + min(first + 31, pt.rows - 1) / a.group;
+        auto ends = [&](int pos) { return a.causal ? min(pos + 1, pt.keys) : pt.keys; };
+        auto begins = [&](int pos) { return a.window > 0 ? max(pos - a.window + 1, 0) : 0; };
+        lane_begin = begins(past + token), lane_end = ends(past + token);
+        begin = begins(p0), end = ends(p1), all_begin = begins(p1), all_end = ends(p0);
+    }
+};
+// counts of visible values that are not finite (1 of +inf, 128 of -inf, 16384 of NaN, of at most 64 keys), added to sums
+__device__ __forceinline__ void add_kinds(const pf16 &kinds, pf16 &o) {
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+        const int k = (int)kinds[r];
+        if (k) o[r] += k >= 16384 || ((k & 127) && k >= 128) ? NAN : k >= 128 ? -INFINITY : INFINITY;
+    }
+}
+// the lane's row, done: divided into Y, or as it is for the join
+template <typename T, int HD>
+__device__ __forceinline__ void prompt_rows_out(const PromptArgs &a, const PromptTile &pt, const PromptRow &pr, int h, float m, float l, const pf16 (&o)[HD / 32]) {
+    l = halves_sum(l);
+    if (!pr.mine) return;
+    if (a.splits > 1) {
+        const size_t part = prompt_part(a, blockIdx.y, pt.q0 + pr.token, pr.head);
+        if (h == 0) a.part_ml[2 * part] = m, a.part_ml[2 * part + 1] = l;
+        float *to = a.part_o + part * a.dim;
+#pragma unroll
+        for (int ot = 0; ot < HD / 32; ot++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int c = 32 * ot + 8 * (r / 4) + 4 * h;
+                if (c < a.dim) *reinterpret_cast<float4 *>(to + c) = make_float4(o[ot][r], o[ot][r + 1], o[ot][r + 2], o[ot][r + 3]);
+            }
+        return;
+    }
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T *y = static_cast<T *>(a.y) + a.y_stride * (pt.q0 + pr.token) + (int64_t)pr.head * a.dim;
+#pragma unroll
+    for (int ot = 0; ot < HD / 32; ot++)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int c = 32 * ot + 8 * (r / 4) + 4 * h;
+            if (c < a.dim) *reinterpret_cast<T4 *>(y + c) = T4{(T)(o[ot][r] * inv), (T)(o[ot][r + 1] * inv), (T)(o[ot][r + 2] * inv), (T)(o[ot][r + 3] * inv)};
+        }
+}
+
 template <int HD, int W, int KT>
-__global__ void __launch_bounds__(64 * W) prompt_tiles_kernel(const PromptArgs a) {
+__global__ void __launch_bounds__(64 * W, HD > 128 || (HD == 128 && W == 2) ? 1 : 2) prompt_tiles_kernel(const PromptArgs a) {
     constexpr int PITCH = HD <= 64 ? 64 : HD <= 128 ? 128 : 256;   // halfs of an LDS row
     constexpr int TILE = KT * PITCH * 2;                           // bytes of a tile of K, or of V
     constexpr int CHUNKS = PITCH / 8, RPI = 512 / PITCH;           // 16-byte chunks of a row; rows of a 1 KiB load
@@ -156,35 +225,16 @@ __global__ void __launch_bounds__(64 * W) prompt_tiles_kernel(const PromptArgs a
     PromptTile pt;
     if (!prompt_tile(a, a.tiles - 1 - (int)(blockIdx.x / heads), 32 * W, &pt)) return;
 
-    const int past = pt.keys - pt.len_q;                              // position of the sequence's first query row
-    const int last_row = min(pt.r0 + 32 * W, pt.rows) - 1;
-    const int k_end = a.causal ? min(max(past + last_row / a.group + 1, 0), pt.keys) : pt.keys;
-    const int k_begin = a.window > 0 ? max(past + pt.r0 / a.group - a.window + 1, 0) : 0;
-    int t0 = k_begin / KT, t1 = k_end > k_begin ? (k_end + KT - 1) / KT : t0;
-    if (a.splits > 1) {
-        const int per = (t1 - t0 + a.splits - 1) / a.splits;
-        t0 += (int)blockIdx.y * per, t1 = min(t1, t0 + per);
-    }
-
-    // the lane's query row
-    const int wr0 = pt.r0 + 32 * wave, row = wr0 + n;
-    const bool mine = row < pt.rows;
-    const int token = row / a.group, head = kvh * a.group + (row - token * a.group), pos = past + token;
-    const int lane_end = a.causal ? min(pos + 1, pt.keys) : pt.keys, lane_begin = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
-    // ... and the wavefront's: the first row's and the last's ends
-    const int w_last = min(wr0 + 31, pt.rows - 1);
-    const int w_pos0 = past + wr0 / a.group, w_pos1 = past + w_last / a.group;
-    const bool w_any = wr0 < pt.rows;
-    const int w_end = a.causal ? min(w_pos1 + 1, pt.keys) : pt.keys, w_begin = a.window > 0 ? max(w_pos0 - a.window + 1, 0) : 0;
-    const int w_all_end = a.causal ? min(w_pos0 + 1, pt.keys) : pt.keys, w_all_begin = a.window > 0 ? max(w_pos1 - a.window + 1, 0) : 0;
+    const PromptSpan sp(a, pt, 32 * W, KT);
+    const PromptRow pr(a, pt, pt.r0 + 32 * wave, n, kvh);
 
     ph8 qf[HD / 16];
     {
-        const _Float16 *q = static_cast<const _Float16 *>(a.q) + a.q_stride * (pt.q0 + (mine ? token : 0)) + (int64_t)(mine ? head : 0) * a.dim;
+        const _Float16 *q = static_cast<const _Float16 *>(a.q) + a.q_stride * (pt.q0 + (pr.mine ? pr.token : 0)) + (int64_t)(pr.mine ? pr.head : 0) * a.dim;
 #pragma unroll
         for (int c = 0; c < HD / 16; c++) {
             ph8 v = {};
-            if (mine && 16 * c + 8 * h < a.dim) v = *reinterpret_cast<const ph8 *>(q + 16 * c + 8 * h);
+            if (pr.mine && 16 * c + 8 * h < a.dim) v = *reinterpret_cast<const ph8 *>(q + 16 * c + 8 * h);
             qf[c] = a.scale < 0.f ? -v : v;
         }
     }
@@ -228,13 +278,13 @@ __global__ void __launch_bounds__(64 * W) prompt_tiles_kernel(const PromptArgs a
     for (int i = 0; i < HD / 32; i++) o[i] = pf16{};
     float m = -INFINITY, l = 0.f;
 
-    if (t0 < t1) fetch(t0, 0);
-    for (int t = t0; t < t1; t++) {
-        const int buf = (t - t0) & 1;
+    if (sp.t0 < sp.t1) fetch(sp.t0, 0);
+    for (int t = sp.t0; t < sp.t1; t++) {
+        const int buf = (t - sp.t0) & 1;
         // this tile has arrived, and every wavefront is done with the other buffer
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (t + 1 < t1) fetch(t + 1, buf ^ 1);
-        if (!w_any || t * KT >= w_end || (t + 1) * KT <= w_begin) continue;
+        if (t + 1 < sp.t1) fetch(t + 1, buf ^ 1);
+        if (!pr.any || t * KT >= pr.end || (t + 1) * KT <= pr.begin) continue;
         const char *ks = smem + buf * 2 * TILE, *vs = ks + TILE;
 
         pf16 s[KT / 32];
@@ -245,14 +295,14 @@ __global__ void __launch_bounds__(64 * W) prompt_tiles_kernel(const PromptArgs a
             for (int c = 0; c < HD / 16; c++)
                 s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const ph8 *>(ks + k_at[c & 3] + (c >> 2) * 128 + b * 64 * PITCH), qf[c], s[b], 0, 0, 0);
         }
-        const bool masked = (t + 1) * KT > w_all_end || t * KT < w_all_begin;
+        const bool masked = (t + 1) * KT > pr.all_end || t * KT < pr.all_begin;
         if (masked) {
 #pragma unroll
             for (int b = 0; b < KT / 32; b++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const int key = t * KT + 32 * b + 8 * (r / 4) + 4 * h + r % 4;
-                    s[b][r] = key >= lane_begin && key < lane_end ? s[b][r] : -INFINITY;
+                    s[b][r] = key >= pr.lane_begin && key < pr.lane_end ? s[b][r] : -INFINITY;
                 }
         }
         float mx = s[0][0];
@@ -313,16 +363,12 @@ __global__ void __launch_bounds__(64 * W) prompt_tiles_kernel(const PromptArgs a
                             // 1 of +inf, 128 of -inf, 16384 of NaN: a tile's counts of each stay apart
                             if ((bits & 0x7c00) == 0x7c00) kind[j] = (_Float16)((bits & 0x3ff) ? 16384.f : bits >> 15 ? 128.f : 1.f), v[j] = (_Float16)0;
                             const int key = t * KT + 16 * u + 8 * (j / 4) + 4 * h + j % 4;
-                            seen[j] = (_Float16)(key >= lane_begin && key < lane_end ? 1.f : 0.f);
+                            seen[j] = (_Float16)(key >= pr.lane_begin && key < pr.lane_end ? 1.f : 0.f);
                         }
                         o[ot] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u], o[ot], 0, 0, 0);
                         kinds = __builtin_amdgcn_mfma_f32_32x32x16_f16(kind, seen, kinds, 0, 0, 0);
                     }
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int k = (int)kinds[r];
-                        if (k) o[ot][r] += k >= 16384 || ((k & 127) && k >= 128) ? NAN : k >= 128 ? -INFINITY : INFINITY;
-                    }
+                    add_kinds(kinds, o[ot]);
                 }
                 continue;
             }
@@ -332,31 +378,226 @@ __global__ void __launch_bounds__(64 * W) prompt_tiles_kernel(const PromptArgs a
 #pragma unroll
             for (int u = 0; u < KT / 16; u++) o[ot] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_part(ot, u), p[u], o[ot], 0, 0, 0);
     }
-    l = halves_sum(l);
-    if (!mine) return;
-    if (a.splits > 1) {
-        const size_t part = prompt_part(a, blockIdx.y, pt.q0 + token, head);
-        if (h == 0) a.part_ml[2 * part] = m, a.part_ml[2 * part + 1] = l;
-        float *to = a.part_o + part * a.dim;
+    prompt_rows_out<_Float16, HD>(a, pt, pr, h, m, l, o);
+}
+
+// ---------------------------------------------------------------------------------- on the matrix cores, f32
+//
+// The same products of f32 factors, each as three bf16 terms (8 bits a term, together the value's 24): of the nine products of
+// terms the six that matter at 2^-24 are formed, smallest first. K and V are split once on their way into LDS, a plane a term; a
+// tile's values wait in registers while the tile before is multiplied.
+typedef __bf16 pb8 __attribute__((ext_vector_type(8)));
+typedef __bf16 pb2 __attribute__((ext_vector_type(2)));
+typedef float pf2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ float bf16_up(uint32_t bits) { return __uint_as_float(bits << 16); }
+// two values as three pairs of bf16; a value that is not finite is its first term, whole
+__device__ __forceinline__ void split3(float x, float y, uint32_t (&term)[3]) {
+    constexpr float most = 3.3895314e38f;   // bf16's largest: rounding up from it would be an infinity
+    const bool fx = fabsf(x) <= 3.4028235e38f, fy = fabsf(y) <= 3.4028235e38f;
+    const pf2 a = {fx ? __builtin_amdgcn_fmed3f(x, -most, most) : x, fy ? __builtin_amdgcn_fmed3f(y, -most, most) : y};
+    term[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector(a, pb2));
+    const pf2 r = {fx ? x - bf16_up(term[0]) : 0.f, fy ? y - __uint_as_float(term[0] & 0xffff0000u) : 0.f};
+    term[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, pb2));
+    const pf2 q = {r.x - bf16_up(term[1]), r.y - __uint_as_float(term[1] & 0xffff0000u)};
+    term[2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(q, pb2));
+}
+__device__ __forceinline__ pf16 mfma_terms(const pb8 (&x)[3], const pb8 (&y)[3], pf16 acc) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[2], y[0], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], y[2], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], y[1], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], y[0], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], y[1], acc, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], y[0], acc, 0, 0, 0);
+}
+
+template <int HD, int W>
+__global__ void __launch_bounds__(64 * W, HD > 128 ? 1 : 2) prompt_terms_kernel(const PromptArgs a) {
+    constexpr int KT = 32;
+    constexpr int PITCH = HD <= 64 ? 64 : HD <= 128 ? 128 : 256;   // bf16 of an LDS row
+    constexpr int PLANE = KT * PITCH * 2;                          // bytes of a term of a tile
+    constexpr int CHUNKS = HD / 8;                                 // units of eight channels of a row
+    constexpr int EACH = (KT * CHUNKS + 64 * W - 1) / (64 * W);    // ... of a tile, per thread
+    __shared__ __attribute__((aligned(1024))) char smem[6 * PLANE];   // [K, V][term]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 31, h = lane >> 5;
+
+    const int heads = a.n_q_heads / a.group, kvh = (int)(blockIdx.x % heads);
+    PromptTile pt;
+    if (!prompt_tile(a, a.tiles - 1 - (int)(blockIdx.x / heads), 32 * W, &pt)) return;
+    const PromptSpan sp(a, pt, 32 * W, KT);
+    const PromptRow pr(a, pt, pt.r0 + 32 * wave, n, kvh);
+
+    pb8 qf[HD / 16][3];
+    {
+        const float *q = static_cast<const float *>(a.q) + a.q_stride * (pt.q0 + (pr.mine ? pr.token : 0)) + (int64_t)(pr.mine ? pr.head : 0) * a.dim;
+#pragma unroll
+        for (int c = 0; c < HD / 16; c++) {
+            float4 v[2] = {};
+            if (pr.mine && 16 * c + 8 * h < a.dim) {
+                v[0] = *reinterpret_cast<const float4 *>(q + 16 * c + 8 * h);
+                v[1] = *reinterpret_cast<const float4 *>(q + 16 * c + 8 * h + 4);
+            }
+            const float *x = reinterpret_cast<const float *>(v);
+            uint32_t term[4][3];
+#pragma unroll
+            for (int j = 0; j < 4; j++) split3(x[2 * j], x[2 * j + 1], term[j]);
+#pragma unroll
+            for (int e = 0; e < 3; e++) qf[c][e] = __builtin_bit_cast(pb8, pu4{term[0][e], term[1][e], term[2][e], term[3][e]});
+        }
+    }
+    const float c2 = a.scale * kLog2e;
+
+    const float *kb = static_cast<const float *>(a.k) + a.k_stride * pt.k0 + (int64_t)kvh * a.dim;
+    const float *vb = static_cast<const float *>(a.v) + a.v_stride * pt.k0 + (int64_t)kvh * a.dim;
+    float4 held[2][EACH][2];
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const int unit = tid + e * 64 * W, r = unit / CHUNKS, c = (unit - r * CHUNKS) * 8;
+            const bool there = unit < KT * CHUNKS && t * KT + r < pt.keys && c < a.dim;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                held[0][e][j] = there ? *reinterpret_cast<const float4 *>(kb + a.k_stride * (t * KT + r) + c + 4 * j) : float4{};
+                held[1][e][j] = there ? *reinterpret_cast<const float4 *>(vb + a.v_stride * (t * KT + r) + c + 4 * j) : float4{};
+            }
+        }
+    };
+    auto store = [&]() {
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const int unit = tid + e * 64 * W, r = unit / CHUNKS, chunk = unit - r * CHUNKS;
+            if (unit >= KT * CHUNKS) break;
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                const float *x = reinterpret_cast<const float *>(held[w][e]);
+                uint32_t term[4][3];
+#pragma unroll
+                for (int j = 0; j < 4; j++) split3(x[2 * j], x[2 * j + 1], term[j]);
+                char *to = smem + w * 3 * PLANE + r * PITCH * 2 + (chunk ^ (w ? (r & 3) << 1 : r & 7)) * 16;
+#pragma unroll
+                for (int k = 0; k < 3; k++) *reinterpret_cast<pu4 *>(to + k * PLANE) = pu4{term[0][k], term[1][k], term[2][k], term[3][k]};
+            }
+        }
+    };
+
+    const int i16 = lane & 15;
+    uint32_t k_at[4], v_at[2];
+#pragma unroll
+    for (int c = 0; c < 4; c++) k_at[c] = n * PITCH * 2 + (((2 * c + h) ^ (n & 7)) * 16);
+#pragma unroll
+    for (int o = 0; o < 2; o++) v_at[o] = (4 * h + (i16 >> 2)) * PITCH * 2 + (((4 * o + 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1)) ^ ((i16 >> 2) << 1)) * 16) + (i16 & 1) * 8;
+
+    pf16 o[HD / 32];
+#pragma unroll
+    for (int i = 0; i < HD / 32; i++) o[i] = pf16{};
+    float m = -INFINITY, l = 0.f;
+    if (sp.t0 < sp.t1) fetch(sp.t0);
+    for (int t = sp.t0; t < sp.t1; t++) {
+        __syncthreads();   // everybody is done with the tile before
+        store();
+        __syncthreads();
+        if (t + 1 < sp.t1) fetch(t + 1);
+        if (!pr.any || t * KT >= pr.end || (t + 1) * KT <= pr.begin) continue;
+
+        pf16 s = pf16{};
+#pragma unroll
+        for (int c = 0; c < HD / 16; c++) {
+            pb8 kf[3];
+#pragma unroll
+            for (int e = 0; e < 3; e++) kf[e] = *reinterpret_cast<const pb8 *>(smem + e * PLANE + k_at[c & 3] + (c >> 2) * 128);
+            s = mfma_terms(kf, qf[c], s);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] *= c2;
+        const bool masked = (t + 1) * KT > pr.all_end || t * KT < pr.all_begin;
+        if (masked) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int key = t * KT + 8 * (r / 4) + 4 * h + r % 4;
+                s[r] = key >= pr.lane_begin && key < pr.lane_end ? s[r] : -INFINITY;
+            }
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; r++) mx = fmaxf(mx, s[r]);
+        mx = halves_max(mx);
+        if (__any(mx > m + kRescaleAt)) {
+            const float grown = mx > m + kRescaleAt ? mx : m, keep = grown == m ? 1.f : __builtin_amdgcn_exp2f(m - grown);
+            m = grown, l *= keep;
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[i][r] *= keep;
+        }
+        const float shift = m == -INFINITY ? 0.f : m;
+        pb8 p[2][3];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            uint32_t term[4][3];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float x = __builtin_amdgcn_exp2f(s[8 * u + 2 * j] - shift), y = __builtin_amdgcn_exp2f(s[8 * u + 2 * j + 1] - shift);
+                l += x + y;
+                split3(x, y, term[j]);
+            }
+#pragma unroll
+            for (int e = 0; e < 3; e++) p[u][e] = __builtin_bit_cast(pb8, pu4{term[0][e], term[1][e], term[2][e], term[3][e]});
+        }
+        auto v_part = [&](int e, int ot, int u) {
+            const char *at = smem + (3 + e) * PLANE + v_at[ot & 1] + (ot >> 1) * 128 + u * 32 * PITCH;
+            const ps4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ps4 *)(at));
+            const ps4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ps4 *)(at + 16 * PITCH));
+            return __builtin_bit_cast(pb8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        // Infinities and NaN of V (whole in its first term): in the product zeros stand for them -- a weight's later terms may be
+        // zero or negative -- and a second product finds out what the rows that see them get.
+        uint32_t bad = 0;
 #pragma unroll
         for (int ot = 0; ot < HD / 32; ot++)
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const int c = 32 * ot + 8 * (r / 4) + 4 * h;
-                if (c < a.dim) *reinterpret_cast<float4 *>(to + c) = make_float4(o[ot][r], o[ot][r + 1], o[ot][r + 2], o[ot][r + 3]);
+            for (int u = 0; u < 2; u++) {
+                const pu4 w = __builtin_bit_cast(pu4, v_part(0, ot, u));
+#pragma unroll
+                for (int j = 0; j < 4; j++) bad |= ((w[j] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
             }
-        return;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    _Float16 *y = static_cast<_Float16 *>(a.y) + a.y_stride * (pt.q0 + token) + (int64_t)head * a.dim;
+        const bool any_bad = __any(bad != 0);
 #pragma unroll
-    for (int ot = 0; ot < HD / 32; ot++)
+        for (int ot = 0; ot < HD / 32; ot++)
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int c = 32 * ot + 8 * (r / 4) + 4 * h;
-            if (c < a.dim)
-                *reinterpret_cast<ph4 *>(y + c) = ph4{(_Float16)(o[ot][r] * inv), (_Float16)(o[ot][r + 1] * inv), (_Float16)(o[ot][r + 2] * inv), (_Float16)(o[ot][r + 3] * inv)};
+            for (int u = 0; u < 2; u++) {
+                pb8 v[3];
+#pragma unroll
+                for (int e = 0; e < 3; e++) v[e] = v_part(e, ot, u);
+                if (any_bad) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if ((__builtin_bit_cast(uint16_t, (__bf16)v[0][j]) & 0x7f80) == 0x7f80) v[0][j] = (__bf16)0.f;
+                }
+                o[ot] = mfma_terms(v, p[u], o[ot]);
+            }
+        if (any_bad) {
+#pragma unroll
+            for (int ot = 0; ot < HD / 32; ot++) {
+                pf16 kinds = pf16{};
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const pb8 v = v_part(0, ot, u);
+                    pb8 kind = {}, seen = {};
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const uint16_t bits = __builtin_bit_cast(uint16_t, (__bf16)v[j]);
+                        if ((bits & 0x7f80) == 0x7f80) kind[j] = (__bf16)((bits & 0x7f) ? 16384.f : bits >> 15 ? 128.f : 1.f);
+                        const int key = t * KT + 16 * u + 8 * (j / 4) + 4 * h + j % 4;
+                        seen[j] = (__bf16)(key >= pr.lane_begin && key < pr.lane_end ? 1.f : 0.f);
+                    }
+                    kinds = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kind, seen, kinds, 0, 0, 0);
+                }
+                add_kinds(kinds, o[ot]);
+            }
         }
+    }
+    prompt_rows_out<float, HD>(a, pt, pr, h, m, l, o);
 }
 
 // The ranges of keys that several workgroups had of the same rows, joined: one wavefront per row and head.
@@ -388,23 +629,51 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs a) {
         if (lane + 64 * i < a.dim) y[lane + 64 * i] = (T)(acc[i] * inv);
 }
 
-template <int HD, int W, int KT>
-int prompt_tiles(hipc_ctx *ctx, PromptArgs a, int splits) {
+size_t prompt_parts_bytes(const PromptArgs &a, int splits) { return splits > 1 ? (size_t)splits * a.total_q * a.n_q_heads * (a.dim + 2) * 4 : 0; }
+
+template <typename T, int HD, int W>
+int prompt_launch(hipc_ctx *ctx, PromptArgs a, int splits) {
     const int64_t tiles = ceil_div((int64_t)a.total_q * a.group, 32 * W) + a.n_seqs;   // (at most: a sequence may leave one unfinished)
     a.tiles = (int)tiles, a.splits = splits;
     if (splits > 1) {
         const size_t rows = (size_t)splits * a.total_q * a.n_q_heads;
         void *s = nullptr;
-        if (int rc = scratch_get(ctx, kScratchPrompt, rows * (a.dim + 2) * 4, &s)) return rc;
+        if (int rc = scratch_get(ctx, kScratchPrompt, prompt_parts_bytes(a, splits), &s)) return rc;
         a.part_o = static_cast<float *>(s), a.part_ml = a.part_o + rows * a.dim;
     }
-    hipLaunchKernelGGL((prompt_tiles_kernel<HD, W, KT>), dim3((unsigned)(tiles * (a.n_q_heads / a.group)), splits), 64 * W, 0, ctx->stream, a);
+    const dim3 grid((unsigned)(tiles * (a.n_q_heads / a.group)), splits);
+    if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((prompt_tiles_kernel<HD, W, (HD > 128 ? 32 : 64)>), grid, 64 * W, 0, ctx->stream, a);
+    else hipLaunchKernelGGL((prompt_terms_kernel<HD, W>), grid, 64 * W, 0, ctx->stream, a);
     HIPC_LAUNCHED(ctx);
     if (splits > 1) {
-        hipLaunchKernelGGL((prompt_join_kernel<_Float16>), (unsigned)ceil_div((int64_t)a.total_q * a.n_q_heads, 4), 256, 0, ctx->stream, a);
+        hipLaunchKernelGGL((prompt_join_kernel<T>), (unsigned)ceil_div((int64_t)a.total_q * a.n_q_heads, 4), 256, 0, ctx->stream, a);
         HIPC_LAUNCHED(ctx);
     }
     return HIPC_OK;
+}
+
+// How many wavefronts a workgroup has, and how many workgroups share the keys of a tile of rows. Both go by what the host knows:
+// rows, keys and sequences in all. Measured (us, 2 / 4 / 8 wavefronts): 8192 rows in one sequence, 32 query and 8 kv heads of 128, f16
+// 886 / 618 / 604; eight sequences of up to 1024 85 / 63 / 72 (the longest sequence's last tiles end the launch); two of up to 1500 in f32, whose
+// tiles are split once for all wavefronts, 357 / 265 / 236. Sharing keys costs a join and pays while CUs are left: 16 rows behind 8000 keys
+// 210 alone, 36 shared by 16; 2000 rows of four heads of 256 seeing 512 keys 46 alone, 34 by four, 52 by sixteen.
+template <typename T>
+int prompt_matrix(hipc_ctx *ctx, const PromptArgs &a) {
+    const int64_t rows = (int64_t)a.total_q * a.group, kv = a.n_q_heads / a.group, cus = ctx->cu_count;
+    int waves = rows <= 64 * (int64_t)a.n_seqs ? 2 : 4;
+    if (a.dim <= 128 && waves == 4 && rows * kv >= 256 * cus * (sizeof(T) == 2 ? 4 : 1)) waves = 8;
+    if (ctx->tune.prompt_waves > 0) waves = ctx->tune.prompt_waves;
+    const int64_t groups = std::max<int64_t>(ceil_div(rows, 32 * waves), a.n_seqs) * kv;
+    int64_t keys = a.total_k / a.n_seqs;
+    if (a.window > 0) keys = std::min<int64_t>(keys, a.window + 32 * waves / a.group);
+    const int64_t key_tiles = keys / (sizeof(T) == 2 && a.dim <= 128 ? 64 : 32);
+    int splits = groups < cus ? (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / groups, key_tiles / 4, 32})) : 1;
+    if (ctx->tune.prompt_split > 0) splits = ctx->tune.prompt_split;
+    splits = std::min(splits, 256);
+    if (!scratch_fits(ctx, kScratchPrompt, prompt_parts_bytes(a, splits))) splits = 1;
+    if (a.dim <= 64) return waves >= 8 ? prompt_launch<T, 64, 8>(ctx, a, splits) : waves >= 4 ? prompt_launch<T, 64, 4>(ctx, a, splits) : prompt_launch<T, 64, 2>(ctx, a, splits);
+    if (a.dim <= 128) return waves >= 8 ? prompt_launch<T, 128, 8>(ctx, a, splits) : waves >= 4 ? prompt_launch<T, 128, 4>(ctx, a, splits) : prompt_launch<T, 128, 2>(ctx, a, splits);
+    return waves >= 4 ? prompt_launch<T, 256, 4>(ctx, a, splits) : prompt_launch<T, 256, 2>(ctx, a, splits);
 }
 
 }  // namespace
@@ -436,12 +705,11 @@ int hipc_prompt_attention(hipc_ctx *ctx, const hipc_attention_heads *heads, int 
         a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.y_stride = y_stride;
         a.n_seqs = (int)n_seqs, a.total_q = (int)total_q, a.total_k = (int)total_k, a.n_q_heads = heads->n_q_heads, a.group = heads->n_q_heads / heads->n_kv_heads;
         a.dim = heads->head_dim, a.causal = heads->causal != 0, a.window = heads->window;
-        if (dtype == HIPC_F16 && heads->head_dim % 8 == 0 && heads->head_dim <= 256 && aligned(Q, 16) && aligned(K, 16) && aligned(V, 16) && aligned(Y, 8) &&
-            q_stride % 8 == 0 && k_stride % 8 == 0 && v_stride % 8 == 0 && y_stride % 4 == 0 && k_stride <= 1 << 23 && v_stride <= 1 << 23 &&
-            (total_q * a.group + (int64_t)n_seqs * 256) * heads->n_kv_heads < (int64_t)1 << 31) {
-            const int d = heads->head_dim;
-            return d <= 64 ? prompt_tiles<64, 8, 64>(ctx, a, 1) : d <= 128 ? prompt_tiles<128, 8, 64>(ctx, a, 1) : prompt_tiles<256, 4, 32>(ctx, a, 1);
-        }
+        const int64_t unit = dtype == HIPC_F16 ? 8 : 4;   // elements of 16 bytes
+        if (heads->head_dim % 8 == 0 && heads->head_dim <= 256 && aligned(Q, 16) && aligned(K, 16) && aligned(V, 16) && aligned(Y, 16) && q_stride % unit == 0 &&
+            k_stride % unit == 0 && v_stride % unit == 0 && y_stride % unit == 0 && k_stride <= 1 << 23 && v_stride <= 1 << 23 &&
+            (total_q * a.group + n_seqs * 256) * heads->n_kv_heads < (int64_t)1 << 31)
+            return dtype == HIPC_F16 ? prompt_matrix<_Float16>(ctx, a) : prompt_matrix<float>(ctx, a);
         const dim3 grid((unsigned)total_q, heads->n_q_heads);
         if (dtype == HIPC_F16) hipLaunchKernelGGL((prompt_rows_kernel<_Float16>), grid, 64, 0, ctx->stream, a);
         else hipLaunchKernelGGL((prompt_rows_kernel<float>), grid, 64, 0, ctx->stream, a);

@@ -40,7 +40,7 @@
 
 namespace hipc {
 
-constexpr int kScratchSlots = 6;
+constexpr int kScratchSlots = 7;
 
 // grow-only device scratch reused by operators that need a temporary (packed
 // B of a raw call, the i32 accumulator of a QLinear op). One in-order stream
@@ -321,6 +321,8 @@ int allow_dynamic_lds(hipc_ctx *ctx, K kernel, size_t bytes, bool (&done)[kMaxDe
 // Returns ctx->scratch[slot] grown to at least `bytes`. Growth allocates, so it is
 // refused while a capture is open.
 int scratch_get(hipc_ctx *ctx, int slot, size_t bytes, void **out);
+// words of device memory set by a kernel (context.hip)
+__global__ void fill_words(uint32_t *dst, size_t words, uint32_t value);
 // whether it would: inside a capture only what the slot has grown to before. A call that was never run eagerly takes a route
 // that needs no scratch memory there, where it has one
 inline bool scratch_fits(const hipc_ctx *ctx, int slot, size_t bytes) { return !ctx->capturing || ctx->scratch[slot].bytes >= bytes; }

@@ -64,6 +64,32 @@ __device__ __forceinline__ void kv4_values(uint32_t w, kvh2 scale, kvh2 lowest, 
     v[3] = __builtin_elementwise_fma(part(w & 0x00f000f0u, 0x54005400u) - k64, scale, lowest);
 }
 
+// the same where every pair of values has a scale and a lowest value of its own (four pairs each, as bits)
+typedef uint32_t kv4_pairs __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void kv4_values(uint32_t w, kv4_pairs scale, kv4_pairs lowest, kvh2 (&v)[4]) {
+    auto part = [](uint32_t bits) { return __builtin_bit_cast(kvh2, bits); };
+    const kvh2 k1024 = {(_Float16)1024.f, (_Float16)1024.f}, k64 = {(_Float16)64.f, (_Float16)64.f};
+    v[0] = __builtin_elementwise_fma(part((w & 0x000f000fu) | 0x64006400u) - k1024, part(scale[0]), part(lowest[0]));
+    v[1] = __builtin_elementwise_fma(part((w & 0x00f000f0u) | 0x54005400u) - k64, part(scale[1]), part(lowest[1]));
+    w >>= 8;
+    v[2] = __builtin_elementwise_fma(part((w & 0x000f000fu) | 0x64006400u) - k1024, part(scale[2]), part(lowest[2]));
+    v[3] = __builtin_elementwise_fma(part((w & 0x00f000f0u) | 0x54005400u) - k64, part(scale[3]), part(lowest[3]));
+}
+
+// eight elements as floats; `wide`: they lie on 16 bytes
+template <typename T>
+__device__ __forceinline__ void kv4_load8(const T *p, bool wide, float (&x)[8]) {
+    typedef T T8 __attribute__((ext_vector_type(8)));
+    if (wide) {
+        const T8 v = *reinterpret_cast<const T8 *>(p);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (float)v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (float)p[i];
+    }
+}
+
 // host side: what every call of the cache checks
 int kv4_check(hipc_ctx *ctx, const char *who, const hipc_kv4_cache *c);
 // the heads of an attention call, and the scale it uses

@@ -1,4 +1,6 @@
 // Attention of the newest tokens of many sequences over the paged 4-bit cache (hipc_kv4_attention).
+#include <type_traits>
+
 #include "kv4.h"
 #include "lanes.h"
 
@@ -11,47 +13,458 @@ struct Kv4Attend {
     const void *q;
     void *y;
     int64_t q_stride, y_stride;
-    int tokens, n_q_heads, window;
+    int tokens, n_q_heads, group, window, row_blocks, wide;   // wide: rows of Q and Y on 16 bytes
     float scale;
+    float *parts;        // [workgroup][2] parts of a unit: rows x channels sums, then (maximum, sum) pairs
+    uint32_t *arrived;   // [workgroup]: parts of the unit that began here and went on; all zero between calls
 };
 
-// One wavefront per query row: one key after the other, the running maximum and sum of the softmax beside the sums.
-template <typename T>
-__global__ void __launch_bounds__(64) kv4_attend_kernel(const Kv4Attend a) {
-    const int lane = threadIdx.x, dim = a.cache.head_dim;
-    const int64_t row = blockIdx.x;
-    const int seq = (int)(row / a.tokens), h = blockIdx.y, kvh = h / (a.n_q_heads / a.cache.n_kv_heads);
-    const int pos = kv4_length(a.cache, seq) - a.tokens + (int)(row - (int64_t)seq * a.tokens);
-    const T *q = static_cast<const T *>(a.q) + row * a.q_stride + (int64_t)h * dim;
-    T *y = static_cast<T *>(a.y) + row * a.y_stride + (int64_t)h * dim;
-    constexpr int C = kKv4MaxHead / 64;
-    float qv[C], acc[C] = {};
+typedef _Float16 kvh8 __attribute__((ext_vector_type(8)));
+typedef float kvf4 __attribute__((ext_vector_type(4)));
+typedef uint32_t kvu2 __attribute__((ext_vector_type(2)));
+typedef uint32_t kvu4 __attribute__((ext_vector_type(4)));
+typedef int kvi2 __attribute__((ext_vector_type(2)));
+
+constexpr int kScratchKv4 = 6;     // scratch slot of this operator alone
+constexpr int kKv4Rows = 16;       // query rows of a unit
+constexpr int kKv4Tile = 64;       // keys a wavefront takes at a time
+constexpr int kKv4Waves = 4;
+constexpr float kKv4Log2e = 1.4426950408889634f;
+constexpr float kKv4RescaleAt = 8.f;   // the running maximum may fall behind by 2^8 before sums are rescaled ...
+constexpr float kKv4Up = 7.f;          // ... and weights are kept 2^7 times as large: up to 2^15, so that two f16 terms hold 22 bits of more of them
+
+// the four groups of 16 lanes, in all lanes
+__device__ __forceinline__ float groups_max(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float groups_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// The key tiles a sequence's newest tokens see: [first, first + count).
+struct Kv4Span {
+    int length, first, count;
+    __device__ __forceinline__ Kv4Span(const Kv4Attend &a, int seq) {
+        length = a.cache.n_pages > 0 ? kv4_length(a.cache, seq) : 0;
+        const int begin = a.window > 0 ? max(length - a.tokens - a.window + 1, 0) : 0;
+        first = begin / kKv4Tile;
+        count = length > 0 ? (length + kKv4Tile - 1) / kKv4Tile - first : 0;
+    }
+};
+
+// Which unit -- (sequence, kv head, block of 16 query rows), in this order -- the tile number `at` of all units' tiles
+// belongs to; `before` is the number of its first tile.
+struct Kv4Unit {
+    int seq, inner;       // inner = kv head * row_blocks + block
+    int count;            // its tiles
+    int64_t before;
+};
+__device__ __forceinline__ int wave_scan(int v) {   // inclusive
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int i = 0; i < C; i++) qv[i] = lane + 64 * i < dim ? (float)q[lane + 64 * i] * a.scale : 0.f;
-    float m = -INFINITY, l = 0.f;
-    for (int t = a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0; t <= pos; t++) {
-        const Kv4Place place = kv4_place(a.cache, seq, t);
-        if (!place.there) continue;
-        const int64_t r = place.slot + (int64_t)kvh * a.cache.page_size;
-        auto value = [&](const void *codes, const void *params, int c) -> float {
-            const int n = (static_cast<const uint8_t *>(codes)[r * (dim / 2) + c / 2] >> (4 * (c & 1))) & 15;
-            const kvh2 p = static_cast<const kvh2 *>(params)[r * (dim / kKv4Group) + c / kKv4Group];
-            return (float)__builtin_fmaf16((_Float16)n, p.x, p.y);
-        };
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < C; i++)
-            if (lane + 64 * i < dim) s = __builtin_fmaf(qv[i], value(a.cache.k_codes, a.cache.k_params, lane + 64 * i), s);
-        s = lean_wave_sum(s);
-        const float grown = fmaxf(m, s), keep = m == -INFINITY ? 0.f : expf(m - grown), p = expf(s - grown);
-        m = grown, l = l * keep + p;
-#pragma unroll
-        for (int i = 0; i < C; i++)
-            if (lane + 64 * i < dim) acc[i] = acc[i] * keep + p * value(a.cache.v_codes, a.cache.v_params, lane + 64 * i);
+    for (int d = 1; d < 64; d <<= 1) {
+        const int up = __shfl_up(v, d);
+        if (lane >= d) v += up;
+    }
+    return v;
+}
+__device__ __forceinline__ bool kv4_find(const Kv4Attend &a, int per_seq, int64_t at, Kv4Unit *u) {
+    const int lane = threadIdx.x & 63;
+    int64_t before = 0;
+    for (int base = 0; base < a.cache.n_seqs; base += 64) {
+        const int n = base + lane < a.cache.n_seqs ? Kv4Span(a, base + lane).count : 0;
+        const int sum = wave_scan(n);
+        const uint64_t over = __ballot(before + (int64_t)sum * per_seq > at);
+        if (over) {
+            const int l = __builtin_ctzll(over);
+            const int tiles = __builtin_amdgcn_readlane(n, l);
+            const int64_t first = before + (int64_t)(__builtin_amdgcn_readlane(sum, l) - tiles) * per_seq;
+            u->seq = base + l, u->count = tiles;
+            u->inner = (int)((at - first) / tiles);
+            u->before = first + (int64_t)u->inner * tiles;
+            return true;
+        }
+        before += (int64_t)__builtin_amdgcn_readlane(sum, 63) * per_seq;
+    }
+    return false;
+}
+
+// One launch for everything. All units' key tiles are laid end to end and dealt to the workgroups in equal runs, so that sequences of any
+// lengths keep the whole device busy; a unit that lies in one run is finished there, and of one that lies in several the workgroup that
+// comes last joins the parts, in their order.
+//
+// A wavefront takes 64 keys of one kv head at a time, for 16 query rows (tokens times the heads of the group):
+//   S^T = K Q^T     16x16x32: of tile t (16 keys) row m is key 16 (m / 4) + 4 t + m % 4, so that a lane ends up with the scores of 16
+//                   consecutive keys of one query (query = lane % 16, keys 16 (lane / 16) ..): two steps of the second product
+//   O^T = V^T P^T   P as the lanes hold it, V^T by the transposing 4-bit load from the packed rows in LDS (16 keys of a channel per lane)
+// The codes become f16 values on their way into the operands (exactly what the cache stands for), weights are two f16 terms, f32 queries
+// two terms of the row times a power of two. Keys come straight from memory into operand registers, a tile ahead; values (codes, and
+// the parameters of the keys that are seen, zeros for the others) pass through the wavefront's own LDS, without a barrier.
+template <int HD, int QT>
+__global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_kernel(const Kv4Attend a) {
+    constexpr int WPL = HD / 32;                              // words of codes of a key per lane; also groups of a row
+    constexpr int UNITS = HD <= 32 ? 2 : HD <= 64 ? 4 : HD <= 128 ? 8 : 16;   // 8-byte units of an LDS row of codes
+    constexpr int PER = 16 / UNITS;                           // rows of 128 bytes
+    constexpr int NP = WPL % 4 == 0 ? WPL / 4 : WPL <= 2 ? 1 : WPL;           // parameters of a key a lane needs for its words
+    constexpr int MT = HD / 16;                               // 16-channel tiles
+    constexpr int CODES = kKv4Tile * UNITS * 8, PARAMS = WPL * 256;           // LDS of a wavefront
+    constexpr int SUMS = kKv4Waves * HD * kKv4Rows * 4;
+    constexpr int STAGE = kKv4Waves * (CODES + PARAMS);
+    typedef typename std::conditional<QT == 1, _Float16, float>::type T;
+    __shared__ __attribute__((aligned(1024))) char smem[STAGE > SUMS ? STAGE : SUMS];
+    __shared__ float ml[kKv4Waves][2][kKv4Rows];
+    __shared__ int last_here;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, q4 = lane >> 4;
+    char *codes = smem + wave * (CODES + PARAMS), *params = codes + CODES;
+    const int shift = 31 - __builtin_clz((unsigned)a.cache.page_size), page_mask = a.cache.page_size - 1;
+    const int per_seq = a.cache.n_kv_heads * a.row_blocks;
+
+    // this workgroup's run of tiles: at least a tile for each wavefront, and long units in few enough parts that joining them is not the longer half
+    int64_t total = 0;
+    int longest = 0;
+    for (int base = 0; base < a.cache.n_seqs; base += 64) {
+        const int c = base + lane < a.cache.n_seqs ? Kv4Span(a, base + lane).count : 0;
+        total += (int64_t)__builtin_amdgcn_readlane(wave_scan(c), 63) * per_seq;
+        longest = max(longest, c);
     }
 #pragma unroll
-    for (int i = 0; i < C; i++)
-        if (lane + 64 * i < dim) y[lane + 64 * i] = (T)(l > 0.f ? acc[i] / l : l);
+    for (int d = 32; d >= 1; d >>= 1) longest = max(longest, __shfl_xor(longest, d));
+    const int64_t even = (total + gridDim.x - 1) / gridDim.x;
+    const int least = max(kKv4Waves, (int)sqrtf((float)longest * (1.f / 7.f)));
+    const int64_t share = even > least ? even : least;
+    const int64_t run0 = share * blockIdx.x, run1 = run0 + share < total ? run0 + share : total;
+
+    if (blockIdx.x == 0) {   // rows that see nothing for want of keys
+        for (int s = wave; s < a.cache.n_seqs; s += kKv4Waves)
+            if (Kv4Span(a, s).count == 0)
+                for (int r = 0; r < a.tokens; r++)
+                    for (int c = lane; c < a.n_q_heads * HD; c += 64) static_cast<T *>(a.y)[((int64_t)s * a.tokens + r) * a.y_stride + c] = (T)0.f;
+    }
+    if (run0 >= run1) return;
+
+    Kv4Unit u;
+    if (!kv4_find(a, per_seq, run0, &u)) return;
+    int64_t at = run0;
+    while (at < run1) {
+        const Kv4Span span(a, u.seq);
+        const int kvh = u.inner / a.row_blocks, block = u.inner - kvh * a.row_blocks;
+        const int from = (int)(at - u.before), to = (int)((run1 - u.before) < u.count ? run1 - u.before : u.count);   // its tiles of this run
+
+        // the lane's query row
+        const int rows = min(a.tokens * a.group - block * kKv4Rows, kKv4Rows);
+        const int row = block * kKv4Rows + n, token = min(row, a.tokens * a.group - 1) / a.group, g = row - token * a.group;
+        const bool mine = n < rows;
+        const int pos = span.length - a.tokens + token;
+        const int lane_begin = a.window > 0 ? max(pos - a.window + 1, 0) : 0, lane_end = mine ? pos + 1 : 0;
+        const int pos0 = span.length - a.tokens + block * kKv4Rows / a.group;                       // the first row's and the last's
+        const int pos1 = span.length - a.tokens + (block * kKv4Rows + rows - 1) / a.group;
+        const int any_begin = a.window > 0 ? max(pos0 - a.window + 1, 0) : 0, all_begin = a.window > 0 ? max(pos1 - a.window + 1, 0) : 0;
+
+        kvh8 qf[WPL][QT];
+        float c2 = fabsf(a.scale) * kKv4Log2e;
+        {
+            const T *q = static_cast<const T *>(a.q) + ((int64_t)u.seq * a.tokens + (mine ? token : 0)) * a.q_stride + (int64_t)(kvh * a.group + (mine ? g : 0)) * HD;
+            const float sign = a.scale < 0.f ? -1.f : 1.f;
+            float x[WPL][8], most = 0.f;
+#pragma unroll
+            for (int w = 0; w < WPL; w++) {
+                kv4_load8(q + 8 * (q4 * WPL + w), a.wide, x[w]);
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[w][j] *= sign, most = fmaxf(most, fabsf(x[w][j]));
+            }
+            if (QT == 2) {
+                most = groups_max(most);
+                // the row's largest value into [2^14, 2^15); an infinity stays where it is
+                const int up = most > 0.f && most < INFINITY ? 14 - ilogbf(most) : 0;
+                c2 = ldexpf(c2, -up);
+#pragma unroll
+                for (int w = 0; w < WPL; w++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[w][j] = ldexpf(x[w][j], up);
+            }
+#pragma unroll
+            for (int w = 0; w < WPL; w++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float v = x[w][(j & 1) * 4 + (j >> 1)];   // the order the codes unpack in: 0 4 1 5 2 6 3 7
+                    const _Float16 hi = (_Float16)v;
+                    qf[w][0][j] = hi;
+                    if (QT == 2) qf[w][QT - 1][j] = (_Float16)(v - (float)hi);
+                }
+        }
+
+        kvf4 o[MT];
+#pragma unroll
+        for (int i = 0; i < MT; i++) o[i] = kvf4{};
+        float m = -INFINITY, l = 0.f;
+
+        // a tile's loads. Blocks of 16 positions lie in one page: block n / 4 for the lane's keys, block q4 for its value row
+        struct Loads {
+            uint32_t k[4][WPL], kp[4][NP], v[WPL][4], vp[WPL];
+            bool k_there, v_there;
+        };
+        const int *table = static_cast<const int *>(a.cache.table) + (int64_t)u.seq * a.cache.table_width;
+        auto page_row = [&](int key, bool *there) -> int64_t {
+            const int entry = min(key >> shift, (int)a.cache.table_width - 1);
+            const int page = table[entry];
+            *there = page >= 0 && page < a.cache.n_pages;
+            return (((int64_t)(*there ? page : 0) * a.cache.n_kv_heads + kvh) << shift) + (key & page_mask);
+        };
+        auto load = [&](int tile, Loads &d) {
+            const int key0 = (span.first + tile) * kKv4Tile;
+            const int64_t k_row = page_row(key0 + 16 * (n >> 2) + (n & 3), &d.k_there);
+            const uint32_t *kc = reinterpret_cast<const uint32_t *>(static_cast<const char *>(a.cache.k_codes) + k_row * (HD / 2)) + q4 * WPL;
+            const uint32_t *kp = static_cast<const uint32_t *>(a.cache.k_params) + k_row * WPL;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+#pragma unroll
+                for (int w = 0; w < WPL; w++) d.k[t][w] = kc[t * 4 * (HD / 8) + w];
+#pragma unroll
+                for (int i = 0; i < NP; i++) d.kp[t][i] = kp[t * 4 * WPL + (WPL % 4 == 0 ? q4 * (WPL / 4) + i : (q4 * WPL + i) / 4)];
+            }
+            const int64_t v_row = page_row(key0 + lane, &d.v_there);
+            const uint32_t *vp = static_cast<const uint32_t *>(a.cache.v_params) + v_row * WPL;
+#pragma unroll
+            for (int i = 0; i < WPL; i++) d.vp[i] = vp[i];
+            // 16-byte chunks of 64 rows: row (64 e + lane) / WPL, found through the lane that has that row's place
+#pragma unroll
+            for (int e = 0; e < WPL; e++) {
+                const int id = 64 * e + lane, r = id / WPL, c = id - r * WPL;
+                const uint32_t lo = __shfl((uint32_t)v_row, r), hi = __shfl((uint32_t)(v_row >> 32), r);
+                const kvu4 w = *reinterpret_cast<const kvu4 *>(static_cast<const char *>(a.cache.v_codes) + (int64_t)((uint64_t)hi << 32 | lo) * (HD / 2) + c * 16);
+#pragma unroll
+                for (int j = 0; j < 4; j++) d.v[e][j] = w[j];
+            }
+        };
+
+        auto multiply = [&](int tile, Loads &d) {
+            const int key0 = (span.first + tile) * kKv4Tile;
+            const bool pages = __all(d.v_there);
+            const bool masked = key0 + kKv4Tile > pos0 + 1 || key0 < all_begin || !pages;
+            // values to LDS: codes in 8-byte units, unit x of row r at x ^ (r / PER), so that the 16 rows of a transposing load lie in different banks
+#pragma unroll
+            for (int e = 0; e < WPL; e++) {
+                const int id = 64 * e + lane, r = id / WPL, c = id - r * WPL, x = (r / PER) & (UNITS - 1);
+                const kvu4 w = x & 1 ? kvu4{d.v[e][2], d.v[e][3], d.v[e][0], d.v[e][1]} : kvu4{d.v[e][0], d.v[e][1], d.v[e][2], d.v[e][3]};
+                *reinterpret_cast<kvu4 *>(codes + r * (UNITS * 8) + (c ^ (x >> 1)) * 16) = w;
+            }
+            // parameters of eight keys of a group together, in pairs as the codes unpack: scales of keys (i, i + 4), then lowest values
+            const int key = key0 + lane;
+            bool seen = true;
+            uint32_t odd_groups = 0;   // (several tokens) groups of the lane's key whose parameters are not finite
+            if (masked) {
+                seen = key < span.length && key >= any_begin && d.v_there;
+                if (a.tokens > 1) {
+#pragma unroll
+                    for (int i = 0; i < WPL; i++)
+                        if (((((d.vp[i] & 0x7c007c00u) + 0x04000400u) & 0x80008000u) != 0) && seen) odd_groups |= 1u << i;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < WPL; i++) {
+                const uint32_t w = seen && !(odd_groups >> i & 1) ? d.vp[i] : 0u;
+                char *to = params + i * 256 + (lane >> 3) * 32 + (lane & 3) * 4 + ((lane >> 2) & 1) * 2;
+                *reinterpret_cast<uint16_t *>(to) = (uint16_t)w;
+                *reinterpret_cast<uint16_t *>(to + 16) = (uint16_t)(w >> 16);
+            }
+
+            kvf4 s[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                s[t] = kvf4{};
+#pragma unroll
+                for (int w = 0; w < WPL; w++) {
+                    const kvh2 p = __builtin_bit_cast(kvh2, d.kp[t][WPL % 4 == 0 ? w / 4 : NP == 1 ? 0 : w]);
+                    kvh2 v[4];
+                    kv4_values(d.k[t][w], kvh2{p.x, p.x}, kvh2{p.y, p.y}, v);
+                    const kvh8 kf = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
+#pragma unroll
+                    for (int e = QT - 1; e >= 0; e--) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[w][e], s[t], 0, 0, 0);
+                }
+            }
+            if (masked) {
+                const uint64_t there = __ballot(d.v_there);
+                const bool block_there = (there >> (16 * q4)) & 1;   // the lane's 16 keys are one block's
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int k = key0 + 16 * q4 + 4 * t + r;
+                        s[t][r] = block_there && k >= lane_begin && k < lane_end ? s[t][r] : -INFINITY;
+                    }
+            }
+            float mx = s[0][0];
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) mx = fmaxf(mx, s[t][r]);
+            mx = groups_max(mx) * c2;
+            if (__any(mx > m + kKv4RescaleAt)) {
+                const float grown = mx > m + kKv4RescaleAt ? mx : m, keep = grown == m ? 1.f : __builtin_amdgcn_exp2f(m - grown);   // (a row goes by its own scores)
+                m = grown, l *= keep;
+#pragma unroll
+                for (int i = 0; i < MT; i++) o[i] *= keep;
+            }
+            const float down = (m == -INFINITY ? 0.f : m) - kKv4Up;
+            kvh8 p[2][2];   // [step][term]
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int f = 0; f < 2; f++) {
+                        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * h + f][r], c2, -down));
+                        const _Float16 hi = (_Float16)w;
+                        l += w;
+                        p[h][0][2 * r + f] = hi, p[h][1][2 * r + f] = (_Float16)(w - (float)hi);
+                    }
+
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+                // (row 16 q4 + n of the codes, unit i; the result: this lane's channel 16 i + n, keys 16 q4 .. + 15)
+                const int r = 16 * q4 + n;
+                const kvi2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) kvi2 *)(codes + r * (UNITS * 8) + ((i ^ (r / PER)) & (UNITS - 1)) * 8));
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const char *pp = params + (i / 2) * 256 + (2 * q4 + h) * 32;
+                    const kvu4 sc = *reinterpret_cast<const kvu4 *>(pp), lo = *reinterpret_cast<const kvu4 *>(pp + 16);
+                    kvh2 v[4];
+                    kv4_values((uint32_t)w[h], sc, lo, v);
+                    const kvh8 vf = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p[h][1], o[i], 0, 0, 0);
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p[h][0], o[i], 0, 0, 0);
+                }
+            }
+            if (masked && a.tokens > 1) {
+                // a key with parameters that are not finite was left out above: what rows that see it get is NaN, the other tokens' rows nothing
+                for (uint64_t left = __ballot(odd_groups != 0); left; left &= left - 1) {
+                    const int b = __builtin_ctzll(left), k = key0 + b;
+                    const uint32_t odd = __builtin_amdgcn_readlane(odd_groups, b);
+                    const bool sees = k >= lane_begin && k < lane_end;
+#pragma unroll
+                    for (int i = 0; i < MT; i++)
+                        if ((odd >> (i / 2) & 1) && sees) o[i] += kvf4{NAN, NAN, NAN, NAN};
+                }
+            }
+        };
+
+        {
+            Loads now, next;
+            int tile = from + wave;
+            if (tile < to) load(tile, now);
+            for (; tile < to; tile += kKv4Waves) {
+                if (tile + kKv4Waves < to) load(tile + kKv4Waves, next);
+                multiply(tile, now);
+                now = next;
+            }
+        }
+
+        // the wavefronts' sums, joined in LDS
+        l = groups_sum(l);
+        __syncthreads();   // (the codes' LDS becomes the sums')
+        if (q4 == 0) ml[wave][0][n] = m, ml[wave][1][n] = l;
+        __syncthreads();
+        float best = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kKv4Waves; w++) best = fmaxf(best, ml[w][0][n]);
+#pragma unroll
+        for (int w = 0; w < kKv4Waves; w++) sum += ml[w][1][n] == 0.f ? 0.f : ml[w][1][n] * __builtin_amdgcn_exp2f(ml[w][0][n] - best);
+        {
+            const float keep = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - best);
+            float4 *mine_o = reinterpret_cast<float4 *>(smem) + wave * MT * 64 + lane;
+#pragma unroll
+            for (int i = 0; i < MT; i++) mine_o[i * 64] = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[i][0] * keep, o[i][1] * keep, o[i][2] * keep, o[i][3] * keep);
+        }
+        __syncthreads();
+        const bool whole = from == 0 && to == u.count;
+        auto store_row = [&](int r, int c, const float4 &v, float inv) {
+            const int rr = block * kKv4Rows + r, tk = rr / a.group;
+            T *y = static_cast<T *>(a.y) + ((int64_t)u.seq * a.tokens + tk) * a.y_stride + (int64_t)(kvh * a.group + rr - tk * a.group) * HD + c;
+            typedef T T4 __attribute__((ext_vector_type(4)));
+            const T4 out = {(T)(v.x * inv), (T)(v.y * inv), (T)(v.z * inv), (T)(v.w * inv)};
+            if (a.wide) {
+                *reinterpret_cast<T4 *>(y) = out;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) y[j] = out[j];
+            }
+        };
+        // workgroup w's part of a unit that began in an earlier run (0), or begins here and goes on (1): [row][channel] sums, then maxima and sums
+        auto part_of = [&](int64_t w, int which) { return a.parts + (w * 2 + which) * (int64_t)(kKv4Rows * (HD + 2)); };
+        float *part = part_of(blockIdx.x, from == 0 ? 1 : 0);
+        for (int i = wave; i < MT; i += kKv4Waves) {   // thread (i, lane): channels 16 i + 4 q4 .. + 3 of row n
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kKv4Waves; w++) {
+                const float4 x = reinterpret_cast<const float4 *>(smem)[(w * MT + i) * 64 + lane];
+                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+            }
+            if (!mine) continue;
+            if (whole) {
+                store_row(n, 16 * i + 4 * q4, v, sum == 0.f ? 0.f : 1.f / sum);
+            } else {
+                float *to_part = part + n * HD + 16 * i + 4 * q4;
+                const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) __hip_atomic_store(to_part + j, x[j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+        if (!whole) {
+            if (wave == 0 && q4 == 0 && mine) {
+                __hip_atomic_store(part + kKv4Rows * HD + 2 * n, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(part + kKv4Rows * HD + 2 * n + 1, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's stores are where everyone sees them
+            __syncthreads();
+            const int64_t w0 = u.before / share, w1 = (u.before + u.count - 1) / share;   // the workgroups that have parts of it
+            if (tid == 0) {
+                const uint32_t others = __hip_atomic_fetch_add(a.arrived + w0, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+                last_here = others == (uint32_t)(w1 - w0);
+                if (last_here) __hip_atomic_store(a.arrived + w0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next call
+            }
+            __syncthreads();
+            if (last_here) {
+                for (int i = tid; i < rows * (HD / 4); i += 64 * kKv4Waves) {
+                    const int r = i / (HD / 4), c = (i - r * (HD / 4)) * 4;
+                    auto read = [&](const float *x) { return __hip_atomic_load(x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+                    float top = -INFINITY;
+                    for (int64_t w = w0; w <= w1; w++) top = fmaxf(top, read(part_of(w, w == w0) + kKv4Rows * HD + 2 * r));
+                    float all = 0.f;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int64_t w = w0; w <= w1; w++) {
+                        const float *x = part_of(w, w == w0);
+                        const float pm = read(x + kKv4Rows * HD + 2 * r), ps = read(x + kKv4Rows * HD + 2 * r + 1);
+                        const float x0 = read(x + r * HD + c), x1 = read(x + r * HD + c + 1), x2 = read(x + r * HD + c + 2), x3 = read(x + r * HD + c + 3);
+                        if (ps == 0.f) continue;   // nothing the row sees
+                        const float keep = __builtin_amdgcn_exp2f(pm - top);
+                        all += ps * keep, v.x += x0 * keep, v.y += x1 * keep, v.z += x2 * keep, v.w += x3 * keep;
+                    }
+                    store_row(r, c, v, all == 0.f ? 0.f : 1.f / all);
+                }
+            }
+        }
+        __syncthreads();   // LDS is free for the next unit
+
+        at = u.before + u.count;
+        if (at < run1 && ++u.inner < per_seq) {
+            u.before = at;
+        } else if (at < run1 && !kv4_find(a, per_seq, at, &u)) {
+            break;
+        }
+    }
+}
+
+template <int HD>
+void kv4_launch(hipc_ctx *ctx, const Kv4Attend &a, int dtype, unsigned grid) {
+    if (dtype == HIPC_F16) hipLaunchKernelGGL((kv4_attend_kernel<HD, 1>), grid, 64 * kKv4Waves, 0, ctx->stream, a);
+    else hipLaunchKernelGGL((kv4_attend_kernel<HD, 2>), grid, 64 * kKv4Waves, 0, ctx->stream, a);
 }
 
 }  // namespace
@@ -94,10 +507,32 @@ int hipc_kv4_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_at
         HIPC_REQUIRE(ctx, q_stride >= width && y_stride >= width && q_stride <= (int64_t)1 << 40 && y_stride <= (int64_t)1 << 40,
                      "%s: rows %lld and %lld apart, of %lld values", who, (long long)q_stride, (long long)y_stride, (long long)width);
         a.cache = *cache, a.q = Q, a.y = Y, a.q_stride = q_stride, a.y_stride = y_stride;
-        a.tokens = (int)tokens, a.n_q_heads = heads->n_q_heads, a.window = heads->window;
-        const dim3 grid((unsigned)(cache->n_seqs * tokens), heads->n_q_heads);
-        if (dtype == HIPC_F16) hipLaunchKernelGGL((kv4_attend_kernel<_Float16>), grid, 64, 0, ctx->stream, a);
-        else hipLaunchKernelGGL((kv4_attend_kernel<float>), grid, 64, 0, ctx->stream, a);
+        a.tokens = (int)tokens, a.n_q_heads = heads->n_q_heads, a.group = (int)group, a.window = heads->window;
+        a.row_blocks = (int)ceil_div(tokens * group, kKv4Rows);
+        const int64_t unit = dtype == HIPC_F16 ? 8 : 4;
+        a.wide = aligned(Q, 16) && aligned(Y, 16) && q_stride % unit == 0 && y_stride % unit == 0;
+        // two workgroups a CU; what they exchange, and the words they count in, in a scratch slot of this operator's own: the words are zero
+        // between calls, so a new block is cleared once
+        const unsigned grid = 2 * ctx->cu_count;
+        const size_t count_bytes = (grid * 4 + 255) & ~(size_t)255;
+        const void *before = ctx->scratch[kScratchKv4].ptr;
+        void *block = nullptr;
+        if (int rc = scratch_get(ctx, kScratchKv4, count_bytes + (size_t)grid * 2 * kKv4Rows * (kKv4MaxHead + 2) * 4, &block)) return rc;
+        a.arrived = static_cast<uint32_t *>(block), a.parts = reinterpret_cast<float *>(static_cast<char *>(block) + count_bytes);
+        if (block != before) {
+            hipLaunchKernelGGL((fill_words), 1, 256, 0, ctx->stream, a.arrived, count_bytes / 4, 0u);
+            HIPC_LAUNCHED(ctx);
+        }
+        switch (heads->head_dim / 32) {
+            case 1: kv4_launch<32>(ctx, a, dtype, grid); break;
+            case 2: kv4_launch<64>(ctx, a, dtype, grid); break;
+            case 3: kv4_launch<96>(ctx, a, dtype, grid); break;
+            case 4: kv4_launch<128>(ctx, a, dtype, grid); break;
+            case 5: kv4_launch<160>(ctx, a, dtype, grid); break;
+            case 6: kv4_launch<192>(ctx, a, dtype, grid); break;
+            case 7: kv4_launch<224>(ctx, a, dtype, grid); break;
+            default: kv4_launch<256>(ctx, a, dtype, grid); break;
+        }
         HIPC_LAUNCHED(ctx);
         return HIPC_OK;
     });

@@ -32,19 +32,6 @@ __device__ __forceinline__ Kv4Unit kv4_unit(const Kv4Rows &a, int u) {
     return {h, (r - h * per_head) * 8, value};
 }
 
-template <typename T>
-__device__ __forceinline__ void kv4_load8(const T *p, bool wide, float (&x)[8]) {
-    typedef T T8 __attribute__((ext_vector_type(8)));
-    if (wide) {
-        const T8 v = *reinterpret_cast<const T8 *>(p);
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = (float)v[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = (float)p[i];
-    }
-}
-
 __device__ __forceinline__ float quad_min(float v) {
     v = fminf(v, lean_dpp<0xB1>(v));
     return fminf(v, lean_dpp<0x4E>(v));

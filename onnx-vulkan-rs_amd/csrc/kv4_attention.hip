@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
             __syncthreads();
             const int64_t w0 = u.before / share, w1 = (u.before + u.count - 1) / share;   // the workgroups that have parts of it
             if (tid == 0) {
-                const uint32_t others = __hip_atomic_fetch_add(a.arrived + w0, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+                const uint32_t others = __hip_atomic_fetch_add(a.arrived + w0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 last_here = others == (uint32_t)(w1 - w0);
                 if (last_here) __hip_atomic_store(a.arrived + w0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next call
             }

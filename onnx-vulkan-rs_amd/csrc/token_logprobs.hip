@@ -2,8 +2,10 @@
 #include <hip/hip_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "internal.h"
+#include "lanes.h"
 
 namespace hipc {
 
@@ -11,8 +13,9 @@ namespace {
 
 constexpr int kScratchLogprobs = 7;   // scratch slot of this operator alone
 constexpr int kLogWaves = 4;
-constexpr int kLogChunk = 2048;       // logits a wavefront holds at a time: 32 a lane
-constexpr int kLogWorkgroups = 2048;  // at most that many share rows
+constexpr int kLogChunk = 1024;       // logits a wavefront holds at a time: 16 a lane
+constexpr int kLogWorkgroups = 1024;  // at most that many share rows
+constexpr int kLogParts = 64;         // ... a row
 constexpr int kLogBuffer = 256;       // candidates a wavefront ranks at a time
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -34,7 +37,7 @@ struct LogSum {
 struct LogPart {
     LogSum sum;
     uint32_t pad;
-    uint64_t best[HIPC_TOP_MAX];   // keys, largest first; 0 where there are fewer
+    uint64_t best[kLogWaves][HIPC_TOP_MAX];   // of each wavefront: keys, largest first; 0 where there are fewer
 };
 
 // A logit and its place as one whole number that orders as the alternatives do: by value, the lower id first among equals.
@@ -61,83 +64,172 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
     return v;
 }
 
-// A wavefront's `top` largest keys so far, the j-th in lane j (0: none), and N more of each lane to take in.
-// Those that can count are written side by side into the wavefront's LDS, with the list, and ranked by counting the larger ones. Where
-// too many pass the list's last -- a list that is not full yet, or ascending logits -- the top-th largest of the lanes' own largest is the bar:
-// at least `top` keys are at or above it. If equal values still leave too many, one key after the other is picked.
-template <int N, typename Key>
-__device__ __forceinline__ void log_take(uint64_t &list, int top, uint64_t *buffer, Key key) {
+// What a wavefront knows of a row's largest logits: keys in its LDS, `count` of them, and the least value that counts. Keys that pass are
+// written side by side; they are ranked, and all but the `top` largest dropped, when there is no room left and at the end. The first bar is the
+// top-th largest of the lanes' largest logits: at least `top` reach it, and few more. All of this is short loops with little LDS latency
+// in a row: it runs a few times in a launch, one wavefront's time after the other's (a wavefront's first chunk 1 us, ranking 0.5 us).
+struct LogBuffer {
+    float stage[kLogChunk];                          // a chunk's logits: the lane's i-th at 64 i + lane
+    uint64_t key[kLogBuffer], ranked[HIPC_TOP_MAX];
+};
+
+__device__ __forceinline__ uint32_t wave_least(uint32_t v) {
+    auto dpp = [](uint32_t x, auto ctrl) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf, 0xf, true); };
+    v = min(v, dpp(v, std::integral_constant<int, 0xB1>()));
+    v = min(v, dpp(v, std::integral_constant<int, 0x4E>()));
+    v = min(v, dpp(v, std::integral_constant<int, 0x124>()));
+    v = min(v, dpp(v, std::integral_constant<int, 0x128>()));
+    auto lane = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+    return min(min(lane(0), lane(16)), min(lane(32), lane(48)));
+}
+// the largest whole number that at least `top` of the lanes' are at or above: the least of those that fewer than `top` are above
+__device__ __forceinline__ uint32_t log_reach(uint32_t v, int top) {
+    int above = 0;
+#pragma unroll 16
+    for (int j = 0; j < 64; j++) above += (uint32_t)__builtin_amdgcn_readlane((int)v, j) > v;
+    return wave_least(above < top ? v : 0xffffffffu);
+}
+__device__ __forceinline__ int log_before(uint64_t lanes) {   // those in front of this one
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
+}
+// the `top` largest of `count` keys of the buffer, the j-th in lane j (one wavefront's LDS accesses are done in their order)
+__device__ __forceinline__ uint64_t log_rank(int top, LogBuffer &buffer, int count) {
     const int lane = threadIdx.x & 63;
-    uint64_t bar = lane_key(list, top - 1);   // (keys at or below it cannot count)
-    int count = 0;
-    for (int round = 0;; round++) {
-        count = 0;
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const uint64_t k = key(i);
-            const uint64_t in = __ballot(k > bar);
-            const int at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
-            if (k > bar && at < kLogBuffer - HIPC_TOP_MAX) buffer[at] = k;
-            count += __popcll(in);
-        }
-        if (count <= kLogBuffer - HIPC_TOP_MAX) break;
-        if (round == 1) {
-            count = -1;
-            break;
-        }
-        // the value of the top-th largest of the lanes' largest keys, bit by bit
-        uint64_t own = 0;
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const uint64_t k = key(i);
-            own = k > own ? k : own;
-        }
-        const uint32_t v = (uint32_t)(own >> 32);
-        uint32_t reach = 0;
-        for (int b = 31; b >= 0; b--) {
-            const uint32_t next = reach | 1u << b;
-            if (__popcll(__ballot(v >= next)) >= top) reach = next;
-        }
-        const uint64_t higher = reach ? ((uint64_t)reach << 32) - 1 : 0;
-        bar = higher > bar ? higher : bar;
-    }
-    if (count == 0) return;
-    if (count < 0) {
-        uint64_t last = ~(uint64_t)0, mine = 0;
-        for (int j = 0; j < top; j++) {
-            uint64_t own = list < last ? list : 0;
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const uint64_t k = key(i);
-                own = k < last && k > own ? k : own;
-            }
-            last = wave_max(own);
-            if (lane == j) mine = last;
-            if (last == 0) break;
-        }
-        list = mine;
-        return;
-    }
-    if (lane < top) buffer[count + lane] = list;
-    const int all = count + top;
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    uint64_t sorted = 0;
-    for (int base = 0; base < all; base += 64) {
-        const bool have = base + lane < all;
-        const uint64_t k = have ? buffer[base + lane] : 0;
+    constexpr int STEP = 16;
+    if (lane < STEP) buffer.key[count + lane] = 0;
+    if (lane < top) buffer.ranked[lane] = 0;
+#pragma unroll 1
+    for (int base = 0; base < count; base += 64) {
+        const uint64_t k = base + lane < count ? buffer.key[base + lane] : 0;
         int rank = 0;
-        for (int j = 0; j < all; j++) rank += buffer[j] > k;
-        // the lane of that rank takes it (empty places of the list, key 0, are taken by nobody)
-        for (uint64_t left = __ballot(k != 0 && rank < top); left; left &= left - 1) {
-            const int b = __builtin_ctzll(left);
-            const uint64_t moved = lane_key(k, b);
-            if (lane == __builtin_amdgcn_readlane(rank, b)) sorted = moved;
-        }
+#pragma unroll 1
+        for (int j = 0; j < count; j += STEP)
+#pragma unroll
+            for (int e = 0; e < STEP; e++) rank += buffer.key[j + e] > k;
+        if (k != 0 && rank < top) buffer.ranked[rank] = k;
     }
-    list = sorted;
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (read before the next call writes)
+    return lane < top ? buffer.ranked[lane] : 0;
+}
+constexpr int kLogRoom = kLogBuffer - 16;
+
+struct LogBest {
+    int count = 0;
+    uint32_t least = 0;   // as in log_key; 0: not known yet
+    float bar = -INFINITY;   // the value of `least`
+
+    __device__ __forceinline__ void raise(uint32_t to) {
+        if (to > least) least = to, bar = key_value((uint64_t)to << 32);
+    }
+    __device__ __forceinline__ void rank(int top, LogBuffer &buffer) {
+        keep(top, buffer, log_rank(top, buffer, count));
+    }
+    __device__ __forceinline__ void keep(int top, LogBuffer &buffer, uint64_t list) {
+        const int lane = threadIdx.x & 63;
+        if (lane < top) buffer.key[lane] = list;
+        count = __popcll(__ballot(list != 0));
+        const uint64_t lowest = lane_key(list, top - 1);
+        if (lowest) raise((uint32_t)(lowest >> 32) + 1);   // (later logits have higher ids: an equal one does not count)
+    }
+    // A chunk's logits x, of which the lane's largest is `largest`; id(i) is the place of the lane's i-th, below 0 behind the row's ends.
+    template <int N, typename Id>
+    __device__ __forceinline__ void scan(int top, LogBuffer &buffer, float largest, const float (&x)[N], Id id) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < N; i++) buffer.stage[64 * i + lane] = x[i];
+        bool tight = false;   // the bar is this chunk's own
+        if (least == 0) {
+            raise(log_reach((uint32_t)(log_key(largest, 0) >> 32), top));
+            tight = true;
+        }
+        for (;;) {
+            uint32_t pass = 0;
+#pragma unroll
+            for (int i = 0; i < N; i++) pass |= x[i] >= bar ? 1u << i : 0u;
+            int now = count;
+#pragma unroll 1
+            while (__any(pass != 0) && now <= kLogRoom) {
+                const int i = pass ? __builtin_ctz(pass) : 0, at = id(i);
+                const bool counts = pass != 0 && at >= 0;
+                pass &= pass - 1;
+                const uint64_t in = __ballot(counts);
+                const int place = now + log_before(in);
+                if (counts && place < kLogRoom) buffer.key[place] = log_key(buffer.stage[64 * i + lane], at);
+                now += __popcll(in);
+            }
+            if (now <= kLogRoom) {
+                count = now;
+                break;
+            }
+            // no room: what was there is ranked, then the chunk's own bar is taken, and at last (equal values) one key after the other
+            if (count > top) {
+                rank(top, buffer);
+            } else if (!tight) {
+                raise(log_reach((uint32_t)(log_key(largest, 0) >> 32), top));
+                tight = true;
+            } else {
+                uint64_t last = ~(uint64_t)0, mine = 0;
+                const uint64_t had = lane < count ? buffer.key[lane] : 0;
+#pragma unroll 1
+                for (int j = 0; j < top; j++) {
+                    uint64_t own = had < last ? had : 0;
+#pragma unroll 1
+                    for (int i = 0; i < N; i++) {
+                        const float v = buffer.stage[64 * i + lane];
+                        const int at = id(i);
+                        const uint64_t k = v == v && at >= 0 ? log_key(v, at) : 0;
+                        own = k < last && k > own ? k : own;
+                    }
+                    last = wave_max(own);
+                    if (lane == j) mine = last;
+                    if (last == 0) break;
+                }
+                keep(top, buffer, mine);
+                break;
+            }
+        }
+        if (tight) raise(least + 1);   // (for the chunks behind)
+        if (count >= 2 * top) rank(top, buffer);
+    }
+};
+
+// what another workgroup stored is read from where it stored it
+__device__ __forceinline__ uint64_t key_of_all(const uint64_t *at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ LogSum sum_of_all(const LogSum *at) {
+    auto get = [](const float *v) { return __hip_atomic_load(v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    return {get(&at->m), get(&at->l), get(&at->w)};
 }
 
+// The `top` largest keys of up to 64 sorted lists (0: none behind a list's last), one per lane, the lane's at `mine` (any address where `have` is
+// false). The top-th largest of the lists' first keys is a bar that at least `top` keys reach.
+__device__ __forceinline__ uint64_t log_merge(int top, LogBuffer &buffer, const uint64_t *mine, bool have) {
+    uint64_t early[4];   // most lists count with fewer keys than these; they are on their way together
+#pragma unroll
+    for (int r = 0; r < 4; r++) early[r] = key_of_all(mine + min(r, top - 1));
+    const uint32_t reach = log_reach(have ? (uint32_t)(early[0] >> 32) : 0u, top);
+    const uint64_t bar = reach ? ((uint64_t)reach << 32) - 1 : 0;
+    int count = 0;
+#pragma unroll 1
+    for (int r = 0; r < top; r++) {
+        const uint64_t v = r == 0 ? early[0] : r == 1 ? early[1] : r == 2 ? early[2] : r == 3 ? early[3] : key_of_all(mine + r);
+        const uint64_t k = have ? v : 0, in = __ballot(k > bar);
+        if (!in) break;
+        if (count + __popcll(in) > kLogRoom) {   // (equal values)
+            const uint64_t list = log_rank(top, buffer, count);
+            if ((int)(threadIdx.x & 63) < top) buffer.key[threadIdx.x & 63] = list;
+            count = __popcll(__ballot(list != 0));
+        }
+        if (k > bar) buffer.key[count + log_before(in)] = k;
+        count += __popcll(in);
+    }
+    return log_rank(top, buffer, count);
+}
+
+// the lanes' sums as one: each in units of the largest value of all
+__device__ __forceinline__ LogSum log_wave(const LogSum &s) {
+    const float m = lean_wave_max(s.m);
+    const float d = s.m == m ? 0.f : (s.m - m) * kLog2e, f = s.l == 0.f ? 0.f : __builtin_amdgcn_exp2f(d);
+    return {m, lean_wave_sum(s.l == 0.f ? 0.f : s.l * f), lean_wave_sum(s.l == 0.f || f == 0.f ? 0.f : f * __builtin_fmaf(s.l, d, s.w))};
+}
 __device__ __forceinline__ LogSum log_join(const LogSum &a, const LogSum &b) {
     const float m = fmaxf(a.m, b.m);
     // a side without a value above -inf adds nothing (its difference to m may be no number)
@@ -165,21 +257,21 @@ __device__ void log_finish(const LogprobArgs &a, int64_t row, const LogSum &s, u
     }
 }
 
-// A row is read once, by a.parts workgroups; a wavefront streams 2048 logits at a time, the next ones on their way meanwhile, with a running
+// A row is read once, by a.parts workgroups; a wavefront streams 1024 logits at a time, the next ones on their way meanwhile, with a running
 // maximum and sums per lane and without a barrier. The alternatives cost a comparison per logit; only where one passes the list's last is there
 // more to do, which after the first few thousand logits is rare.
 template <typename T>
-__global__ void __launch_bounds__(64 * kLogWaves) logprob_kernel(const LogprobArgs a) {
+__global__ void __launch_bounds__(64 * kLogWaves, 4) logprob_kernel(const LogprobArgs a) {
     constexpr int VEC = 16 / sizeof(T), LOADS = kLogChunk / 64 / VEC;
     typedef T TV __attribute__((ext_vector_type(VEC)));
-    __shared__ uint64_t buffers[kLogWaves][kLogBuffer];
+    __shared__ LogBuffer buffers[kLogWaves];
     __shared__ LogSum sums[kLogWaves];
     __shared__ uint64_t lists[kLogWaves][HIPC_TOP_MAX];
     __shared__ int last_here;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t row = blockIdx.x / a.parts;
     const int part = (int)(blockIdx.x - row * a.parts);
-    uint64_t *buffer = buffers[wave];
+    LogBuffer &buffer = buffers[wave];
 
     // the row in pieces of 16 aligned bytes: the first and the last may hold less of it
     const T *x = static_cast<const T *>(a.x) + row * a.row_stride;
@@ -189,26 +281,33 @@ __global__ void __launch_bounds__(64 * kLogWaves) logprob_kernel(const LogprobAr
     const int per = (chunks + a.parts * kLogWaves - 1) / (a.parts * kLogWaves);   // of a wavefront, one behind the other
     const int c0 = (part * kLogWaves + wave) * per, c1 = min(c0 + per, chunks);
 
-    TV now[LOADS], next[LOADS];
+    float m = -INFINITY, l = 0.f, w = 0.f;
+    LogBest best;
+    TV now[LOADS], next[LOADS] = {};
+    // (below 2^31: the vocabulary is at most 2^30)
+    auto first_of = [&](int chunk) { return (chunk * LOADS * 64 + lane) * VEC - head; };
     auto load = [&](int chunk, TV (&v)[LOADS]) {
+        const int first = first_of(chunk);
+        if (chunk != 0 && chunk != chunks - 1) {
+#pragma unroll
+            for (int e = 0; e < LOADS; e++) v[e] = __builtin_nontemporal_load(reinterpret_cast<const TV *>(x + first + e * 64 * VEC));
+            return;
+        }
 #pragma unroll
         for (int e = 0; e < LOADS; e++) {
-            const int64_t at = ((int64_t)(chunk * LOADS + e) * 64 + lane) * VEC - head;   // of the row
+            const int at = first + e * 64 * VEC;
             if (at >= 0 && at + VEC <= a.vocab) {
-                v[e] = __builtin_nontemporal_load(reinterpret_cast<const TV *>(x + at));
+                v[e] = *reinterpret_cast<const TV *>(x + at);
             } else {
 #pragma unroll
                 for (int j = 0; j < VEC; j++) v[e][j] = at + j >= 0 && at + j < a.vocab ? x[at + j] : (T)-INFINITY;
             }
         }
     };
-    float m = -INFINITY, l = 0.f, w = 0.f;
-    uint64_t list = 0;
-    float bar = -INFINITY;
-    bool full = false;
     if (c0 < c1) load(c0, now);
     for (int c = c0; c < c1; c++) {
         if (c + 1 < c1) load(c + 1, next);
+        const int first = first_of(c);
         float most = -INFINITY;
 #pragma unroll
         for (int e = 0; e < LOADS; e++)
@@ -230,15 +329,14 @@ __global__ void __launch_bounds__(64 * kLogWaves) logprob_kernel(const LogprobAr
                 l2 += y, w2 = __builtin_fmaf(y, fmaxf(t, -200.f), w2);
             }
         l += l2, w += w2;
-        if (a.top > 0 && (__any(most > bar) || !full)) {
-            log_take<LOADS * VEC>(list, a.top, buffer, [&](int i) -> uint64_t {
-                const float v = (float)now[i / VEC][i % VEC];
-                const int64_t id = ((int64_t)(c * LOADS + i / VEC) * 64 + lane) * VEC - head + i % VEC;
-                return v == v && id >= 0 && id < a.vocab ? log_key(v, (int)id) : 0;
+        if (a.top > 0 && __any(most >= best.bar)) {
+            float values[LOADS * VEC];
+#pragma unroll
+            for (int i = 0; i < LOADS * VEC; i++) values[i] = (float)now[i / VEC][i % VEC];
+            best.scan(a.top, buffer, most, values, [&](int i) -> int {
+                const int at = first + i / VEC * 64 * VEC + i % VEC;
+                return at >= 0 && at < a.vocab ? at : -1;
             });
-            const uint64_t lowest = lane_key(list, a.top - 1);
-            full = lowest != 0;
-            if (full) bar = key_value(lowest);   // (later logits have higher ids: an equal one does not count)
         }
 #pragma unroll
         for (int e = 0; e < LOADS; e++) now[e] = next[e];
@@ -246,61 +344,53 @@ __global__ void __launch_bounds__(64 * kLogWaves) logprob_kernel(const LogprobAr
 
     // lanes, then wavefronts
     LogSum s{m, l, w};
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) s = log_join(s, LogSum{__shfl_xor(s.m, d), __shfl_xor(s.l, d), __shfl_xor(s.w, d)});
-    if (lane == 0) sums[wave] = s;
-    if (lane < HIPC_TOP_MAX) lists[wave][lane] = list;
-    __syncthreads();
-    if (wave == 0) {
-        for (int v = 1; v < kLogWaves; v++) s = log_join(s, sums[v]);
-        if (a.top > 0) {
-            uint64_t more[(kLogWaves - 1) * HIPC_TOP_MAX / 64 + 1] = {};
-            constexpr int N = sizeof more / sizeof more[0];
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int at = i * 64 + lane;
-                if (at < (kLogWaves - 1) * HIPC_TOP_MAX) more[i] = lists[1 + at / HIPC_TOP_MAX][at % HIPC_TOP_MAX];
-            }
-            log_take<N>(list, a.top, buffer, [&](int i) { return more[i]; });
-        }
-    }
-    if (a.parts == 1) {
-        if (wave == 0) log_finish<T>(a, row, s, list);
-        return;
-    }
-    // several workgroups: the one that comes last joins what they found
+    s = log_wave(s);
     LogPart *mine = a.part + row * a.parts;
-    if (wave == 0) {
-        auto put = [](void *to, uint32_t v) { __hip_atomic_store(static_cast<uint32_t *>(to), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-        if (lane == 0) put(&mine[part].sum.m, __float_as_uint(s.m)), put(&mine[part].sum.l, __float_as_uint(s.l)), put(&mine[part].sum.w, __float_as_uint(s.w));
-        if (lane < a.top) __hip_atomic_store(&mine[part].best[lane], list, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the stores are where everyone sees them
-        if (lane == 0) {
-            const uint32_t before = __hip_atomic_fetch_add(a.arrived + row, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-            last_here = before == (uint32_t)a.parts - 1;
-            if (last_here) __hip_atomic_store(a.arrived + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next call
-        }
+    const bool alone = a.parts == 1;
+    uint64_t list = a.top > 0 && best.count > 0 ? log_rank(a.top, buffer, best.count) : 0;
+    if (lane == 0) sums[wave] = s;
+    if (lane < a.top) {
+        if (alone) lists[wave][lane] = list;
+        else __hip_atomic_store(&mine[part].best[wave][lane], list, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the stores are where everyone sees them
     __syncthreads();
-    if (!last_here || wave != 0) return;
-    auto get = [](const void *at) { return __hip_atomic_load(static_cast<const uint32_t *>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-    s = {-INFINITY, 0.f, 0.f};
-    for (int q = lane; q < a.parts; q += 64)
-        s = log_join(s, LogSum{__uint_as_float(get(&mine[q].sum.m)), __uint_as_float(get(&mine[q].sum.l)), __uint_as_float(get(&mine[q].sum.w))});
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) s = log_join(s, LogSum{__shfl_xor(s.m, d), __shfl_xor(s.l, d), __shfl_xor(s.w, d)});
-    list = 0;
-    if (a.top > 0) {
-        constexpr int N = 8;
-        for (int from = 0; from < a.parts * a.top; from += 64 * N) {
-            uint64_t more[N];
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int at = from + i * 64 + lane, q = at / a.top;
-                more[i] = at < a.parts * a.top ? __hip_atomic_load(&mine[q].best[at - q * a.top], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+    if (wave != 0 && (alone || a.top == 0)) return;
+    if (!alone) {
+        // several workgroups: the one that comes last joins what they found
+        if (wave == 0) {
+#pragma unroll 1
+            for (int v = 1; v < kLogWaves; v++) s = log_join(s, sums[v]);
+            if (lane == 0) {
+                auto put = [](float *to, float v) { __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+                put(&mine[part].sum.m, s.m), put(&mine[part].sum.l, s.l), put(&mine[part].sum.w, s.w);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                last_here = __hip_atomic_fetch_add(a.arrived + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)a.parts - 1;
             }
-            log_take<N>(list, a.top, buffer, [&](int i) { return more[i]; });
         }
+        if (a.top > 0) __syncthreads();
+        if (!last_here) return;
+        if (tid == 0) __hip_atomic_store(a.arrived + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next call
+        static_assert(kLogParts * kLogWaves <= 64 * kLogWaves, "a list per thread");
+        if (a.top > 0) {
+            const bool have = tid < a.parts * kLogWaves;
+            list = log_merge(a.top, buffer, &mine[have ? tid / kLogWaves : 0].best[tid % kLogWaves][0], have);
+            if (lane < a.top) lists[wave][lane] = list;
+        }
+        s = {-INFINITY, 0.f, 0.f};
+        if (wave == 0) {
+            for (int q = lane; q < a.parts; q += 64) s = log_join(s, sum_of_all(&mine[q].sum));
+            s = log_wave(s);
+        }
+        if (a.top > 0) __syncthreads();
+        if (wave != 0) return;
+    } else {
+#pragma unroll 1
+        for (int v = 1; v < kLogWaves; v++) s = log_join(s, sums[v]);
+    }
+    if (a.top > 0) {
+        for (int i = lane; i < kLogWaves * a.top; i += 64) buffer.key[i] = lists[i / a.top][i % a.top];
+        list = log_rank(a.top, buffer, kLogWaves * a.top);
     }
     log_finish<T>(a, row, s, list);
 }
@@ -328,10 +418,10 @@ int hipc_token_logprobs(hipc_ctx *ctx, int dtype, const void *logits, int64_t ro
         HIPC_REQUIRE(ctx, aligned(tokens, 4) && aligned(logprob, 4) && aligned(entropy, 4) && aligned(top_ids, 4) && aligned(top_logprobs, 4), "%s: a pointer off its elements", who);
         LogprobArgs a{logits, row_stride, (int)vocab, top, 1, static_cast<const int *>(tokens), static_cast<float *>(logprob), static_cast<float *>(entropy),
                       static_cast<float *>(top_logprobs), static_cast<int *>(top_ids), nullptr, nullptr};
-        // few rows are shared by several workgroups, each wavefront of which has 2048 logits at least
+        // few rows are shared by several workgroups, each wavefront of which has 1024 logits at least
         const size_t count_bytes = kLogWorkgroups * sizeof(uint32_t), bytes = count_bytes + kLogWorkgroups * sizeof(LogPart);
         if (scratch_fits(ctx, kScratchLogprobs, bytes))
-            a.parts = (int)std::max<int64_t>(1, std::min<int64_t>(kLogWorkgroups / rows, ceil_div(vocab, kLogWaves * kLogChunk)));
+            a.parts = (int)std::max<int64_t>(1, std::min<int64_t>({kLogWorkgroups / rows, ceil_div(vocab, kLogWaves * kLogChunk), kLogParts}));
         if (a.parts > 1) {
             const void *before = ctx->scratch[kScratchLogprobs].ptr;
             void *block = nullptr;

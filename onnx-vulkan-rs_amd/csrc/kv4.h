@@ -53,28 +53,30 @@ __device__ __forceinline__ int kv4_length(const hipc_kv4_cache &c, int s) {
 
 // Eight codes as f16 values, each lowest + code * scale rounded once: the code's bits under the exponent of 1024 (or, four
 // bits further up, of 64) are that number plus the code; the subtraction is exact, and so is the product inside the fma.
-__device__ __forceinline__ void kv4_values(uint32_t w, kvh2 scale, kvh2 lowest, kvh2 (&v)[4]) {
-    auto part = [](uint32_t bits, uint32_t magic) { return __builtin_bit_cast(kvh2, bits | magic); };
-    const kvh2 k1024 = {(_Float16)1024.f, (_Float16)1024.f}, k64 = {(_Float16)64.f, (_Float16)64.f};
-    // nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7
-    v[0] = __builtin_elementwise_fma(part(w & 0x000f000fu, 0x64006400u) - k1024, scale, lowest);
-    v[1] = __builtin_elementwise_fma(part(w & 0x00f000f0u, 0x54005400u) - k64, scale, lowest);
-    w >>= 8;
-    v[2] = __builtin_elementwise_fma(part(w & 0x000f000fu, 0x64006400u) - k1024, scale, lowest);
-    v[3] = __builtin_elementwise_fma(part(w & 0x00f000f0u, 0x54005400u) - k64, scale, lowest);
-}
-
-// the same where every pair of values has a scale and a lowest value of its own (four pairs each, as bits)
-typedef uint32_t kv4_pairs __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ void kv4_values(uint32_t w, kv4_pairs scale, kv4_pairs lowest, kvh2 (&v)[4]) {
-    auto part = [](uint32_t bits) { return __builtin_bit_cast(kvh2, bits); };
-    const kvh2 k1024 = {(_Float16)1024.f, (_Float16)1024.f}, k64 = {(_Float16)64.f, (_Float16)64.f};
-    v[0] = __builtin_elementwise_fma(part((w & 0x000f000fu) | 0x64006400u) - k1024, part(scale[0]), part(lowest[0]));
-    v[1] = __builtin_elementwise_fma(part((w & 0x00f000f0u) | 0x54005400u) - k64, part(scale[1]), part(lowest[1]));
-    w >>= 8;
-    v[2] = __builtin_elementwise_fma(part((w & 0x000f000fu) | 0x64006400u) - k1024, part(scale[2]), part(lowest[2]));
-    v[3] = __builtin_elementwise_fma(part((w & 0x00f000f0u) | 0x54005400u) - k64, part(scale[3]), part(lowest[3]));
-}
+// (A mask in a scalar register and the exponents in vector registers: one instruction takes the bits out and puts them in.)
+struct Kv4Unpack {
+    uint32_t low = 0x000f000fu, high = 0x00f000f0u, e1024 = 0x64006400u, e64 = 0x54005400u;
+    __device__ __forceinline__ Kv4Unpack() {
+        HIPC_PIN_SGPR(low);
+        HIPC_PIN_SGPR(high);
+        HIPC_PIN_VGPR(e1024);
+        HIPC_PIN_VGPR(e64);
+    }
+    // nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7; a pair's scales and lowest values by scale(i), lowest(i)
+    template <typename Scale, typename Lowest>
+    __device__ __forceinline__ void operator()(uint32_t w, Scale scale, Lowest lowest, kvh2 (&v)[4]) const {
+        auto part = [](uint32_t bits) { return __builtin_bit_cast(kvh2, bits); };
+        const kvh2 k1024 = {(_Float16)1024.f, (_Float16)1024.f}, k64 = {(_Float16)64.f, (_Float16)64.f};
+        v[0] = __builtin_elementwise_fma(part((w & low) | e1024) - k1024, scale(0), lowest(0));
+        v[1] = __builtin_elementwise_fma(part((w & high) | e64) - k64, scale(1), lowest(1));
+        w >>= 8;
+        v[2] = __builtin_elementwise_fma(part((w & low) | e1024) - k1024, scale(2), lowest(2));
+        v[3] = __builtin_elementwise_fma(part((w & high) | e64) - k64, scale(3), lowest(3));
+    }
+    __device__ __forceinline__ void operator()(uint32_t w, kvh2 scale, kvh2 lowest, kvh2 (&v)[4]) const {
+        (*this)(w, [=](int) { return scale; }, [=](int) { return lowest; }, v);
+    }
+};
 
 // eight elements as floats; `wide`: they lie on 16 bytes
 template <typename T>

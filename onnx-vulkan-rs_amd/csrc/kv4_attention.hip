@@ -125,6 +125,7 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
     char *codes = smem + wave * (CODES + PARAMS), *params = codes + CODES;
     const int shift = 31 - __builtin_clz((unsigned)a.cache.page_size), page_mask = a.cache.page_size - 1;
     const int per_seq = a.cache.n_kv_heads * a.row_blocks;
+    const Kv4Unpack unpack;
 
     // this workgroup's run of tiles: at least a tile for each wavefront, and long units in few enough parts that joining them is not the longer half
     int64_t total = 0;
@@ -205,75 +206,93 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
         for (int i = 0; i < MT; i++) o[i] = kvf4{};
         float m = -INFINITY, l = 0.f;
 
-        // a tile's loads. Blocks of 16 positions lie in one page: block n / 4 for the lane's keys, block q4 for its value row
-        struct Loads {
-            uint32_t k[4][WPL], kp[4][NP], v[WPL][4], vp[WPL];
-            bool k_there, v_there;
-        };
+        // A tile's loads. Blocks of 16 positions lie in one page: block n / 4 for the lane's keys, block q4 for the parameters of its value row.
+        // Page numbers are asked for two tiles ahead, values and keys one: the values' registers are free once they are in LDS, the keys' once they
+        // are multiplied.
+        uint32_t k_codes[4][WPL], k_params[4][NP], v_codes[WPL][4], v_params[WPL];
         const int *table = static_cast<const int *>(a.cache.table) + (int64_t)u.seq * a.cache.table_width;
-        auto page_row = [&](int key, bool *there) -> int64_t {
-            const int entry = min(key >> shift, (int)a.cache.table_width - 1);
-            const int page = table[entry];
-            *there = page >= 0 && page < a.cache.n_pages;
-            return (((int64_t)(*there ? page : 0) * a.cache.n_kv_heads + kvh) << shift) + (key & page_mask);
+        auto page_at = [&](int tile, int block) { return table[min(((span.first + tile) * kKv4Tile + 16 * block) >> shift, (int)a.cache.table_width - 1)]; };
+        auto is_page = [&](int page) { return page >= 0 && page < a.cache.n_pages; };
+        auto row_of = [&](int page, int key) -> int64_t {
+            return (((int64_t)(is_page(page) ? page : 0) * a.cache.n_kv_heads + kvh) << shift) + (key & page_mask);
         };
-        auto load = [&](int tile, Loads &d) {
+        auto load_values = [&](int tile, int page) {   // page: of block q4
             const int key0 = (span.first + tile) * kKv4Tile;
-            const int64_t k_row = page_row(key0 + 16 * (n >> 2) + (n & 3), &d.k_there);
-            const uint32_t *kc = reinterpret_cast<const uint32_t *>(static_cast<const char *>(a.cache.k_codes) + k_row * (HD / 2)) + q4 * WPL;
-            const uint32_t *kp = static_cast<const uint32_t *>(a.cache.k_params) + k_row * WPL;
+            const int64_t row = row_of(page, key0 + lane);
+            const uint32_t *vp = static_cast<const uint32_t *>(a.cache.v_params) + row * WPL;
+#pragma unroll
+            for (int i = 0; i < WPL; i++) v_params[i] = vp[i];
+            // 16-byte chunks of the 64 rows, in their order: chunk 64 e + lane is of row (64 e + lane) / WPL
+            auto row_at = [&](int r) -> int64_t {   // uniform r: the lane that has that row
+                return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(row >> 32), r) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)row, r));
+            };
+            const char *vc = static_cast<const char *>(a.cache.v_codes);
+#pragma unroll
+            for (int e = 0; e < WPL; e++) {
+                const char *at;
+                if (WPL == 4 || WPL == 8) {   // the rows of a load lie in one block: side by side
+                    at = vc + row_at(64 / WPL * e) * (HD / 2) + lane * 16;
+                } else if (WPL == 1) {
+                    at = vc + row * (HD / 2);
+                } else {
+                    const int id = 64 * e + lane, r = id / WPL;
+                    const uint32_t lo = __shfl((uint32_t)row, r), hi = __shfl((uint32_t)(row >> 32), r);
+                    at = vc + (int64_t)((uint64_t)hi << 32 | lo) * (HD / 2) + (id - r * WPL) * 16;
+                }
+                const kvu4 w = *reinterpret_cast<const kvu4 *>(at);
+#pragma unroll
+                for (int j = 0; j < 4; j++) v_codes[e][j] = w[j];
+            }
+        };
+        auto load_keys = [&](int tile, int page) {   // page: of block n / 4
+            const int64_t row = row_of(page, (span.first + tile) * kKv4Tile + 16 * (n >> 2) + (n & 3));
+            const uint32_t *kc = reinterpret_cast<const uint32_t *>(static_cast<const char *>(a.cache.k_codes) + row * (HD / 2)) + q4 * WPL;
+            const uint32_t *kp = static_cast<const uint32_t *>(a.cache.k_params) + row * WPL;
 #pragma unroll
             for (int t = 0; t < 4; t++) {
 #pragma unroll
-                for (int w = 0; w < WPL; w++) d.k[t][w] = kc[t * 4 * (HD / 8) + w];
+                for (int w = 0; w < WPL; w++) k_codes[t][w] = kc[t * 4 * (HD / 8) + w];
 #pragma unroll
-                for (int i = 0; i < NP; i++) d.kp[t][i] = kp[t * 4 * WPL + (WPL % 4 == 0 ? q4 * (WPL / 4) + i : (q4 * WPL + i) / 4)];
-            }
-            const int64_t v_row = page_row(key0 + lane, &d.v_there);
-            const uint32_t *vp = static_cast<const uint32_t *>(a.cache.v_params) + v_row * WPL;
-#pragma unroll
-            for (int i = 0; i < WPL; i++) d.vp[i] = vp[i];
-            // 16-byte chunks of 64 rows: row (64 e + lane) / WPL, found through the lane that has that row's place
-#pragma unroll
-            for (int e = 0; e < WPL; e++) {
-                const int id = 64 * e + lane, r = id / WPL, c = id - r * WPL;
-                const uint32_t lo = __shfl((uint32_t)v_row, r), hi = __shfl((uint32_t)(v_row >> 32), r);
-                const kvu4 w = *reinterpret_cast<const kvu4 *>(static_cast<const char *>(a.cache.v_codes) + (int64_t)((uint64_t)hi << 32 | lo) * (HD / 2) + c * 16);
-#pragma unroll
-                for (int j = 0; j < 4; j++) d.v[e][j] = w[j];
+                for (int i = 0; i < NP; i++) k_params[t][i] = kp[t * 4 * WPL + (WPL % 4 == 0 ? q4 * (WPL / 4) + i : (q4 * WPL + i) / 4)];
             }
         };
-
-        auto multiply = [&](int tile, Loads &d) {
+        int tile = from + wave, v_page = 0, k_page = 0, v_page1 = 0, k_page1 = 0;
+        if (tile < to) v_page = page_at(tile, q4), k_page = page_at(tile, n >> 2);
+        if (tile + kKv4Waves < to) v_page1 = page_at(tile + kKv4Waves, q4), k_page1 = page_at(tile + kKv4Waves, n >> 2);
+        if (tile < to) load_values(tile, v_page), load_keys(tile, k_page);
+        for (; tile < to; tile += kKv4Waves) {
+            const bool more = tile + kKv4Waves < to;
             const int key0 = (span.first + tile) * kKv4Tile;
-            const bool pages = __all(d.v_there);
-            const bool masked = key0 + kKv4Tile > pos0 + 1 || key0 < all_begin || !pages;
+            const bool v_there = is_page(v_page), masked = key0 + kKv4Tile > pos0 + 1 || key0 < all_begin || !__all(v_there);
+            int v_page2 = 0, k_page2 = 0;
+            if (tile + 2 * kKv4Waves < to) v_page2 = page_at(tile + 2 * kKv4Waves, q4), k_page2 = page_at(tile + 2 * kKv4Waves, n >> 2);
             // values to LDS: codes in 8-byte units, unit x of row r at x ^ (r / PER), so that the 16 rows of a transposing load lie in different banks
 #pragma unroll
             for (int e = 0; e < WPL; e++) {
                 const int id = 64 * e + lane, r = id / WPL, c = id - r * WPL, x = (r / PER) & (UNITS - 1);
-                const kvu4 w = x & 1 ? kvu4{d.v[e][2], d.v[e][3], d.v[e][0], d.v[e][1]} : kvu4{d.v[e][0], d.v[e][1], d.v[e][2], d.v[e][3]};
+                const kvu4 w = x & 1 ? kvu4{v_codes[e][2], v_codes[e][3], v_codes[e][0], v_codes[e][1]} : kvu4{v_codes[e][0], v_codes[e][1], v_codes[e][2], v_codes[e][3]};
                 *reinterpret_cast<kvu4 *>(codes + r * (UNITS * 8) + (c ^ (x >> 1)) * 16) = w;
             }
             // parameters of eight keys of a group together, in pairs as the codes unpack: scales of keys (i, i + 4), then lowest values
-            const int key = key0 + lane;
             bool seen = true;
             uint32_t odd_groups = 0;   // (several tokens) groups of the lane's key whose parameters are not finite
             if (masked) {
-                seen = key < span.length && key >= any_begin && d.v_there;
+                const int key = key0 + lane;
+                seen = key < span.length && key >= any_begin && v_there;
                 if (a.tokens > 1) {
 #pragma unroll
                     for (int i = 0; i < WPL; i++)
-                        if (((((d.vp[i] & 0x7c007c00u) + 0x04000400u) & 0x80008000u) != 0) && seen) odd_groups |= 1u << i;
+                        if (((((v_params[i] & 0x7c007c00u) + 0x04000400u) & 0x80008000u) != 0) && seen) odd_groups |= 1u << i;
                 }
             }
 #pragma unroll
             for (int i = 0; i < WPL; i++) {
-                const uint32_t w = seen && !(odd_groups >> i & 1) ? d.vp[i] : 0u;
-                char *to = params + i * 256 + (lane >> 3) * 32 + (lane & 3) * 4 + ((lane >> 2) & 1) * 2;
-                *reinterpret_cast<uint16_t *>(to) = (uint16_t)w;
-                *reinterpret_cast<uint16_t *>(to + 16) = (uint16_t)(w >> 16);
+                const uint32_t w = seen && !(odd_groups >> i & 1) ? v_params[i] : 0u;
+                char *to_lds = params + i * 256 + (lane >> 3) * 32 + (lane & 3) * 4 + ((lane >> 2) & 1) * 2;
+                *reinterpret_cast<uint16_t *>(to_lds) = (uint16_t)w;
+                *reinterpret_cast<uint16_t *>(to_lds + 16) = (uint16_t)(w >> 16);
             }
+            if (more) load_values(tile + kKv4Waves, v_page1);
 
             kvf4 s[4];
 #pragma unroll
@@ -281,16 +300,17 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
                 s[t] = kvf4{};
 #pragma unroll
                 for (int w = 0; w < WPL; w++) {
-                    const kvh2 p = __builtin_bit_cast(kvh2, d.kp[t][WPL % 4 == 0 ? w / 4 : NP == 1 ? 0 : w]);
+                    const kvh2 p = __builtin_bit_cast(kvh2, k_params[t][WPL % 4 == 0 ? w / 4 : NP == 1 ? 0 : w]);
                     kvh2 v[4];
-                    kv4_values(d.k[t][w], kvh2{p.x, p.x}, kvh2{p.y, p.y}, v);
+                    unpack(k_codes[t][w], kvh2{p.x, p.x}, kvh2{p.y, p.y}, v);
                     const kvh8 kf = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
 #pragma unroll
                     for (int e = QT - 1; e >= 0; e--) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[w][e], s[t], 0, 0, 0);
                 }
             }
+            if (more) load_keys(tile + kKv4Waves, k_page1);
             if (masked) {
-                const uint64_t there = __ballot(d.v_there);
+                const uint64_t there = __ballot(v_there);
                 const bool block_there = (there >> (16 * q4)) & 1;   // the lane's 16 keys are one block's
 #pragma unroll
                 for (int t = 0; t < 4; t++)
@@ -336,7 +356,8 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
                     const char *pp = params + (i / 2) * 256 + (2 * q4 + h) * 32;
                     const kvu4 sc = *reinterpret_cast<const kvu4 *>(pp), lo = *reinterpret_cast<const kvu4 *>(pp + 16);
                     kvh2 v[4];
-                    kv4_values((uint32_t)w[h], sc, lo, v);
+                    auto pair = [](uint32_t bits) { return __builtin_bit_cast(kvh2, bits); };
+                    unpack((uint32_t)w[h], [&](int j) { return pair(sc[j]); }, [&](int j) { return pair(lo[j]); }, v);
                     const kvh8 vf = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
                     o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p[h][1], o[i], 0, 0, 0);
                     o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p[h][0], o[i], 0, 0, 0);
@@ -353,17 +374,7 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
                         if ((odd >> (i / 2) & 1) && sees) o[i] += kvf4{NAN, NAN, NAN, NAN};
                 }
             }
-        };
-
-        {
-            Loads now, next;
-            int tile = from + wave;
-            if (tile < to) load(tile, now);
-            for (; tile < to; tile += kKv4Waves) {
-                if (tile + kKv4Waves < to) load(tile + kKv4Waves, next);
-                multiply(tile, now);
-                now = next;
-            }
+            v_page = v_page1, k_page = k_page1, v_page1 = v_page2, k_page1 = k_page2;
         }
 
         // the wavefronts' sums, joined in LDS

@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Rows a) {
         const uint32_t codes = *reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(unit.value ? a.cache.v_codes : a.cache.k_codes) +
                                                                    r * (a.cache.head_dim / 2) + unit.channel / 2);
         const kvh2 p = static_cast<const kvh2 *>(unit.value ? a.cache.v_params : a.cache.k_params)[r * (a.cache.head_dim / kKv4Group) + unit.channel / kKv4Group];
-        kv4_values(codes, kvh2{p.x, p.x}, kvh2{p.y, p.y}, v);
+        Kv4Unpack()(codes, kvh2{p.x, p.x}, kvh2{p.y, p.y}, v);
     }
     typedef T T8 __attribute__((ext_vector_type(8)));
     const T8 y = {(T)v[0].x, (T)v[1].x, (T)v[2].x, (T)v[3].x, (T)v[0].y, (T)v[1].y, (T)v[2].y, (T)v[3].y};

@@ -50,44 +50,48 @@ __device__ __forceinline__ float groups_sum(float v) {
 // The key tiles a sequence's newest tokens see: [first, first + count).
 struct Kv4Span {
     int length, first, count;
-    __device__ __forceinline__ Kv4Span(const Kv4Attend &a, int seq) {
-        length = a.cache.n_pages > 0 ? kv4_length(a.cache, seq) : 0;
-        const int begin = a.window > 0 ? max(length - a.tokens - a.window + 1, 0) : 0;
-        first = begin / kKv4Tile;
-        count = length > 0 ? (length + kKv4Tile - 1) / kKv4Tile - first : 0;
-    }
 };
+__device__ __forceinline__ Kv4Span kv4_span(const Kv4Attend &a, int seq) {
+    const int length = a.cache.n_pages > 0 ? kv4_length(a.cache, seq) : 0;
+    const int begin = a.window > 0 ? max(length - a.tokens - a.window + 1, 0) : 0;
+    return {length, begin / kKv4Tile, length > 0 ? (length + kKv4Tile - 1) / kKv4Tile - begin / kKv4Tile : 0};
+}
 
 // Which unit -- (sequence, kv head, block of 16 query rows), in this order -- the tile number `at` of all units' tiles
 // belongs to; `before` is the number of its first tile.
 struct Kv4Unit {
+    Kv4Span span;
     int seq, inner;       // inner = kv head * row_blocks + block
-    int count;            // its tiles
     int64_t before;
 };
-__device__ __forceinline__ int wave_scan(int v) {   // inclusive
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int up = __shfl_up(v, d);
-        if (lane >= d) v += up;
-    }
+__device__ __forceinline__ int wave_scan(int v) {   // inclusive: within rows of 16 lanes, then the rows' last lanes onwards
+    auto add = [&](auto ctrl, auto rows) { v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false); };
+    using std::integral_constant;
+    add(integral_constant<int, 0x111>(), integral_constant<int, 0xf>());   // row_shr:1, 2, 4, 8
+    add(integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
+    add(integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
+    add(integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
+    add(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());   // lane 15 to the row behind it
+    add(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());   // lane 31 to the two rows behind it
     return v;
 }
+// a division of whole numbers that are hardly ever beyond 32 bits (one of 64 bits is some 100 instructions)
+__device__ __forceinline__ int64_t kv4_div(int64_t x, int64_t y) { return ((uint64_t)(x | y) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y; }
 __device__ __forceinline__ bool kv4_find(const Kv4Attend &a, int per_seq, int64_t at, Kv4Unit *u) {
     const int lane = threadIdx.x & 63;
     int64_t before = 0;
     for (int base = 0; base < a.cache.n_seqs; base += 64) {
-        const int n = base + lane < a.cache.n_seqs ? Kv4Span(a, base + lane).count : 0;
+        const Kv4Span s = kv4_span(a, min(base + lane, a.cache.n_seqs - 1));
+        const int n = base + lane < a.cache.n_seqs ? s.count : 0;
         const int sum = wave_scan(n);
         const uint64_t over = __ballot(before + (int64_t)sum * per_seq > at);
         if (over) {
             const int l = __builtin_ctzll(over);
-            const int tiles = __builtin_amdgcn_readlane(n, l);
-            const int64_t first = before + (int64_t)(__builtin_amdgcn_readlane(sum, l) - tiles) * per_seq;
-            u->seq = base + l, u->count = tiles;
-            u->inner = (int)((at - first) / tiles);
-            u->before = first + (int64_t)u->inner * tiles;
+            u->span = {__builtin_amdgcn_readlane(s.length, l), __builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(n, l)};
+            const int64_t first = before + (int64_t)(__builtin_amdgcn_readlane(sum, l) - u->span.count) * per_seq;
+            u->seq = base + l;
+            u->inner = (int)kv4_div(at - first, u->span.count);
+            u->before = first + (int64_t)u->inner * u->span.count;
             return true;
         }
         before += (int64_t)__builtin_amdgcn_readlane(sum, 63) * per_seq;
@@ -129,34 +133,32 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
 
     // this workgroup's run of tiles: at least a tile for each wavefront, and long units in few enough parts that joining them is not the longer half
     int64_t total = 0;
-    int longest = 0;
+    float longest = 0.f;
     for (int base = 0; base < a.cache.n_seqs; base += 64) {
-        const int c = base + lane < a.cache.n_seqs ? Kv4Span(a, base + lane).count : 0;
+        const bool is = base + lane < a.cache.n_seqs;
+        const int c = is ? kv4_span(a, base + lane).count : 0;
         total += (int64_t)__builtin_amdgcn_readlane(wave_scan(c), 63) * per_seq;
-        longest = max(longest, c);
+        longest = fmaxf(longest, lean_wave_max((float)c));
+        if (blockIdx.x == gridDim.x - 1 && wave == 0)   // rows that see nothing for want of keys
+            for (uint64_t none = __ballot(is && c == 0); none; none &= none - 1) {
+                const int64_t s = base + __builtin_ctzll(none);
+                for (int r = 0; r < a.tokens; r++)
+                    for (int i = lane; i < a.n_q_heads * HD; i += 64) static_cast<T *>(a.y)[(s * a.tokens + r) * a.y_stride + i] = (T)0.f;
+            }
     }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) longest = max(longest, __shfl_xor(longest, d));
-    const int64_t even = (total + gridDim.x - 1) / gridDim.x;
-    const int least = max(kKv4Waves, (int)sqrtf((float)longest * (1.f / 7.f)));
+    const int64_t even = kv4_div(total + gridDim.x - 1, gridDim.x);
+    const int least = max(kKv4Waves, (int)sqrtf(longest * (1.f / 7.f)));
     const int64_t share = even > least ? even : least;
     const int64_t run0 = share * blockIdx.x, run1 = run0 + share < total ? run0 + share : total;
-
-    if (blockIdx.x == 0) {   // rows that see nothing for want of keys
-        for (int s = wave; s < a.cache.n_seqs; s += kKv4Waves)
-            if (Kv4Span(a, s).count == 0)
-                for (int r = 0; r < a.tokens; r++)
-                    for (int c = lane; c < a.n_q_heads * HD; c += 64) static_cast<T *>(a.y)[((int64_t)s * a.tokens + r) * a.y_stride + c] = (T)0.f;
-    }
     if (run0 >= run1) return;
 
     Kv4Unit u;
     if (!kv4_find(a, per_seq, run0, &u)) return;
     int64_t at = run0;
     while (at < run1) {
-        const Kv4Span span(a, u.seq);
+        const Kv4Span span = u.span;
         const int kvh = u.inner / a.row_blocks, block = u.inner - kvh * a.row_blocks;
-        const int from = (int)(at - u.before), to = (int)((run1 - u.before) < u.count ? run1 - u.before : u.count);   // its tiles of this run
+        const int from = (int)(at - u.before), to = (int)((run1 - u.before) < u.span.count ? run1 - u.before : u.span.count);   // its tiles of this run
 
         // the lane's query row
         const int rows = min(a.tokens * a.group - block * kKv4Rows, kKv4Rows);
@@ -394,7 +396,7 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
             for (int i = 0; i < MT; i++) mine_o[i * 64] = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[i][0] * keep, o[i][1] * keep, o[i][2] * keep, o[i][3] * keep);
         }
         __syncthreads();
-        const bool whole = from == 0 && to == u.count;
+        const bool whole = from == 0 && to == u.span.count;
         auto store_row = [&](int r, int c, const float4 &v, float inv) {
             const int rr = block * kKv4Rows + r, tk = rr / a.group;
             T *y = static_cast<T *>(a.y) + ((int64_t)u.seq * a.tokens + tk) * a.y_stride + (int64_t)(kvh * a.group + rr - tk * a.group) * HD + c;
@@ -410,6 +412,14 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
         // workgroup w's part of a unit that began in an earlier run (0), or begins here and goes on (1): [row][channel] sums, then maxima and sums
         auto part_of = [&](int64_t w, int which) { return a.parts + (w * 2 + which) * (int64_t)(kKv4Rows * (HD + 2)); };
         float *part = part_of(blockIdx.x, from == 0 ? 1 : 0);
+        // two floats at a time, stored where (and read from where) every workgroup sees them
+        auto put = [](float *to_pair, float x, float y) {
+            __hip_atomic_store(reinterpret_cast<uint64_t *>(to_pair), (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        };
+        auto get = [](const float *pair) {
+            const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t *>(pair), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+        };
         for (int i = wave; i < MT; i += kKv4Waves) {   // thread (i, lane): channels 16 i + 4 q4 .. + 3 of row n
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -422,19 +432,16 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
                 store_row(n, 16 * i + 4 * q4, v, sum == 0.f ? 0.f : 1.f / sum);
             } else {
                 float *to_part = part + n * HD + 16 * i + 4 * q4;
-                const float x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int j = 0; j < 4; j++) __hip_atomic_store(to_part + j, x[j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                put(to_part, v.x, v.y), put(to_part + 2, v.z, v.w);
             }
         }
         if (!whole) {
             if (wave == 0 && q4 == 0 && mine) {
-                __hip_atomic_store(part + kKv4Rows * HD + 2 * n, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                __hip_atomic_store(part + kKv4Rows * HD + 2 * n + 1, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                put(part + kKv4Rows * HD + 2 * n, best, sum);
             }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's stores are where everyone sees them
             __syncthreads();
-            const int64_t w0 = u.before / share, w1 = (u.before + u.count - 1) / share;   // the workgroups that have parts of it
+            const int64_t w0 = kv4_div(u.before, share), w1 = kv4_div(u.before + u.span.count - 1, share);   // the workgroups that have parts of it
             if (tid == 0) {
                 const uint32_t others = __hip_atomic_fetch_add(a.arrived + w0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 last_here = others == (uint32_t)(w1 - w0);
@@ -444,18 +451,29 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
             if (last_here) {
                 for (int i = tid; i < rows * (HD / 4); i += 64 * kKv4Waves) {
                     const int r = i / (HD / 4), c = (i - r * (HD / 4)) * 4;
-                    auto read = [&](const float *x) { return __hip_atomic_load(x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-                    float top = -INFINITY;
-                    for (int64_t w = w0; w <= w1; w++) top = fmaxf(top, read(part_of(w, w == w0) + kKv4Rows * HD + 2 * r));
-                    float all = 0.f;
+                    float top = -INFINITY, all = 0.f;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int64_t w = w0; w <= w1; w++) {
-                        const float *x = part_of(w, w == w0);
-                        const float pm = read(x + kKv4Rows * HD + 2 * r), ps = read(x + kKv4Rows * HD + 2 * r + 1);
-                        const float x0 = read(x + r * HD + c), x1 = read(x + r * HD + c + 1), x2 = read(x + r * HD + c + 2), x3 = read(x + r * HD + c + 3);
-                        if (ps == 0.f) continue;   // nothing the row sees
-                        const float keep = __builtin_amdgcn_exp2f(pm - top);
-                        all += ps * keep, v.x += x0 * keep, v.y += x1 * keep, v.z += x2 * keep, v.w += x3 * keep;
+                    constexpr int N = 8;   // parts on their way together
+                    for (int64_t w = w0; w <= w1; w += N) {
+                        float2 msum[N], x01[N], x23[N];
+#pragma unroll
+                        for (int e = 0; e < N; e++) {
+                            const int64_t at_w = w + e < w1 ? w + e : w1;
+                            const float *x = part_of(at_w, at_w == w0);
+                            msum[e] = get(x + kKv4Rows * HD + 2 * r), x01[e] = get(x + r * HD + c), x23[e] = get(x + r * HD + c + 2);
+                            if (w + e > w1) msum[e] = make_float2(-INFINITY, 0.f);
+                        }
+                        float higher = top;
+#pragma unroll
+                        for (int e = 0; e < N; e++) higher = fmaxf(higher, msum[e].x);
+                        const float back = all == 0.f ? 0.f : __builtin_amdgcn_exp2f(top - higher);
+                        top = higher, all *= back, v.x *= back, v.y *= back, v.z *= back, v.w *= back;
+#pragma unroll
+                        for (int e = 0; e < N; e++) {
+                            if (msum[e].y == 0.f) continue;   // nothing the row sees
+                            const float keep = __builtin_amdgcn_exp2f(msum[e].x - top);
+                            all += msum[e].y * keep, v.x += x01[e].x * keep, v.y += x01[e].y * keep, v.z += x23[e].x * keep, v.w += x23[e].y * keep;
+                        }
                     }
                     store_row(r, c, v, all == 0.f ? 0.f : 1.f / all);
                 }
@@ -463,7 +481,7 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
         }
         __syncthreads();   // LDS is free for the next unit
 
-        at = u.before + u.count;
+        at = u.before + u.span.count;
         if (at < run1 && ++u.inner < per_seq) {
             u.before = at;
         } else if (at < run1 && !kv4_find(a, per_seq, at, &u)) {

@@ -57,12 +57,11 @@ __device__ __forceinline__ Kv4Span kv4_span(const Kv4Attend &a, int seq) {
     return {length, begin / kKv4Tile, length > 0 ? (length + kKv4Tile - 1) / kKv4Tile - begin / kKv4Tile : 0};
 }
 
-// Which unit -- (sequence, kv head, block of 16 query rows), in this order -- the tile number `at` of all units' tiles
-// belongs to; `before` is the number of its first tile.
+// A unit: (sequence, kv head, block of 16 query rows), counted in this order.
 struct Kv4Unit {
     Kv4Span span;
     int seq, inner;       // inner = kv head * row_blocks + block
-    int64_t before;
+    int64_t before;       // steps of all units in front of it
 };
 __device__ __forceinline__ int wave_scan(int v) {   // inclusive: within rows of 16 lanes, then the rows' last lanes onwards
     auto add = [&](auto ctrl, auto rows) { v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false); };
@@ -77,31 +76,62 @@ __device__ __forceinline__ int wave_scan(int v) {   // inclusive: within rows of
 }
 // a division of whole numbers that are hardly ever beyond 32 bits (one of 64 bits is some 100 instructions)
 __device__ __forceinline__ int64_t kv4_div(int64_t x, int64_t y) { return ((uint64_t)(x | y) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y; }
-__device__ __forceinline__ bool kv4_find(const Kv4Attend &a, int per_seq, int64_t at, Kv4Unit *u) {
+// Steps of a unit: its tiles, or (cut > 0) its parts of up to `cut` tiles. The unit that step number `at` of all units' belongs to.
+__device__ __forceinline__ int kv4_steps(int tiles, int cut) { return cut > 0 ? (tiles + cut - 1) / cut : tiles; }
+__device__ __forceinline__ bool kv4_find(const Kv4Attend &a, const Kv4Span &early, int per_seq, int64_t at, int cut, Kv4Unit *u) {
     const int lane = threadIdx.x & 63;
     int64_t before = 0;
     for (int base = 0; base < a.cache.n_seqs; base += 64) {
-        const Kv4Span s = kv4_span(a, min(base + lane, a.cache.n_seqs - 1));
-        const int n = base + lane < a.cache.n_seqs ? s.count : 0;
+        const Kv4Span s = base == 0 ? early : kv4_span(a, min(base + lane, a.cache.n_seqs - 1));
+        const int n = base + lane < a.cache.n_seqs ? kv4_steps(s.count, cut) : 0;
         const int sum = wave_scan(n);
         const uint64_t over = __ballot(before + (int64_t)sum * per_seq > at);
         if (over) {
-            const int l = __builtin_ctzll(over);
-            u->span = {__builtin_amdgcn_readlane(s.length, l), __builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(n, l)};
-            const int64_t first = before + (int64_t)(__builtin_amdgcn_readlane(sum, l) - u->span.count) * per_seq;
+            const int l = __builtin_ctzll(over), steps = __builtin_amdgcn_readlane(n, l);
+            u->span = {__builtin_amdgcn_readlane(s.length, l), __builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.count, l)};
+            const int64_t first = before + (int64_t)(__builtin_amdgcn_readlane(sum, l) - steps) * per_seq;
             u->seq = base + l;
-            u->inner = (int)kv4_div(at - first, u->span.count);
-            u->before = first + (int64_t)u->inner * u->span.count;
+            u->inner = (int)kv4_div(at - first, steps);
+            u->before = first + (int64_t)u->inner * steps;
             return true;
         }
         before += (int64_t)__builtin_amdgcn_readlane(sum, 63) * per_seq;
     }
     return false;
 }
+// steps of all units
+__device__ __forceinline__ int64_t kv4_total(const Kv4Attend &a, const Kv4Span &early, int per_seq, int cut, float *longest) {
+    const int lane = threadIdx.x & 63;
+    int64_t total = 0;
+    float most = 0.f;
+    for (int base = 0; base < a.cache.n_seqs; base += 64) {
+        const int c = base + lane >= a.cache.n_seqs ? 0 : base == 0 ? early.count : kv4_span(a, base + lane).count;
+        total += (int64_t)__builtin_amdgcn_readlane(wave_scan(kv4_steps(c, cut)), 63) * per_seq;
+        most = fmaxf(most, lean_wave_max((float)c));
+    }
+    *longest = most;
+    return total;
+}
 
-// One launch for everything. All units' key tiles are laid end to end and dealt to the workgroups in equal runs, so that sequences of any
-// lengths keep the whole device busy; a unit that lies in one run is finished there, and of one that lies in several the workgroup that
-// comes last joins the parts, in their order.
+// rows that see nothing for want of keys
+template <typename T, int HD>
+__device__ void kv4_zero_rows(const Kv4Attend &a) {
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < a.cache.n_seqs; base += 64) {
+        const bool is = base + lane < a.cache.n_seqs;
+        for (uint64_t none = __ballot(is && kv4_span(a, is ? base + lane : 0).count == 0); none; none &= none - 1) {
+            const int64_t s = base + __builtin_ctzll(none);
+            for (int r = 0; r < a.tokens; r++)
+                for (int i = threadIdx.x; i < a.n_q_heads * HD; i += blockDim.x) static_cast<T *>(a.y)[(s * a.tokens + r) * a.y_stride + i] = (T)0.f;
+        }
+    }
+}
+
+// One launch for everything. Where there are fewer units than workgroups, units are cut into parts of at most so many tiles that there is a
+// workgroup for each; otherwise all units' tiles are laid end to end and dealt to the workgroups in equal runs. So sequences of any lengths
+// keep the whole device busy. A unit that lies in one part is finished there; of one that lies in several the workgroup that comes last joins the
+// parts, in their order. (Runs everywhere: a workgroup mostly has the end of one unit and the beginning of another, and starting on a unit and
+// leaving it costs some 6 us beside 3 us a tile.)
 //
 // A wavefront takes 64 keys of one kv head at a time, for 16 query rows (tokens times the heads of the group):
 //   S^T = K Q^T     16x16x32: of tile t (16 keys) row m is key 16 (m / 4) + 4 t + m % 4, so that a lane ends up with the scores of 16
@@ -131,34 +161,43 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
     const int per_seq = a.cache.n_kv_heads * a.row_blocks;
     const Kv4Unpack unpack;
 
-    // this workgroup's run of tiles: at least a tile for each wavefront, and long units in few enough parts that joining them is not the longer half
-    int64_t total = 0;
-    float longest = 0.f;
-    for (int base = 0; base < a.cache.n_seqs; base += 64) {
-        const bool is = base + lane < a.cache.n_seqs;
-        const int c = is ? kv4_span(a, base + lane).count : 0;
-        total += (int64_t)__builtin_amdgcn_readlane(wave_scan(c), 63) * per_seq;
-        longest = fmaxf(longest, lean_wave_max((float)c));
-        if (blockIdx.x == gridDim.x - 1 && wave == 0)   // rows that see nothing for want of keys
-            for (uint64_t none = __ballot(is && c == 0); none; none &= none - 1) {
-                const int64_t s = base + __builtin_ctzll(none);
-                for (int r = 0; r < a.tokens; r++)
-                    for (int i = lane; i < a.n_q_heads * HD; i += 64) static_cast<T *>(a.y)[(s * a.tokens + r) * a.y_stride + i] = (T)0.f;
-            }
+    // at least a tile for each wavefront, and long units in few enough parts that joining them is not the longer half
+    const int groups = (int)gridDim.x;
+    const Kv4Span early = kv4_span(a, min(lane, a.cache.n_seqs - 1));   // of the first 64 sequences, which mostly are all
+    float longest, same;
+    const int64_t tiles = kv4_total(a, early, per_seq, 0, &longest);
+    if (tiles == 0) {
+        if (blockIdx.x == gridDim.x - 1) kv4_zero_rows<T, HD>(a);
+        return;
     }
-    const int64_t even = kv4_div(total + gridDim.x - 1, gridDim.x);
+    const int64_t even = kv4_div(tiles + groups - 1, groups);
     const int least = max(kKv4Waves, (int)sqrtf(longest * (1.f / 7.f)));
-    const int64_t share = even > least ? even : least;
-    const int64_t run0 = share * blockIdx.x, run1 = run0 + share < total ? run0 + share : total;
-    if (run0 >= run1) return;
-
+    int64_t share = even > least ? even : least;
+    int cut = 0;
+    if (kv4_total(a, early, per_seq, 1 << 30, &same) <= groups) {
+        cut = (int)share;
+        for (;;) {   // (longer parts make fewer of them; with one a unit it ends)
+            const int64_t parts = kv4_total(a, early, per_seq, cut, &same);
+            if (parts <= groups) break;
+            cut = max(cut + 1, (int)min((float)cut * (float)parts / (float)groups, longest));
+        }
+        share = 1;
+    }
+    int64_t at = share * blockIdx.x;
     Kv4Unit u;
-    if (!kv4_find(a, per_seq, run0, &u)) return;
-    int64_t at = run0;
-    while (at < run1) {
+    if (blockIdx.x == gridDim.x - 1) kv4_zero_rows<T, HD>(a);
+    if (!kv4_find(a, early, per_seq, at, cut, &u)) return;
+    const int64_t run1 = at + share;
+    for (;;) {
         const Kv4Span span = u.span;
         const int kvh = u.inner / a.row_blocks, block = u.inner - kvh * a.row_blocks;
-        const int from = (int)(at - u.before), to = (int)((run1 - u.before) < u.span.count ? run1 - u.before : u.span.count);   // its tiles of this run
+        // its tiles of this workgroup
+        const int steps = kv4_steps(span.count, cut);
+        int from = (int)(at - u.before), to = run1 - u.before < steps ? (int)(run1 - u.before) : steps;
+        if (cut > 0) {   // in parts as equal as whole tiles allow
+            const int part = from, each = (span.count + steps - 1) / steps;
+            from = min(part * each, span.count), to = min(from + each, span.count);
+        }
 
         // the lane's query row
         const int rows = min(a.tokens * a.group - block * kKv4Rows, kKv4Rows);
@@ -170,37 +209,11 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
         const int pos1 = span.length - a.tokens + (block * kKv4Rows + rows - 1) / a.group;
         const int any_begin = a.window > 0 ? max(pos0 - a.window + 1, 0) : 0, all_begin = a.window > 0 ? max(pos1 - a.window + 1, 0) : 0;
 
-        kvh8 qf[WPL][QT];
-        float c2 = fabsf(a.scale) * kKv4Log2e;
+        float qx[WPL][8];
         {
             const T *q = static_cast<const T *>(a.q) + ((int64_t)u.seq * a.tokens + (mine ? token : 0)) * a.q_stride + (int64_t)(kvh * a.group + (mine ? g : 0)) * HD;
-            const float sign = a.scale < 0.f ? -1.f : 1.f;
-            float x[WPL][8], most = 0.f;
 #pragma unroll
-            for (int w = 0; w < WPL; w++) {
-                kv4_load8(q + 8 * (q4 * WPL + w), a.wide, x[w]);
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[w][j] *= sign, most = fmaxf(most, fabsf(x[w][j]));
-            }
-            if (QT == 2) {
-                most = groups_max(most);
-                // the row's largest value into [2^14, 2^15); an infinity stays where it is
-                const int up = most > 0.f && most < INFINITY ? 14 - ilogbf(most) : 0;
-                c2 = ldexpf(c2, -up);
-#pragma unroll
-                for (int w = 0; w < WPL; w++)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x[w][j] = ldexpf(x[w][j], up);
-            }
-#pragma unroll
-            for (int w = 0; w < WPL; w++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float v = x[w][(j & 1) * 4 + (j >> 1)];   // the order the codes unpack in: 0 4 1 5 2 6 3 7
-                    const _Float16 hi = (_Float16)v;
-                    qf[w][0][j] = hi;
-                    if (QT == 2) qf[w][QT - 1][j] = (_Float16)(v - (float)hi);
-                }
+            for (int w = 0; w < WPL; w++) kv4_load8(q + 8 * (q4 * WPL + w), a.wide, qx[w]);
         }
 
         kvf4 o[MT];
@@ -262,6 +275,36 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
         if (tile < to) v_page = page_at(tile, q4), k_page = page_at(tile, n >> 2);
         if (tile + kKv4Waves < to) v_page1 = page_at(tile + kKv4Waves, q4), k_page1 = page_at(tile + kKv4Waves, n >> 2);
         if (tile < to) load_values(tile, v_page), load_keys(tile, k_page);
+        // the queries as operands, while the first tile is on its way
+        kvh8 qf[WPL][QT];
+        float c2 = fabsf(a.scale) * kKv4Log2e;
+        {
+            const float sign = a.scale < 0.f ? -1.f : 1.f;
+            float most = 0.f;
+#pragma unroll
+            for (int w = 0; w < WPL; w++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) qx[w][j] *= sign, most = fmaxf(most, fabsf(qx[w][j]));
+            if (QT == 2) {
+                most = groups_max(most);
+                // the row's largest value into [2^14, 2^15); an infinity stays where it is
+                const int up = most > 0.f && most < INFINITY ? 14 - ilogbf(most) : 0;
+                c2 = ldexpf(c2, -up);
+#pragma unroll
+                for (int w = 0; w < WPL; w++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) qx[w][j] = ldexpf(qx[w][j], up);
+            }
+#pragma unroll
+            for (int w = 0; w < WPL; w++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float v = qx[w][(j & 1) * 4 + (j >> 1)];   // the order the codes unpack in: 0 4 1 5 2 6 3 7
+                    const _Float16 hi = (_Float16)v;
+                    qf[w][0][j] = hi;
+                    if (QT == 2) qf[w][QT - 1][j] = (_Float16)(v - (float)hi);
+                }
+        }
         for (; tile < to; tile += kKv4Waves) {
             const bool more = tile + kKv4Waves < to;
             const int key0 = (span.first + tile) * kKv4Tile;
@@ -411,7 +454,7 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
         };
         // workgroup w's part of a unit that began in an earlier run (0), or begins here and goes on (1): [row][channel] sums, then maxima and sums
         auto part_of = [&](int64_t w, int which) { return a.parts + (w * 2 + which) * (int64_t)(kKv4Rows * (HD + 2)); };
-        float *part = part_of(blockIdx.x, from == 0 ? 1 : 0);
+        float *part = part_of(blockIdx.x, cut == 0 && from == 0 ? 1 : 0);
         // two floats at a time, stored where (and read from where) every workgroup sees them
         auto put = [](float *to_pair, float x, float y) {
             __hip_atomic_store(reinterpret_cast<uint64_t *>(to_pair), (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -441,7 +484,7 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
             }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's stores are where everyone sees them
             __syncthreads();
-            const int64_t w0 = kv4_div(u.before, share), w1 = kv4_div(u.before + u.span.count - 1, share);   // the workgroups that have parts of it
+            const int64_t w0 = kv4_div(u.before, share), w1 = kv4_div(u.before + steps - 1, share);   // the workgroups that have parts of it
             if (tid == 0) {
                 const uint32_t others = __hip_atomic_fetch_add(a.arrived + w0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 last_here = others == (uint32_t)(w1 - w0);
@@ -459,7 +502,7 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
 #pragma unroll
                         for (int e = 0; e < N; e++) {
                             const int64_t at_w = w + e < w1 ? w + e : w1;
-                            const float *x = part_of(at_w, at_w == w0);
+                            const float *x = part_of(at_w, cut == 0 && at_w == w0);
                             msum[e] = get(x + kKv4Rows * HD + 2 * r), x01[e] = get(x + r * HD + c), x23[e] = get(x + r * HD + c + 2);
                             if (w + e > w1) msum[e] = make_float2(-INFINITY, 0.f);
                         }
@@ -481,12 +524,10 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
         }
         __syncthreads();   // LDS is free for the next unit
 
-        at = u.before + u.span.count;
-        if (at < run1 && ++u.inner < per_seq) {
-            u.before = at;
-        } else if (at < run1 && !kv4_find(a, per_seq, at, &u)) {
-            break;
-        }
+        at = u.before + steps;
+        if (at >= run1) break;
+        if (++u.inner < per_seq) u.before = at;
+        else if (!kv4_find(a, early, per_seq, at, cut, &u)) break;
     }
 }
 

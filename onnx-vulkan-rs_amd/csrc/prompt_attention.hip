@@ -179,19 +179,19 @@ __device__ __forceinline__ void add_kinds(const pf16 &kinds, pf16 &o) {
     }
 }
 // the lane's row, done: divided into Y, or as it is for the join
-template <typename T, int HD>
-__device__ __forceinline__ void prompt_rows_out(const PromptArgs &a, const PromptTile &pt, const PromptRow &pr, int h, float m, float l, const pf16 (&o)[HD / 32]) {
+template <typename T, int HC>
+__device__ __forceinline__ void prompt_rows_out(const PromptArgs &a, const PromptTile &pt, const PromptRow &pr, int h, int c0, float m, float l, const pf16 (&o)[HC / 32]) {
     l = halves_sum(l);
     if (!pr.mine) return;
     if (a.splits > 1) {
         const size_t part = prompt_part(a, blockIdx.y, pt.q0 + pr.token, pr.head);
-        if (h == 0) a.part_ml[2 * part] = m, a.part_ml[2 * part + 1] = l;
+        if (h == 0 && c0 == 0) a.part_ml[2 * part] = m, a.part_ml[2 * part + 1] = l;
         float *to = a.part_o + part * a.dim;
 #pragma unroll
-        for (int ot = 0; ot < HD / 32; ot++)
+        for (int ot = 0; ot < HC / 32; ot++)
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
-                const int c = 32 * ot + 8 * (r / 4) + 4 * h;
+                const int c = c0 + 32 * ot + 8 * (r / 4) + 4 * h;
                 if (c < a.dim) *reinterpret_cast<float4 *>(to + c) = make_float4(o[ot][r], o[ot][r + 1], o[ot][r + 2], o[ot][r + 3]);
             }
         return;
@@ -200,22 +200,27 @@ __device__ __forceinline__ void prompt_rows_out(const PromptArgs &a, const Promp
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T *y = static_cast<T *>(a.y) + a.y_stride * (pt.q0 + pr.token) + (int64_t)pr.head * a.dim;
 #pragma unroll
-    for (int ot = 0; ot < HD / 32; ot++)
+    for (int ot = 0; ot < HC / 32; ot++)
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
-            const int c = 32 * ot + 8 * (r / 4) + 4 * h;
+            const int c = c0 + 32 * ot + 8 * (r / 4) + 4 * h;
             if (c < a.dim) *reinterpret_cast<T4 *>(y + c) = T4{(T)(o[ot][r] * inv), (T)(o[ot][r + 1] * inv), (T)(o[ot][r + 2] * inv), (T)(o[ot][r + 3] * inv)};
         }
 }
 
+// Heads wider than 128 channels are shared by C = 2 wavefronts: each multiplies its half of the channels, they add up their scores through
+// LDS, and each sums its half of the channels of the result (one wavefront with all 256 needs 512 registers and has its SIMD to itself:
+// 4096 rows of 16 query and 4 kv heads 280 us, shared @SHARED@).
 template <int HD, int W, int KT>
-__global__ void __launch_bounds__(64 * W, HD > 128 || (HD == 128 && W == 2) ? 1 : 2) prompt_tiles_kernel(const PromptArgs a) {
+__global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tiles_kernel(const PromptArgs a) {
+    constexpr int C = HD > 128 ? 2 : 1, HC = HD / C;               // wavefronts of a row, channels of each
     constexpr int PITCH = HD <= 64 ? 64 : HD <= 128 ? 128 : 256;   // halfs of an LDS row
     constexpr int TILE = KT * PITCH * 2;                           // bytes of a tile of K, or of V
     constexpr int CHUNKS = PITCH / 8, RPI = 512 / PITCH;           // 16-byte chunks of a row; rows of a 1 KiB load
     constexpr int LOADS = TILE / 1024;                             // loads of a tile
     constexpr int EACH = (LOADS + W - 1) / W;
     __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];   // [buffer][K, V]
+    __shared__ float4 scores[C > 1 ? W : 1][KT / 8][64];              // a wavefront's own, for the other
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_char *)smem;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
@@ -223,18 +228,18 @@ __global__ void __launch_bounds__(64 * W, HD > 128 || (HD == 128 && W == 2) ? 1 
     // the heaviest tiles (the last of a causal sequence) first; kv heads change fastest, so a head stays with its XCDs
     const int heads = a.n_q_heads / a.group, kvh = (int)(blockIdx.x % heads);
     PromptTile pt;
-    if (!prompt_tile(a, a.tiles - 1 - (int)(blockIdx.x / heads), 32 * W, &pt)) return;
+    if (!prompt_tile(a, a.tiles - 1 - (int)(blockIdx.x / heads), 32 * W / C, &pt)) return;
+    const PromptSpan sp(a, pt, 32 * W / C, KT);
+    const PromptRow pr(a, pt, pt.r0 + 32 * (wave / C), n, kvh);
+    const int c0 = C > 1 ? (wave & 1) * HC : 0;   // the wavefront's first channel
 
-    const PromptSpan sp(a, pt, 32 * W, KT);
-    const PromptRow pr(a, pt, pt.r0 + 32 * wave, n, kvh);
-
-    ph8 qf[HD / 16];
+    ph8 qf[HC / 16];
     {
         const _Float16 *q = static_cast<const _Float16 *>(a.q) + a.q_stride * (pt.q0 + (pr.mine ? pr.token : 0)) + (int64_t)(pr.mine ? pr.head : 0) * a.dim;
 #pragma unroll
-        for (int c = 0; c < HD / 16; c++) {
+        for (int c = 0; c < HC / 16; c++) {
             ph8 v = {};
-            if (pr.mine && 16 * c + 8 * h < a.dim) v = *reinterpret_cast<const ph8 *>(q + 16 * c + 8 * h);
+            if (pr.mine && c0 + 16 * c + 8 * h < a.dim) v = *reinterpret_cast<const ph8 *>(q + c0 + 16 * c + 8 * h);
             qf[c] = a.scale < 0.f ? -v : v;
         }
     }
@@ -269,13 +274,13 @@ __global__ void __launch_bounds__(64 * W, HD > 128 || (HD == 128 && W == 2) ? 1 
     const int i16 = lane & 15;
     uint32_t k_at[4], v_at[2];
 #pragma unroll
-    for (int c = 0; c < 4; c++) k_at[c] = n * PITCH * 2 + (((2 * c + h) ^ (n & 7)) * 16);
+    for (int c = 0; c < 4; c++) k_at[c] = n * PITCH * 2 + (((2 * c + h) ^ (n & 7)) * 16) + 2 * c0;
 #pragma unroll
-    for (int o = 0; o < 2; o++) v_at[o] = (4 * h + (i16 >> 2)) * PITCH * 2 + (((4 * o + 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1)) ^ ((i16 >> 2) << 1)) * 16) + (i16 & 1) * 8;
+    for (int o = 0; o < 2; o++) v_at[o] = (4 * h + (i16 >> 2)) * PITCH * 2 + (((4 * o + 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1)) ^ ((i16 >> 2) << 1)) * 16) + (i16 & 1) * 8 + 2 * c0;
 
-    pf16 o[HD / 32];
+    pf16 o[HC / 32];
 #pragma unroll
-    for (int i = 0; i < HD / 32; i++) o[i] = pf16{};
+    for (int i = 0; i < HC / 32; i++) o[i] = pf16{};
     float m = -INFINITY, l = 0.f;
 
     if (sp.t0 < sp.t1) fetch(sp.t0, 0);
@@ -284,7 +289,8 @@ __global__ void __launch_bounds__(64 * W, HD > 128 || (HD == 128 && W == 2) ? 1 
         // this tile has arrived, and every wavefront is done with the other buffer
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (t + 1 < sp.t1) fetch(t + 1, buf ^ 1);
-        if (!pr.any || t * KT >= pr.end || (t + 1) * KT <= pr.begin) continue;
+        const bool active = pr.any && t * KT < pr.end && (t + 1) * KT > pr.begin;
+        if (C == 1 && !active) continue;
         const char *ks = smem + buf * 2 * TILE, *vs = ks + TILE;
 
         pf16 s[KT / 32];
@@ -292,8 +298,19 @@ __global__ void __launch_bounds__(64 * W, HD > 128 || (HD == 128 && W == 2) ? 1 
         for (int b = 0; b < KT / 32; b++) {
             s[b] = pf16{};
 #pragma unroll
-            for (int c = 0; c < HD / 16; c++)
+            for (int c = 0; c < HC / 16; c++)
                 s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const ph8 *>(ks + k_at[c & 3] + (c >> 2) * 128 + b * 64 * PITCH), qf[c], s[b], 0, 0, 0);
+        }
+        if (C > 1) {
+#pragma unroll
+            for (int i = 0; i < KT / 8; i++) scores[wave][i][lane] = make_float4(s[i / 4][i % 4 * 4], s[i / 4][i % 4 * 4 + 1], s[i / 4][i % 4 * 4 + 2], s[i / 4][i % 4 * 4 + 3]);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (!active) continue;
+#pragma unroll
+            for (int i = 0; i < KT / 8; i++) {
+                const float4 v = scores[wave ^ 1][i][lane];
+                s[i / 4][i % 4 * 4] += v.x, s[i / 4][i % 4 * 4 + 1] += v.y, s[i / 4][i % 4 * 4 + 2] += v.z, s[i / 4][i % 4 * 4 + 3] += v.w;
+            }
         }
         const bool masked = (t + 1) * KT > pr.all_end || t * KT < pr.all_begin;
         if (masked) {
@@ -315,7 +332,7 @@ __global__ void __launch_bounds__(64 * W, HD > 128 || (HD == 128 && W == 2) ? 1 
             const float grown = mx > m + kRescaleAt ? mx : m, keep = grown == m ? 1.f : __builtin_amdgcn_exp2f(m - grown);   // (a row goes by its own scores)
             m = grown, l *= keep;
 #pragma unroll
-            for (int i = 0; i < HD / 32; i++)
+            for (int i = 0; i < HC / 32; i++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) o[i][r] *= keep;
         }
@@ -343,7 +360,7 @@ __global__ void __launch_bounds__(64 * W, HD > 128 || (HD == 128 && W == 2) ? 1 
             // zeros in their places, and a second one finds out what the rows that see them get.
             uint32_t bad = 0;
 #pragma unroll
-            for (int ot = 0; ot < HD / 32; ot++)
+            for (int ot = 0; ot < HC / 32; ot++)
 #pragma unroll
                 for (int u = 0; u < KT / 16; u++) {
                     const pu4 w = __builtin_bit_cast(pu4, v_part(ot, u));
@@ -352,7 +369,7 @@ __global__ void __launch_bounds__(64 * W, HD > 128 || (HD == 128 && W == 2) ? 1 
                 }
             if (__any(bad != 0)) {
 #pragma unroll
-                for (int ot = 0; ot < HD / 32; ot++) {
+                for (int ot = 0; ot < HC / 32; ot++) {
                     pf16 kinds = pf16{};
 #pragma unroll
                     for (int u = 0; u < KT / 16; u++) {
@@ -374,11 +391,11 @@ __global__ void __launch_bounds__(64 * W, HD > 128 || (HD == 128 && W == 2) ? 1 
             }
         }
 #pragma unroll
-        for (int ot = 0; ot < HD / 32; ot++)
+        for (int ot = 0; ot < HC / 32; ot++)
 #pragma unroll
             for (int u = 0; u < KT / 16; u++) o[ot] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_part(ot, u), p[u], o[ot], 0, 0, 0);
     }
-    prompt_rows_out<_Float16, HD>(a, pt, pr, h, m, l, o);
+    prompt_rows_out<_Float16, HC>(a, pt, pr, h, c0, m, l, o);
 }
 
 // ---------------------------------------------------------------------------------- on the matrix cores, f32
@@ -412,31 +429,34 @@ __device__ __forceinline__ pf16 mfma_terms(const pb8 (&x)[3], const pb8 (&y)[3],
 }
 
 template <int HD, int W>
-__global__ void __launch_bounds__(64 * W, HD > 128 ? 1 : 2) prompt_terms_kernel(const PromptArgs a) {
+__global__ void __launch_bounds__(64 * W, W == 2 || (HD > 128 && W == 4) ? 1 : 2) prompt_terms_kernel(const PromptArgs a) {
+    constexpr int C = HD > 128 ? 2 : 1, HC = HD / C;
     constexpr int KT = 32;
     constexpr int PITCH = HD <= 64 ? 64 : HD <= 128 ? 128 : 256;   // bf16 of an LDS row
     constexpr int PLANE = KT * PITCH * 2;                          // bytes of a term of a tile
     constexpr int CHUNKS = HD / 8;                                 // units of eight channels of a row
     constexpr int EACH = (KT * CHUNKS + 64 * W - 1) / (64 * W);    // ... of a tile, per thread
     __shared__ __attribute__((aligned(1024))) char smem[6 * PLANE];   // [K, V][term]
+    __shared__ float4 scores[C > 1 ? W : 1][4][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
 
     const int heads = a.n_q_heads / a.group, kvh = (int)(blockIdx.x % heads);
     PromptTile pt;
-    if (!prompt_tile(a, a.tiles - 1 - (int)(blockIdx.x / heads), 32 * W, &pt)) return;
-    const PromptSpan sp(a, pt, 32 * W, KT);
-    const PromptRow pr(a, pt, pt.r0 + 32 * wave, n, kvh);
+    if (!prompt_tile(a, a.tiles - 1 - (int)(blockIdx.x / heads), 32 * W / C, &pt)) return;
+    const PromptSpan sp(a, pt, 32 * W / C, KT);
+    const PromptRow pr(a, pt, pt.r0 + 32 * (wave / C), n, kvh);
+    const int c0 = C > 1 ? (wave & 1) * HC : 0;
 
-    pb8 qf[HD / 16][3];
+    pb8 qf[HC / 16][3];
     {
         const float *q = static_cast<const float *>(a.q) + a.q_stride * (pt.q0 + (pr.mine ? pr.token : 0)) + (int64_t)(pr.mine ? pr.head : 0) * a.dim;
 #pragma unroll
-        for (int c = 0; c < HD / 16; c++) {
+        for (int c = 0; c < HC / 16; c++) {
             float4 v[2] = {};
-            if (pr.mine && 16 * c + 8 * h < a.dim) {
-                v[0] = *reinterpret_cast<const float4 *>(q + 16 * c + 8 * h);
-                v[1] = *reinterpret_cast<const float4 *>(q + 16 * c + 8 * h + 4);
+            if (pr.mine && c0 + 16 * c + 8 * h < a.dim) {
+                v[0] = *reinterpret_cast<const float4 *>(q + c0 + 16 * c + 8 * h);
+                v[1] = *reinterpret_cast<const float4 *>(q + c0 + 16 * c + 8 * h + 4);
             }
             const float *x = reinterpret_cast<const float *>(v);
             uint32_t term[4][3];
@@ -484,13 +504,13 @@ __global__ void __launch_bounds__(64 * W, HD > 128 ? 1 : 2) prompt_terms_kernel(
     const int i16 = lane & 15;
     uint32_t k_at[4], v_at[2];
 #pragma unroll
-    for (int c = 0; c < 4; c++) k_at[c] = n * PITCH * 2 + (((2 * c + h) ^ (n & 7)) * 16);
+    for (int c = 0; c < 4; c++) k_at[c] = n * PITCH * 2 + (((2 * c + h) ^ (n & 7)) * 16) + 2 * c0;
 #pragma unroll
-    for (int o = 0; o < 2; o++) v_at[o] = (4 * h + (i16 >> 2)) * PITCH * 2 + (((4 * o + 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1)) ^ ((i16 >> 2) << 1)) * 16) + (i16 & 1) * 8;
+    for (int o = 0; o < 2; o++) v_at[o] = (4 * h + (i16 >> 2)) * PITCH * 2 + (((4 * o + 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1)) ^ ((i16 >> 2) << 1)) * 16) + (i16 & 1) * 8 + 2 * c0;
 
-    pf16 o[HD / 32];
+    pf16 o[HC / 32];
 #pragma unroll
-    for (int i = 0; i < HD / 32; i++) o[i] = pf16{};
+    for (int i = 0; i < HC / 32; i++) o[i] = pf16{};
     float m = -INFINITY, l = 0.f;
     if (sp.t0 < sp.t1) fetch(sp.t0);
     for (int t = sp.t0; t < sp.t1; t++) {
@@ -498,15 +518,27 @@ __global__ void __launch_bounds__(64 * W, HD > 128 ? 1 : 2) prompt_terms_kernel(
         store();
         __syncthreads();
         if (t + 1 < sp.t1) fetch(t + 1);
-        if (!pr.any || t * KT >= pr.end || (t + 1) * KT <= pr.begin) continue;
+        const bool active = pr.any && t * KT < pr.end && (t + 1) * KT > pr.begin;
+        if (C == 1 && !active) continue;
 
         pf16 s = pf16{};
 #pragma unroll
-        for (int c = 0; c < HD / 16; c++) {
+        for (int c = 0; c < HC / 16; c++) {
             pb8 kf[3];
 #pragma unroll
             for (int e = 0; e < 3; e++) kf[e] = *reinterpret_cast<const pb8 *>(smem + e * PLANE + k_at[c & 3] + (c >> 2) * 128);
             s = mfma_terms(kf, qf[c], s);
+        }
+        if (C > 1) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) scores[wave][i][lane] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+            __syncthreads();
+            if (!active) continue;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float4 v = scores[wave ^ 1][i][lane];
+                s[4 * i] += v.x, s[4 * i + 1] += v.y, s[4 * i + 2] += v.z, s[4 * i + 3] += v.w;
+            }
         }
 #pragma unroll
         for (int r = 0; r < 16; r++) s[r] *= c2;
@@ -526,7 +558,7 @@ __global__ void __launch_bounds__(64 * W, HD > 128 ? 1 : 2) prompt_terms_kernel(
             const float grown = mx > m + kRescaleAt ? mx : m, keep = grown == m ? 1.f : __builtin_amdgcn_exp2f(m - grown);
             m = grown, l *= keep;
 #pragma unroll
-            for (int i = 0; i < HD / 32; i++)
+            for (int i = 0; i < HC / 32; i++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) o[i][r] *= keep;
         }
@@ -554,7 +586,7 @@ __global__ void __launch_bounds__(64 * W, HD > 128 ? 1 : 2) prompt_terms_kernel(
         // zero or negative -- and a second product finds out what the rows that see them get.
         uint32_t bad = 0;
 #pragma unroll
-        for (int ot = 0; ot < HD / 32; ot++)
+        for (int ot = 0; ot < HC / 32; ot++)
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const pu4 w = __builtin_bit_cast(pu4, v_part(0, ot, u));
@@ -563,7 +595,7 @@ __global__ void __launch_bounds__(64 * W, HD > 128 ? 1 : 2) prompt_terms_kernel(
             }
         const bool any_bad = __any(bad != 0);
 #pragma unroll
-        for (int ot = 0; ot < HD / 32; ot++)
+        for (int ot = 0; ot < HC / 32; ot++)
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 pb8 v[3];
@@ -578,7 +610,7 @@ __global__ void __launch_bounds__(64 * W, HD > 128 ? 1 : 2) prompt_terms_kernel(
             }
         if (any_bad) {
 #pragma unroll
-            for (int ot = 0; ot < HD / 32; ot++) {
+            for (int ot = 0; ot < HC / 32; ot++) {
                 pf16 kinds = pf16{};
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
@@ -597,7 +629,7 @@ __global__ void __launch_bounds__(64 * W, HD > 128 ? 1 : 2) prompt_terms_kernel(
             }
         }
     }
-    prompt_rows_out<float, HD>(a, pt, pr, h, m, l, o);
+    prompt_rows_out<float, HC>(a, pt, pr, h, c0, m, l, o);
 }
 
 // The ranges of keys that several workgroups had of the same rows, joined: one wavefront per row and head.
@@ -633,7 +665,7 @@ size_t prompt_parts_bytes(const PromptArgs &a, int splits) { return splits > 1 ?
 
 template <typename T, int HD, int W>
 int prompt_launch(hipc_ctx *ctx, PromptArgs a, int splits) {
-    const int64_t tiles = ceil_div((int64_t)a.total_q * a.group, 32 * W) + a.n_seqs;   // (at most: a sequence may leave one unfinished)
+    const int64_t tiles = ceil_div((int64_t)a.total_q * a.group, 32 * W / (HD > 128 ? 2 : 1)) + a.n_seqs;   // (at most: a sequence may leave one unfinished)
     a.tiles = (int)tiles, a.splits = splits;
     if (splits > 1) {
         const size_t rows = (size_t)splits * a.total_q * a.n_q_heads;
@@ -660,20 +692,21 @@ int prompt_launch(hipc_ctx *ctx, PromptArgs a, int splits) {
 template <typename T>
 int prompt_matrix(hipc_ctx *ctx, const PromptArgs &a) {
     const int64_t rows = (int64_t)a.total_q * a.group, kv = a.n_q_heads / a.group, cus = ctx->cu_count;
-    int waves = rows <= 64 * (int64_t)a.n_seqs ? 2 : 4;
-    if (a.dim <= 128 && waves == 4 && rows * kv >= 256 * cus * (sizeof(T) == 2 ? 4 : 1)) waves = 8;
+    const int shared = a.dim > 128 ? 2 : 1;   // wavefronts of a row
+    int waves = rows <= 64 * (int64_t)a.n_seqs ? 2 * shared : 4;
+    if (waves == 4 && rows * kv * shared >= 256 * cus * (sizeof(T) == 2 ? 4 : 1)) waves = 8;
     if (ctx->tune.prompt_waves > 0) waves = ctx->tune.prompt_waves;
-    const int64_t groups = std::max<int64_t>(ceil_div(rows, 32 * waves), a.n_seqs) * kv;
+    const int tile_rows = 32 * waves / shared;
+    const int64_t groups = std::max<int64_t>(ceil_div(rows, tile_rows), a.n_seqs) * kv;
     int64_t keys = a.total_k / a.n_seqs;
-    if (a.window > 0) keys = std::min<int64_t>(keys, a.window + 32 * waves / a.group);
+    if (a.window > 0) keys = std::min<int64_t>(keys, a.window + tile_rows / a.group);
     const int64_t key_tiles = keys / (sizeof(T) == 2 && a.dim <= 128 ? 64 : 32);
     int splits = groups < cus ? (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / groups, key_tiles / 4, 32})) : 1;
-    if (ctx->tune.prompt_split > 0) splits = ctx->tune.prompt_split;
-    splits = std::min(splits, 256);
+    if (ctx->tune.prompt_split > 0) splits = std::min(ctx->tune.prompt_split, 256);
     if (!scratch_fits(ctx, kScratchPrompt, prompt_parts_bytes(a, splits))) splits = 1;
     if (a.dim <= 64) return waves >= 8 ? prompt_launch<T, 64, 8>(ctx, a, splits) : waves >= 4 ? prompt_launch<T, 64, 4>(ctx, a, splits) : prompt_launch<T, 64, 2>(ctx, a, splits);
     if (a.dim <= 128) return waves >= 8 ? prompt_launch<T, 128, 8>(ctx, a, splits) : waves >= 4 ? prompt_launch<T, 128, 4>(ctx, a, splits) : prompt_launch<T, 128, 2>(ctx, a, splits);
-    return waves >= 4 ? prompt_launch<T, 256, 4>(ctx, a, splits) : prompt_launch<T, 256, 2>(ctx, a, splits);
+    return waves >= 8 ? prompt_launch<T, 256, 8>(ctx, a, splits) : waves >= 4 ? prompt_launch<T, 256, 4>(ctx, a, splits) : prompt_launch<T, 256, 2>(ctx, a, splits);
 }
 
 }  // namespace

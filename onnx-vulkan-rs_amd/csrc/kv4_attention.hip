@@ -63,17 +63,6 @@ struct Kv4Unit {
     int seq, inner;       // inner = kv head * row_blocks + block
     int64_t before;       // steps of all units in front of it
 };
-__device__ __forceinline__ int wave_scan(int v) {   // inclusive: within rows of 16 lanes, then the rows' last lanes onwards
-    auto add = [&](auto ctrl, auto rows) { v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false); };
-    using std::integral_constant;
-    add(integral_constant<int, 0x111>(), integral_constant<int, 0xf>());   // row_shr:1, 2, 4, 8
-    add(integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
-    add(integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
-    add(integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
-    add(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());   // lane 15 to the row behind it
-    add(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());   // lane 31 to the two rows behind it
-    return v;
-}
 // a division of whole numbers that are hardly ever beyond 32 bits (one of 64 bits is some 100 instructions)
 __device__ __forceinline__ int64_t kv4_div(int64_t x, int64_t y) { return ((uint64_t)(x | y) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y; }
 // Steps of a unit: its tiles, or (cut > 0) its parts of up to `cut` tiles. The unit that step number `at` of all units' belongs to.

@@ -36,5 +36,18 @@ __device__ __forceinline__ float lean_wave_max(float v) {
     return fmaxf(fmaxf(lean_lane(v, 0), lean_lane(v, 16)), fmaxf(lean_lane(v, 32), lean_lane(v, 48)));
 }
 
+// inclusive sums over the lanes: within rows of 16, then the rows' last lanes onwards
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int lane_scan_step(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+    v = lane_scan_step<0x111, 0xf>(v);   // row_shr:1, 2, 4, 8
+    v = lane_scan_step<0x112, 0xf>(v);
+    v = lane_scan_step<0x114, 0xf>(v);
+    v = lane_scan_step<0x118, 0xf>(v);
+    v = lane_scan_step<0x142, 0xa>(v);   // lanes 15 and 47 to the rows behind them
+    return lane_scan_step<0x143, 0xc>(v);   // lane 31 to the two rows behind it
+}
 
 }  // namespace hipc

@@ -93,14 +93,11 @@ __device__ __forceinline__ bool prompt_tile(const PromptArgs &a, int tile, int r
     int before = 0;
     for (int base = 0; base < a.n_seqs; base += 64) {
         const int s = min(base + lane, a.n_seqs - 1);
-        const int from = max(a.q_starts[s], 0), to = min(a.q_starts[s + 1], a.total_q);
+        // (all four on their way together)
+        const int q_from = a.q_starts[s], q_to = a.q_starts[s + 1], k_from = a.k_starts[s], k_to = a.k_starts[s + 1];
+        const int from = max(q_from, 0), to = min(q_to, a.total_q), keys_from = max(k_from, 0), keys = max(min(k_to, a.total_k) - keys_from, 0);
         const int n = base + lane < a.n_seqs && to > from ? ((to - from) * a.group + rows_per_tile - 1) / rows_per_tile : 0;
-        int sum = n;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int up = __shfl_up(sum, d);
-            if (lane >= d) sum += up;
-        }
+        const int sum = wave_scan(n);
         const uint64_t over = __ballot(before + sum > tile);
         if (over) {
             const int l = __builtin_ctzll(over);
@@ -110,8 +107,8 @@ __device__ __forceinline__ bool prompt_tile(const PromptArgs &a, int tile, int r
             out->len_q = __builtin_amdgcn_readlane(to, l) - out->q0;
             out->rows = out->len_q * a.group;
             out->r0 = (tile - first) * rows_per_tile;
-            out->k0 = max(a.k_starts[out->seq], 0);
-            out->keys = max(min(a.k_starts[out->seq + 1], a.total_k) - out->k0, 0);
+            out->k0 = __builtin_amdgcn_readlane(keys_from, l);
+            out->keys = __builtin_amdgcn_readlane(keys, l);
             return true;
         }
         before += __builtin_amdgcn_readlane(sum, 63);
@@ -401,23 +398,17 @@ __global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tile
 // ---------------------------------------------------------------------------------- on the matrix cores, f32
 //
 // The same products of f32 factors, each as three bf16 terms (8 bits a term, together the value's 24): of the nine products of
-// terms the six that matter at 2^-24 are formed, smallest first. K and V are split once on their way into LDS, a plane a term; a
+// terms six are formed, smallest first; the three left out are below 2^-21 of the whole together (2^-23 on average). K and V are split once on their way into LDS, a plane a term; a
 // tile's values wait in registers while the tile before is multiplied.
 typedef __bf16 pb8 __attribute__((ext_vector_type(8)));
-typedef __bf16 pb2 __attribute__((ext_vector_type(2)));
-typedef float pf2 __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ float bf16_up(uint32_t bits) { return __uint_as_float(bits << 16); }
-// two values as three pairs of bf16; a value that is not finite is its first term, whole
+// Two values as three pairs of bf16, cut off rather than rounded: 8 bits each, so their sum is the value, and no term passes the type's range. (A
+// value that is not finite is its first term; the others are NaN.)
 __device__ __forceinline__ void split3(float x, float y, uint32_t (&term)[3]) {
-    constexpr float most = 3.3895314e38f;   // bf16's largest: rounding up from it would be an infinity
-    const bool fx = fabsf(x) <= 3.4028235e38f, fy = fabsf(y) <= 3.4028235e38f;
-    const pf2 a = {fx ? __builtin_amdgcn_fmed3f(x, -most, most) : x, fy ? __builtin_amdgcn_fmed3f(y, -most, most) : y};
-    term[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector(a, pb2));
-    const pf2 r = {fx ? x - bf16_up(term[0]) : 0.f, fy ? y - __uint_as_float(term[0] & 0xffff0000u) : 0.f};
-    term[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, pb2));
-    const pf2 q = {r.x - bf16_up(term[1]), r.y - __uint_as_float(term[1] & 0xffff0000u)};
-    term[2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(q, pb2));
+    auto top = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); };
+    auto pair = [](float v, float w) { return __builtin_amdgcn_perm(__float_as_uint(w), __float_as_uint(v), 0x07060302u); };   // the upper halves
+    const float rx = x - top(x), ry = y - top(y);
+    term[0] = pair(x, y), term[1] = pair(rx, ry), term[2] = pair(rx - top(rx), ry - top(ry));
 }
 __device__ __forceinline__ pf16 mfma_terms(const pb8 (&x)[3], const pb8 (&y)[3], pf16 acc) {
     acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[2], y[0], acc, 0, 0, 0);
@@ -583,7 +574,7 @@ __global__ void __launch_bounds__(64 * W, W == 2 || (HD > 128 && W == 4) ? 1 : 2
             return __builtin_bit_cast(pb8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         };
         // Infinities and NaN of V (whole in its first term): in the product zeros stand for them -- a weight's later terms may be
-        // zero or negative -- and a second product finds out what the rows that see them get.
+        // zero -- and a second product finds out what the rows that see them get.
         uint32_t bad = 0;
 #pragma unroll
         for (int ot = 0; ot < HC / 32; ot++)
@@ -604,7 +595,7 @@ __global__ void __launch_bounds__(64 * W, W == 2 || (HD > 128 && W == 4) ? 1 : 2
                 if (any_bad) {
 #pragma unroll
                     for (int j = 0; j < 8; j++)
-                        if ((__builtin_bit_cast(uint16_t, (__bf16)v[0][j]) & 0x7f80) == 0x7f80) v[0][j] = (__bf16)0.f;
+                        if ((__builtin_bit_cast(uint16_t, (__bf16)v[0][j]) & 0x7f80) == 0x7f80) v[0][j] = v[1][j] = v[2][j] = (__bf16)0.f;
                 }
                 o[ot] = mfma_terms(v, p[u], o[ot]);
             }

@@ -230,16 +230,6 @@ __global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tile
     const PromptRow pr(a, pt, pt.r0 + 32 * (wave / C), n, kvh);
     const int c0 = C > 1 ? (wave & 1) * HC : 0;   // the wavefront's first channel
 
-    ph8 qf[HC / 16];
-    {
-        const _Float16 *q = static_cast<const _Float16 *>(a.q) + a.q_stride * (pt.q0 + (pr.mine ? pr.token : 0)) + (int64_t)(pr.mine ? pr.head : 0) * a.dim;
-#pragma unroll
-        for (int c = 0; c < HC / 16; c++) {
-            ph8 v = {};
-            if (pr.mine && c0 + 16 * c + 8 * h < a.dim) v = *reinterpret_cast<const ph8 *>(q + c0 + 16 * c + 8 * h);
-            qf[c] = a.scale < 0.f ? -v : v;
-        }
-    }
     const float c2 = fabsf(a.scale) * kLog2e;
 
     // the tile's loads of this wavefront: offsets stay, the descriptor's base moves along the keys
@@ -281,6 +271,16 @@ __global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tile
     float m = -INFINITY, l = 0.f;
 
     if (sp.t0 < sp.t1) fetch(sp.t0, 0);
+    ph8 qf[HC / 16];
+    {
+        const _Float16 *q = static_cast<const _Float16 *>(a.q) + a.q_stride * (pt.q0 + (pr.mine ? pr.token : 0)) + (int64_t)(pr.mine ? pr.head : 0) * a.dim;
+#pragma unroll
+        for (int c = 0; c < HC / 16; c++) {
+            ph8 v = {};
+            if (pr.mine && c0 + 16 * c + 8 * h < a.dim) v = *reinterpret_cast<const ph8 *>(q + c0 + 16 * c + 8 * h);
+            qf[c] = a.scale < 0.f ? -v : v;
+        }
+    }
     for (int t = sp.t0; t < sp.t1; t++) {
         const int buf = (t - sp.t0) & 1;
         // this tile has arrived, and every wavefront is done with the other buffer
@@ -439,24 +439,6 @@ __global__ void __launch_bounds__(64 * W, W == 2 || (HD > 128 && W == 4) ? 1 : 2
     const PromptRow pr(a, pt, pt.r0 + 32 * (wave / C), n, kvh);
     const int c0 = C > 1 ? (wave & 1) * HC : 0;
 
-    pb8 qf[HC / 16][3];
-    {
-        const float *q = static_cast<const float *>(a.q) + a.q_stride * (pt.q0 + (pr.mine ? pr.token : 0)) + (int64_t)(pr.mine ? pr.head : 0) * a.dim;
-#pragma unroll
-        for (int c = 0; c < HC / 16; c++) {
-            float4 v[2] = {};
-            if (pr.mine && c0 + 16 * c + 8 * h < a.dim) {
-                v[0] = *reinterpret_cast<const float4 *>(q + c0 + 16 * c + 8 * h);
-                v[1] = *reinterpret_cast<const float4 *>(q + c0 + 16 * c + 8 * h + 4);
-            }
-            const float *x = reinterpret_cast<const float *>(v);
-            uint32_t term[4][3];
-#pragma unroll
-            for (int j = 0; j < 4; j++) split3(x[2 * j], x[2 * j + 1], term[j]);
-#pragma unroll
-            for (int e = 0; e < 3; e++) qf[c][e] = __builtin_bit_cast(pb8, pu4{term[0][e], term[1][e], term[2][e], term[3][e]});
-        }
-    }
     const float c2 = a.scale * kLog2e;
 
     const float *kb = static_cast<const float *>(a.k) + a.k_stride * pt.k0 + (int64_t)kvh * a.dim;
@@ -504,6 +486,24 @@ __global__ void __launch_bounds__(64 * W, W == 2 || (HD > 128 && W == 4) ? 1 : 2
     for (int i = 0; i < HC / 32; i++) o[i] = pf16{};
     float m = -INFINITY, l = 0.f;
     if (sp.t0 < sp.t1) fetch(sp.t0);
+    pb8 qf[HC / 16][3];
+    {
+        const float *q = static_cast<const float *>(a.q) + a.q_stride * (pt.q0 + (pr.mine ? pr.token : 0)) + (int64_t)(pr.mine ? pr.head : 0) * a.dim;
+#pragma unroll
+        for (int c = 0; c < HC / 16; c++) {
+            float4 v[2] = {};
+            if (pr.mine && c0 + 16 * c + 8 * h < a.dim) {
+                v[0] = *reinterpret_cast<const float4 *>(q + c0 + 16 * c + 8 * h);
+                v[1] = *reinterpret_cast<const float4 *>(q + c0 + 16 * c + 8 * h + 4);
+            }
+            const float *x = reinterpret_cast<const float *>(v);
+            uint32_t term[4][3];
+#pragma unroll
+            for (int j = 0; j < 4; j++) split3(x[2 * j], x[2 * j + 1], term[j]);
+#pragma unroll
+            for (int e = 0; e < 3; e++) qf[c][e] = __builtin_bit_cast(pb8, pu4{term[0][e], term[1][e], term[2][e], term[3][e]});
+        }
+    }
     for (int t = sp.t0; t < sp.t1; t++) {
         __syncthreads();   // everybody is done with the tile before
         store();
@@ -512,14 +512,16 @@ __global__ void __launch_bounds__(64 * W, W == 2 || (HD > 128 && W == 4) ? 1 : 2
         const bool active = pr.any && t * KT < pr.end && (t + 1) * KT > pr.begin;
         if (C == 1 && !active) continue;
 
-        pf16 s = pf16{};
+        pf16 s = pf16{}, odd = pf16{};   // (two chains of products, which wait for each other's results half as long)
 #pragma unroll
         for (int c = 0; c < HC / 16; c++) {
             pb8 kf[3];
 #pragma unroll
             for (int e = 0; e < 3; e++) kf[e] = *reinterpret_cast<const pb8 *>(smem + e * PLANE + k_at[c & 3] + (c >> 2) * 128);
-            s = mfma_terms(kf, qf[c], s);
+            if (c & 1) odd = mfma_terms(kf, qf[c], odd);
+            else s = mfma_terms(kf, qf[c], s);
         }
+        s += odd;
         if (C > 1) {
 #pragma unroll
             for (int i = 0; i < 4; i++) scores[wave][i][lane] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);

@@ -41,8 +41,20 @@ __device__ __forceinline__ float quad_max(float v) {
     return fmaxf(v, lean_dpp<0x4E>(v));
 }
 
-// The quantizer's arithmetic is that of exact numbers up to its named roundings: a quotient next to the border of two codes
-// is told from the border by the remainder, in 64 bits, where products of a code (4 bits) and a scale (11) are exact.
+// The quantizer's arithmetic is that of exact numbers up to its named roundings. A quotient is formed in f32 (off by less than 2^-17 below 31; beyond,
+// the code is held to 0 or 15 either way) and decides unless it lies within 2^-14 of the border between two codes; then the remainder does, in 64 bits, where the difference and the
+// product of a code (5 bits) and a scale (11) are exact. In 64 bits throughout, the kernel was bound by its 45 instructions a value
+// (16000 rows of 8 heads of 128, f32: 36.8 us, and 26.0 this way, 5.8 TB/s).
+__device__ __forceinline__ int kv4_code(float x, float lowest, float scale, float inverse) {
+    const float q = (x - lowest) * inverse, r = __builtin_rintf(q);
+    int c = (int)r;
+    if (__builtin_fabsf(__builtin_fabsf(q - r) - 0.5f) < 0x1p-14f) {
+        const double d = (double)x - (double)lowest, rest = __builtin_fma(-(double)r, (double)scale, d), over = __builtin_fabs(rest) - 0.5 * (double)scale;
+        if (over > 0.0 || (over == 0.0 && (c & 1))) c += rest > 0.0 ? 1 : -1;
+    }
+    return min(max(c, 0), 15);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Rows a) {
     const int w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
@@ -70,21 +82,15 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Rows a) {
     }
     lo = quad_min(lo), hi = quad_max(hi);
     nan = quad_max(nan ? 1.f : 0.f) != 0.f;
-    float step = (float)(((double)hi - (double)lo) / 15.0);
+    // (max - min) / 15: the product with 1 / 15, corrected by its remainder
+    const double range = (double)hi - (double)lo, about = range * (1.0 / 15.0);
+    float step = (float)__builtin_fma(__builtin_fma(-15.0, about, range), 1.0 / 15.0, about);
     HIPC_PIN_VGPR(step);   // the two roundings stay two (f32, then f16): left alone, the compiler makes one conversion of them
     const _Float16 lowest = (_Float16)lo, scale = (_Float16)step;
-    const double s = (double)(float)scale, z = (double)(float)lowest, inverse = scale > (_Float16)0 ? 1.0 / s : 0.0;
+    const float inverse = scale > (_Float16)0 ? __builtin_amdgcn_rcpf((float)scale) : 0.f;
     uint32_t codes = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const double d = (double)x[i] - z;
-        double c = __builtin_rint(d * inverse);
-        const double rest = __builtin_fma(-c, s, d), over = __builtin_fabs(rest) - 0.5 * s;
-        const bool odd = ((int)c & 1) != 0;
-        if (scale > (_Float16)0 && (over > 0.0 || (over == 0.0 && odd))) c += rest > 0.0 ? 1.0 : -1.0;
-        const int n = (int)c;
-        codes |= (uint32_t)(n < 0 ? 0 : n > 15 ? 15 : n) << (4 * i);
-    }
+    for (int i = 0; i < 8; i++) codes |= (uint32_t)kv4_code(x[i], (float)lowest, (float)scale, inverse) << (4 * i);
     if (!mine) return;
     const int64_t r = place.slot + (int64_t)unit.head * a.cache.page_size;
     uint8_t *to = static_cast<uint8_t *>(unit.value ? a.cache.v_codes : a.cache.k_codes) + r * (a.cache.head_dim / 2) + unit.channel / 2;

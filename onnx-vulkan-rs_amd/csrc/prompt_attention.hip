@@ -1,5 +1,6 @@
 // Attention over packed prompts (hipc_prompt_attention).
 #include <algorithm>
+#include <type_traits>
 
 #include "kv4.h"
 #include "lanes.h"
@@ -205,74 +206,28 @@ __device__ __forceinline__ void prompt_rows_out(const PromptArgs &a, const Promp
         }
 }
 
-// Heads wider than 128 channels are shared by C = 2 wavefronts: each multiplies its half of the channels, they add up their scores through
-// LDS, and each sums its half of the channels of the result (one wavefront with all 256 needs 512 registers and has its SIMD to itself:
-// 4096 rows of 16 query and 4 kv heads 280 us, shared @SHARED@).
-template <int HD, int W, int KT>
-__global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tiles_kernel(const PromptArgs a) {
-    constexpr int C = HD > 128 ? 2 : 1, HC = HD / C;               // wavefronts of a row, channels of each
-    constexpr int PITCH = HD <= 64 ? 64 : HD <= 128 ? 128 : 256;   // halfs of an LDS row
-    constexpr int TILE = KT * PITCH * 2;                           // bytes of a tile of K, or of V
-    constexpr int CHUNKS = PITCH / 8, RPI = 512 / PITCH;           // 16-byte chunks of a row; rows of a 1 KiB load
-    constexpr int LOADS = TILE / 1024;                             // loads of a tile
-    constexpr int EACH = (LOADS + W - 1) / W;
-    __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];   // [buffer][K, V]
-    __shared__ float4 scores[C > 1 ? W : 1][KT / 8][64];              // a wavefront's own, for the other
-    const uint32_t lds = (uint32_t)(uintptr_t)(lds_char *)smem;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n = lane & 31, h = lane >> 5;
-
-    // the heaviest tiles (the last of a causal sequence) first; kv heads change fastest, so a head stays with its XCDs
-    const int heads = a.n_q_heads / a.group, kvh = (int)(blockIdx.x % heads);
-    PromptTile pt;
-    if (!prompt_tile(a, a.tiles - 1 - (int)(blockIdx.x / heads), 32 * W / C, &pt)) return;
-    const PromptSpan sp(a, pt, 32 * W / C, KT);
-    const PromptRow pr(a, pt, pt.r0 + 32 * (wave / C), n, kvh);
-    const int c0 = C > 1 ? (wave & 1) * HC : 0;   // the wavefront's first channel
-
-    const float c2 = fabsf(a.scale) * kLog2e;
-
-    // the tile's loads of this wavefront: offsets stay, the descriptor's base moves along the keys
-    const uint32_t k_row = (uint32_t)a.k_stride * 2, v_row = (uint32_t)a.v_stride * 2;
-    const char *kb = static_cast<const char *>(a.k) + (a.k_stride * pt.k0 + (int64_t)kvh * a.dim) * 2;
-    const char *vb = static_cast<const char *>(a.v) + (a.v_stride * pt.k0 + (int64_t)kvh * a.dim) * 2;
-    uint32_t k_off[EACH], v_off[EACH];
-#pragma unroll
-    for (int e = 0; e < EACH; e++) {
-        const int r = (wave + e * W) * RPI + lane / CHUNKS, chunk = lane % CHUNKS;
-        const int kc = chunk ^ (r & 7), vc = chunk ^ ((r & 3) << 1);
-        k_off[e] = 8 * kc < a.dim ? r * k_row + 16 * kc : 0x80000000u;
-        v_off[e] = 8 * vc < a.dim ? r * v_row + 16 * vc : 0x80000000u;
-    }
-    auto fetch = [&](int t, int buf) {
-        const int left = min(pt.keys - t * KT, KT);
-        const pu4 kr = descriptor(kb + (int64_t)t * KT * k_row, (uint32_t)(left - 1) * k_row + 2 * a.dim);
-        const pu4 vr = descriptor(vb + (int64_t)t * KT * v_row, (uint32_t)(left - 1) * v_row + 2 * a.dim);
-#pragma unroll
-        for (int e = 0; e < EACH; e++)
-            if (LOADS % W == 0 || wave + e * W < LOADS) {
-                const uint32_t to = lds + buf * 2 * TILE + (wave + e * W) * 1024;
-                to_lds(to, kr, k_off[e]);
-                to_lds(to + TILE, vr, v_off[e]);
-            }
-    };
-
-    // where the lane reads: K row n, chunk 2 c + h; V rows 4 h + i / 4 (+ 8, + 16 u), 16 channels of 32 ot a half of the 32 lanes
-    const int i16 = lane & 15;
-    uint32_t k_at[4], v_at[2];
-#pragma unroll
-    for (int c = 0; c < 4; c++) k_at[c] = n * PITCH * 2 + (((2 * c + h) ^ (n & 7)) * 16) + 2 * c0;
-#pragma unroll
-    for (int o = 0; o < 2; o++) v_at[o] = (4 * h + (i16 >> 2)) * PITCH * 2 + (((4 * o + 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1)) ^ ((i16 >> 2) << 1)) * 16) + (i16 & 1) * 8 + 2 * c0;
-
-    pf16 o[HC / 32];
-#pragma unroll
-    for (int i = 0; i < HC / 32; i++) o[i] = pf16{};
-    float m = -INFINITY, l = 0.f;
-
-    if (sp.t0 < sp.t1) fetch(sp.t0, 0);
+// A wavefront's 32 query rows, HC channels of them from channel c0 on, over key tiles of KT rows of PITCH halfs in LDS.
+template <int HC, int KT, int PITCH>
+struct PromptRows {
     ph8 qf[HC / 16];
-    {
+    pf16 o[HC / 32];
+    float m = -INFINITY, l = 0.f, c2;
+    uint32_t k_at[4], v_at[2];
+    int h;
+
+    __device__ __forceinline__ PromptRows(const PromptArgs &a, int lane, int c0) {
+        const int n = lane & 31, i16 = lane & 15;
+        h = lane >> 5;
+        c2 = fabsf(a.scale) * kLog2e;
+        // where the lane reads: K row n, chunk 2 c + h; V rows 4 h + i / 4 (+ 8, + 16 u), 16 channels of 32 ot a half of the 32 lanes
+#pragma unroll
+        for (int c = 0; c < 4; c++) k_at[c] = n * PITCH * 2 + (((2 * c + h) ^ (n & 7)) * 16) + 2 * c0;
+#pragma unroll
+        for (int i = 0; i < 2; i++) v_at[i] = (4 * h + (i16 >> 2)) * PITCH * 2 + (((4 * i + 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1)) ^ ((i16 >> 2) << 1)) * 16) + (i16 & 1) * 8 + 2 * c0;
+#pragma unroll
+        for (int i = 0; i < HC / 32; i++) o[i] = pf16{};
+    }
+    __device__ __forceinline__ void queries(const PromptArgs &a, const PromptTile &pt, const PromptRow &pr, int c0) {
         const _Float16 *q = static_cast<const _Float16 *>(a.q) + a.q_stride * (pt.q0 + (pr.mine ? pr.token : 0)) + (int64_t)(pr.mine ? pr.head : 0) * a.dim;
 #pragma unroll
         for (int c = 0; c < HC / 16; c++) {
@@ -281,16 +236,7 @@ __global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tile
             qf[c] = a.scale < 0.f ? -v : v;
         }
     }
-    for (int t = sp.t0; t < sp.t1; t++) {
-        const int buf = (t - sp.t0) & 1;
-        // this tile has arrived, and every wavefront is done with the other buffer
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (t + 1 < sp.t1) fetch(t + 1, buf ^ 1);
-        const bool active = pr.any && t * KT < pr.end && (t + 1) * KT > pr.begin;
-        if (C == 1 && !active) continue;
-        const char *ks = smem + buf * 2 * TILE, *vs = ks + TILE;
-
-        pf16 s[KT / 32];
+    __device__ __forceinline__ void scores(const char *ks, pf16 (&s)[KT / 32]) const {
 #pragma unroll
         for (int b = 0; b < KT / 32; b++) {
             s[b] = pf16{};
@@ -298,24 +244,15 @@ __global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tile
             for (int c = 0; c < HC / 16; c++)
                 s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const ph8 *>(ks + k_at[c & 3] + (c >> 2) * 128 + b * 64 * PITCH), qf[c], s[b], 0, 0, 0);
         }
-        if (C > 1) {
-#pragma unroll
-            for (int i = 0; i < KT / 8; i++) scores[wave][i][lane] = make_float4(s[i / 4][i % 4 * 4], s[i / 4][i % 4 * 4 + 1], s[i / 4][i % 4 * 4 + 2], s[i / 4][i % 4 * 4 + 3]);
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (!active) continue;
-#pragma unroll
-            for (int i = 0; i < KT / 8; i++) {
-                const float4 v = scores[wave ^ 1][i][lane];
-                s[i / 4][i % 4 * 4] += v.x, s[i / 4][i % 4 * 4 + 1] += v.y, s[i / 4][i % 4 * 4 + 2] += v.z, s[i / 4][i % 4 * 4 + 3] += v.w;
-            }
-        }
-        const bool masked = (t + 1) * KT > pr.all_end || t * KT < pr.all_begin;
+    }
+    // the scores of keys key0 .. become weights
+    __device__ __forceinline__ void weights(pf16 (&s)[KT / 32], int key0, bool masked, const PromptRow &pr, ph8 (&p)[KT / 16]) {
         if (masked) {
 #pragma unroll
             for (int b = 0; b < KT / 32; b++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    const int key = t * KT + 32 * b + 8 * (r / 4) + 4 * h + r % 4;
+                    const int key = key0 + 32 * b + 8 * (r / 4) + 4 * h + r % 4;
                     s[b][r] = key >= pr.lane_begin && key < pr.lane_end ? s[b][r] : -INFINITY;
                 }
         }
@@ -334,7 +271,6 @@ __global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tile
                 for (int r = 0; r < 16; r++) o[i][r] *= keep;
         }
         const float shift = m == -INFINITY ? 0.f : m;
-        ph8 p[KT / 16];
 #pragma unroll
         for (int u = 0; u < KT / 16; u++)
 #pragma unroll
@@ -346,12 +282,14 @@ __global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tile
                 p[u][j] = w16.x, p[u][j + 1] = w16.y;
                 l = __builtin_amdgcn_fdot2(w16, ph2{(_Float16)1.f, (_Float16)1.f}, l, false);
             }
-        auto v_part = [&](int ot, int u) {
-            const char *at = vs + v_at[ot & 1] + (ot >> 1) * 128 + u * 32 * PITCH;
-            const ps4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ps4 *)(at));
-            const ps4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ps4 *)(at + 16 * PITCH));
-            return __builtin_bit_cast(ph8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-        };
+    }
+    __device__ __forceinline__ ph8 v_part(const char *vs, int ot, int u) const {
+        const char *at = vs + v_at[ot & 1] + (ot >> 1) * 128 + u * 32 * PITCH;
+        const ps4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ps4 *)(at));
+        const ps4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ps4 *)(at + 16 * PITCH));
+        return __builtin_bit_cast(ph8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    __device__ __forceinline__ void values(const char *vs, int key0, bool masked, const PromptRow &pr, const ph8 (&p)[KT / 16]) {
         if (masked) {
             // A hidden key's weight is zero, but zero times an infinity is not: where the tile has such values, the product takes
             // zeros in their places, and a second one finds out what the rows that see them get.
@@ -360,7 +298,7 @@ __global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tile
             for (int ot = 0; ot < HC / 32; ot++)
 #pragma unroll
                 for (int u = 0; u < KT / 16; u++) {
-                    const pu4 w = __builtin_bit_cast(pu4, v_part(ot, u));
+                    const pu4 w = __builtin_bit_cast(pu4, v_part(vs, ot, u));
 #pragma unroll
                     for (int j = 0; j < 4; j++) bad |= ((w[j] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
                 }
@@ -370,13 +308,13 @@ __global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tile
                     pf16 kinds = pf16{};
 #pragma unroll
                     for (int u = 0; u < KT / 16; u++) {
-                        ph8 v = v_part(ot, u), kind = {}, seen = {};
+                        ph8 v = v_part(vs, ot, u), kind = {}, seen = {};
 #pragma unroll
                         for (int j = 0; j < 8; j++) {
                             const uint16_t bits = __builtin_bit_cast(uint16_t, (_Float16)v[j]);
                             // 1 of +inf, 128 of -inf, 16384 of NaN: a tile's counts of each stay apart
                             if ((bits & 0x7c00) == 0x7c00) kind[j] = (_Float16)((bits & 0x3ff) ? 16384.f : bits >> 15 ? 128.f : 1.f), v[j] = (_Float16)0;
-                            const int key = t * KT + 16 * u + 8 * (j / 4) + 4 * h + j % 4;
+                            const int key = key0 + 16 * u + 8 * (j / 4) + 4 * h + j % 4;
                             seen[j] = (_Float16)(key >= pr.lane_begin && key < pr.lane_end ? 1.f : 0.f);
                         }
                         o[ot] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u], o[ot], 0, 0, 0);
@@ -384,15 +322,181 @@ __global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tile
                     }
                     add_kinds(kinds, o[ot]);
                 }
-                continue;
+                return;
             }
         }
 #pragma unroll
         for (int ot = 0; ot < HC / 32; ot++)
 #pragma unroll
-            for (int u = 0; u < KT / 16; u++) o[ot] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_part(ot, u), p[u], o[ot], 0, 0, 0);
+            for (int u = 0; u < KT / 16; u++) o[ot] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_part(vs, ot, u), p[u], o[ot], 0, 0, 0);
     }
-    prompt_rows_out<_Float16, HC>(a, pt, pr, h, c0, m, l, o);
+};
+
+// The loads of KT rows of K and V by W wavefronts, of which this is number `wave`: offsets stay, the descriptors' bases move along the keys.
+template <int KT, int PITCH, int W>
+struct PromptFetch {
+    static constexpr int CHUNKS = PITCH / 8, RPI = 512 / PITCH;   // 16-byte chunks of a row; rows of a 1 KiB load
+    static constexpr int LOADS = KT / RPI, EACH = (LOADS + W - 1) / W;
+    const char *k, *v;
+    uint32_t k_row, v_row, k_off[EACH], v_off[EACH];
+    int keys, width, wave;
+
+    __device__ __forceinline__ PromptFetch(const PromptArgs &a, const PromptTile &pt, int kvh, int wave_, int lane) : keys(pt.keys), width(2 * a.dim), wave(wave_) {
+        k_row = (uint32_t)a.k_stride * 2, v_row = (uint32_t)a.v_stride * 2;
+        k = static_cast<const char *>(a.k) + (a.k_stride * pt.k0 + (int64_t)kvh * a.dim) * 2;
+        v = static_cast<const char *>(a.v) + (a.v_stride * pt.k0 + (int64_t)kvh * a.dim) * 2;
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const int r = (wave + e * W) * RPI + lane / CHUNKS, chunk = lane % CHUNKS;
+            const int kc = chunk ^ (r & 7), vc = chunk ^ ((r & 3) << 1);
+            k_off[e] = 8 * kc < a.dim ? r * k_row + 16 * kc : 0x80000000u;
+            v_off[e] = 8 * vc < a.dim ? r * v_row + 16 * vc : 0x80000000u;
+        }
+    }
+    __device__ __forceinline__ void rows(const char *base, uint32_t row, const uint32_t (&off)[EACH], int t, uint32_t to) const {
+        const pu4 r = descriptor(base + (int64_t)t * KT * row, (uint32_t)(min(keys - t * KT, KT) - 1) * row + width);
+#pragma unroll
+        for (int e = 0; e < EACH; e++)
+            if (LOADS % W == 0 || wave + e * W < LOADS) to_lds(to + (wave + e * W) * 1024, r, off[e]);
+    }
+    __device__ __forceinline__ void keys_of(int t, uint32_t to) const { rows(k, k_row, k_off, t, to); }
+    __device__ __forceinline__ void values_of(int t, uint32_t to) const { rows(v, v_row, v_off, t, to); }
+};
+
+// Heads wider than 128 channels are shared by C = 2 wavefronts: each multiplies its half of the channels, they add up their scores through
+// LDS, and each sums its half of the channels of the result (one wavefront with all 256 needs 512 registers and has its SIMD to itself:
+// 4096 rows of 16 query and 4 kv heads 280 us, shared 235).
+template <int HD, int W, int KT>
+__global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tiles_kernel(const PromptArgs a) {
+    constexpr int C = HD > 128 ? 2 : 1, HC = HD / C;               // wavefronts of a row, channels of each
+    constexpr int PITCH = HD <= 64 ? 64 : HD <= 128 ? 128 : 256;   // halfs of an LDS row
+    constexpr int TILE = KT * PITCH * 2;                           // bytes of a tile of K, or of V
+    __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];   // [buffer][K, V]
+    __shared__ float4 scores[C > 1 ? W : 1][KT / 8][64];              // a wavefront's own, for the other
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_char *)smem;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+    // the heaviest tiles (the last of a causal sequence) first; kv heads change fastest, so a head stays with its XCDs
+    const int heads = a.n_q_heads / a.group, kvh = (int)(blockIdx.x % heads);
+    PromptTile pt;
+    if (!prompt_tile(a, a.tiles - 1 - (int)(blockIdx.x / heads), 32 * W / C, &pt)) return;
+    const PromptSpan sp(a, pt, 32 * W / C, KT);
+    const PromptRow pr(a, pt, pt.r0 + 32 * (wave / C), lane & 31, kvh);
+    const int c0 = C > 1 ? (wave & 1) * HC : 0;   // the wavefront's first channel
+    const PromptFetch<KT, PITCH, W> from(a, pt, kvh, wave, lane);
+    PromptRows<HC, KT, PITCH> rows(a, lane, c0);
+    auto fetch = [&](int t, int buf) {
+        from.keys_of(t, lds + buf * 2 * TILE);
+        from.values_of(t, lds + buf * 2 * TILE + TILE);
+    };
+    if (sp.t0 < sp.t1) fetch(sp.t0, 0);
+    rows.queries(a, pt, pr, c0);
+    for (int t = sp.t0; t < sp.t1; t++) {
+        const int buf = (t - sp.t0) & 1;
+        // this tile has arrived, and every wavefront is done with the other buffer
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (t + 1 < sp.t1) fetch(t + 1, buf ^ 1);
+        const bool active = pr.any && t * KT < pr.end && (t + 1) * KT > pr.begin;
+        if (C == 1 && !active) continue;
+        const char *ks = smem + buf * 2 * TILE;
+        pf16 s[KT / 32];
+        rows.scores(ks, s);
+        if (C > 1) {
+#pragma unroll
+            for (int i = 0; i < KT / 8; i++) scores[wave][i][lane] = make_float4(s[i / 4][i % 4 * 4], s[i / 4][i % 4 * 4 + 1], s[i / 4][i % 4 * 4 + 2], s[i / 4][i % 4 * 4 + 3]);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (!active) continue;
+#pragma unroll
+            for (int i = 0; i < KT / 8; i++) {
+                const float4 v = scores[wave ^ 1][i][lane];
+                s[i / 4][i % 4 * 4] += v.x, s[i / 4][i % 4 * 4 + 1] += v.y, s[i / 4][i % 4 * 4 + 2] += v.z, s[i / 4][i % 4 * 4 + 3] += v.w;
+            }
+        }
+        const bool masked = (t + 1) * KT > pr.all_end || t * KT < pr.all_begin;
+        ph8 p[KT / 16];
+        rows.weights(s, t * KT, masked, pr, p);
+        rows.values(ks + TILE, t * KT, masked, pr, p);
+    }
+    prompt_rows_out<_Float16, HC>(a, pt, pr, rows.h, c0, rows.m, rows.l, rows.o);
+}
+
+// Few rows: a workgroup has 32 of them, and its four wavefronts take the key tiles in turn, each through LDS of its own, so that none waits for
+// another before the end. The keys' half of that LDS is free for the next tile once they are multiplied, the values' half once those are; both are
+// asked for then, and waited for by count (loads end in the order they were issued in).
+template <int HD>
+__global__ void __launch_bounds__(256, HD > 128 ? 1 : 2) prompt_few_kernel(const PromptArgs a) {
+    constexpr int W = 4, KT = 32, PITCH = HD <= 64 ? 64 : HD <= 128 ? 128 : 256, TILE = KT * PITCH * 2;
+    constexpr int SUMS = W * HD * 32 * 4;
+    __shared__ __attribute__((aligned(1024))) char smem[2 * W * TILE > SUMS ? 2 * W * TILE : SUMS];   // [wavefront][K, V]; at last the sums
+    __shared__ float ml[W][2][32];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int heads = a.n_q_heads / a.group, kvh = (int)(blockIdx.x % heads);
+    PromptTile pt;
+    if (!prompt_tile(a, a.tiles - 1 - (int)(blockIdx.x / heads), 32, &pt)) return;
+    const PromptSpan sp(a, pt, 32, KT);
+    const PromptRow pr(a, pt, pt.r0, lane & 31, kvh);
+    const PromptFetch<KT, PITCH, 1> from(a, pt, kvh, 0, lane);
+    constexpr int LOADS = PromptFetch<KT, PITCH, 1>::LOADS;
+    PromptRows<HD, KT, PITCH> rows(a, lane, 0);
+    const char *ks = smem + wave * 2 * TILE, *vs = ks + TILE;
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_char *)smem + wave * 2 * TILE;
+    int t = sp.t0 + wave;
+    if (t < sp.t1) from.keys_of(t, lds), from.values_of(t, lds + TILE);
+    rows.queries(a, pt, pr, 0);
+    for (; t < sp.t1; t += W) {
+        const bool masked = (t + 1) * KT > pr.all_end || t * KT < pr.all_begin, more = t + W < sp.t1;
+        pf16 s[1];
+        ph8 p[2];
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");   // the keys are there; the values may be on their way
+        rows.scores(ks, s);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");             // (the keys have been read)
+        if (more) from.keys_of(t + W, lds);
+        rows.weights(s, t * KT, masked, pr, p);
+        if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        rows.values(vs, t * KT, masked, pr, p);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (more) from.values_of(t + W, lds + TILE);
+    }
+    // the wavefronts' sums, joined in LDS
+    rows.l = halves_sum(rows.l);
+    if (lane < 32) ml[wave][0][lane] = rows.m, ml[wave][1][lane] = rows.l;
+    __syncthreads();
+    const int n = lane & 31;
+    float best = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; w++) best = fmaxf(best, ml[w][0][n]);
+#pragma unroll
+    for (int w = 0; w < W; w++) sum += ml[w][1][n] == 0.f ? 0.f : ml[w][1][n] * __builtin_amdgcn_exp2f(ml[w][0][n] - best);
+    const float keep = rows.l == 0.f ? 0.f : __builtin_amdgcn_exp2f(rows.m - best);
+    float4 *sums = reinterpret_cast<float4 *>(smem);   // [wavefront][four results of a lane][lane]
+#pragma unroll
+    for (int i = 0; i < HD / 8; i++) {
+        const pf16 &x = rows.o[i / 4];
+        const int r = i % 4 * 4;
+        sums[(wave * (HD / 8) + i) * 64 + lane] = rows.l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x[r] * keep, x[r + 1] * keep, x[r + 2] * keep, x[r + 3] * keep);
+    }
+    __syncthreads();
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const size_t part = prompt_part(a, blockIdx.y, pt.q0 + (pr.mine ? pr.token : 0), pr.mine ? pr.head : 0);
+    if (a.splits > 1 && wave == 0 && lane < 32 && pr.mine) a.part_ml[2 * part] = best, a.part_ml[2 * part + 1] = sum;
+#pragma unroll
+    for (int j = 0; j < HD / 8 / W; j++) {
+        const int i = j * W + wave, c = 32 * (i / 4) + 8 * (i % 4) + 4 * rows.h;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            const float4 x = sums[(w * (HD / 8) + i) * 64 + lane];
+            v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+        }
+        if (!pr.mine || c >= a.dim) continue;
+        if (a.splits > 1) {
+            *reinterpret_cast<float4 *>(a.part_o + part * a.dim + c) = v;
+        } else {
+            _Float16 *y = static_cast<_Float16 *>(a.y) + a.y_stride * (pt.q0 + pr.token) + (int64_t)pr.head * a.dim;
+            *reinterpret_cast<ph4 *>(y + c) = ph4{(_Float16)(v.x * inv), (_Float16)(v.y * inv), (_Float16)(v.z * inv), (_Float16)(v.w * inv)};
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------------- on the matrix cores, f32
@@ -656,9 +760,10 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs a) {
 
 size_t prompt_parts_bytes(const PromptArgs &a, int splits) { return splits > 1 ? (size_t)splits * a.total_q * a.n_q_heads * (a.dim + 2) * 4 : 0; }
 
+// W == 1: the kernel for few rows
 template <typename T, int HD, int W>
 int prompt_launch(hipc_ctx *ctx, PromptArgs a, int splits) {
-    const int64_t tiles = ceil_div((int64_t)a.total_q * a.group, 32 * W / (HD > 128 ? 2 : 1)) + a.n_seqs;   // (at most: a sequence may leave one unfinished)
+    const int64_t tiles = ceil_div((int64_t)a.total_q * a.group, W == 1 ? 32 : 32 * W / (HD > 128 ? 2 : 1)) + a.n_seqs;   // (at most: a sequence may leave one unfinished)
     a.tiles = (int)tiles, a.splits = splits;
     if (splits > 1) {
         const size_t rows = (size_t)splits * a.total_q * a.n_q_heads;
@@ -667,7 +772,8 @@ int prompt_launch(hipc_ctx *ctx, PromptArgs a, int splits) {
         a.part_o = static_cast<float *>(s), a.part_ml = a.part_o + rows * a.dim;
     }
     const dim3 grid((unsigned)(tiles * (a.n_q_heads / a.group)), splits);
-    if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((prompt_tiles_kernel<HD, W, (HD > 128 ? 32 : 64)>), grid, 64 * W, 0, ctx->stream, a);
+    if constexpr (sizeof(T) == 2 && W == 1) hipLaunchKernelGGL((prompt_few_kernel<HD>), grid, 256, 0, ctx->stream, a);
+    else if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((prompt_tiles_kernel<HD, W, (HD > 128 ? 32 : 64)>), grid, 64 * W, 0, ctx->stream, a);
     else hipLaunchKernelGGL((prompt_terms_kernel<HD, W>), grid, 64 * W, 0, ctx->stream, a);
     HIPC_LAUNCHED(ctx);
     if (splits > 1) {
@@ -688,18 +794,26 @@ int prompt_matrix(hipc_ctx *ctx, const PromptArgs &a) {
     const int shared = a.dim > 128 ? 2 : 1;   // wavefronts of a row
     int waves = rows <= 64 * (int64_t)a.n_seqs ? 2 * shared : 4;
     if (waves == 4 && rows * kv * shared >= 256 * cus * (sizeof(T) == 2 ? 4 : 1)) waves = 8;
+    if (sizeof(T) == 2 && std::max<int64_t>(ceil_div(rows, 32), a.n_seqs) * kv <= 2 * cus) waves = 1;
     if (ctx->tune.prompt_waves > 0) waves = ctx->tune.prompt_waves;
-    const int tile_rows = 32 * waves / shared;
+    if (sizeof(T) != 2) waves = std::max(waves, 2);
+    const int tile_rows = waves == 1 ? 32 : 32 * waves / shared;
     const int64_t groups = std::max<int64_t>(ceil_div(rows, tile_rows), a.n_seqs) * kv;
     int64_t keys = a.total_k / a.n_seqs;
     if (a.window > 0) keys = std::min<int64_t>(keys, a.window + tile_rows / a.group);
-    const int64_t key_tiles = keys / (sizeof(T) == 2 && a.dim <= 128 ? 64 : 32);
-    int splits = groups < cus ? (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / groups, key_tiles / 4, 32})) : 1;
+    const int64_t key_tiles = keys / (waves == 1 ? 128 : sizeof(T) == 2 && a.dim <= 128 ? 64 : 32);
+    int splits = groups < cus ? (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / groups, key_tiles / (waves == 1 ? 8 : 4), 32})) : 1;
     if (ctx->tune.prompt_split > 0) splits = std::min(ctx->tune.prompt_split, 256);
     if (!scratch_fits(ctx, kScratchPrompt, prompt_parts_bytes(a, splits))) splits = 1;
-    if (a.dim <= 64) return waves >= 8 ? prompt_launch<T, 64, 8>(ctx, a, splits) : waves >= 4 ? prompt_launch<T, 64, 4>(ctx, a, splits) : prompt_launch<T, 64, 2>(ctx, a, splits);
-    if (a.dim <= 128) return waves >= 8 ? prompt_launch<T, 128, 8>(ctx, a, splits) : waves >= 4 ? prompt_launch<T, 128, 4>(ctx, a, splits) : prompt_launch<T, 128, 2>(ctx, a, splits);
-    return waves >= 8 ? prompt_launch<T, 256, 8>(ctx, a, splits) : waves >= 4 ? prompt_launch<T, 256, 4>(ctx, a, splits) : prompt_launch<T, 256, 2>(ctx, a, splits);
+    auto launch = [&](auto width) -> int {
+        constexpr int HD = decltype(width)::value;
+        if (waves >= 8) return prompt_launch<T, HD, 8>(ctx, a, splits);
+        if (waves >= 4) return prompt_launch<T, HD, 4>(ctx, a, splits);
+        if (waves >= 2 || sizeof(T) != 2) return prompt_launch<T, HD, 2>(ctx, a, splits);
+        if constexpr (sizeof(T) == 2) return prompt_launch<T, HD, 1>(ctx, a, splits);
+        return HIPC_OK;
+    };
+    return a.dim <= 64 ? launch(std::integral_constant<int, 64>()) : a.dim <= 128 ? launch(std::integral_constant<int, 128>()) : launch(std::integral_constant<int, 256>());
 }
 
 }  // namespace

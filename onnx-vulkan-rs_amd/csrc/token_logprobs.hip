@@ -14,7 +14,7 @@ namespace {
 constexpr int kScratchLogprobs = 7;   // scratch slot of this operator alone
 constexpr int kLogWaves = 4;
 constexpr int kLogChunk = 1024;       // logits a wavefront holds at a time: 16 a lane
-constexpr int kLogWorkgroups = 1024;  // at most that many share rows
+constexpr int kLogWorkgroups = 512;   // at most that many share rows
 constexpr int kLogParts = 64;         // ... a row
 constexpr int kLogBuffer = 256;       // candidates a wavefront ranks at a time
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;

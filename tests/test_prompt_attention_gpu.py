@@ -162,11 +162,11 @@ def test_a_recorded_call_follows_the_starts(ctx, pkg):
 
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
-@pytest.mark.parametrize("waves", [2, 4, 8])
+@pytest.mark.parametrize("waves", [1, 2, 4, 8])
 @pytest.mark.parametrize("split", [1, 2, 5])
 @pytest.mark.parametrize("heads,kv,dim", [(4, 1, 256), (6, 2, 128), (3, 1, 64)])
 def test_every_launch_shape(ctx, pkg, dtype, waves, split, heads, kv, dim):
-    """Workgroups of 2, 4 and 8 wavefronts, alone with their keys or sharing them, over sequences that end anywhere in a tile."""
+    """Workgroups of 2, 4 and 8 wavefronts, and of 32 rows (1), alone with their keys or sharing them, over sequences that end anywhere in a tile."""
     q_lengths, k_lengths = [70, 3, 1], [200, 3, 90]
     q, k, v = operands(np.random.default_rng(dim + split), dtype, 74, 293, heads, kv, dim)
     with ctx.options(HIPC_PROMPT_WAVES=waves, HIPC_PROMPT_SPLIT=split):

@@ -76,7 +76,7 @@ void *hipc_stream(hipc_ctx *ctx);
  * `name` is one of HIPC_GEMV_T, HIPC_GEMV_WAVES, HIPC_GEMV_PER_CU, HIPC_GEMM_TILE, HIPC_GEMM_BIG,
  * HIPC_GEMM_SMALL, HIPC_GEMM_SKINNY, HIPC_CONV_ROW, HIPC_PREFILL_TILE, HIPC_PREFILL_SPLIT, HIPC_PREFILL_DIRECT, HIPC_PREFILL_GROUPS,
  * HIPC_DEC_FUSED_GLUE, HIPC_DEC_FUSED_ATTN, HIPC_DEC_FUSED_ARGMAX, HIPC_GEMV_LEAN, HIPC_DEC_LEAN, HIPC_DEC_RESIDENT, HIPC_DEC_WAIT, HIPC_DEC_WIDE, HIPC_DEC_POLLS,
- * HIPC_DEC_PREFETCH, HIPC_DQL_WAIT; a context starts from the environment variables of the same names; value < 0 returns the choice to the library. */
+ * HIPC_DEC_PREFETCH, HIPC_DQL_WAIT, HIPC_PROMPT_WAVES, HIPC_PROMPT_SPLIT; a context starts from the environment variables of the same names; value < 0 returns the choice to the library. */
 int hipc_set_option(hipc_ctx *ctx, const char *name, int value);
 
 /* ------------------------------------------------------------------ buffers */
@@ -420,12 +420,15 @@ typedef struct {
  *   the keys k_starts[s] .. k_starts[s + 1] - 1. With len_q and len_k of them, query row i stands at position
  *   len_k - len_q + i among the keys, so a prompt that comes in pieces passes the earlier keys along with the new ones.
  * A row that sees no key (a position below 0) is zero. Rows of Q and Y in front of the first and behind the last sequence are
- * neither read nor written. Starts are held to [0, total]; a sequence that would end before it starts has no rows.
- * Keys and values that a row does not see do not enter its result, whatever they hold (infinities and NaN too).
+ * neither read nor written. Starts ascend; they are held to [0, total], and a sequence that would end before it starts has no rows.
+ * Keys and values that a row does not see do not enter its result, whatever they hold (infinities and NaN too). A row that sees an
+ * infinity or a NaN gets what these make of it; in f32 an infinite query or key that a row sees makes it NaN.
  * f16: products of the f16 values as they are, sums in f32, softmax in f32, its weights rounded to f16 for the second
- * product. f32: every factor as three bf16 terms (24 bits), sums in f32. head_dim is at most 512; one that is a multiple
- * of 8, up to 256, with rows and strides on 16 bytes runs on the matrix cores, any other on a kernel that computes in f32 on
- * the vector units. n_seqs <= 2^20; totals <= 2^31 - 1. Q, K and V may not overlap Y.
+ * product. f32: every factor as three bf16 terms (24 bits), sums in f32. Weighted values are summed before they are divided by
+ * the weights' sum: f32 values above some 2^100 may pass the type's range on the way. head_dim is at most 512; one that is a
+ * multiple of 8, up to 256, with rows and strides (up to 2^23 elements) on 16 bytes runs on the matrix cores, any other on a kernel that
+ * computes in f32 on the vector units. n_seqs <= 2^20; totals <= 2^30. Q, K and V may not overlap Y. With few rows, keys are shared by
+ * several workgroups whose parts lie in scratch memory; a call recorded before any like it ran does without (another order of the sums).
  */
 int hipc_prompt_attention(hipc_ctx *ctx, const hipc_attention_heads *heads, int dtype, const void *Q, int64_t q_stride,
                           const void *K, int64_t k_stride, const void *V, int64_t v_stride, const void *q_starts,
@@ -441,7 +444,8 @@ int hipc_prompt_attention(hipc_ctx *ctx, const hipc_attention_heads *heads, int 
  * table[s * table_width + t / page_size], at place t % page_size; table [n_seqs, table_width] and lengths [n_seqs] are i32 on the
  * device, so a recorded call follows what is written there between its replays. A page number outside [0, n_pages) is no page:
  * what would be stored there is not, what would be read there is zero, and attention does not see its positions (pages
- * behind every window may so be given back). Lengths are held to [0, table_width * page_size].
+ * behind every window may so be given back). So are positions behind the table, whatever the lengths say; a length below 0 counts as 0.
+ * table_width * page_size <= 2^30.
  */
 typedef struct {
     void *k_codes, *k_params, *v_codes, *v_params;
@@ -472,7 +476,8 @@ int hipc_kv4_read(hipc_ctx *ctx, const hipc_kv4_cache *cache, int dtype, const v
  * lengths[s] - tokens + i. heads->causal has to be set; heads->n_kv_heads and head_dim are the cache's. A row that sees
  * nothing (an empty sequence, a position below 0) is zero. The cache's values enter exactly, f16 queries too, f32 queries
  * with 22 bits of a row's largest value; weights with 22 bits; sums in f32. tokens * n_q_heads / n_kv_heads <= 1024.
- * The order of the sums is fixed by the shapes, the lengths and the device: results repeat bit for bit.
+ * The order of the sums is fixed by the shapes, the lengths and the device: results repeat bit for bit. The call needs a scratch block of
+ * fixed size: run one on the context before recording one.
  */
 int hipc_kv4_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_attention_heads *heads, int dtype, int64_t tokens,
                        const void *Q, int64_t q_stride, void *Y, int64_t y_stride);
@@ -488,7 +493,8 @@ int hipc_kv4_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_at
  *   top_ids [rows, top] i32, top_logprobs [rows, top] f32: the `top` (0 to HIPC_TOP_MAX) largest logits, largest first, the lower id
  *                            first among equals; NaN never counts; where fewer than `top` logits compare the rest is -1 and NaN
  * A row without a finite largest logit (all -inf, a +inf or a NaN in it) has no distribution: its logprob, entropy and
- * top_logprobs are NaN. The logits are read once. vocab <= 2^30.
+ * top_logprobs are NaN. The logits are read once. vocab <= 2^30. Few rows are shared by several workgroups, which need a scratch block of fixed
+ * size; a call recorded before any other ran does without (another order of the sums).
  */
 #define HIPC_TOP_MAX 32
 int hipc_token_logprobs(hipc_ctx *ctx, int dtype, const void *logits, int64_t row_stride, int64_t rows, int64_t vocab,

@@ -332,6 +332,9 @@ int stage_upload(hipc_ctx *ctx, void *dst, const void *host, size_t bytes);
 // variant that allocates nothing, and keeps it in ctx->dql_static (dynamic_quantize.hip)
 int dql_static_init(hipc_ctx *ctx);
 
+// a launch counts its threads along an axis in 32 bits
+inline bool grid_fits(int64_t workgroups, int threads) { return workgroups > 0 && workgroups * threads < (int64_t)1 << 32; }
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline bool is_pow2(int64_t v) { return v > 0 && (v & (v - 1)) == 0; }
 inline bool is_byte_dtype(int dt) { return dt == HIPC_U8 || dt == HIPC_I8; }

@@ -11,6 +11,7 @@ namespace hipc {
 
 constexpr int kKv4Group = 32;      // channels that share a scale and a lowest value
 constexpr int kKv4MaxHead = 256;
+constexpr int kKv4MaxPositions = 1 << 30;   // of a sequence
 
 typedef _Float16 kvh2 __attribute__((ext_vector_type(2)));
 
@@ -44,12 +45,9 @@ __device__ __forceinline__ Kv4Place kv4_place(const hipc_kv4_cache &c, int s, in
     if (page < 0 || page >= c.n_pages) return {0, false};
     return {((int64_t)page * c.n_kv_heads << shift) + (t & (c.page_size - 1)), true};
 }
-// lengths are held to what the table can name
-__device__ __forceinline__ int kv4_length(const hipc_kv4_cache &c, int s) {
-    const int64_t most = c.table_width * c.page_size;
-    const int n = static_cast<const int *>(c.lengths)[s];
-    return n < 0 ? 0 : n > most ? (int)most : n;
-}
+// what a sequence's length says, and the positions below it that the table has room for
+__device__ __forceinline__ int kv4_length(const hipc_kv4_cache &c, int s) { return max(static_cast<const int *>(c.lengths)[s], 0); }
+__device__ __forceinline__ int kv4_held(const hipc_kv4_cache &c, int length) { return min(length, (int)(c.table_width * c.page_size)); }
 
 // Eight codes as f16 values, each lowest + code * scale rounded once: the code's bits under the exponent of 1024 (or, four
 // bits further up, of 64) are that number plus the code; the subtraction is exact, and so is the product inside the fma.

@@ -1,4 +1,5 @@
 // Attention of the newest tokens of many sequences over the paged 4-bit cache (hipc_kv4_attention).
+#include <algorithm>
 #include <type_traits>
 
 #include "kv4.h"
@@ -52,9 +53,9 @@ struct Kv4Span {
     int length, first, count;
 };
 __device__ __forceinline__ Kv4Span kv4_span(const Kv4Attend &a, int seq) {
-    const int length = a.cache.n_pages > 0 ? kv4_length(a.cache, seq) : 0;
+    const int length = a.cache.n_pages > 0 ? kv4_length(a.cache, seq) : 0, held = kv4_held(a.cache, length);
     const int begin = a.window > 0 ? max(length - a.tokens - a.window + 1, 0) : 0;
-    return {length, begin / kKv4Tile, length > 0 ? (length + kKv4Tile - 1) / kKv4Tile - begin / kKv4Tile : 0};
+    return {length, begin / kKv4Tile, held > begin ? (held + kKv4Tile - 1) / kKv4Tile - begin / kKv4Tile : 0};
 }
 
 // A unit: (sequence, kv head, block of 16 query rows), counted in this order.
@@ -215,7 +216,10 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
         // are multiplied.
         uint32_t k_codes[4][WPL], k_params[4][NP], v_codes[WPL][4], v_params[WPL];
         const int *table = static_cast<const int *>(a.cache.table) + (int64_t)u.seq * a.cache.table_width;
-        auto page_at = [&](int tile, int block) { return table[min(((span.first + tile) * kKv4Tile + 16 * block) >> shift, (int)a.cache.table_width - 1)]; };
+        auto page_at = [&](int tile, int block) {
+            const int entry = ((span.first + tile) * kKv4Tile + 16 * block) >> shift, last = (int)a.cache.table_width - 1, page = table[min(entry, last)];
+            return entry <= last ? page : -1;
+        };
         auto is_page = [&](int page) { return page >= 0 && page < a.cache.n_pages; };
         auto row_of = [&](int page, int key) -> int64_t {
             return (((int64_t)(is_page(page) ? page : 0) * a.cache.n_kv_heads + kvh) << shift) + (key & page_mask);
@@ -566,7 +570,7 @@ int hipc_kv4_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_at
         HIPC_REQUIRE(ctx, q_stride >= width && y_stride >= width && q_stride <= (int64_t)1 << 40 && y_stride <= (int64_t)1 << 40,
                      "%s: rows %lld and %lld apart, of %lld values", who, (long long)q_stride, (long long)y_stride, (long long)width);
         a.cache = *cache, a.q = Q, a.y = Y, a.q_stride = q_stride, a.y_stride = y_stride;
-        a.tokens = (int)tokens, a.n_q_heads = heads->n_q_heads, a.group = (int)group, a.window = heads->window;
+        a.tokens = (int)tokens, a.n_q_heads = heads->n_q_heads, a.group = (int)group, a.window = std::min(heads->window, kKv4MaxPositions);
         a.row_blocks = (int)ceil_div(tokens * group, kKv4Rows);
         const int64_t unit = dtype == HIPC_F16 ? 8 : 4;
         a.wide = aligned(Q, 16) && aligned(Y, 16) && q_stride % unit == 0 && y_stride % unit == 0;

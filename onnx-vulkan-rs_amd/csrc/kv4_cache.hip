@@ -146,7 +146,7 @@ int rows_check(hipc_ctx *ctx, const char *who, const hipc_kv4_cache *c, int dtyp
     a->cache = *c, a->starts = static_cast<const int *>(starts), a->k = K, a->v = V, a->k_stride = k_stride, a->v_stride = v_stride, a->total = (int)total;
     a->units = (int)(width / 4), a->chunks = (int)ceil_div(a->units, 64);
     a->wide = aligned(K, 16) && aligned(V, 16) && k_stride * size % 16 == 0 && v_stride * size % 16 == 0;
-    HIPC_REQUIRE(ctx, ceil_div(total * a->chunks, 4) <= 0x7fffffff / 4, "%s: too many rows of too many heads in one call", who);
+    HIPC_REFUSE(ctx, !grid_fits(ceil_div(total * a->chunks, 4), 256), "%s: %lld rows of %lld values: too many for one call", who, (long long)total, (long long)width);
     return HIPC_OK;
 }
 
@@ -154,11 +154,11 @@ int rows_check(hipc_ctx *ctx, const char *who, const hipc_kv4_cache *c, int dtyp
 
 int kv4_check(hipc_ctx *ctx, const char *who, const hipc_kv4_cache *c) {
     HIPC_REQUIRE(ctx, c, "%s: null cache", who);
-    HIPC_REQUIRE(ctx, c->n_kv_heads > 0 && c->n_kv_heads <= 65536 && c->n_seqs >= 0 && c->n_seqs <= 1 << 20, "%s: %d kv heads, %d sequences", who, c->n_kv_heads, c->n_seqs);
+    HIPC_REQUIRE(ctx, c->n_kv_heads > 0 && c->n_kv_heads <= 65535 && c->n_seqs >= 0 && c->n_seqs <= 1 << 20, "%s: %d kv heads, %d sequences", who, c->n_kv_heads, c->n_seqs);
     HIPC_REFUSE(ctx, c->head_dim <= 0 || c->head_dim > kKv4MaxHead || c->head_dim % kKv4Group != 0, "%s: head_dim %d (multiples of %d up to %d are taken)", who, c->head_dim, kKv4Group, kKv4MaxHead);
     HIPC_REFUSE(ctx, c->page_size < 16 || !is_pow2(c->page_size), "%s: pages of %d positions (powers of two from 16 on are taken)", who, c->page_size);
     HIPC_REQUIRE(ctx, c->n_pages >= 0 && c->n_pages <= 0x7fffffff && c->table_width >= 0, "%s: %lld pages, %lld a sequence", who, (long long)c->n_pages, (long long)c->table_width);
-    HIPC_REQUIRE(ctx, c->table_width <= 0x7fffffff / c->page_size, "%s: a table of %lld pages of %d positions passes 2^31 positions", who, (long long)c->table_width, c->page_size);
+    HIPC_REQUIRE(ctx, c->table_width <= kKv4MaxPositions / c->page_size, "%s: a table of %lld pages of %d positions passes 2^30 positions", who, (long long)c->table_width, c->page_size);
     // (rows of the cache, one per position and kv head, are counted in 64 bits on the device)
     HIPC_REQUIRE(ctx, c->n_pages == 0 || (c->k_codes && c->k_params && c->v_codes && c->v_params), "%s: null pointer", who);
     HIPC_REQUIRE(ctx, aligned(c->k_codes, 16) && aligned(c->k_params, 16) && aligned(c->v_codes, 16) && aligned(c->v_params, 16), "%s: the cache's arrays lie on 16 bytes", who);

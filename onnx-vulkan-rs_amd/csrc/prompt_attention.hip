@@ -832,7 +832,7 @@ int hipc_prompt_attention(hipc_ctx *ctx, const hipc_attention_heads *heads, int 
         PromptArgs a{};
         if (int rc = attention_check(ctx, who, heads, dtype, &a.scale)) return rc;
         HIPC_REFUSE(ctx, heads->head_dim > kPromptMaxHead, "%s: head_dim %d (up to %d is taken)", who, heads->head_dim, kPromptMaxHead);
-        HIPC_REQUIRE(ctx, n_seqs >= 0 && n_seqs <= 1 << 20 && total_q >= 0 && total_q <= 0x7fffffff && total_k >= 0 && total_k <= 0x7fffffff,
+        HIPC_REQUIRE(ctx, n_seqs >= 0 && n_seqs <= 1 << 20 && total_q >= 0 && total_q <= 1 << 30 && total_k >= 0 && total_k <= 1 << 30,
                      "%s: %lld sequences, %lld query rows, %lld keys", who, (long long)n_seqs, (long long)total_q, (long long)total_k);
         if (n_seqs == 0 || total_q == 0) return HIPC_OK;
         const size_t size = dtype == HIPC_F16 ? 2 : 4;
@@ -844,12 +844,13 @@ int hipc_prompt_attention(hipc_ctx *ctx, const hipc_attention_heads *heads, int 
         a.q = Q, a.k = K, a.v = V, a.y = Y, a.q_starts = static_cast<const int *>(q_starts), a.k_starts = static_cast<const int *>(k_starts);
         a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.y_stride = y_stride;
         a.n_seqs = (int)n_seqs, a.total_q = (int)total_q, a.total_k = (int)total_k, a.n_q_heads = heads->n_q_heads, a.group = heads->n_q_heads / heads->n_kv_heads;
-        a.dim = heads->head_dim, a.causal = heads->causal != 0, a.window = heads->window;
+        a.dim = heads->head_dim, a.causal = heads->causal != 0, a.window = std::min(heads->window, 1 << 30);
         const int64_t unit = dtype == HIPC_F16 ? 8 : 4;   // elements of 16 bytes
         if (heads->head_dim % 8 == 0 && heads->head_dim <= 256 && aligned(Q, 16) && aligned(K, 16) && aligned(V, 16) && aligned(Y, 16) && q_stride % unit == 0 &&
             k_stride % unit == 0 && v_stride % unit == 0 && y_stride % unit == 0 && k_stride <= 1 << 23 && v_stride <= 1 << 23 &&
-            (total_q * a.group + n_seqs * 256) * heads->n_kv_heads < (int64_t)1 << 31)
+            grid_fits((total_q * a.group / 32 + n_seqs + 1) * heads->n_kv_heads, 512) && grid_fits(ceil_div(total_q * heads->n_q_heads, 4), 256))
             return dtype == HIPC_F16 ? prompt_matrix<_Float16>(ctx, a) : prompt_matrix<float>(ctx, a);
+        HIPC_REFUSE(ctx, !grid_fits(total_q, 64), "%s: %lld rows: too many for one call of such heads", who, (long long)total_q);
         const dim3 grid((unsigned)total_q, heads->n_q_heads);
         if (dtype == HIPC_F16) hipLaunchKernelGGL((prompt_rows_kernel<_Float16>), grid, 64, 0, ctx->stream, a);
         else hipLaunchKernelGGL((prompt_rows_kernel<float>), grid, 64, 0, ctx->stream, a);

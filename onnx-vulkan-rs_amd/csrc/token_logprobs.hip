@@ -432,7 +432,7 @@ int hipc_token_logprobs(hipc_ctx *ctx, int dtype, const void *logits, int64_t ro
                 HIPC_LAUNCHED(ctx);
             }
         }
-        HIPC_REQUIRE(ctx, rows * a.parts <= 0x7fffffff, "%s: too many rows", who);
+        HIPC_REFUSE(ctx, !grid_fits(rows * a.parts, 64 * kLogWaves), "%s: %lld rows: too many for one call", who, (long long)rows);
         const unsigned grid = (unsigned)(rows * a.parts);
         if (dtype == HIPC_F16) hipLaunchKernelGGL((logprob_kernel<_Float16>), grid, 64 * kLogWaves, 0, ctx->stream, a);
         else hipLaunchKernelGGL((logprob_kernel<float>), grid, 64 * kLogWaves, 0, ctx->stream, a);

@@ -106,11 +106,11 @@ class Cache:
         scale = scale or 1.0 / math.sqrt(q.shape[2])
         y, weight, size = np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape[:2] + (1,))
         for s, n in enumerate(lengths):
-            n = max(0, min(int(n), self.table.shape[1] * self.page))
+            n = max(0, int(n))
             for i in range(tokens):
                 pos = n - tokens + i
                 first = max(0, pos - window + 1) if window else 0
-                seen = [t for t in range(first, pos + 1) if self.place(s, t) is not None]
+                seen = [t for t in range(first, min(pos + 1, self.table.shape[1] * self.page)) if self.place(s, t) is not None]
                 if not seen:
                     continue
                 k, v = (np.stack([self.load(w, s, t) for t in seen], 1) for w in (0, 1))

@@ -173,15 +173,92 @@ def test_pages_that_are_no_pages(ctx, pkg):
 
 
 def test_lengths_past_the_table_and_below_zero(ctx, pkg):
+    """Positions behind the table lie on no page: rows that would go there are not stored (and nothing else is written over), read as
+    zeros, and are not seen, though they count where a window does."""
     p = Pair(ctx, pkg, np.random.default_rng(4), 2, 2, 16, 1, 64)
     p.append([32, 32])
     q = p.rng.standard_normal((2, 2, 64)).astype(np.float16)
-    want = p.gpu.attention(q)
+    want, held = p.gpu.attention(q), p.gpu.read([32, 32])
     p.gpu.set_lengths([1 << 30, -5])
     got = p.gpu.attention(q)
     assert np.array_equal(bits(got[0]), bits(want[0])) and not got[1].any()
     k, _ = p.gpu.read([2, 2])
-    assert k[:2].any() and not k[2:].any()
+    assert not k.any()
+    p.gpu.set_lengths([35, 0])
+    rows = p.rng.standard_normal((6, 1, 64)).astype(np.float16)
+    p.gpu.append(rows[:5], rows[:5], [5, 0])              # positions 30 .. 34: two of them lie in the table
+    k, _ = p.gpu.read([35, 0])
+    assert np.array_equal(bits(k[:30]), bits(held[0][:30])) and k[30].any() and not np.array_equal(k[30], held[0][30]) and not k[32:].any()
+    for s, n in ((0, 35), (1, 0)):
+        p.lengths[s] = n
+    for i in range(2):
+        p.ref.store(0, 30 + i, (rows[i], rows[i]))
+    for window in (0, 10, 3):
+        y = p.check(ctx, pkg, 4, 1, np.float16, window)
+        assert y[0].any() == (window != 3)
+    p.gpu.set_lengths([-5, 2147483647])
+    assert not p.gpu.attention(q)[0].any()
+    p.gpu.free()
+
+
+def test_a_nan_that_only_the_newest_token_sees(ctx, pkg):
+    """Parameters that are not finite at the last position: that token's rows are NaN in their channels, the token before it is as without."""
+    p = Pair(ctx, pkg, np.random.default_rng(14), 2, 5, 16, 1, 96)
+    p.append([70, 3])
+    q = p.rng.standard_normal((4, 3, 96)).astype(np.float16)
+    want = p.gpu.attention(q, tokens=2)
+    page, place = p.ref.place(0, 69)
+    params = ctx.download(p.gpu.buffers[3], np.float16, p.ref.params[1].shape)
+    params[page, 0, place, 1] = np.nan                     # channels 32 .. 63 of the value
+    ctx.upload(params, p.gpu.buffers[3])
+    got = p.gpu.attention(q, tokens=2).astype(np.float32)
+    assert np.array_equal(got[[0, 2, 3]], want[[0, 2, 3]].astype(np.float32))
+    assert np.isnan(got[1, :, 32:64]).all() and np.array_equal(got[1, :, :32], want[1, :, :32].astype(np.float32)) and np.array_equal(got[1, :, 64:], want[1, :, 64:].astype(np.float32))
+    p.gpu.free()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
+@pytest.mark.parametrize("off,pad", [(0, 0), (1, 0), (0, 3), (3, 5)])
+def test_rows_anywhere(ctx, pkg, dtype, off, pad):
+    """Rows apart by odd numbers of elements and off 16 bytes: stored, read and attended to as if they were side by side."""
+    kv, dim, heads, n = 2, 64, 6, 37
+    p, r = (Pair(ctx, pkg, np.random.default_rng(15), 1, 3, 16, kv, dim) for _ in range(2))
+    k, v = r.append([n], dtype)
+    width, size, code = kv * dim + pad, np.dtype(dtype).itemsize, pkg.runtime.hipc_dtype(dtype)
+    def strided(x, w):
+        buf = np.full(off + x.shape[0] * w + 8, 7, dtype)
+        for i in range(x.shape[0]):
+            buf[off + i * w:off + i * w + x[i].size] = x[i].reshape(-1)
+        return buf
+    dK, dV, dS = ctx.upload(strided(k, width)), ctx.upload(strided(v, width)), ctx.upload(np.array([0, n], np.int32))
+    p.gpu.set_lengths([n])
+    pkg.ops.kv4_append_device(ctx, p.gpu.cache, code, dS, n, dK.at(off * size), width, dV.at(off * size), width)
+    dB = ctx.upload(strided(np.zeros_like(k), width)), ctx.upload(strided(np.zeros_like(k), width))
+    pkg.ops.kv4_read_device(ctx, p.gpu.cache, code, dS, n, dB[0].at(off * size), width, dB[1].at(off * size), width)
+    for d, want in zip(dB, r.gpu.read([n], dtype)):
+        assert np.array_equal(bits(ctx.download(d, dtype, (off + n * width + 8,))), bits(strided(want, width)))
+    q = np.random.default_rng(16).standard_normal((1, heads, dim)).astype(dtype)
+    w = heads * dim + pad
+    dQ, dY = ctx.upload(strided(q, w)), ctx.upload(strided(np.zeros_like(q), w))
+    pkg.ops.kv4_attention_device(ctx, p.gpu.cache, pkg.AttentionHeads(heads, kv, dim, 1, 0, 0.0), code, 1, dQ.at(off * size), w, dY.at(off * size), w)
+    assert np.array_equal(bits(ctx.download(dY, dtype, (off + w + 8,))), bits(strided(r.gpu.attention(q), w)))
+    for b in (dK, dV, dS, dQ, dY) + dB:
+        b.free()
+    p.gpu.free(), r.gpu.free()
+
+
+def test_many_sequences(ctx, pkg):
+    """More sequences than a wavefront has lanes, most of them empty, and more units than workgroups."""
+    rng = np.random.default_rng(17)
+    seqs = 150
+    lengths = np.where(rng.random(seqs) < 0.5, 0, rng.integers(1, 40, seqs))
+    p = Pair(ctx, pkg, rng, seqs, 3, 16, 2, 32)
+    p.append([int(n) for n in lengths])
+    y = p.check(ctx, pkg, 4, 1, np.float16)
+    assert not y[lengths == 0].any()
+    p.check(ctx, pkg, 34, 2, np.float32)                   # 34 query rows a kv head: three blocks, 450 units and more
+    k, v = p.gpu.read([int(n) for n in lengths])
+    assert np.array_equal(bits(k), bits(p.rows(0, lengths))) and np.array_equal(bits(v), bits(p.rows(1, lengths)))
     p.gpu.free()
 
 
@@ -279,7 +356,7 @@ def test_refusals(ctx, pkg):
         assert rows(fn, head_dim=48) == 2 and rows(fn, head_dim=288) == 2 and rows(fn, head_dim=0) == 2
         assert rows(fn, page_size=8) == 2 and rows(fn, page_size=48) == 2
         assert rows(fn, n_kv_heads=0) == 1 and rows(fn, n_seqs=-1) == 1 and rows(fn, n_pages=-1) == 1 and rows(fn, table_width=-1) == 1
-        assert rows(fn, table_width=1 << 28) == 1
+        assert rows(fn, table_width=1 << 27) == 1
         assert rows(fn, k_codes=None) == 1 and rows(fn, v_params=good["v_params"] + 4) == 1
         assert rows(fn, lengths=None) == 1 and rows(fn, table=None) == 1
         assert rows(fn, starts=None) == 1 and rows(fn, k=None) == 1 and rows(fn, k=d.ptr + 1) == 1

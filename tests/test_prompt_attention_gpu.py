@@ -193,7 +193,7 @@ def test_refusals(ctx, pkg):
     assert call(q=None) == 1 and call(y=None) == 1 and call(starts=None) == 1
     assert call(qs=127) == 1 and call(ks=63) == 1
     assert call(q=d.ptr + 1) == 1 and call(starts=d.ptr + 2) == 1
-    assert call(total=-1) == 1 and call(n=-1) == 1 and call(total=1 << 31) == 1
+    assert call(total=-1) == 1 and call(n=-1) == 1 and call(total=(1 << 30) + 1) == 1
     assert b"hipc_prompt_attention" in ctx.lib.hipc_last_error(ctx.handle)
     assert call(n=0) == 0 and call(total=0) == 0           # nothing to do
     d.free()

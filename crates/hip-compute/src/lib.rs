@@ -20,7 +20,7 @@ use std::ffi::{CStr, CString};
 use std::os::raw::{c_int, c_void};
 use std::ptr;
 
-pub use sys::{hipc_conv_geom as ConvGeom, hipc_decoder_config as DecoderConfig};
+pub use sys::{hipc_attention_heads as AttentionHeads, hipc_conv_geom as ConvGeom, hipc_decoder_config as DecoderConfig, hipc_kv4_cache as Kv4Cache, HIPC_TOP_MAX};
 
 /// What went wrong, in the interpreter's terms.
 #[derive(Clone, Copy, Debug, PartialEq, Eq)]
@@ -200,6 +200,24 @@ pub struct ScaleBias<'a> {
 pub struct QParams {
     pub scale: f32,
     pub zero_point: i32,
+}
+
+/// The rows of an attention operand: a region and the elements from one row to the next.
+#[derive(Clone, Copy, Debug)]
+pub struct Rows<'a> {
+    pub at: BufferSlice<'a>,
+    pub stride: i64,
+}
+
+/// What `token_logprobs` writes; what is `None` is not computed.
+#[derive(Clone, Copy, Debug, Default)]
+pub struct TokenLogprobs<'a> {
+    /// the given tokens (i32 per row) and where their log-probabilities go (f32 per row)
+    pub given: Option<(BufferSlice<'a>, BufferSlice<'a>)>,
+    /// f32 per row
+    pub entropy: Option<BufferSlice<'a>>,
+    /// the most likely ids and their log-probabilities ([rows, top] i32 and f32), and how many (up to `HIPC_TOP_MAX`)
+    pub top: Option<(BufferSlice<'a>, BufferSlice<'a>, i32)>,
 }
 
 /// One process-wide runtime object, like `VkContext` (`crates/vk-compute/src/lib.rs:16-20`).
@@ -568,6 +586,46 @@ impl HipContext {
         })
     }
 
+    // ------------------------- attention over prompts and a cache in 4 bits
+
+    /// Prompts of different lengths packed one behind the other (`GroupQueryAttention`'s prompt form, interp.rs:7514-7949):
+    /// `q` [total_q, n_q_heads, head_dim], `k` / `v` [total_k, n_kv_heads, head_dim], `y` like `q`, all of `dtype`; the starts
+    /// [n_seqs + 1] i32 lie on the device.
+    pub fn prompt_attention(
+        &self, heads: &AttentionHeads, dtype: DType, q: Rows<'_>, k: Rows<'_>, v: Rows<'_>, q_starts: BufferSlice<'_>, k_starts: BufferSlice<'_>,
+        n_seqs: i64, total_q: i64, total_k: i64, y: Rows<'_>,
+    ) -> Result<()> {
+        self.check(unsafe {
+            sys::hipc_prompt_attention(
+                self.raw, heads, dtype.raw(), q.at.ptr(), q.stride, k.at.ptr(), k.stride, v.at.ptr(), v.stride, q_starts.ptr(), k_starts.ptr(),
+                n_seqs, total_q, total_k, y.at.ptr(), y.stride,
+            )
+        })
+    }
+    /// Store the rows of `k` and `v` as the last positions of their sequences (`cache.lengths` counts them already).
+    pub fn kv4_append(&self, cache: &Kv4Cache, dtype: DType, starts: BufferSlice<'_>, total: i64, k: Rows<'_>, v: Rows<'_>) -> Result<()> {
+        self.check(unsafe { sys::hipc_kv4_append(self.raw, cache, dtype.raw(), starts.ptr(), total, k.at.ptr(), k.stride, v.at.ptr(), v.stride) })
+    }
+    /// The values those rows stand for.
+    pub fn kv4_read(&self, cache: &Kv4Cache, dtype: DType, starts: BufferSlice<'_>, total: i64, k: Rows<'_>, v: Rows<'_>) -> Result<()> {
+        self.check(unsafe { sys::hipc_kv4_read(self.raw, cache, dtype.raw(), starts.ptr(), total, k.at.ptr(), k.stride, v.at.ptr(), v.stride) })
+    }
+    /// Attention of the newest `tokens` positions of every sequence over the cache; run one before recording one.
+    pub fn kv4_attention(&self, cache: &Kv4Cache, heads: &AttentionHeads, dtype: DType, tokens: i64, q: Rows<'_>, y: Rows<'_>) -> Result<()> {
+        self.check(unsafe { sys::hipc_kv4_attention(self.raw, cache, heads, dtype.raw(), tokens, q.at.ptr(), q.stride, y.at.ptr(), y.stride) })
+    }
+
+    // ----------------------------------------- probabilities of the answers
+
+    /// Log-probabilities of given tokens, entropies and the most likely alternatives of rows of logits (f16 or f32).
+    pub fn token_logprobs(&self, dtype: DType, logits: Rows<'_>, rows: i64, vocab: i64, out: &TokenLogprobs<'_>) -> Result<()> {
+        let (tokens, logprob) = out.given.map_or((ptr::null_mut(), ptr::null_mut()), |(t, l)| (t.ptr(), l.ptr()));
+        let (ids, probs, top) = out.top.map_or((ptr::null_mut(), ptr::null_mut(), 0), |(i, p, n)| (i.ptr(), p.ptr(), n));
+        self.check(unsafe {
+            sys::hipc_token_logprobs(self.raw, dtype.raw(), logits.at.ptr(), logits.stride, rows, vocab, tokens, logprob, opt_ptr(out.entropy), top as c_int, ids, probs)
+        })
+    }
+
     // ------------------------------------------------------------ decode step
 
     /// Caches, scratch and the `{token, position}` state of one decoder, all on the device.
@@ -747,6 +805,12 @@ impl Decoder<'_> {
         let (mut k, mut v) = (ptr::null_mut(), ptr::null_mut());
         self.ctx.check(unsafe { sys::hipc_decoder_kv_cache(self.ctx.raw, self.raw, layer as c_int, &mut k, &mut v) })?;
         Ok((k, v))
+    }
+    /// Device address of the last step's logits, [vocab] f32 (for `HipContext::token_logprobs` through `GpuBuffer::from_raw`).
+    pub fn logits(&self) -> Result<*mut c_void> {
+        let mut p = ptr::null_mut();
+        self.ctx.check(unsafe { sys::hipc_decoder_logits(self.ctx.raw, self.raw, &mut p) })?;
+        Ok(p)
     }
     /// positions per row of the transposed value cache: max_seq rounded up to a multiple of 64
     pub fn v_stride(&self) -> usize {

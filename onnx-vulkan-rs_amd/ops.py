@@ -410,14 +410,29 @@ def kv4_attention_device(ctx, cache: Kv4Cache, heads: AttentionHeads, dtype, tok
     ctx._check(ctx.lib.hipc_kv4_attention(ctx.handle, cache, heads, dtype, tokens, _ptr(Q), q_stride, _ptr(Y), y_stride))
 
 
+def _rows_match(what, arrays, shapes, dtype):
+    """The device reads every operand by the first one's type and shape."""
+    for x, shape in zip(arrays, shapes):
+        if x.dtype != dtype or x.shape != shape:
+            raise ValueError(f"{what}: {x.dtype} {x.shape} beside {dtype} {shape}")
+
+
+def _starts(what, lengths, n_seqs, rows):
+    n = np.asarray(lengths, np.int64)
+    if n.shape != (n_seqs,) or (n < 0).any() or n.sum() > rows:
+        raise ValueError(f"{what}: lengths {list(lengths)} of {n_seqs} sequences in {rows} rows")
+    return np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+
+
 def prompt_attention(ctx: Context, q, k, v, q_lengths, k_lengths=None, causal=True, window=0, scale=0.0):
     """Attention over packed prompts on numpy operands: ``q [rows, heads, dim]``, ``k`` / ``v [keys, kv heads, dim]``, float16 or
     float32; the lengths of the sequences in rows and in keys (by default the same)."""
     q, k, v = (np.ascontiguousarray(x) for x in (q, k, v))
     if k_lengths is None:
         k_lengths = q_lengths
+    _rows_match("prompt_attention", (k, v), (k.shape[:2] + q.shape[2:],) * 2, q.dtype)
     heads = AttentionHeads(q.shape[1], k.shape[1], q.shape[2], int(causal), window, scale)
-    starts = [np.concatenate([[0], np.cumsum(n)]).astype(np.int32) for n in (q_lengths, k_lengths)]
+    starts = [_starts("prompt_attention", n, len(q_lengths), x.shape[0]) for n, x in ((q_lengths, q), (k_lengths, k))]
     dQ, dK, dV, dqs, dks = (ctx.upload(x) for x in (q, k, v, *starts))
     dY = ctx.upload(np.zeros_like(q))
     row = [x.shape[1] * x.shape[2] for x in (q, k, v)]
@@ -434,8 +449,10 @@ class Kv4Pages:
 
     def __init__(self, ctx: Context, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, table):
         """``table [sequences, width]``: the page numbers of every sequence."""
-        self.ctx, self.n_kv_heads, self.head_dim = ctx, n_kv_heads, head_dim
         table = np.ascontiguousarray(table, np.int32)
+        if table.ndim != 2:
+            raise ValueError(f"Kv4Pages: a table of shape {table.shape}")
+        self.ctx, self.n_kv_heads, self.head_dim, self.n_seqs, self.width = ctx, n_kv_heads, head_dim, *table.shape
         rows = n_pages * n_kv_heads * page_size
         codes, params = np.zeros(rows * head_dim // 2, np.uint8), np.zeros(rows * (head_dim // KV4_GROUP) * 2, np.float16)
         self.buffers = [ctx.upload(x) for x in (codes, params, codes, params)]
@@ -445,15 +462,21 @@ class Kv4Pages:
                               self.table.ptr, table.shape[1])
 
     def set_lengths(self, lengths):
-        self.ctx.upload(np.ascontiguousarray(lengths, np.int32), self.lengths)
+        lengths = np.ascontiguousarray(lengths, np.int32)
+        _rows_match("set_lengths", (lengths,), ((self.n_seqs,),), np.int32)
+        self.ctx.upload(lengths, self.lengths)
 
     def set_table(self, table):
-        self.ctx.upload(np.ascontiguousarray(table, np.int32), self.table)
+        table = np.ascontiguousarray(table, np.int32)
+        _rows_match("set_table", (table,), ((self.n_seqs, self.width),), np.int32)
+        self.ctx.upload(table, self.table)
 
     def append(self, k, v, new):
         """Packed rows ``[sum(new), kv heads, dim]`` become the last ``new[s]`` positions of sequence s (lengths count them already)."""
         k, v = np.ascontiguousarray(k), np.ascontiguousarray(v)
-        dK, dV, ds = self.ctx.upload(k), self.ctx.upload(v), self.ctx.upload(np.concatenate([[0], np.cumsum(new)]).astype(np.int32))
+        _rows_match("append", (k, v), ((k.shape[0], self.n_kv_heads, self.head_dim),) * 2, k.dtype)
+        starts = _starts("append", new, self.n_seqs, k.shape[0])
+        dK, dV, ds = self.ctx.upload(k), self.ctx.upload(v), self.ctx.upload(starts)
         row = self.n_kv_heads * self.head_dim
         kv4_append_device(self.ctx, self.cache, hipc_dtype(k.dtype), ds, k.shape[0], dK, row, dV, row)
         for b in (dK, dV, ds):
@@ -462,8 +485,8 @@ class Kv4Pages:
     def read(self, count, dtype=np.float16):
         """The last ``count[s]`` positions of every sequence, packed: (keys, values)."""
         shape = (int(np.sum(count)), self.n_kv_heads, self.head_dim)
-        zero = np.zeros(shape, dtype)
-        dK, dV, ds = self.ctx.upload(zero), self.ctx.upload(zero), self.ctx.upload(np.concatenate([[0], np.cumsum(count)]).astype(np.int32))
+        starts, zero = _starts("read", count, self.n_seqs, shape[0]), np.zeros(shape, dtype)
+        dK, dV, ds = self.ctx.upload(zero), self.ctx.upload(zero), self.ctx.upload(starts)
         row = self.n_kv_heads * self.head_dim
         kv4_read_device(self.ctx, self.cache, hipc_dtype(np.dtype(dtype)), ds, shape[0], dK, row, dV, row)
         out = self.ctx.download(dK, dtype, shape), self.ctx.download(dV, dtype, shape)
@@ -474,6 +497,7 @@ class Kv4Pages:
     def attention(self, q, tokens=1, window=0, scale=0.0):
         """``q [sequences * tokens, heads, dim]``: the newest tokens of every sequence over its cache."""
         q = np.ascontiguousarray(q)
+        _rows_match("attention", (q,), ((self.n_seqs * tokens, q.shape[1], self.head_dim),), q.dtype)
         heads = AttentionHeads(q.shape[1], self.n_kv_heads, self.head_dim, 1, window, scale)
         dQ, dY = self.ctx.upload(q), self.ctx.upload(np.zeros_like(q))
         row = q.shape[1] * q.shape[2]
@@ -500,9 +524,10 @@ def token_logprobs_device(ctx, dtype, logits, row_stride, rows, vocab, tokens, l
 def token_logprobs(ctx: Context, logits, tokens, top=0):
     """``logits [rows, vocab]`` float16 or float32, ``tokens [rows]``: (logprob, entropy, ids and log probabilities of the ``top``
     best)."""
-    logits = np.ascontiguousarray(logits)
+    logits, tokens = np.ascontiguousarray(logits), np.ascontiguousarray(tokens, np.int32)
     rows, vocab = logits.shape
-    dX, dT = ctx.upload(logits), ctx.upload(np.ascontiguousarray(tokens, np.int32))
+    _rows_match("token_logprobs", (tokens,), ((rows,),), np.int32)
+    dX, dT = ctx.upload(logits), ctx.upload(tokens)
     dL, dE = ctx.alloc(max(4 * rows, 4)), ctx.alloc(max(4 * rows, 4))
     dI, dP = (ctx.alloc(4 * rows * top), ctx.alloc(4 * rows * top)) if rows * top else (None, None)
     token_logprobs_device(ctx, hipc_dtype(logits.dtype), dX, vocab, rows, vocab, dT, dL, dE, top, dI, dP)

@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tile
 // another before the end. The keys' half of that LDS is free for the next tile once they are multiplied, the values' half once those are; both are
 // asked for then, and waited for by count (loads end in the order they were issued in).
 template <int HD>
-__global__ void __launch_bounds__(256, HD > 128 ? 1 : 2) prompt_few_kernel(const PromptArgs a) {
+__global__ void __launch_bounds__(256, 2) prompt_few_kernel(const PromptArgs a) {
     constexpr int W = 4, KT = 32, PITCH = HD <= 64 ? 64 : HD <= 128 ? 128 : 256, TILE = KT * PITCH * 2;
     constexpr int SUMS = W * HD * 32 * 4;
     __shared__ __attribute__((aligned(1024))) char smem[2 * W * TILE > SUMS ? 2 * W * TILE : SUMS];   // [wavefront][K, V]; at last the sums
@@ -729,33 +729,63 @@ __global__ void __launch_bounds__(64 * W, W == 2 || (HD > 128 && W == 4) ? 1 : 2
     prompt_rows_out<float, HC>(a, pt, pr, h, c0, m, l, o);
 }
 
-// The ranges of keys that several workgroups had of the same rows, joined: one wavefront per row and head.
-template <typename T>
+// The ranges of keys that several workgroups had of the same rows, joined: four channels of a row and head per thread. What a range counts for and its
+// part are on their way together, AT_ONCE ranges at a time, and rows are looked up meanwhile. (Looked up, weighed and read one behind the other,
+// 31 ranges of 64 rows of four heads of 256 took 40 us of the call's 54.)
+template <typename T, int AT_ONCE>
 __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int row = __builtin_amdgcn_readfirstlane((int)(w / a.n_q_heads)), head = __builtin_amdgcn_readfirstlane((int)(w % a.n_q_heads));
-    if (row >= a.total_q) return;
-    int seq, first, end;
-    if (!packed_sequence(a.q_starts, a.n_seqs, a.total_q, row, &seq, &first, &end)) return;
+    const int quads = a.dim / 4;
+    const int64_t rows = (int64_t)a.total_q * a.n_q_heads, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const bool in = at < rows * quads;
+    const int64_t of = in ? at / quads : rows - 1;   // row and head, as in the parts
+    const int c = in ? (int)(at - of * quads) * 4 : 0, row = (int)(of / a.n_q_heads), head = (int)(of - (int64_t)row * a.n_q_heads);
     float m = -INFINITY, l = 0.f;
-    for (int z = 0; z < a.splits; z++) m = fmaxf(m, a.part_ml[2 * prompt_part(a, z, row, head)]);
-    float acc[kPromptMaxHead / 64] = {};
-    for (int z = 0; z < a.splits; z++) {
-        const size_t part = prompt_part(a, z, row, head);
-        const float pm = a.part_ml[2 * part], pl = a.part_ml[2 * part + 1];
-        if (pl == 0.f) continue;   // the range has nothing the row sees
-        const float keep = pm == m ? 1.f : __builtin_amdgcn_exp2f(pm - m);
-        l += pl * keep;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto join = [&](int z0, const float2 (&ml)[AT_ONCE], const float4 (&o)[AT_ONCE]) {
+        float most = m;
 #pragma unroll
-        for (int i = 0; i < kPromptMaxHead / 64; i++)
-            if (lane + 64 * i < a.dim) acc[i] += keep * a.part_o[part * a.dim + lane + 64 * i];
+        for (int e = 0; e < AT_ONCE; e++)
+            if (z0 + e < a.splits && ml[e].y != 0.f) most = fmaxf(most, ml[e].x);
+        const float before = m == most ? 1.f : __builtin_amdgcn_exp2f(m - most);
+        m = most;
+        if (l != 0.f) l *= before, acc.x *= before, acc.y *= before, acc.z *= before, acc.w *= before;
+#pragma unroll
+        for (int e = 0; e < AT_ONCE; e++) {
+            if (z0 + e >= a.splits || ml[e].y == 0.f) continue;   // (the range has nothing the row sees, and its part may hold anything)
+            const float keep = ml[e].x == m ? 1.f : __builtin_amdgcn_exp2f(ml[e].x - m);
+            l = __builtin_fmaf(ml[e].y, keep, l);
+            acc.x = __builtin_fmaf(keep, o[e].x, acc.x), acc.y = __builtin_fmaf(keep, o[e].y, acc.y);
+            acc.z = __builtin_fmaf(keep, o[e].z, acc.z), acc.w = __builtin_fmaf(keep, o[e].w, acc.w);
+        }
+    };
+    float2 ml[AT_ONCE];
+    float4 o[AT_ONCE];
+    auto load = [&](int z0) {
+#pragma unroll
+        for (int e = 0; e < AT_ONCE; e++) {
+            const int64_t part = min(z0 + e, a.splits - 1) * rows + of;
+            ml[e] = reinterpret_cast<const float2 *>(a.part_ml)[part];
+            o[e] = *reinterpret_cast<const float4 *>(a.part_o + part * a.dim + c);
+        }
+    };
+    load(0);
+    // (a wavefront's lanes may lie in several rows)
+    bool mine = false;
+    const int last = __builtin_amdgcn_readlane(row, 63);
+    for (int r = __builtin_amdgcn_readfirstlane(row); r <= last; r++) {
+        int seq, first, end;
+        const bool has = packed_sequence(a.q_starts, a.n_seqs, a.total_q, r, &seq, &first, &end);
+        mine |= has && r == row;
     }
+    join(0, ml, o);
+    for (int z = AT_ONCE; z < a.splits; z += AT_ONCE) {
+        load(z);
+        join(z, ml, o);
+    }
+    if (!in || !mine) return;
+    typedef T T4 __attribute__((ext_vector_type(4)));
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    T *y = static_cast<T *>(a.y) + a.y_stride * row + (int64_t)head * a.dim;
-#pragma unroll
-    for (int i = 0; i < kPromptMaxHead / 64; i++)
-        if (lane + 64 * i < a.dim) y[lane + 64 * i] = (T)(acc[i] * inv);
+    *reinterpret_cast<T4 *>(static_cast<T *>(a.y) + a.y_stride * row + (int64_t)head * a.dim + c) = T4{(T)(acc.x * inv), (T)(acc.y * inv), (T)(acc.z * inv), (T)(acc.w * inv)};
 }
 
 size_t prompt_parts_bytes(const PromptArgs &a, int splits) { return splits > 1 ? (size_t)splits * a.total_q * a.n_q_heads * (a.dim + 2) * 4 : 0; }
@@ -777,41 +807,54 @@ int prompt_launch(hipc_ctx *ctx, PromptArgs a, int splits) {
     else hipLaunchKernelGGL((prompt_terms_kernel<HD, W>), grid, 64 * W, 0, ctx->stream, a);
     HIPC_LAUNCHED(ctx);
     if (splits > 1) {
-        hipLaunchKernelGGL((prompt_join_kernel<T>), (unsigned)ceil_div((int64_t)a.total_q * a.n_q_heads, 4), 256, 0, ctx->stream, a);
+        const unsigned threads = (unsigned)ceil_div((int64_t)a.total_q * a.n_q_heads * a.dim / 4, 256);
+        if (splits <= 4) hipLaunchKernelGGL((prompt_join_kernel<T, 4>), threads, 256, 0, ctx->stream, a);
+        else hipLaunchKernelGGL((prompt_join_kernel<T, 8>), threads, 256, 0, ctx->stream, a);
         HIPC_LAUNCHED(ctx);
     }
     return HIPC_OK;
 }
 
 // How many wavefronts a workgroup has, and how many workgroups share the keys of a tile of rows. Both go by what the host knows:
-// rows, keys and sequences in all. Measured (us, 2 / 4 / 8 wavefronts): 8192 rows in one sequence, 32 query and 8 kv heads of 128, f16
-// 886 / 618 / 604; eight sequences of up to 1024 85 / 63 / 72 (the longest sequence's last tiles end the launch); two of up to 1500 in f32, whose
-// tiles are split once for all wavefronts, 357 / 265 / 236. Sharing keys costs a join and pays while CUs are left: 16 rows behind 8000 keys
-// 210 alone, 36 shared by 16; 2000 rows of four heads of 256 seeing 512 keys 46 alone, 34 by four, 52 by sixteen.
+// rows, keys and sequences in all. Measured in us, inputs not in the caches nearest the CUs, heads 32 / 8 of 128 in f16 unless said.
+// Wavefronts (2 / 4 / 8): 8192 rows in one sequence 886 / 618 / 604; eight sequences of up to 1024 86 / 62 / 63 (the longest sequence's last tiles
+// end the launch); two of up to 1500 in f32, whose tiles are split once for all wavefronts, 357 / 265 / 236.
+// The kernel for few rows against the better of 2 and 4 wavefronts: 16 rows behind 4000 keys 15 / 17, 60 20 / 23, 500 alone 11 / 18; 200 seeing 512 keys 12 / 20;
+// past 512 workgroups it loses: four prompts of up to 400 22 / 17. Channels up to 64 carry it to twice as many (two prompts of up to 1000, 14 / 2 heads 13 / 20);
+// wider than 128, its 32 rows a workgroup take in the keys too often (two pieces of 1000 that see 512 keys, 4 / 1 heads of 256: 33 / 25).
+// Sharing keys costs the parts' way out and back and a join, and pays while CUs are left and there are keys enough (alone / 2 / 4 / 8 / 16):
+// 64 rows behind 4000 keys, 4 / 1 heads of 256 173 / 94 / 52 / 32 / 23; 600 rows behind 4000 keys 100 / 82 / 79; 600 that see 512 21 / 30 / 32.
 template <typename T>
 int prompt_matrix(hipc_ctx *ctx, const PromptArgs &a) {
     const int64_t rows = (int64_t)a.total_q * a.group, kv = a.n_q_heads / a.group, cus = ctx->cu_count;
     const int shared = a.dim > 128 ? 2 : 1;   // wavefronts of a row
     int waves = rows <= 64 * (int64_t)a.n_seqs ? 2 * shared : 4;
     if (waves == 4 && rows * kv * shared >= 256 * cus * (sizeof(T) == 2 ? 4 : 1)) waves = 8;
-    if (sizeof(T) == 2 && std::max<int64_t>(ceil_div(rows, 32), a.n_seqs) * kv <= 2 * cus) waves = 1;
+    if (sizeof(T) == 2 && a.dim <= 128 && std::max<int64_t>(ceil_div(rows, 32), a.n_seqs) * kv <= (a.dim <= 64 ? 4 : 2) * cus) waves = 1;
     if (ctx->tune.prompt_waves > 0) waves = ctx->tune.prompt_waves;
-    if (sizeof(T) != 2) waves = std::max(waves, 2);
+    if (sizeof(T) != 2 || a.dim > 128) waves = std::max(waves, 2);
     const int tile_rows = waves == 1 ? 32 : 32 * waves / shared;
     const int64_t groups = std::max<int64_t>(ceil_div(rows, tile_rows), a.n_seqs) * kv;
     int64_t keys = a.total_k / a.n_seqs;
     if (a.window > 0) keys = std::min<int64_t>(keys, a.window + tile_rows / a.group);
-    const int64_t key_tiles = keys / (waves == 1 ? 128 : sizeof(T) == 2 && a.dim <= 128 ? 64 : 32);
-    int splits = groups < cus ? (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / groups, key_tiles / (waves == 1 ? 8 : 4), 32})) : 1;
+    const int64_t key_tiles = ceil_div(keys, waves == 1 ? 128 : sizeof(T) == 2 && a.dim <= 128 ? 64 : 32);
+    // us: a tile of keys 1.2 (f32: 4), the join 4, and for each range its part out and in, at 4.4 TB/s, and its start
+    const double tile = sizeof(T) == 2 ? 1.2 : 4.0, part = (double)a.total_q * a.n_q_heads * a.dim * 4 / 2.2e6 + 0.15;
+    int splits = 1;
+    double best = tile * key_tiles;
+    for (int s = 2; s <= std::min<int64_t>(32, key_tiles) && s * groups <= 2 * cus && groups < cus; s++) {
+        const double time = tile * ceil_div(key_tiles, s) + 4.0 + s * part;
+        if (time < best) best = time, splits = s;
+    }
     if (ctx->tune.prompt_split > 0) splits = std::min(ctx->tune.prompt_split, 256);
     if (!scratch_fits(ctx, kScratchPrompt, prompt_parts_bytes(a, splits))) splits = 1;
     auto launch = [&](auto width) -> int {
         constexpr int HD = decltype(width)::value;
         if (waves >= 8) return prompt_launch<T, HD, 8>(ctx, a, splits);
         if (waves >= 4) return prompt_launch<T, HD, 4>(ctx, a, splits);
-        if (waves >= 2 || sizeof(T) != 2) return prompt_launch<T, HD, 2>(ctx, a, splits);
-        if constexpr (sizeof(T) == 2) return prompt_launch<T, HD, 1>(ctx, a, splits);
-        return HIPC_OK;
+        if constexpr (sizeof(T) == 2 && HD <= 128)
+            if (waves == 1) return prompt_launch<T, HD, 1>(ctx, a, splits);
+        return prompt_launch<T, HD, 2>(ctx, a, splits);
     };
     return a.dim <= 64 ? launch(std::integral_constant<int, 64>()) : a.dim <= 128 ? launch(std::integral_constant<int, 128>()) : launch(std::integral_constant<int, 256>());
 }
@@ -848,7 +891,7 @@ int hipc_prompt_attention(hipc_ctx *ctx, const hipc_attention_heads *heads, int 
         const int64_t unit = dtype == HIPC_F16 ? 8 : 4;   // elements of 16 bytes
         if (heads->head_dim % 8 == 0 && heads->head_dim <= 256 && aligned(Q, 16) && aligned(K, 16) && aligned(V, 16) && aligned(Y, 16) && q_stride % unit == 0 &&
             k_stride % unit == 0 && v_stride % unit == 0 && y_stride % unit == 0 && k_stride <= 1 << 23 && v_stride <= 1 << 23 &&
-            grid_fits((total_q * a.group / 32 + n_seqs + 1) * heads->n_kv_heads, 512) && grid_fits(ceil_div(total_q * heads->n_q_heads, 4), 256))
+            grid_fits((total_q * a.group / 32 + n_seqs + 1) * heads->n_kv_heads, 512) && grid_fits(ceil_div(total_q * qw, 1024), 256))
             return dtype == HIPC_F16 ? prompt_matrix<_Float16>(ctx, a) : prompt_matrix<float>(ctx, a);
         HIPC_REFUSE(ctx, !grid_fits(total_q, 64), "%s: %lld rows: too many for one call of such heads", who, (long long)total_q);
         const dim3 grid((unsigned)total_q, heads->n_q_heads);

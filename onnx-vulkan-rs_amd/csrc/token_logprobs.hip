@@ -16,6 +16,7 @@ constexpr int kLogWaves = 4;
 constexpr int kLogChunk = 1024;       // logits a wavefront holds at a time: 16 a lane
 constexpr int kLogWorkgroups = 512;   // at most that many share rows
 constexpr int kLogParts = 64;         // ... a row
+constexpr int kLogHeld = 4;           // chunks that a wavefront's registers hold
 constexpr int kLogBuffer = 256;       // candidates a wavefront ranks at a time
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -30,13 +31,15 @@ struct LogprobArgs {
     uint32_t *arrived;       // [row], zero between calls
 };
 
+// of a row that begins `head` elements behind 16 aligned bytes
+__host__ __device__ inline int log_chunks(int vocab, int head, int vec) { return (int)(((int64_t)vocab + head + vec - 1) / vec + kLogChunk / vec - 1) / (kLogChunk / vec); }
+
 // What a stretch of a row amounts to: its largest value m, sum of e = exp(x - m), and sum of e log2(e).
 struct LogSum {
     float m, l, w;
 };
 struct LogPart {
-    LogSum sum;
-    uint32_t pad;
+    LogSum sum[kLogWaves];
     uint64_t best[kLogWaves][HIPC_TOP_MAX];   // of each wavefront: keys, largest first; 0 where there are fewer
 };
 
@@ -82,8 +85,15 @@ __device__ __forceinline__ uint32_t wave_least(uint32_t v) {
     auto lane = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
     return min(min(lane(0), lane(16)), min(lane(32), lane(48)));
 }
-// the largest whole number that at least `top` of the lanes' are at or above: the least of those that fewer than `top` are above
+__device__ __forceinline__ uint32_t wave_most(uint32_t v) { return ~wave_least(~v); }
+// The largest whole number that at least `top` of the lanes' are at or above (lanes with 0 have none: 0 where there are fewer). The lanes' numbers are
+// gone through from the largest on while that takes fewer steps than to count, for every lane, those above it.
 __device__ __forceinline__ uint32_t log_reach(uint32_t v, int top) {
+    if (top <= 6) {
+        uint32_t most = wave_most(v);
+        while (most != 0 && __popcll(__ballot(v >= most)) < top) most = wave_most(v < most ? v : 0u);
+        return most;
+    }
     int above = 0;
 #pragma unroll 16
     for (int j = 0; j < 64; j++) above += (uint32_t)__builtin_amdgcn_readlane((int)v, j) > v;
@@ -111,6 +121,32 @@ __device__ __forceinline__ uint64_t log_rank(int top, LogBuffer &buffer, int cou
     return lane < top ? buffer.ranked[lane] : 0;
 }
 constexpr int kLogRoom = kLogBuffer - 16;
+// The `top` largest keys of the wavefronts' lists, each sorted and with zeros behind its last: a key's rank is its place in its own list and, by
+// halving, the number of larger ones in the others.
+__device__ __forceinline__ uint64_t log_lists(int top, LogBuffer &buffer, const uint64_t (&lists)[kLogWaves][HIPC_TOP_MAX]) {
+    static_assert(HIPC_TOP_MAX == 32 && kLogWaves == 4, "two lists a wavefront's lanes");
+    const int lane = threadIdx.x & 63, place = lane & 31, own = lane >> 5;
+    uint64_t k[2];
+    int larger[2][3] = {};
+#pragma unroll
+    for (int r = 0; r < 2; r++) k[r] = lists[2 * r + own][place];
+    if (lane < top) buffer.ranked[lane] = 0;
+#pragma unroll
+    for (int s = 0; s < 6; s++) {
+        const int step = s == 5 ? 1 : 16 >> s;
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+#pragma unroll
+            for (int o = 0; o < 3; o++)
+                if (lists[(2 * r + own + 1 + o) & 3][larger[r][o] + step - 1] > k[r]) larger[r][o] += step;
+    }
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const int rank = place + larger[r][0] + larger[r][1] + larger[r][2];
+        if (k[r] != 0 && rank < top) buffer.ranked[rank] = k[r];
+    }
+    return lane < top ? buffer.ranked[lane] : 0;
+}
 
 struct LogBest {
     int count = 0;
@@ -134,13 +170,13 @@ struct LogBest {
     template <int N, typename Id>
     __device__ __forceinline__ void scan(int top, LogBuffer &buffer, float largest, const float (&x)[N], Id id) {
         const int lane = threadIdx.x & 63;
-#pragma unroll
-        for (int i = 0; i < N; i++) buffer.stage[64 * i + lane] = x[i];
         bool tight = false;   // the bar is this chunk's own
         if (least == 0) {
             raise(log_reach((uint32_t)(log_key(largest, 0) >> 32), top));
             tight = true;
         }
+#pragma unroll
+        for (int i = 0; i < N; i++) buffer.stage[64 * i + lane] = x[i];
         for (;;) {
             uint32_t pass = 0;
 #pragma unroll
@@ -239,16 +275,13 @@ __device__ __forceinline__ LogSum log_join(const LogSum &a, const LogSum &b) {
     return {m, (a.l == 0.f ? 0.f : a.l * fa) + (b.l == 0.f ? 0.f : b.l * fb), wa + wb};
 }
 
-template <typename T>
-__device__ void log_finish(const LogprobArgs &a, int64_t row, const LogSum &s, uint64_t list) {
+// `token` is the row's given one and `given` its logit
+__device__ __forceinline__ void log_finish(const LogprobArgs &a, int64_t row, int token, float given, const LogSum &s, uint64_t list) {
     const int lane = threadIdx.x & 63;
     // no finite largest value: no distribution (a NaN among the logits has made l one; +inf too, by inf - inf)
     const float log_l = logf(s.l), lse = s.m == -INFINITY ? NAN : s.m + log_l;
     if (lane == 0) {
-        if (a.logprob) {
-            const int t = a.tokens[row];
-            a.logprob[row] = t == -1 ? 0.f : t < 0 || t >= a.vocab ? NAN : (float)static_cast<const T *>(a.x)[row * a.row_stride + t] - lse;
-        }
+        if (a.logprob) a.logprob[row] = token == -1 ? 0.f : token < 0 || token >= a.vocab ? NAN : given - lse;
         if (a.entropy) a.entropy[row] = s.m == -INFINITY ? NAN : log_l - kLn2 * (s.w / s.l);
     }
     if (lane < a.top) {
@@ -257,10 +290,12 @@ __device__ void log_finish(const LogprobArgs &a, int64_t row, const LogSum &s, u
     }
 }
 
-// A row is read once, by a.parts workgroups; a wavefront streams 1024 logits at a time, the next ones on their way meanwhile, with a running
+// A row is read once, by a.parts workgroups. A wavefront streams 1024 logits at a time, the next ones on their way meanwhile, with a running
 // maximum and sums per lane and without a barrier. The alternatives cost a comparison per logit; only where one passes the list's last is there
-// more to do, which after the first few thousand logits is rare.
-template <typename T>
+// more to do, which after the first few thousand logits is rare. HELD: a wavefront's share is kLogHeld chunks at most; they are on their way together
+// and stay in registers, so that one bar, of them all, is there before the first is compared (64 rows of 100003 in f16: with the
+// five best 15.5 us, 16.4 streamed; with twenty 19.1 and 21.3).
+template <typename T, bool HELD>
 __global__ void __launch_bounds__(64 * kLogWaves, 4) logprob_kernel(const LogprobArgs a) {
     constexpr int VEC = 16 / sizeof(T), LOADS = kLogChunk / 64 / VEC;
     typedef T TV __attribute__((ext_vector_type(VEC)));
@@ -276,14 +311,16 @@ __global__ void __launch_bounds__(64 * kLogWaves, 4) logprob_kernel(const Logpro
     // the row in pieces of 16 aligned bytes: the first and the last may hold less of it
     const T *x = static_cast<const T *>(a.x) + row * a.row_stride;
     const int head = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-    const int pieces = (int)(((int64_t)a.vocab + head + VEC - 1) / VEC);
-    const int chunks = (pieces + 64 * LOADS - 1) / (64 * LOADS);
+    const int chunks = log_chunks(a.vocab, head, VEC);
     const int per = (chunks + a.parts * kLogWaves - 1) / (a.parts * kLogWaves);   // of a wavefront, one behind the other
     const int c0 = (part * kLogWaves + wave) * per, c1 = min(c0 + per, chunks);
 
+    // the given token's logit, which any workgroup may turn out to need at the end, is on its way with the others
+    const int token = a.logprob ? a.tokens[row] : -1;
+    float given = token >= 0 && token < a.vocab ? (float)x[token] : 0.f;
+
     float m = -INFINITY, l = 0.f, w = 0.f;
     LogBest best;
-    TV now[LOADS], next[LOADS] = {};
     // (below 2^31: the vocabulary is at most 2^30)
     auto first_of = [&](int chunk) { return (chunk * LOADS * 64 + lane) * VEC - head; };
     auto load = [&](int chunk, TV (&v)[LOADS]) {
@@ -304,20 +341,15 @@ __global__ void __launch_bounds__(64 * kLogWaves, 4) logprob_kernel(const Logpro
             }
         }
     };
-    if (c0 < c1) load(c0, now);
-    for (int c = c0; c < c1; c++) {
-        if (c + 1 < c1) load(c + 1, next);
-        const int first = first_of(c);
+    auto largest = [&](const TV (&v)[LOADS]) {
         float most = -INFINITY;
 #pragma unroll
         for (int e = 0; e < LOADS; e++)
 #pragma unroll
-            for (int j = 0; j < VEC; j++) most = fmaxf(most, (float)now[e][j]);
-        if (most > m) {
-            const float f = l == 0.f ? 0.f : __builtin_amdgcn_exp2f((m - most) * kLog2e);
-            w = f == 0.f ? 0.f : f * __builtin_fmaf(l, (m - most) * kLog2e, w), l *= f;
-            m = most;
-        }
+            for (int j = 0; j < VEC; j++) most = fmaxf(most, (float)v[e][j]);
+        return most;
+    };
+    auto add = [&](const TV (&v)[LOADS]) {
         const float shift = m == -INFINITY ? 0.f : m;   // (subtracted before the scaling: a row at its type's lowest value times log2 e would be an infinity)
         float l2 = 0.f, w2 = 0.f;
 #pragma unroll
@@ -325,74 +357,110 @@ __global__ void __launch_bounds__(64 * kLogWaves, 4) logprob_kernel(const Logpro
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
                 // (a masked logit: t = -inf, its exponential 0, and 0 times the held t; a NaN stays one through the exponential)
-                const float t = ((float)now[e][j] - shift) * kLog2e, y = __builtin_amdgcn_exp2f(t);
+                const float t = ((float)v[e][j] - shift) * kLog2e, y = __builtin_amdgcn_exp2f(t);
                 l2 += y, w2 = __builtin_fmaf(y, fmaxf(t, -200.f), w2);
             }
         l += l2, w += w2;
-        if (a.top > 0 && __any(most >= best.bar)) {
-            float values[LOADS * VEC];
+    };
+    auto look = [&](int chunk, float most, const TV (&v)[LOADS]) {
+        if (!__any(most >= best.bar)) return;
+        const int first = first_of(chunk);
+        float values[LOADS * VEC];
 #pragma unroll
-            for (int i = 0; i < LOADS * VEC; i++) values[i] = (float)now[i / VEC][i % VEC];
-            best.scan(a.top, buffer, most, values, [&](int i) -> int {
-                const int at = first + i / VEC * 64 * VEC + i % VEC;
-                return at >= 0 && at < a.vocab ? at : -1;
-            });
+        for (int i = 0; i < LOADS * VEC; i++) values[i] = (float)v[i / VEC][i % VEC];
+        best.scan(a.top, buffer, most, values, [&](int i) -> int {
+            const int at = first + i / VEC * 64 * VEC + i % VEC;
+            return at >= 0 && at < a.vocab ? at : -1;
+        });
+    };
+    if constexpr (HELD) {
+        TV held[kLogHeld][LOADS];
+        float most[kLogHeld];
+#pragma unroll
+        for (int i = 0; i < kLogHeld; i++)
+            if (c0 + i < c1) load(c0 + i, held[i]);
+#pragma unroll
+        for (int i = 0; i < kLogHeld; i++) {
+            most[i] = c0 + i < c1 ? largest(held[i]) : -INFINITY;
+            m = fmaxf(m, most[i]);
         }
 #pragma unroll
-        for (int e = 0; e < LOADS; e++) now[e] = next[e];
+        for (int i = 0; i < kLogHeld; i++)
+            if (c0 + i < c1) add(held[i]);
+        if (a.top > 0) {
+            best.raise(log_reach((uint32_t)(log_key(m, 0) >> 32), a.top));
+#pragma unroll
+            for (int i = 0; i < kLogHeld; i++)
+                if (c0 + i < c1) look(c0 + i, most[i], held[i]);
+        }
+    } else {
+        TV now[LOADS], next[LOADS] = {};
+        if (c0 < c1) load(c0, now);
+        for (int c = c0; c < c1; c++) {
+            if (c + 1 < c1) load(c + 1, next);
+            const float most = largest(now);
+            if (most > m) {
+                const float f = l == 0.f ? 0.f : __builtin_amdgcn_exp2f((m - most) * kLog2e);
+                w = f == 0.f ? 0.f : f * __builtin_fmaf(l, (m - most) * kLog2e, w), l *= f;
+                m = most;
+            }
+            add(now);
+            if (a.top > 0) look(c, most, now);
+#pragma unroll
+            for (int e = 0; e < LOADS; e++) now[e] = next[e];
+        }
     }
+
+    HIPC_PIN_VGPR(given);
 
     // lanes, then wavefronts
     LogSum s{m, l, w};
     s = log_wave(s);
-    LogPart *mine = a.part + row * a.parts;
-    const bool alone = a.parts == 1;
     uint64_t list = a.top > 0 && best.count > 0 ? log_rank(a.top, buffer, best.count) : 0;
-    if (lane == 0) sums[wave] = s;
-    if (lane < a.top) {
-        if (alone) lists[wave][lane] = list;
-        else __hip_atomic_store(&mine[part].best[wave][lane], list, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the stores are where everyone sees them
-    __syncthreads();
-    if (wave != 0 && (alone || a.top == 0)) return;
-    if (!alone) {
-        // several workgroups: the one that comes last joins what they found
-        if (wave == 0) {
+    if (a.parts == 1) {
+        if (lane == 0) sums[wave] = s;
+        if (lane < HIPC_TOP_MAX) lists[wave][lane] = list;
+        __syncthreads();
+        if (wave != 0) return;
 #pragma unroll 1
-            for (int v = 1; v < kLogWaves; v++) s = log_join(s, sums[v]);
-            if (lane == 0) {
-                auto put = [](float *to, float v) { __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-                put(&mine[part].sum.m, s.m), put(&mine[part].sum.l, s.l), put(&mine[part].sum.w, s.w);
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                last_here = __hip_atomic_fetch_add(a.arrived + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)a.parts - 1;
-            }
-        }
+        for (int v = 1; v < kLogWaves; v++) s = log_join(s, sums[v]);
+    } else {
+        // several workgroups: the one that comes last joins what they found
+        LogPart *all = a.part + row * a.parts;
+        auto put = [](auto *to, auto v) { __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+        LogSum *sum = &all[part].sum[wave];
+        if (lane == 0) put(&sum->m, s.m), put(&sum->l, s.l), put(&sum->w, s.w);
+        if (lane < a.top) put(&all[part].best[wave][lane], list);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the stores are where everyone sees them
+        __syncthreads();
+        if (tid == 0) last_here = __hip_atomic_fetch_add(a.arrived + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)a.parts - 1;
+        if (wave != 0 && a.top == 0) return;
         if (a.top > 0) __syncthreads();
         if (!last_here) return;
-        if (tid == 0) __hip_atomic_store(a.arrived + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next call
+        if (tid == 0) put(a.arrived + row, 0u);   // for the next call
         static_assert(kLogParts * kLogWaves <= 64 * kLogWaves, "a list per thread");
+        LogSum found[kLogWaves];
+        if (wave == 0) {
+#pragma unroll
+            for (int v = 0; v < kLogWaves; v++) found[v] = sum_of_all(&all[min(lane, a.parts - 1)].sum[v]);
+        }
         if (a.top > 0) {
             const bool have = tid < a.parts * kLogWaves;
-            list = log_merge(a.top, buffer, &mine[have ? tid / kLogWaves : 0].best[tid % kLogWaves][0], have);
-            if (lane < a.top) lists[wave][lane] = list;
+            list = log_merge(a.top, buffer, &all[have ? tid / kLogWaves : 0].best[tid % kLogWaves][0], have);
+            if (lane < HIPC_TOP_MAX) lists[wave][lane] = list;
         }
-        s = {-INFINITY, 0.f, 0.f};
         if (wave == 0) {
-            for (int q = lane; q < a.parts; q += 64) s = log_join(s, sum_of_all(&mine[q].sum));
+            s = found[0];
+#pragma unroll
+            for (int v = 1; v < kLogWaves; v++) s = log_join(s, found[v]);
+            if (lane >= a.parts) s = {-INFINITY, 0.f, 0.f};
             s = log_wave(s);
         }
         if (a.top > 0) __syncthreads();
         if (wave != 0) return;
-    } else {
-#pragma unroll 1
-        for (int v = 1; v < kLogWaves; v++) s = log_join(s, sums[v]);
     }
-    if (a.top > 0) {
-        for (int i = lane; i < kLogWaves * a.top; i += 64) buffer.key[i] = lists[i / a.top][i % a.top];
-        list = log_rank(a.top, buffer, kLogWaves * a.top);
-    }
-    log_finish<T>(a, row, s, list);
+    if (a.top > 0) list = log_lists(a.top, buffer, lists);
+    log_finish(a, row, token, given, s, list);
 }
 
 }  // namespace
@@ -434,8 +502,15 @@ int hipc_token_logprobs(hipc_ctx *ctx, int dtype, const void *logits, int64_t ro
         }
         HIPC_REFUSE(ctx, !grid_fits(rows * a.parts, 64 * kLogWaves), "%s: %lld rows: too many for one call", who, (long long)rows);
         const unsigned grid = (unsigned)(rows * a.parts);
-        if (dtype == HIPC_F16) hipLaunchKernelGGL((logprob_kernel<_Float16>), grid, 64 * kLogWaves, 0, ctx->stream, a);
-        else hipLaunchKernelGGL((logprob_kernel<float>), grid, 64 * kLogWaves, 0, ctx->stream, a);
+        auto launch = [&](auto held) {
+            constexpr bool HELD = decltype(held)::value;
+            if (dtype == HIPC_F16) hipLaunchKernelGGL((logprob_kernel<_Float16, HELD>), grid, 64 * kLogWaves, 0, ctx->stream, a);
+            else hipLaunchKernelGGL((logprob_kernel<float, HELD>), grid, 64 * kLogWaves, 0, ctx->stream, a);
+        };
+        // (rows may begin anywhere within 16 bytes)
+        const int vec = dtype == HIPC_F16 ? 8 : 4;
+        if (log_chunks(a.vocab, vec - 1, vec) <= kLogHeld * kLogWaves * a.parts) launch(std::true_type());
+        else launch(std::false_type());
         HIPC_LAUNCHED(ctx);
         return HIPC_OK;
     });

@@ -52,6 +52,31 @@ def test_ties_orders_and_masks(ctx, pkg, dtype, kind):
 
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
+@pytest.mark.parametrize("rows,vocab", [(1, 131077), (300, 9001), (300, 20021), (100, 90001)], ids=["shared", "alone", "alone, streamed", "shared, streamed"])
+@pytest.mark.parametrize("top", [1, 5, 32])
+def test_every_way_through_a_row(ctx, pkg, dtype, rows, vocab, top):
+    """Rows that one workgroup has or several, held in registers or streamed, with values that are equal, few, in order or banned."""
+    rng = np.random.default_rng(top + vocab)
+    i = np.arange(vocab)
+    kinds = [np.full(vocab, -2.5), rng.integers(0, 3, vocab), i / vocab, -i / vocab, rng.standard_normal(vocab),
+             np.where(rng.random(vocab) < 0.999, -np.inf, rng.standard_normal(vocab)), np.where(np.isin(i, (5, vocab // 2, vocab - 1)), 1.0, -np.inf),
+             np.where(rng.random(vocab) < 0.9, np.finfo(dtype).min, rng.standard_normal(vocab)), np.where(i < vocab - 7, 0.0, np.nan), np.full(vocab, -np.inf)]
+    x, tokens = np.stack(kinds).astype(dtype), np.full(len(kinds), 5)
+    with np.errstate(all="ignore"):
+        want = ref.token_logprobs(x, tokens, top)
+        bound = [allowed(x, np.where(np.isfinite(want[j]), want[j], 0.0)) for j in (0, 1, 3)]
+    for first in range(0, len(kinds), min(rows, len(kinds))):
+        pick = (first + np.arange(rows)) % len(kinds)
+        got = pkg.ops.token_logprobs(ctx, x[pick], tokens[pick], top)
+        assert np.array_equal(got[2], want[2][pick]), np.argwhere(got[2] != want[2][pick])[:4]
+        for j, limit in zip((0, 1, 3), bound):
+            w = want[j][pick]
+            assert np.array_equal(np.isnan(got[j]), np.isnan(w)) and np.array_equal(np.isinf(got[j]), np.isinf(w))
+            fine = np.isfinite(w)
+            assert np.all(np.abs(got[j][fine].astype(np.float64) - w[fine]) <= limit[pick][fine])
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
 def test_rows_without_a_distribution(ctx, pkg, dtype):
     """All -inf, a +inf, a NaN, nothing but NaN: NaN, with the ids of what compares; the rows around them are untouched by it."""
     rng = np.random.default_rng(4)

@@ -19,7 +19,7 @@ struct PromptArgs {
     int n_seqs, total_q, total_k, n_q_heads, group, dim, causal, window;
     float scale;
     // on the matrix cores
-    int tiles, splits;         // query tiles at most; workgroups that share the keys of a tile
+    int tiles, splits, by_keys;   // query tiles at most; workgroups that share the keys of a tile; tiles are started in the order of the keys they see
     float *part_o, *part_ml;   // of each: [split][row][head][channel] sums, (maximum, sum) pairs
 };
 constexpr int kScratchPrompt = 3;   // scratch slot of the parts
@@ -84,32 +84,69 @@ typedef __attribute__((address_space(3))) char lds_char;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleAt = 8.f;   // in powers of two
 
-// which rows a workgroup of `rows` query rows of one kv head has: tiles are counted through the sequences in order
+// Which ROWS query rows of one kv head a workgroup has; the tiles are started in the order of `at`.
 struct PromptTile {
     int seq, q0, len_q, k0, keys;   // the sequence's rows of Q and K
     int r0, rows;                   // first row of the tile, rows of the sequence (tokens * group)
 };
-__device__ __forceinline__ bool prompt_tile(const PromptArgs &a, int tile, int rows_per_tile, PromptTile *out) {
-    const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int base = 0; base < a.n_seqs; base += 64) {
-        const int s = min(base + lane, a.n_seqs - 1);
+// what a lane knows of a sequence
+struct PromptLengths {
+    int from, keys_from, len, keys, tiles;
+    __device__ __forceinline__ PromptLengths(const PromptArgs &a, int seq, int rows) {
+        const int s = min(seq, a.n_seqs - 1);
         // (all four on their way together)
         const int q_from = a.q_starts[s], q_to = a.q_starts[s + 1], k_from = a.k_starts[s], k_to = a.k_starts[s + 1];
-        const int from = max(q_from, 0), to = min(q_to, a.total_q), keys_from = max(k_from, 0), keys = max(min(k_to, a.total_k) - keys_from, 0);
-        const int n = base + lane < a.n_seqs && to > from ? ((to - from) * a.group + rows_per_tile - 1) / rows_per_tile : 0;
-        const int sum = wave_scan(n);
+        from = max(q_from, 0), keys_from = max(k_from, 0);
+        const int to = min(q_to, a.total_q);
+        len = seq < a.n_seqs && to > from ? to - from : 0, keys = max(min(k_to, a.total_k) - keys_from, 0);
+        tiles = (len * a.group + rows - 1) / rows;
+    }
+    __device__ __forceinline__ void of_lane(const PromptArgs &a, int l, PromptTile *out) const {
+        out->q0 = __builtin_amdgcn_readlane(from, l);
+        out->len_q = __builtin_amdgcn_readlane(len, l);
+        out->rows = out->len_q * a.group;
+        out->k0 = __builtin_amdgcn_readlane(keys_from, l);
+        out->keys = __builtin_amdgcn_readlane(keys, l);
+    }
+};
+template <int ROWS>
+__device__ __forceinline__ bool prompt_tile(const PromptArgs &a, int at, PromptTile *out) {
+    const int lane = threadIdx.x & 63;
+    if (a.by_keys) {
+        // (64 sequences at most) Tiles that see the most keys first, of all sequences: a lane knows how many tiles of its sequence see more than some number of keys, and the
+        // number below which the wanted one lies is found by halving, in steps of 64 keys. (In the sequences' order the first sequence's last tiles,
+        // as long as any, came last: eight of up to 1024, 32 / 8 heads of 128, 61.5 us and 58.7 this way; four of up to 3000, 14 / 2 heads of 64, 79 and 70.)
+        const PromptLengths s(a, lane, ROWS);
+        const int past = s.keys - s.len;
+        // (j + 1) * ROWS / group + past keys are seen by tile j; the clamp keeps the product within the rows' own count
+        auto above = [&](int level) { return s.tiles - (int)min((uint32_t)s.tiles, (uint32_t)(min(max(64 * level - past, 0), s.len + ROWS) * a.group) / ROWS); };
+        auto all = [&](int n) { return __builtin_amdgcn_readlane(wave_scan(n), 63); };
+        if (at >= all(s.tiles)) return false;
+        int low = -1, high = (int)lean_wave_max((float)((max(s.keys, 0) + ROWS) / 64 + 1)) + 1;   // (rounded up past 2^24)
+        while (high - low > 1) {
+            const int mid = (low + high) / 2;
+            if (all(above(mid)) <= at) high = mid;
+            else low = mid;
+        }
+        const int n = above(high), here = (low < 0 ? s.tiles : above(low)) - n, scan = wave_scan(here);
+        const int rank = at - all(n), l = __builtin_ctzll(__ballot(scan > rank));
+        s.of_lane(a, l, out);
+        out->seq = l;
+        out->r0 = (__builtin_amdgcn_readlane(s.tiles - n - 1 - (rank - (scan - here)), l)) * ROWS;
+        return true;
+    }
+    // the last tiles of a causal sequence are the heaviest
+    const int tile = a.tiles - 1 - at;
+    int before = 0;
+    for (int base = 0; base < a.n_seqs; base += 64) {
+        const PromptLengths s(a, base + lane, ROWS);
+        const int sum = wave_scan(s.tiles);
         const uint64_t over = __ballot(before + sum > tile);
         if (over) {
             const int l = __builtin_ctzll(over);
-            const int first = before + __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l);
+            s.of_lane(a, l, out);
             out->seq = base + l;
-            out->q0 = __builtin_amdgcn_readlane(from, l);
-            out->len_q = __builtin_amdgcn_readlane(to, l) - out->q0;
-            out->rows = out->len_q * a.group;
-            out->r0 = (tile - first) * rows_per_tile;
-            out->k0 = __builtin_amdgcn_readlane(keys_from, l);
-            out->keys = __builtin_amdgcn_readlane(keys, l);
+            out->r0 = (tile - (before + __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(s.tiles, l))) * ROWS;
             return true;
         }
         before += __builtin_amdgcn_readlane(sum, 63);
@@ -376,10 +413,10 @@ __global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tile
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_char *)smem;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-    // the heaviest tiles (the last of a causal sequence) first; kv heads change fastest, so a head stays with its XCDs
+    // the heaviest tiles first; kv heads change fastest, so a head stays with its XCDs
     const int heads = a.n_q_heads / a.group, kvh = (int)(blockIdx.x % heads);
     PromptTile pt;
-    if (!prompt_tile(a, a.tiles - 1 - (int)(blockIdx.x / heads), 32 * W / C, &pt)) return;
+    if (!prompt_tile<32 * W / C>(a, (int)(blockIdx.x / heads), &pt)) return;
     const PromptSpan sp(a, pt, 32 * W / C, KT);
     const PromptRow pr(a, pt, pt.r0 + 32 * (wave / C), lane & 31, kvh);
     const int c0 = C > 1 ? (wave & 1) * HC : 0;   // the wavefront's first channel
@@ -432,7 +469,7 @@ __global__ void __launch_bounds__(256, 2) prompt_few_kernel(const PromptArgs a) 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int heads = a.n_q_heads / a.group, kvh = (int)(blockIdx.x % heads);
     PromptTile pt;
-    if (!prompt_tile(a, a.tiles - 1 - (int)(blockIdx.x / heads), 32, &pt)) return;
+    if (!prompt_tile<32>(a, (int)(blockIdx.x / heads), &pt)) return;
     const PromptSpan sp(a, pt, 32, KT);
     const PromptRow pr(a, pt, pt.r0, lane & 31, kvh);
     const PromptFetch<KT, PITCH, 1> from(a, pt, kvh, 0, lane);
@@ -538,7 +575,7 @@ __global__ void __launch_bounds__(64 * W, W == 2 || (HD > 128 && W == 4) ? 1 : 2
 
     const int heads = a.n_q_heads / a.group, kvh = (int)(blockIdx.x % heads);
     PromptTile pt;
-    if (!prompt_tile(a, a.tiles - 1 - (int)(blockIdx.x / heads), 32 * W / C, &pt)) return;
+    if (!prompt_tile<32 * W / C>(a, (int)(blockIdx.x / heads), &pt)) return;
     const PromptSpan sp(a, pt, 32 * W / C, KT);
     const PromptRow pr(a, pt, pt.r0 + 32 * (wave / C), n, kvh);
     const int c0 = C > 1 ? (wave & 1) * HC : 0;
@@ -795,6 +832,8 @@ template <typename T, int HD, int W>
 int prompt_launch(hipc_ctx *ctx, PromptArgs a, int splits) {
     const int64_t tiles = ceil_div((int64_t)a.total_q * a.group, W == 1 ? 32 : 32 * W / (HD > 128 ? 2 : 1)) + a.n_seqs;   // (at most: a sequence may leave one unfinished)
     a.tiles = (int)tiles, a.splits = splits;
+    // (where all tiles run at once, their order is not worth the microsecond that it takes to find it)
+    a.by_keys = W > 1 && a.causal && a.window == 0 && a.n_seqs > 1 && a.n_seqs <= 64 && tiles * (a.n_q_heads / a.group) > 2 * ctx->cu_count;
     if (splits > 1) {
         const size_t rows = (size_t)splits * a.total_q * a.n_q_heads;
         void *s = nullptr;
@@ -829,7 +868,7 @@ int prompt_matrix(hipc_ctx *ctx, const PromptArgs &a) {
     const int64_t rows = (int64_t)a.total_q * a.group, kv = a.n_q_heads / a.group, cus = ctx->cu_count;
     const int shared = a.dim > 128 ? 2 : 1;   // wavefronts of a row
     int waves = rows <= 64 * (int64_t)a.n_seqs ? 2 * shared : 4;
-    if (waves == 4 && rows * kv * shared >= 256 * cus * (sizeof(T) == 2 ? 4 : 1)) waves = 8;
+    if (waves == 4 && rows * kv * shared >= 256 * cus * (sizeof(T) == 2 ? 4 : 1) && (sizeof(T) != 2 || a.total_k >= 2048 * (int64_t)a.n_seqs)) waves = 8;
     if (sizeof(T) == 2 && a.dim <= 128 && std::max<int64_t>(ceil_div(rows, 32), a.n_seqs) * kv <= (a.dim <= 64 ? 4 : 2) * cus) waves = 1;
     if (ctx->tune.prompt_waves > 0) waves = ctx->tune.prompt_waves;
     if (sizeof(T) != 2 || a.dim > 128) waves = std::max(waves, 2);

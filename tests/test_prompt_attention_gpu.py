@@ -64,6 +64,27 @@ def test_pieces_windows_and_rows_that_see_nothing(ctx, pkg, dtype, q_lengths, k_
         assert causal is False or not got[:23].any()     # positions below 0
 
 
+@pytest.mark.parametrize("dtype,waves,dim,many", [(np.float16, 4, 16, True), (np.float16, 8, 16, False), (np.float16, 4, 136, False), (np.float32, 2, 16, True),
+                                                  (np.float32, 4, 72, False)])
+def test_more_tiles_than_run_at_once(ctx, pkg, dtype, waves, dim, many):
+    """Tiles of all sequences are started in the order of the keys they see: sequences of very different lengths, empty ones, ones behind
+    earlier keys and with fewer keys than rows; every row is there."""
+    rng = np.random.default_rng(dim + many)
+    if many:
+        q_lengths = rng.integers(0, 70, 64)
+        k_lengths = np.where(rng.random(64) < 0.3, q_lengths, np.maximum(q_lengths + rng.integers(-20, 90, 64), 0))
+    else:
+        q_lengths, k_lengths = np.array([0, 700, 1, 333, 0, 64, 1005]), np.array([5, 700, 41, 900, 3, 20, 1134])
+    heads, kv = (40, 40) if dim <= 128 else (56, 28)
+    rows, keys = int(q_lengths.sum()), int(k_lengths.sum())
+    tile = 32 * waves // (2 if dim > 128 else 1)
+    assert (-(-rows * (heads // kv) // tile) + len(q_lengths)) * kv > 2 * 256      # (of 256 CUs)
+    q, k, v = operands(rng, dtype, rows, keys, heads, kv, dim)
+    with ctx.options(HIPC_PROMPT_WAVES=waves):
+        got = pkg.ops.prompt_attention(ctx, q, k, v, q_lengths, k_lengths)
+    check(got, q, k, v, q_lengths, k_lengths)
+
+
 @pytest.mark.parametrize("dtype,dim", [(np.float16, 64), (np.float16, 256), (np.float32, 128), (np.float16, 33)])
 def test_what_a_row_does_not_see_does_not_reach_it(ctx, pkg, dtype, dim):
     """Infinities and NaN in keys and values behind the causal border, in front of the window and in other sequences."""

@@ -1,6 +1,7 @@
 // The 4-bit key/value cache: storing rows (hipc_kv4_append) and reading them back (hipc_kv4_read).
 //
-// Both move bytes: 2 or 4 of a value on the outside, 5 bits in the cache. A wavefront takes 64 units of eight channels of one
+// Both move bytes: 2 or 4 of a value on the outside, 5 bits in the cache, and memory bounds both (of two prompts of up to 8000 rows of 8 heads of 128
+// in f32, 221 MB stored and read in 51 us, 4.3 TB/s; a copy's reading and writing 4.8). A wavefront takes 64 units of eight channels of one
 // packed row (keys and values side by side), so a lane's outside access is 16 or 32 consecutive bytes and its codes one
 // word; four neighbouring lanes hold a group and agree on its range without LDS.
 #include <algorithm>
@@ -32,6 +33,14 @@ __device__ __forceinline__ Kv4Unit kv4_unit(const Kv4Rows &a, int u) {
     return {h, (r - h * per_head) * 8, value};
 }
 
+// Which wavefront of all this one is. Workgroups go round the eight XCDs; numbered so, the rows of an XCD lie side by side, and so do the cache
+// lines that several positions share (a line of codes by two at 128 channels, one of parameters by eight). Two prompts of up to 8000 rows of 8 heads of
+// 128 in f32, stored and read: 53.7 us, in the order of the workgroups 58.1.
+__device__ __forceinline__ int kv4_wave() {
+    const int each = (int)gridDim.x >> 3, b = blockIdx.x, at = b < each << 3 ? (b & 7) * each + (b >> 3) : b;
+    return __builtin_amdgcn_readfirstlane(at * 4 + (threadIdx.x >> 6));
+}
+
 __device__ __forceinline__ float quad_min(float v) {
     v = fminf(v, lean_dpp<0xB1>(v));
     return fminf(v, lean_dpp<0x4E>(v));
@@ -44,7 +53,7 @@ __device__ __forceinline__ float quad_max(float v) {
 // The quantizer's arithmetic is that of exact numbers up to its named roundings. A quotient is formed in f32 (off by less than 2^-17 below 31; beyond,
 // the code is held to 0 or 15 either way) and decides unless it lies within 2^-14 of the border between two codes; then the remainder does, in 64 bits, where the difference and the
 // product of a code (5 bits) and a scale (11) are exact. In 64 bits throughout, the kernel was bound by its 45 instructions a value
-// (16000 rows of 8 heads of 128, f32: 36.8 us, and 26.0 this way, 5.8 TB/s).
+// (two prompts of up to 8000 rows of 8 heads of 128, f32, out of the nearest caches: 36.8 us, and 26.0 this way).
 __device__ __forceinline__ int kv4_code(float x, float lowest, float scale, float inverse) {
     const float q = (x - lowest) * inverse, r = __builtin_rintf(q);
     int c = (int)r;
@@ -57,8 +66,7 @@ __device__ __forceinline__ int kv4_code(float x, float lowest, float scale, floa
 
 template <typename T>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Rows a) {
-    const int w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
-    const int row = w / a.chunks, u = (w - row * a.chunks) * 64 + lane;
+    const int w = kv4_wave(), lane = threadIdx.x & 63, row = w / a.chunks, u = (w - row * a.chunks) * 64 + lane;
     if (row >= a.total) return;
     const bool mine = u < a.units;
     const Kv4Unit unit = kv4_unit(a, mine ? u : 0);
@@ -103,31 +111,47 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Rows a) {
 
 template <typename T>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Rows a) {
-    const int w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
-    const int row = w / a.chunks, u = (w - row * a.chunks) * 64 + lane;
+    const int w = kv4_wave(), lane = threadIdx.x & 63, row = w / a.chunks, u = (w - row * a.chunks) * 64 + lane;
     if (row >= a.total) return;
     int seq, first, end;
     if (!packed_sequence(a.starts, a.cache.n_seqs, a.total, row, &seq, &first, &end)) return;
     const Kv4Place place = kv4_place(a.cache, seq, kv4_length(a.cache, seq) - end + row);
-    if (u >= a.units) return;
-    const Kv4Unit unit = kv4_unit(a, u);
-    kvh2 v[4] = {};
-    if (place.there) {
-        const int64_t r = place.slot + (int64_t)unit.head * a.cache.page_size;
-        const uint32_t codes = *reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(unit.value ? a.cache.v_codes : a.cache.k_codes) +
-                                                                   r * (a.cache.head_dim / 2) + unit.channel / 2);
-        const kvh2 p = static_cast<const kvh2 *>(unit.value ? a.cache.v_params : a.cache.k_params)[r * (a.cache.head_dim / kKv4Group) + unit.channel / kKv4Group];
-        Kv4Unpack()(codes, kvh2{p.x, p.x}, kvh2{p.y, p.y}, v);
-    }
-    typedef T T8 __attribute__((ext_vector_type(8)));
-    const T8 y = {(T)v[0].x, (T)v[1].x, (T)v[2].x, (T)v[3].x, (T)v[0].y, (T)v[1].y, (T)v[2].y, (T)v[3].y};
-    T *to = static_cast<T *>(const_cast<void *>(unit.value ? a.v : a.k)) + (unit.value ? a.v_stride : a.k_stride) * row +
-            (int64_t)unit.head * a.cache.head_dim + unit.channel;
-    if (a.wide) {
-        *reinterpret_cast<T8 *>(to) = y;
-    } else {
+    // Eight values a lane: of f16 a unit, 16 bytes; of f32 two halves of units, 64 lanes apart, so that a store is 1 KiB side by side either way. (The
+    // codes unpack as pairs (i, i + 4): the halves' parameters go with them.)
+    constexpr int HALF = sizeof(T) == 4 ? 2 : 1, N = 8 / HALF;
+    typedef T TN __attribute__((ext_vector_type(N)));
+    T *to[HALF];
+    uint32_t codes = 0;
+    kvh2 p[HALF] = {};
 #pragma unroll
-        for (int i = 0; i < 8; i++) to[i] = y[i];
+    for (int i = 0; i < HALF; i++) {
+        const int at = HALF * (u - lane) + 64 * i + lane, half = HALF > 1 ? at & 1 : 0;   // in halves where there are such
+        to[i] = nullptr;
+        if (at >= HALF * a.units) continue;
+        const Kv4Unit unit = kv4_unit(a, HALF > 1 ? at >> 1 : at);
+        to[i] = static_cast<T *>(const_cast<void *>(unit.value ? a.v : a.k)) + (unit.value ? a.v_stride : a.k_stride) * row +
+                (int64_t)unit.head * a.cache.head_dim + unit.channel + 4 * half;
+        if (!place.there) continue;
+        const int64_t r = place.slot + (int64_t)unit.head * a.cache.page_size;
+        const uint8_t *from = static_cast<const uint8_t *>(unit.value ? a.cache.v_codes : a.cache.k_codes) + r * (a.cache.head_dim / 2) + unit.channel / 2 + 2 * half;
+        if (HALF > 1) codes |= (uint32_t) * reinterpret_cast<const uint16_t *>(from) << (16 * i);
+        else codes = *reinterpret_cast<const uint32_t *>(from);
+        p[i] = static_cast<const kvh2 *>(unit.value ? a.cache.v_params : a.cache.k_params)[r * (a.cache.head_dim / kKv4Group) + unit.channel / kKv4Group];
+    }
+    kvh2 v[4];
+    Kv4Unpack()(codes, kvh2{p[0].x, p[HALF - 1].x}, kvh2{p[0].y, p[HALF - 1].y}, v);
+#pragma unroll
+    for (int i = 0; i < HALF; i++) {
+        if (!to[i]) continue;
+        TN y;
+#pragma unroll
+        for (int j = 0; j < N; j++) y[j] = (T)v[j & 3][HALF > 1 ? i : j >> 2];
+        if (a.wide) {
+            __builtin_nontemporal_store(y, reinterpret_cast<TN *>(to[i]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j++) to[i][j] = y[j];
+        }
     }
 }
 

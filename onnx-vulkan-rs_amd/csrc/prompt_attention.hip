@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tile
 // asked for then, and waited for by count (loads end in the order they were issued in).
 template <int HD>
 __global__ void __launch_bounds__(256, 2) prompt_few_kernel(const PromptArgs a) {
-    constexpr int W = 4, KT = 32, PITCH = HD <= 64 ? 64 : HD <= 128 ? 128 : 256, TILE = KT * PITCH * 2;
+    constexpr int W = 4, KT = 32, PITCH = HD <= 64 ? 64 : 128, TILE = KT * PITCH * 2;
     constexpr int SUMS = W * HD * 32 * 4;
     __shared__ __attribute__((aligned(1024))) char smem[2 * W * TILE > SUMS ? 2 * W * TILE : SUMS];   // [wavefront][K, V]; at last the sums
     __shared__ float ml[W][2][32];

@@ -70,7 +70,8 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
 // What a wavefront knows of a row's largest logits: keys in its LDS, `count` of them, and the least value that counts. Keys that pass are
 // written side by side; they are ranked, and all but the `top` largest dropped, when there is no room left and at the end. The first bar is the
 // top-th largest of the lanes' largest logits: at least `top` reach it, and few more. All of this is short loops with little LDS latency
-// in a row: it runs a few times in a launch, one wavefront's time after the other's (a wavefront's first chunk 1 us, ranking 0.5 us).
+// in a row: it runs a few times in a launch, one wavefront's time after the other's (bar and
+// first chunk 1.7 us, ranking 0.5).
 struct LogBuffer {
     float stage[kLogChunk];                          // a chunk's logits: the lane's i-th at 64 i + lane
     uint64_t key[kLogBuffer], ranked[HIPC_TOP_MAX];

@@ -425,10 +425,11 @@ typedef struct {
  * infinity or a NaN gets what these make of it; in f32 an infinite query or key that a row sees makes it NaN.
  * f16: products of the f16 values as they are, sums in f32, softmax in f32, its weights rounded to f16 for the second
  * product. f32: every factor as three bf16 terms (24 bits), sums in f32. Weighted values are summed before they are divided by
- * the weights' sum: f32 values above some 2^100 may pass the type's range on the way. head_dim is at most 512; one that is a
- * multiple of 8, up to 256, with rows and strides (up to 2^23 elements) on 16 bytes runs on the matrix cores, any other on a kernel that
- * computes in f32 on the vector units. n_seqs <= 2^20; totals <= 2^30. Q, K and V may not overlap Y. With few rows, keys are shared by
- * several workgroups whose parts lie in scratch memory; a call recorded before any like it ran does without (another order of the sums).
+ * the weights' sum: f32 values above some 2^100 may pass the type's range on the way. head_dim is at most 512; up to 256 runs on
+ * the matrix cores: straight from the operands where it is a multiple of 8 and rows and strides (of K and V up to 2^23 elements) are on 16
+ * bytes, else through copies in scratch memory. Wider heads run on a kernel that computes in f32 on the vector units.
+ * n_seqs <= 2^20; totals <= 2^30. Q, K and V may not overlap Y. With few rows, keys are shared by several workgroups whose
+ * parts lie in scratch memory; a call recorded before any like it ran does without either (slower; another order of the sums).
  */
 int hipc_prompt_attention(hipc_ctx *ctx, const hipc_attention_heads *heads, int dtype, const void *Q, int64_t q_stride,
                           const void *K, int64_t k_stride, const void *V, int64_t v_stride, const void *q_starts,

@@ -162,6 +162,61 @@ def test_recorded_before_any_ran(pkg):
         free()
 
 
+@pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
+@pytest.mark.parametrize("off,pad,dim", [(1, 3, 64), (0, 0, 36), (0, 1, 250), (2, 2, 9)])
+def test_rows_of_any_kind_with_and_without_scratch_memory(pkg, dtype, off, pad, dim):
+    """Head widths off 8, rows apart by odd numbers of elements and off 16 bytes: recorded on a context that has no scratch memory, eagerly, and
+    recorded again; rows of Y in front of and behind the sequences stay, whatever rows of Q and K there hold."""
+    heads, kv, rows, keys = 6, 2, 70, 150
+    rng = np.random.default_rng(dim)
+    q, k, v = operands(rng, dtype, rows, keys, heads, kv, dim)
+    q[:2], q[66:], k[:3], v[:3], k[140:], v[140:] = np.nan, np.nan, np.nan, np.inf, np.inf, np.nan
+    code, size = pkg.runtime.hipc_dtype(np.dtype(dtype)), np.dtype(dtype).itemsize
+
+    def strided(x):
+        w = x.shape[1] * x.shape[2]
+        buf = np.full(off + x.shape[0] * (w + pad), 7, dtype)
+        buf[off:].reshape(x.shape[0], w + pad)[:, :w] = x.reshape(x.shape[0], w)
+        return buf
+    with pkg.Context(0) as ctx:
+        up = [ctx.upload(strided(x)) for x in (q, k, v, np.full_like(q, 7))]
+        qs, ks = ctx.upload(np.array([2, 30, 30, 66], np.int32)), ctx.upload(np.array([3, 31, 50, 140], np.int32))
+        h, wq, wk = pkg.AttentionHeads(heads, kv, dim, 1, 0, 0.0), heads * dim + pad, kv * dim + pad
+        at = [b.at(off * size) for b in up]
+
+        def call():
+            pkg.ops.prompt_attention_device(ctx, h, code, at[0], wq, at[1], wk, at[2], wk, qs, ks, 3, rows, keys, at[3], wq)
+
+        def result():
+            buf = ctx.download(up[3], dtype, (off + rows * wq,))
+            assert np.all(buf[:off] == 7)
+            y = buf[off:].reshape(rows, wq)
+            assert np.all(y[:, heads * dim:] == 7) and np.all(y[:2] == 7) and np.all(y[66:] == 7)
+            y = y[2:66, :heads * dim].reshape(64, heads, dim)
+            check(y, q[2:66], k[3:140], v[3:140], [28, 0, 36], [28, 19, 90])
+            ctx.upload(strided(np.full_like(q, 7)), up[3])
+            return bits(np.ascontiguousarray(y))
+
+        def recorded():
+            ctx.capture_begin()
+            call()
+            g = ctx.capture_end()
+            for _ in range(2):
+                ctx.graph_launch(g)
+                y = result()
+                call()
+                assert np.array_equal(result(), eager) if eager is not None else True
+            ctx.graph_destroy(g)
+            return y
+        eager = None
+        recorded()
+        call()
+        eager = result()
+        assert np.array_equal(recorded(), eager)
+        for b in up + [qs, ks]:
+            b.free()
+
+
 def test_pages_that_sequences_share(ctx, pkg):
     """Two sequences with one beginning: the same pages in both rows of the table."""
     rng = np.random.default_rng(4)

@@ -29,7 +29,7 @@ typedef int kvi2 __attribute__((ext_vector_type(2)));
 constexpr int kScratchKv4 = 6;     // scratch slot of this operator alone
 constexpr int kKv4Rows = 16;       // query rows of a unit
 constexpr int kKv4Tile = 64;       // keys a wavefront takes at a time
-constexpr int kKv4Waves = 4;
+constexpr int kKv4PerCu = 8;       // wavefronts
 constexpr float kKv4Log2e = 1.4426950408889634f;
 constexpr float kKv4RescaleAt = 8.f;   // the running maximum may fall behind by 2^8 before sums are rescaled ...
 constexpr float kKv4Up = 7.f;          // ... and weights are kept 2^7 times as large: up to 2^15, so that two f16 terms hold 22 bits of more of them
@@ -52,10 +52,28 @@ __device__ __forceinline__ float groups_sum(float v) {
 struct Kv4Span {
     int length, first, count;
 };
-__device__ __forceinline__ Kv4Span kv4_span(const Kv4Attend &a, int seq) {
-    const int length = a.cache.n_pages > 0 ? kv4_length(a.cache, seq) : 0, held = kv4_held(a.cache, length);
+__device__ __forceinline__ Kv4Span kv4_span_of(const Kv4Attend &a, int length) {
+    const int held = kv4_held(a.cache, length);
     const int begin = a.window > 0 ? max(length - a.tokens - a.window + 1, 0) : 0;
     return {length, begin / kKv4Tile, held > begin ? (held + kKv4Tile - 1) / kKv4Tile - begin / kKv4Tile : 0};
+}
+
+__device__ __forceinline__ int kv4_span_length(const Kv4Attend &a, int seq) { return a.cache.n_pages > 0 ? kv4_length(a.cache, min(seq, a.cache.n_seqs - 1)) : 0; }
+__device__ __forceinline__ Kv4Span kv4_span(const Kv4Attend &a, int seq) { return kv4_span_of(a, kv4_span_length(a, seq)); }
+// body(base, spans) for the sequences in chunks of 64, a lane's is base + lane (the last one's, behind it): the first 64 are there, of
+// the others four chunks' lengths are on their way at once. Ends where body is true.
+template <typename Body>
+__device__ __forceinline__ void kv4_sequences(const Kv4Attend &a, const Kv4Span &early, Body body) {
+    if (body(0, early)) return;
+    const int lane = threadIdx.x & 63;
+    for (int base = 64; base < a.cache.n_seqs; base += 256) {
+        int length[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) length[e] = kv4_span_length(a, base + 64 * e + lane);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (base + 64 * e < a.cache.n_seqs && body(base + 64 * e, kv4_span_of(a, length[e]))) return;
+    }
 }
 
 // A unit: (sequence, kv head, block of 16 query rows), counted in this order.
@@ -71,8 +89,8 @@ __device__ __forceinline__ int kv4_steps(int tiles, int cut) { return cut > 0 ? 
 __device__ __forceinline__ bool kv4_find(const Kv4Attend &a, const Kv4Span &early, int per_seq, int64_t at, int cut, Kv4Unit *u) {
     const int lane = threadIdx.x & 63;
     int64_t before = 0;
-    for (int base = 0; base < a.cache.n_seqs; base += 64) {
-        const Kv4Span s = base == 0 ? early : kv4_span(a, min(base + lane, a.cache.n_seqs - 1));
+    bool found = false;
+    kv4_sequences(a, early, [&](int base, const Kv4Span &s) {
         const int n = base + lane < a.cache.n_seqs ? kv4_steps(s.count, cut) : 0;
         const int sum = wave_scan(n);
         const uint64_t over = __ballot(before + (int64_t)sum * per_seq > at);
@@ -83,9 +101,24 @@ __device__ __forceinline__ bool kv4_find(const Kv4Attend &a, const Kv4Span &earl
             u->seq = base + l;
             u->inner = (int)kv4_div(at - first, steps);
             u->before = first + (int64_t)u->inner * steps;
-            return true;
+            found = true;
         }
         before += (int64_t)__builtin_amdgcn_readlane(sum, 63) * per_seq;
+        return over != 0;
+    });
+    return found;
+}
+// the unit behind the last one of its sequence, which ended at step `at`
+__device__ __forceinline__ bool kv4_next(const Kv4Attend &a, int64_t at, int cut, Kv4Unit *u) {
+    const int lane = threadIdx.x & 63;
+    for (int base = u->seq + 1; base < a.cache.n_seqs; base += 64) {
+        const Kv4Span s = kv4_span(a, base + lane);
+        const uint64_t has = __ballot(base + lane < a.cache.n_seqs && kv4_steps(s.count, cut) > 0);
+        if (!has) continue;
+        const int l = __builtin_ctzll(has);
+        u->span = {__builtin_amdgcn_readlane(s.length, l), __builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.count, l)};
+        u->seq = base + l, u->inner = 0, u->before = at;
+        return true;
     }
     return false;
 }
@@ -94,27 +127,28 @@ __device__ __forceinline__ int64_t kv4_total(const Kv4Attend &a, const Kv4Span &
     const int lane = threadIdx.x & 63;
     int64_t total = 0;
     float most = 0.f;
-    for (int base = 0; base < a.cache.n_seqs; base += 64) {
-        const int c = base + lane >= a.cache.n_seqs ? 0 : base == 0 ? early.count : kv4_span(a, base + lane).count;
+    kv4_sequences(a, early, [&](int base, const Kv4Span &s) {
+        const int c = base + lane < a.cache.n_seqs ? s.count : 0;
         total += (int64_t)__builtin_amdgcn_readlane(wave_scan(kv4_steps(c, cut)), 63) * per_seq;
         most = fmaxf(most, lean_wave_max((float)c));
-    }
+        return false;
+    });
     *longest = most;
     return total;
 }
 
 // rows that see nothing for want of keys
 template <typename T, int HD>
-__device__ void kv4_zero_rows(const Kv4Attend &a) {
+__device__ void kv4_zero_rows(const Kv4Attend &a, const Kv4Span &early) {
     const int lane = threadIdx.x & 63;
-    for (int base = 0; base < a.cache.n_seqs; base += 64) {
-        const bool is = base + lane < a.cache.n_seqs;
-        for (uint64_t none = __ballot(is && kv4_span(a, is ? base + lane : 0).count == 0); none; none &= none - 1) {
+    kv4_sequences(a, early, [&](int base, const Kv4Span &span) {
+        for (uint64_t none = __ballot(base + lane < a.cache.n_seqs && span.count == 0); none; none &= none - 1) {
             const int64_t s = base + __builtin_ctzll(none);
             for (int r = 0; r < a.tokens; r++)
                 for (int i = threadIdx.x; i < a.n_q_heads * HD; i += blockDim.x) static_cast<T *>(a.y)[(s * a.tokens + r) * a.y_stride + i] = (T)0.f;
         }
-    }
+        return false;
+    });
 }
 
 // One launch for everything. Where there are fewer units than workgroups, units are cut into parts of at most so many tiles that there is a
@@ -123,6 +157,10 @@ __device__ void kv4_zero_rows(const Kv4Attend &a) {
 // parts, in their order. (Runs everywhere: a workgroup mostly has the end of one unit and the beginning of another, and starting on a unit and
 // leaving it costs some 6 us beside 3 us a tile.)
 //
+// W: a unit's wavefronts. With four a workgroup each takes every fourth tile and they add up in LDS; where units are many a workgroup is one wavefront, and
+// its run of tiles waits for no other's. (us, four / one; 32 / 8 heads of 128 in f16: 20 sequences of up to 8000 27.9 / 32.7, 48 of up to
+// 4000 35.7 / 33.2, 64 of up to 3200 47.8 / 33.6, 256 of up to 800 106 / 56, 1024 of up to 200 189 / 76.)
+//
 // A wavefront takes 64 keys of one kv head at a time, for 16 query rows (tokens times the heads of the group):
 //   S^T = K Q^T     16x16x32: of tile t (16 keys) row m is key 16 (m / 4) + 4 t + m % 4, so that a lane ends up with the scores of 16
 //                   consecutive keys of one query (query = lane % 16, keys 16 (lane / 16) ..): two steps of the second product
@@ -130,19 +168,19 @@ __device__ void kv4_zero_rows(const Kv4Attend &a) {
 // The codes become f16 values on their way into the operands (exactly what the cache stands for), weights are two f16 terms, f32 queries
 // two terms of the row times a power of two. Keys come straight from memory into operand registers, a tile ahead; values (codes, and
 // the parameters of the keys that are seen, zeros for the others) pass through the wavefront's own LDS, without a barrier.
-template <int HD, int QT>
-__global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_kernel(const Kv4Attend a) {
+template <int HD, int QT, int W>
+__global__ void __launch_bounds__(64 * W, HD <= 128 ? 2 : 1) kv4_attend_kernel(const Kv4Attend a) {
     constexpr int WPL = HD / 32;                              // words of codes of a key per lane; also groups of a row
     constexpr int UNITS = HD <= 32 ? 2 : HD <= 64 ? 4 : HD <= 128 ? 8 : 16;   // 8-byte units of an LDS row of codes
     constexpr int PER = 16 / UNITS;                           // rows of 128 bytes
     constexpr int NP = WPL % 4 == 0 ? WPL / 4 : WPL <= 2 ? 1 : WPL;           // parameters of a key a lane needs for its words
     constexpr int MT = HD / 16;                               // 16-channel tiles
     constexpr int CODES = kKv4Tile * UNITS * 8, PARAMS = WPL * 256;           // LDS of a wavefront
-    constexpr int SUMS = kKv4Waves * HD * kKv4Rows * 4;
-    constexpr int STAGE = kKv4Waves * (CODES + PARAMS);
+    constexpr int SUMS = W * HD * kKv4Rows * 4;
+    constexpr int STAGE = W * (CODES + PARAMS);
     typedef typename std::conditional<QT == 1, _Float16, float>::type T;
     __shared__ __attribute__((aligned(1024))) char smem[STAGE > SUMS ? STAGE : SUMS];
-    __shared__ float ml[kKv4Waves][2][kKv4Rows];
+    __shared__ float ml[W][2][kKv4Rows];
     __shared__ int last_here;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, q4 = lane >> 4;
@@ -157,11 +195,11 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
     float longest, same;
     const int64_t tiles = kv4_total(a, early, per_seq, 0, &longest);
     if (tiles == 0) {
-        if (blockIdx.x == gridDim.x - 1) kv4_zero_rows<T, HD>(a);
+        if (blockIdx.x == gridDim.x - 1) kv4_zero_rows<T, HD>(a, early);
         return;
     }
     const int64_t even = kv4_div(tiles + groups - 1, groups);
-    const int least = max(kKv4Waves, (int)sqrtf(longest * (1.f / 7.f)));
+    const int least = max(W, (int)sqrtf(longest * (1.f / 7.f)));
     int64_t share = even > least ? even : least;
     int cut = 0;
     if (kv4_total(a, early, per_seq, 1 << 30, &same) <= groups) {
@@ -175,7 +213,7 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
     }
     int64_t at = share * blockIdx.x;
     Kv4Unit u;
-    if (blockIdx.x == gridDim.x - 1) kv4_zero_rows<T, HD>(a);
+    if (blockIdx.x == gridDim.x - 1) kv4_zero_rows<T, HD>(a, early);
     if (!kv4_find(a, early, per_seq, at, cut, &u)) return;
     const int64_t run1 = at + share;
     for (;;) {
@@ -266,7 +304,7 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
         };
         int tile = from + wave, v_page = 0, k_page = 0, v_page1 = 0, k_page1 = 0;
         if (tile < to) v_page = page_at(tile, q4), k_page = page_at(tile, n >> 2);
-        if (tile + kKv4Waves < to) v_page1 = page_at(tile + kKv4Waves, q4), k_page1 = page_at(tile + kKv4Waves, n >> 2);
+        if (tile + W < to) v_page1 = page_at(tile + W, q4), k_page1 = page_at(tile + W, n >> 2);
         if (tile < to) load_values(tile, v_page), load_keys(tile, k_page);
         // the queries as operands, while the first tile is on its way
         kvh8 qf[WPL][QT];
@@ -298,12 +336,12 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
                     if (QT == 2) qf[w][QT - 1][j] = (_Float16)(v - (float)hi);
                 }
         }
-        for (; tile < to; tile += kKv4Waves) {
-            const bool more = tile + kKv4Waves < to;
+        for (; tile < to; tile += W) {
+            const bool more = tile + W < to;
             const int key0 = (span.first + tile) * kKv4Tile;
             const bool v_there = is_page(v_page), masked = key0 + kKv4Tile > pos0 + 1 || key0 < all_begin || !__all(v_there);
             int v_page2 = 0, k_page2 = 0;
-            if (tile + 2 * kKv4Waves < to) v_page2 = page_at(tile + 2 * kKv4Waves, q4), k_page2 = page_at(tile + 2 * kKv4Waves, n >> 2);
+            if (tile + 2 * W < to) v_page2 = page_at(tile + 2 * W, q4), k_page2 = page_at(tile + 2 * W, n >> 2);
             // values to LDS: codes in 8-byte units, unit x of row r at x ^ (r / PER), so that the 16 rows of a transposing load lie in different banks
 #pragma unroll
             for (int e = 0; e < WPL; e++) {
@@ -330,7 +368,7 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
                 *reinterpret_cast<uint16_t *>(to_lds) = (uint16_t)w;
                 *reinterpret_cast<uint16_t *>(to_lds + 16) = (uint16_t)(w >> 16);
             }
-            if (more) load_values(tile + kKv4Waves, v_page1);
+            if (more) load_values(tile + W, v_page1);
 
             kvf4 s[4];
 #pragma unroll
@@ -346,7 +384,7 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
                     for (int e = QT - 1; e >= 0; e--) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[w][e], s[t], 0, 0, 0);
                 }
             }
-            if (more) load_keys(tile + kKv4Waves, k_page1);
+            if (more) load_keys(tile + W, k_page1);
             if (masked) {
                 const uint64_t there = __ballot(v_there);
                 const bool block_there = (there >> (16 * q4)) & 1;   // the lane's 16 keys are one block's
@@ -422,9 +460,9 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
         __syncthreads();
         float best = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < kKv4Waves; w++) best = fmaxf(best, ml[w][0][n]);
+        for (int w = 0; w < W; w++) best = fmaxf(best, ml[w][0][n]);
 #pragma unroll
-        for (int w = 0; w < kKv4Waves; w++) sum += ml[w][1][n] == 0.f ? 0.f : ml[w][1][n] * __builtin_amdgcn_exp2f(ml[w][0][n] - best);
+        for (int w = 0; w < W; w++) sum += ml[w][1][n] == 0.f ? 0.f : ml[w][1][n] * __builtin_amdgcn_exp2f(ml[w][0][n] - best);
         {
             const float keep = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - best);
             float4 *mine_o = reinterpret_cast<float4 *>(smem) + wave * MT * 64 + lane;
@@ -456,10 +494,10 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
             const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t *>(pair), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
         };
-        for (int i = wave; i < MT; i += kKv4Waves) {   // thread (i, lane): channels 16 i + 4 q4 .. + 3 of row n
+        for (int i = wave; i < MT; i += W) {   // thread (i, lane): channels 16 i + 4 q4 .. + 3 of row n
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < kKv4Waves; w++) {
+            for (int w = 0; w < W; w++) {
                 const float4 x = reinterpret_cast<const float4 *>(smem)[(w * MT + i) * 64 + lane];
                 v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
             }
@@ -485,7 +523,7 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
             }
             __syncthreads();
             if (last_here) {
-                for (int i = tid; i < rows * (HD / 4); i += 64 * kKv4Waves) {
+                for (int i = tid; i < rows * (HD / 4); i += 64 * W) {
                     const int r = i / (HD / 4), c = (i - r * (HD / 4)) * 4;
                     float top = -INFINITY, all = 0.f;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -520,14 +558,20 @@ __global__ void __launch_bounds__(64 * kKv4Waves, HD <= 128 ? 2 : 1) kv4_attend_
         at = u.before + steps;
         if (at >= run1) break;
         if (++u.inner < per_seq) u.before = at;
-        else if (!kv4_find(a, early, per_seq, at, cut, &u)) break;
+        else if (!kv4_next(a, at, cut, &u)) break;
     }
 }
 
 template <int HD>
-void kv4_launch(hipc_ctx *ctx, const Kv4Attend &a, int dtype, unsigned grid) {
-    if (dtype == HIPC_F16) hipLaunchKernelGGL((kv4_attend_kernel<HD, 1>), grid, 64 * kKv4Waves, 0, ctx->stream, a);
-    else hipLaunchKernelGGL((kv4_attend_kernel<HD, 2>), grid, 64 * kKv4Waves, 0, ctx->stream, a);
+void kv4_launch(hipc_ctx *ctx, const Kv4Attend &a, int dtype, bool alone) {
+    auto launch = [&](auto waves) {
+        constexpr int W = decltype(waves)::value;
+        const unsigned grid = kKv4PerCu * ctx->cu_count / W;
+        if (dtype == HIPC_F16) hipLaunchKernelGGL((kv4_attend_kernel<HD, 1, W>), grid, 64 * W, 0, ctx->stream, a);
+        else hipLaunchKernelGGL((kv4_attend_kernel<HD, 2, W>), grid, 64 * W, 0, ctx->stream, a);
+    };
+    if (alone) launch(std::integral_constant<int, 1>());
+    else launch(std::integral_constant<int, 4>());
 }
 
 }  // namespace
@@ -574,9 +618,9 @@ int hipc_kv4_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_at
         a.row_blocks = (int)ceil_div(tokens * group, kKv4Rows);
         const int64_t unit = dtype == HIPC_F16 ? 8 : 4;
         a.wide = aligned(Q, 16) && aligned(Y, 16) && q_stride % unit == 0 && y_stride % unit == 0;
-        // two workgroups a CU; what they exchange, and the words they count in, in a scratch slot of this operator's own: the words are zero
+        // what workgroups exchange, and the words they count in, in a scratch slot of this operator's own: the words are zero
         // between calls, so a new block is cleared once
-        const unsigned grid = 2 * ctx->cu_count;
+        const unsigned grid = kKv4PerCu * ctx->cu_count;   // at most
         const size_t count_bytes = (grid * 4 + 255) & ~(size_t)255;
         const void *before = ctx->scratch[kScratchKv4].ptr;
         void *block = nullptr;
@@ -586,15 +630,17 @@ int hipc_kv4_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_at
             hipLaunchKernelGGL((fill_words), 1, 256, 0, ctx->stream, a.arrived, count_bytes / 4, 0u);
             HIPC_LAUNCHED(ctx);
         }
+        const int64_t units = (int64_t)cache->n_seqs * cache->n_kv_heads * a.row_blocks;
+        const bool alone = units * 2 >= 3 * (int64_t)ctx->cu_count;
         switch (heads->head_dim / 32) {
-            case 1: kv4_launch<32>(ctx, a, dtype, grid); break;
-            case 2: kv4_launch<64>(ctx, a, dtype, grid); break;
-            case 3: kv4_launch<96>(ctx, a, dtype, grid); break;
-            case 4: kv4_launch<128>(ctx, a, dtype, grid); break;
-            case 5: kv4_launch<160>(ctx, a, dtype, grid); break;
-            case 6: kv4_launch<192>(ctx, a, dtype, grid); break;
-            case 7: kv4_launch<224>(ctx, a, dtype, grid); break;
-            default: kv4_launch<256>(ctx, a, dtype, grid); break;
+            case 1: kv4_launch<32>(ctx, a, dtype, alone); break;
+            case 2: kv4_launch<64>(ctx, a, dtype, alone); break;
+            case 3: kv4_launch<96>(ctx, a, dtype, alone); break;
+            case 4: kv4_launch<128>(ctx, a, dtype, alone); break;
+            case 5: kv4_launch<160>(ctx, a, dtype, alone); break;
+            case 6: kv4_launch<192>(ctx, a, dtype, alone); break;
+            case 7: kv4_launch<224>(ctx, a, dtype, alone); break;
+            default: kv4_launch<256>(ctx, a, dtype, alone); break;
         }
         HIPC_LAUNCHED(ctx);
         return HIPC_OK;

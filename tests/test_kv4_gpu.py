@@ -262,6 +262,37 @@ def test_many_sequences(ctx, pkg):
     p.gpu.free()
 
 
+@pytest.mark.parametrize("dtype,kv,dim,heads,tokens,window", [(np.float16, 4, 128, 16, 1, 0), (np.float32, 4, 64, 8, 2, 0), (np.float16, 4, 96, 4, 3, 50),
+                                                               (np.float32, 4, 256, 4, 1, 100), (np.float16, 6, 32, 36, 4, 0)])
+def test_more_units_than_workgroups(ctx, pkg, dtype, kv, dim, heads, tokens, window):
+    """A wavefront to a unit, runs of tiles dealt over sequences of very different lengths, some of which several wavefronts have parts of: against the
+    definition, and twice the same."""
+    rng = np.random.default_rng(dim + tokens)
+    seqs = 100
+    lengths = np.where(rng.random(seqs) < 0.2, 0, rng.integers(1, 40, seqs))
+    lengths[[7, 50, 99]] = 900, 257, 600
+    p = Pair(ctx, pkg, rng, seqs, 57, 16, kv, dim)
+    p.append([int(n) for n in lengths])
+    assert seqs * kv * -(-tokens * heads // kv // 16) >= 384      # (256 CUs)
+    q = rng.standard_normal((seqs * tokens, heads, dim)).astype(dtype)
+    want, weight, size = p.ref.attention(q, p.lengths, tokens, window)
+    got = p.gpu.attention(q, tokens, window)
+    k_most = float(np.nanmax(np.abs(p.ref.params[0].astype(np.float64)))) * 16
+    off = np.abs(got.astype(np.float64) - want) - tolerance(dtype, q.astype(np.float64), 900, want, weight, size, k_most)
+    assert np.all(off <= 0), (float(off.max()), np.unravel_index(np.argmax(off), off.shape))
+    assert not got.reshape(seqs, tokens, -1)[lengths == 0].any()
+    assert np.array_equal(bits(p.gpu.attention(q, tokens, window)), bits(got))
+    # pages that are given back, and one that never was
+    table = p.ref.table.copy()
+    table[50, 3], table[99, :10], table[7, 30] = -1, 1 << 30, -5
+    p.gpu.set_table(table)
+    p.ref.table = table
+    want, weight, size = p.ref.attention(q, p.lengths, tokens, window)
+    off = np.abs(p.gpu.attention(q, tokens, window).astype(np.float64) - want) - tolerance(dtype, q.astype(np.float64), 900, want, weight, size, k_most)
+    assert np.all(off <= 0), (float(off.max()), np.unravel_index(np.argmax(off), off.shape))
+    p.gpu.free()
+
+
 def test_what_lies_behind_a_sequence_does_not_reach_it(ctx, pkg):
     """Positions behind the length, and pages of nobody, hold NaN parameters; so does a position outside the window."""
     p = Pair(ctx, pkg, np.random.default_rng(9), 2, 6, 16, 2, 64)

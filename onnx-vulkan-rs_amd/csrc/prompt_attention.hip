@@ -201,8 +201,7 @@ __device__ __forceinline__ bool prompt_tile(const PromptArgs &a, int at, PromptT
     // the last tiles of a causal sequence are the heaviest
     const int tile = a.tiles - 1 - at;
     int before = 0;
-    for (int base = 0; base < a.n_seqs; base += 64) {
-        const PromptLengths s(a, base + lane, ROWS);
+    auto in = [&](int base, const PromptLengths &s) {
         const int sum = wave_scan(s.tiles);
         const uint64_t over = __ballot(before + sum > tile);
         if (over) {
@@ -210,9 +209,16 @@ __device__ __forceinline__ bool prompt_tile(const PromptArgs &a, int at, PromptT
             s.of_lane(a, l, out);
             out->seq = base + l;
             out->r0 = (tile - (before + __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(s.tiles, l))) * ROWS;
-            return true;
         }
         before += __builtin_amdgcn_readlane(sum, 63);
+        return over != 0;
+    };
+    if (in(0, PromptLengths(a, lane, ROWS))) return true;
+    for (int base = 64; base < a.n_seqs; base += 256) {   // (four chunks on their way at once)
+        const PromptLengths s[4] = {{a, base + lane, ROWS}, {a, base + 64 + lane, ROWS}, {a, base + 128 + lane, ROWS}, {a, base + 192 + lane, ROWS}};
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (in(base + 64 * e, s[e])) return true;
     }
     return false;
 }

@@ -217,6 +217,19 @@ def test_rows_of_any_kind_with_and_without_scratch_memory(pkg, dtype, off, pad, 
             b.free()
 
 
+@pytest.mark.parametrize("waves,dtype,dim", [(-1, np.float16, 64), (4, np.float16, 128), (2, np.float32, 64), (-1, np.float16, 20)])
+def test_seven_hundred_prompts(ctx, pkg, waves, dtype, dim):
+    """More sequences than are looked up at once, many of them empty, one of some length; parts of them behind earlier keys."""
+    rng = np.random.default_rng(5)
+    q_lengths = np.where(rng.random(700) < 0.4, 0, rng.integers(1, 4, 700))
+    q_lengths[[0, 333, 699]] = 0, 90, 5
+    k_lengths = np.where(rng.random(700) < 0.5, q_lengths, q_lengths + rng.integers(0, 9, 700))
+    q, k, v = operands(rng, dtype, int(q_lengths.sum()), int(k_lengths.sum()), 4, 2, dim)
+    with ctx.options(HIPC_PROMPT_WAVES=waves):
+        got = pkg.ops.prompt_attention(ctx, q, k, v, q_lengths, k_lengths)
+    check(got, q, k, v, q_lengths, k_lengths)
+
+
 def test_pages_that_sequences_share(ctx, pkg):
     """Two sequences with one beginning: the same pages in both rows of the table."""
     rng = np.random.default_rng(4)

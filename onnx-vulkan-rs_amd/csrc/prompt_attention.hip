@@ -473,7 +473,7 @@ struct PromptFetch {
 // LDS, and each sums its half of the channels of the result (one wavefront with all 256 needs 512 registers and has its SIMD to itself:
 // 4096 rows of 16 query and 4 kv heads 280 us, shared 235).
 template <int HD, int W, int KT>
-__global__ void __launch_bounds__(64 * W, HD > 64 && W == 2 ? 1 : 2) prompt_tiles_kernel(const PromptArgs a) {
+__global__ void __launch_bounds__(64 * W, 2) prompt_tiles_kernel(const PromptArgs a) {
     constexpr int C = HD > 128 ? 2 : 1, HC = HD / C;               // wavefronts of a row, channels of each
     constexpr int PITCH = HD <= 64 ? 64 : HD <= 128 ? 128 : 256;   // halfs of an LDS row
     constexpr int TILE = KT * PITCH * 2;                           // bytes of a tile of K, or of V
@@ -630,7 +630,7 @@ __device__ __forceinline__ pf16 mfma_terms(const pb8 (&x)[3], const pb8 (&y)[3],
 }
 
 template <int HD, int W>
-__global__ void __launch_bounds__(64 * W, W == 2 || (HD > 128 && W == 4) ? 1 : 2) prompt_terms_kernel(const PromptArgs a) {
+__global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) prompt_terms_kernel(const PromptArgs a) {
     constexpr int C = HD > 128 ? 2 : 1, HC = HD / C;
     constexpr int KT = 32;
     constexpr int PITCH = HD <= 64 ? 64 : HD <= 128 ? 128 : 256;   // bf16 of an LDS row
@@ -925,9 +925,10 @@ int prompt_launch(hipc_ctx *ctx, PromptArgs a, int splits) {
 
 // How many wavefronts a workgroup has, and how many workgroups share the keys of a tile of rows. Both go by what the host knows:
 // rows, keys and sequences in all. Measured in us, inputs not in the caches nearest the CUs, heads 32 / 8 of 128 in f16 unless said.
-// Wavefronts (2 / 4 / 8): 8192 rows in one sequence 886 / 618 / 604; eight sequences of up to 1024 86 / 62 / 63 (the longest sequence's last tiles
-// end the launch); two of up to 1500 in f32, whose tiles are split once for all wavefronts, 357 / 265 / 236.
-// The kernel for few rows against the better of 2 and 4 wavefronts: 16 rows behind 4000 keys 15 / 17, 60 20 / 23, 500 alone 11 / 18; 200 seeing 512 keys 12 / 20;
+// Wavefronts (4 / 8): 8192 rows in one sequence 607 / 585; eight sequences of up to 1024 58.5 / 61.7; two of up to 1500 in f32, whose tiles are split once for
+// all wavefronts, 239 / 217. Two where heads are narrow and prompts short: 1024 of up to 16 rows, 14 / 2 heads of 64, 23 and 31 with four (of 128,
+// where two have a SIMD each to themselves, 147 and 131).
+// The kernel for few rows against four wavefronts: 16 rows behind 4000 keys 15 / 17, 60 20 / 23, 500 alone 11 / 18; 200 seeing 512 keys 12 / 20;
 // past 512 workgroups it loses: four prompts of up to 400 22 / 17. Channels up to 64 carry it to twice as many (two prompts of up to 1000, 14 / 2 heads 13 / 20);
 // wider than 128, its 32 rows a workgroup take in the keys too often (two pieces of 1000 that see 512 keys, 4 / 1 heads of 256: 33 / 25).
 // Sharing keys costs the parts' way out and back and a join, and pays while CUs are left and there are keys enough (alone / 2 / 4 / 8 / 16):
@@ -936,11 +937,13 @@ template <typename T>
 int prompt_matrix(hipc_ctx *ctx, const PromptArgs &a) {
     const int64_t rows = (int64_t)a.total_q * a.group, kv = a.n_q_heads / a.group, cus = ctx->cu_count;
     const int shared = a.dim > 128 ? 2 : 1;   // wavefronts of a row
-    int waves = rows <= 64 * (int64_t)a.n_seqs ? 2 * shared : 4;
-    if (waves == 4 && rows * kv * shared >= 256 * cus * (sizeof(T) == 2 ? 4 : 1) && (sizeof(T) != 2 || a.total_k >= 2048 * (int64_t)a.n_seqs)) waves = 8;
+    int waves = sizeof(T) == 2 && a.dim <= 64 && rows <= 64 * (int64_t)a.n_seqs ? 2 : 4;
+    if (waves == 4 && rows * kv * shared >= 256 * cus * (sizeof(T) == 2 ? 4 : 1) &&
+        (sizeof(T) == 2 ? a.total_k >= 2048 * (int64_t)a.n_seqs : rows >= 1024 * (int64_t)a.n_seqs))
+        waves = 8;
     if (sizeof(T) == 2 && a.dim <= 128 && std::max<int64_t>(ceil_div(rows, 32), a.n_seqs) * kv <= (a.dim <= 64 ? 4 : 2) * cus) waves = 1;
     if (ctx->tune.prompt_waves > 0) waves = ctx->tune.prompt_waves;
-    if (sizeof(T) != 2 || a.dim > 128) waves = std::max(waves, 2);
+    if (waves < 4 && (sizeof(T) != 2 || a.dim > (waves == 1 ? 128 : 64))) waves = 4;
     const int tile_rows = waves == 1 ? 32 : 32 * waves / shared;
     const int64_t groups = std::max<int64_t>(ceil_div(rows, tile_rows), a.n_seqs) * kv;
     int64_t keys = a.total_k / a.n_seqs;
@@ -959,10 +962,11 @@ int prompt_matrix(hipc_ctx *ctx, const PromptArgs &a) {
     auto launch = [&](auto width) -> int {
         constexpr int HD = decltype(width)::value;
         if (waves >= 8) return prompt_launch<T, HD, 8>(ctx, a, splits);
-        if (waves >= 4) return prompt_launch<T, HD, 4>(ctx, a, splits);
         if constexpr (sizeof(T) == 2 && HD <= 128)
             if (waves == 1) return prompt_launch<T, HD, 1>(ctx, a, splits);
-        return prompt_launch<T, HD, 2>(ctx, a, splits);
+        if constexpr (sizeof(T) == 2 && HD <= 64)
+            if (waves < 4) return prompt_launch<T, HD, 2>(ctx, a, splits);
+        return prompt_launch<T, HD, 4>(ctx, a, splits);
     };
     return a.dim <= 64 ? launch(std::integral_constant<int, 64>()) : a.dim <= 128 ? launch(std::integral_constant<int, 128>()) : launch(std::integral_constant<int, 256>());
 }

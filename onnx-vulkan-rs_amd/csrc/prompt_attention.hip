@@ -968,7 +968,12 @@ int prompt_matrix(hipc_ctx *ctx, const PromptArgs &a) {
             if (waves < 4) return prompt_launch<T, HD, 2>(ctx, a, splits);
         return prompt_launch<T, HD, 4>(ctx, a, splits);
     };
-    return a.dim <= 64 ? launch(std::integral_constant<int, 64>()) : a.dim <= 128 ? launch(std::integral_constant<int, 128>()) : launch(std::integral_constant<int, 256>());
+    // (96 beside 128: 6000 rows of 16 / 8 heads of 96 in f16 147 us, as heads of 128 166; two prompts of up to 1500 in f32 135 and 194. A wavefront of
+    // its own for 160 channels spills: 119 us where 256 shared by two take 88.)
+    return a.dim <= 64    ? launch(std::integral_constant<int, 64>())
+           : a.dim <= 96  ? launch(std::integral_constant<int, 96>())
+           : a.dim <= 128 ? launch(std::integral_constant<int, 128>())
+                          : launch(std::integral_constant<int, 256>());
 }
 
 }  // namespace

@@ -529,10 +529,11 @@ __global__ void __launch_bounds__(64 * W, 2) prompt_tiles_kernel(const PromptArg
 // Few rows: a workgroup has 32 of them, and its four wavefronts take the key tiles in turn, each through LDS of its own, so that none waits for
 // another before the end. The keys' half of that LDS is free for the next tile once they are multiplied, the values' half once those are; both are
 // asked for then, and waited for by count (loads end in the order they were issued in).
-template <int HD>
-__global__ void __launch_bounds__(256, 2) prompt_few_kernel(const PromptArgs a) {
-    constexpr int W = 4, KT = 32, PITCH = HD <= 64 ? 64 : 128, TILE = KT * PITCH * 2;
-    constexpr int SUMS = W * HD * 32 * 4;
+// W == 1: a workgroup is one wavefront with all keys of its rows, for short prompts in great number. (1024 of up to 16 rows, 32 / 8 heads of 128: 55 us, with tiles of four wavefronts 130.)
+template <int HD, int W>
+__global__ void __launch_bounds__(64 * W, 2) prompt_few_kernel(const PromptArgs a) {
+    constexpr int KT = 32, PITCH = HD <= 64 ? 64 : 128, TILE = KT * PITCH * 2;
+    constexpr int SUMS = W > 1 ? W * HD * 32 * 4 : 0;
     __shared__ __attribute__((aligned(1024))) char smem[2 * W * TILE > SUMS ? 2 * W * TILE : SUMS];   // [wavefront][K, V]; at last the sums
     __shared__ float ml[W][2][32];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -563,6 +564,10 @@ __global__ void __launch_bounds__(256, 2) prompt_few_kernel(const PromptArgs a) 
         rows.values(vs, t * KT, masked, pr, p);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (more) from.values_of(t + W, lds + TILE);
+    }
+    if (W == 1) {
+        prompt_rows_out<_Float16, HD>(a, pt, pr, rows.h, 0, rows.m, rows.l, rows.o);
+        return;
     }
     // the wavefronts' sums, joined in LDS
     rows.l = halves_sum(rows.l);
@@ -896,13 +901,13 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs a) {
 
 size_t prompt_parts_bytes(const PromptArgs &a, int splits) { return splits > 1 ? (size_t)splits * a.total_q * a.n_q_heads * (a.dim + 2) * 4 : 0; }
 
-// W == 1: the kernel for few rows
+// W == 1: the kernel for few rows; 2: the same with a wavefront by itself
 template <typename T, int HD, int W>
 int prompt_launch(hipc_ctx *ctx, PromptArgs a, int splits) {
-    const int64_t tiles = ceil_div((int64_t)a.total_q * a.group, W == 1 ? 32 : 32 * W / (HD > 128 ? 2 : 1)) + a.n_seqs;   // (at most: a sequence may leave one unfinished)
+    const int64_t tiles = ceil_div((int64_t)a.total_q * a.group, W <= 2 ? 32 : 32 * W / (HD > 128 ? 2 : 1)) + a.n_seqs;   // (at most: a sequence may leave one unfinished)
     a.tiles = (int)tiles, a.splits = splits;
     // (where all tiles run at once, their order is not worth the microsecond that it takes to find it)
-    a.by_keys = W > 1 && a.causal && a.window == 0 && a.n_seqs > 1 && a.n_seqs <= 64 && tiles * (a.n_q_heads / a.group) > 2 * ctx->cu_count;
+    a.by_keys = W > 2 && a.causal && a.window == 0 && a.n_seqs > 1 && a.n_seqs <= 64 && tiles * (a.n_q_heads / a.group) > 2 * ctx->cu_count;
     if (splits > 1) {
         const size_t rows = (size_t)splits * a.total_q * a.n_q_heads;
         void *s = nullptr;
@@ -910,7 +915,7 @@ int prompt_launch(hipc_ctx *ctx, PromptArgs a, int splits) {
         a.part_o = static_cast<float *>(s), a.part_ml = a.part_o + rows * a.dim;
     }
     const dim3 grid((unsigned)(tiles * (a.n_q_heads / a.group)), splits);
-    if constexpr (sizeof(T) == 2 && W == 1) hipLaunchKernelGGL((prompt_few_kernel<HD>), grid, 256, 0, ctx->stream, a);
+    if constexpr (sizeof(T) == 2 && W <= 2) hipLaunchKernelGGL((prompt_few_kernel<HD, W == 1 ? 4 : 1>), grid, W == 1 ? 256 : 64, 0, ctx->stream, a);
     else if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((prompt_tiles_kernel<HD, W, (HD > 128 ? 32 : 64)>), grid, 64 * W, 0, ctx->stream, a);
     else hipLaunchKernelGGL((prompt_terms_kernel<HD, W>), grid, 64 * W, 0, ctx->stream, a);
     HIPC_LAUNCHED(ctx);
@@ -926,8 +931,8 @@ int prompt_launch(hipc_ctx *ctx, PromptArgs a, int splits) {
 // How many wavefronts a workgroup has, and how many workgroups share the keys of a tile of rows. Both go by what the host knows:
 // rows, keys and sequences in all. Measured in us, inputs not in the caches nearest the CUs, heads 32 / 8 of 128 in f16 unless said.
 // Wavefronts (4 / 8): 8192 rows in one sequence 607 / 585; eight sequences of up to 1024 58.5 / 61.7; two of up to 1500 in f32, whose tiles are split once for
-// all wavefronts, 239 / 217. Two where heads are narrow and prompts short: 1024 of up to 16 rows, 14 / 2 heads of 64, 23 and 31 with four (of 128,
-// where two have a SIMD each to themselves, 147 and 131).
+// all wavefronts, 239 / 217. A wavefront by itself for prompts of few rows (with their heads 256 on average), against four: 1024 of up to 16 rows
+// 55 / 130, 256 of up to 64 41 / 51, 64 of up to 256 58 / 54; of 14 / 2 heads of 64 15 / 31.
 // The kernel for few rows against four wavefronts: 16 rows behind 4000 keys 15 / 17, 60 20 / 23, 500 alone 11 / 18; 200 seeing 512 keys 12 / 20;
 // past 512 workgroups it loses: four prompts of up to 400 22 / 17. Channels up to 64 carry it to twice as many (two prompts of up to 1000, 14 / 2 heads 13 / 20);
 // wider than 128, its 32 rows a workgroup take in the keys too often (two pieces of 1000 that see 512 keys, 4 / 1 heads of 256: 33 / 25).
@@ -937,14 +942,17 @@ template <typename T>
 int prompt_matrix(hipc_ctx *ctx, const PromptArgs &a) {
     const int64_t rows = (int64_t)a.total_q * a.group, kv = a.n_q_heads / a.group, cus = ctx->cu_count;
     const int shared = a.dim > 128 ? 2 : 1;   // wavefronts of a row
-    int waves = sizeof(T) == 2 && a.dim <= 64 && rows <= 64 * (int64_t)a.n_seqs ? 2 : 4;
+    const bool brief = sizeof(T) == 2 && a.dim <= 128 && rows <= 256 * (int64_t)a.n_seqs;
+    int waves = brief ? 2 : 4;
     if (waves == 4 && rows * kv * shared >= 256 * cus * (sizeof(T) == 2 ? 4 : 1) &&
         (sizeof(T) == 2 ? a.total_k >= 2048 * (int64_t)a.n_seqs : rows >= 1024 * (int64_t)a.n_seqs))
         waves = 8;
-    if (sizeof(T) == 2 && a.dim <= 128 && std::max<int64_t>(ceil_div(rows, 32), a.n_seqs) * kv <= (a.dim <= 64 ? 4 : 2) * cus) waves = 1;
+    if (sizeof(T) == 2 && a.dim <= 128 && std::max<int64_t>(ceil_div(rows, 32), a.n_seqs) * kv <= (a.dim <= 64 ? 4 : 2) * cus &&
+        !(brief && a.total_k <= 128 * (int64_t)a.n_seqs))
+        waves = 1;
     if (ctx->tune.prompt_waves > 0) waves = ctx->tune.prompt_waves;
-    if (waves < 4 && (sizeof(T) != 2 || a.dim > (waves == 1 ? 128 : 64))) waves = 4;
-    const int tile_rows = waves == 1 ? 32 : 32 * waves / shared;
+    if (waves < 4 && (sizeof(T) != 2 || a.dim > 128)) waves = 4;
+    const int tile_rows = waves <= 2 ? 32 : 32 * waves / shared;
     const int64_t groups = std::max<int64_t>(ceil_div(rows, tile_rows), a.n_seqs) * kv;
     int64_t keys = a.total_k / a.n_seqs;
     if (a.window > 0) keys = std::min<int64_t>(keys, a.window + tile_rows / a.group);
@@ -962,10 +970,10 @@ int prompt_matrix(hipc_ctx *ctx, const PromptArgs &a) {
     auto launch = [&](auto width) -> int {
         constexpr int HD = decltype(width)::value;
         if (waves >= 8) return prompt_launch<T, HD, 8>(ctx, a, splits);
-        if constexpr (sizeof(T) == 2 && HD <= 128)
+        if constexpr (sizeof(T) == 2 && HD <= 128) {
             if (waves == 1) return prompt_launch<T, HD, 1>(ctx, a, splits);
-        if constexpr (sizeof(T) == 2 && HD <= 64)
             if (waves < 4) return prompt_launch<T, HD, 2>(ctx, a, splits);
+        }
         return prompt_launch<T, HD, 4>(ctx, a, splits);
     };
     // (96 beside 128: 6000 rows of 16 / 8 heads of 96 in f16 147 us, as heads of 128 166; two prompts of up to 1500 in f32 135 and 194. A wavefront of

@@ -75,7 +75,7 @@ def test_more_tiles_than_run_at_once(ctx, pkg, dtype, waves, dim, many):
         k_lengths = np.where(rng.random(64) < 0.3, q_lengths, np.maximum(q_lengths + rng.integers(-20, 90, 64), 0))
     else:
         q_lengths, k_lengths = np.array([0, 700, 1, 333, 0, 64, 1005]), np.array([5, 700, 41, 900, 3, 20, 1134])
-    heads, kv = (40, 40) if dim <= 128 else (56, 28)
+    heads, kv = (40, 40) if dim <= 128 else (16, 8)
     rows, keys = int(q_lengths.sum()), int(k_lengths.sum())
     tile = 32 * waves // (2 if dim > 128 else 1)
     assert (-(-rows * (heads // kv) // tile) + len(q_lengths)) * kv > 2 * 256      # (of 256 CUs)
@@ -187,7 +187,7 @@ def test_a_recorded_call_follows_the_starts(ctx, pkg):
 @pytest.mark.parametrize("split", [1, 2, 5])
 @pytest.mark.parametrize("heads,kv,dim", [(4, 1, 256), (6, 2, 128), (3, 1, 64)])
 def test_every_launch_shape(ctx, pkg, dtype, waves, split, heads, kv, dim):
-    """Workgroups of 2, 4 and 8 wavefronts, and of 32 rows (1), alone with their keys or sharing them, over sequences that end anywhere in a tile."""
+    """Workgroups of 4 and 8 wavefronts, of four that share 32 rows (1) and of one (2), alone with their keys or sharing them, over sequences that end anywhere in a tile."""
     q_lengths, k_lengths = [70, 3, 1], [200, 3, 90]
     q, k, v = operands(np.random.default_rng(dim + split), dtype, 74, 293, heads, kv, dim)
     with ctx.options(HIPC_PROMPT_WAVES=waves, HIPC_PROMPT_SPLIT=split):

@@ -424,10 +424,12 @@ typedef struct {
  * Keys and values that a row does not see do not enter its result, whatever they hold (infinities and NaN too). A row that sees an
  * infinity or a NaN gets what these make of it; in f32 an infinite query or key that a row sees makes it NaN.
  * f16: products of the f16 values as they are, sums in f32, softmax in f32, its weights rounded to f16 for the second
- * product. f32: every factor as three bf16 terms (24 bits), sums in f32. Weighted values are summed before they are divided by
- * the weights' sum: f32 values above some 2^100 may pass the type's range on the way. head_dim is at most 512; up to 256 runs on
- * the matrix cores: straight from the operands where it is a multiple of 8 and rows and strides (of K and V up to 2^23 elements) are on 16
- * bytes, else through copies in scratch memory. Wider heads run on a kernel that computes in f32 on the vector units.
+ * product and for the sum it is divided by: each is off by at most 2^-11 of itself or, below 2^-21 of the row's heaviest,
+ * 2^-32 of that. f32: every factor as three bf16 terms (24 bits), sums in f32. Weighted values are summed before they are
+ * divided by the weights' sum: f32 values above some 2^100 may pass the type's range on the way. head_dim is at most 512; up
+ * to 256 runs on the matrix cores: straight from the operands where it is a multiple of 8 and rows and strides (of K and V up
+ * to 2^23 elements) are on 16 bytes, else through copies in scratch memory. Wider heads run on a kernel that computes in f32
+ * on the vector units.
  * n_seqs <= 2^20; totals <= 2^30. Q, K and V may not overlap Y. With few rows, keys are shared by several workgroups whose
  * parts lie in scratch memory; a call recorded before any like it ran does without either (slower; another order of the sums).
  */

@@ -132,7 +132,10 @@ __global__ void __launch_bounds__(256) prompt_pad_kernel(const PromptPadded a) {
 //   O^T = V^T P^T    the lane's weights are the second operand as they lie, with the keys of a step numbered the way the scores came out;
 //                    V^T is read from row-major LDS rows by the transposing loads
 // so maximum, sum and rescale of the softmax are numbers of one lane, exchanged once between the two halves of the wavefront.
-// The running maximum is let grow by up to 2^8 before sums are rescaled (weights up to 2^8 in f16 round like others).
+// The running maximum is let grow by up to 2^8 before sums are rescaled, and weights are kept 2^7 times as large: up to 2^15 in f16, whose ordinary
+// numbers then reach down to 2^-21 of the heaviest weight and whose subnormal ones, off by up to 2^-32 of it, to 2^-31. (Around 1, f16 loses weights below
+// 2^-25: of 60000 keys that together weigh 2^-10 of one more, all.) That weights are rounded to f16 at all is a choice: as two terms each they would take half as
+// many products again of a kernel that these bound, to bring errors of 1.2 to 1.35 times what rounding the results alone makes down to that.
 // Tiles of K and V go from memory to LDS without a register, one tile ahead; 16-byte chunks of a row lie at chunk ^ f(row), so
 // that the eight (K) and four (V) rows a read takes per cycle lie in different banks. Chunks behind head_dim and rows behind the
 // sequence are zeros (the buffer's range check).
@@ -146,6 +149,7 @@ typedef __attribute__((address_space(3))) char lds_char;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleAt = 8.f;   // in powers of two
+constexpr float kWeightUp = 7.f;    // ... f16 weights
 
 // Which ROWS query rows of one kv head a workgroup has; the tiles are started in the order of `at`.
 struct PromptTile {
@@ -376,7 +380,7 @@ struct PromptRows {
 #pragma unroll
                 for (int r = 0; r < 16; r++) o[i][r] *= keep;
         }
-        const float shift = m == -INFINITY ? 0.f : m;
+        const float shift = (m == -INFINITY ? 0.f : m) - kWeightUp;
 #pragma unroll
         for (int u = 0; u < KT / 16; u++)
 #pragma unroll

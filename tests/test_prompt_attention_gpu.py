@@ -218,3 +218,28 @@ def test_refusals(ctx, pkg):
     assert b"hipc_prompt_attention" in ctx.lib.hipc_last_error(ctx.handle)
     assert call(n=0) == 0 and call(total=0) == 0           # nothing to do
     d.free()
+
+
+@pytest.mark.parametrize("waves,split", [(1, 1), (1, 4), (2, 1), (4, 1), (4, 3), (8, 1), (-1, -1)])
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("at", ["first", "middle", "last"])
+def test_many_keys_far_below_one(ctx, pkg, waves, split, dim, at):
+    """One key e^18 times as heavy as each of 60000 others, which together weigh 9e-4: they are not lost. A weight in f16 is off by half a step, 2^-11 of
+    itself, or where it is subnormal by 2^-25; weights are kept 2^7 times as large, so that is 2^-32 of the heaviest one a key,
+    in the weighted sum (times |v|) and in the sum it is divided by."""
+    rng = np.random.default_rng(dim)
+    keys, heads, rows = 60001, 2, 3
+    q, k, v = np.zeros((rows, heads, dim), np.float16), np.zeros((keys, 1, dim), np.float16), np.zeros((keys, 1, dim), np.float16)
+    q[:, :, 0] = np.sqrt(dim)                                   # a score is the key's first channel
+    k[:, 0, 0] = rng.uniform(-0.2, 0.2, keys)
+    v[:, 0, :] = 1 + np.arange(dim) / dim
+    one = {"first": 5, "middle": 31007, "last": keys - 7}[at]
+    k[one, 0, 0], v[one] = 18.0, 0.0
+    v[one, 0, ::3] = 0.01
+    with ctx.options(HIPC_PROMPT_WAVES=waves, HIPC_PROMPT_SPLIT=split):
+        got = pkg.ops.prompt_attention(ctx, q, k, v, [rows], [keys])
+    want, weight, size = ref.prompt(q, k, v, [rows], [keys])
+    assert 8e-4 < want[0, 0, 1] < 4e-3
+    tol = tolerance(np.float16, dim, keys, want, weight, size) + keys * 2.0 ** -32 * (2.0 + np.abs(want))
+    off = np.abs(got.astype(np.float64) - want) - tol
+    assert np.all(off <= 0), (float(off.max()), float(got[0, 0, 1]), want[0, 0, 1])

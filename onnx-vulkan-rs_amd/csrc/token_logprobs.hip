@@ -49,6 +49,7 @@ __device__ __forceinline__ uint64_t log_key(float x, int id) {
     const uint32_t b = __float_as_uint(x + 0.f);   // (-0 is 0)
     return (uint64_t)(b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u)) << 32 | (uint32_t)~id;
 }
+constexpr uint32_t kLogLowest = 0x007fffffu;   // of -inf
 __device__ __forceinline__ float key_value(uint64_t k) {
     const uint32_t b = (uint32_t)(k >> 32);
     return __uint_as_float(b >> 31 ? b ^ 0x80000000u : ~b);
@@ -171,11 +172,9 @@ struct LogBest {
     template <int N, typename Id>
     __device__ __forceinline__ void scan(int top, LogBuffer &buffer, float largest, const float (&x)[N], Id id) {
         const int lane = threadIdx.x & 63;
-        bool tight = false;   // the bar is this chunk's own
-        if (least == 0) {
-            raise(log_reach((uint32_t)(log_key(largest, 0) >> 32), top));
-            tight = true;
-        }
+        uint32_t reach = 0;   // not 0: what at least `top` of this chunk's logits reach, and the bar is no lower
+        auto of_chunk = [&] { raise(reach = log_reach((uint32_t)(log_key(largest, 0) >> 32), top)); };
+        if (least == 0) of_chunk();
 #pragma unroll
         for (int i = 0; i < N; i++) buffer.stage[64 * i + lane] = x[i];
         for (;;) {
@@ -200,9 +199,8 @@ struct LogBest {
             // no room: what was there is ranked, then the chunk's own bar is taken, and at last (equal values) one key after the other
             if (count > top) {
                 rank(top, buffer);
-            } else if (!tight) {
-                raise(log_reach((uint32_t)(log_key(largest, 0) >> 32), top));
-                tight = true;
+            } else if (reach == 0) {
+                of_chunk();
             } else {
                 uint64_t last = ~(uint64_t)0, mine = 0;
                 const uint64_t had = lane < count ? buffer.key[lane] : 0;
@@ -224,7 +222,9 @@ struct LogBest {
                 break;
             }
         }
-        if (tight) raise(least + 1);   // (for the chunks behind)
+        // For the chunks behind, whose ids are higher: of those `top` one of the same value counts no more. (The reach is passed and not the bar, which the
+        // list may have raised past it; and not -inf, with which lanes that have nothing which compares are counted.)
+        if (reach > kLogLowest) raise(reach + 1);
         if (count >= 2 * top) rank(top, buffer);
     }
 };

@@ -179,3 +179,90 @@ def test_refusals(ctx, pkg):
     assert b"hipc_token_logprobs" in ctx.lib.hipc_last_error(ctx.handle)
     assert call(rows=0) == 0 and call(rows=0, x=None, ids=None, best=None) == 0
     d.free()
+
+
+def places(vocab):
+    """Ids all over a row: in the first chunks, in later ones of the same wavefront, in other wavefronts and workgroups, and the last."""
+    return sorted({1, 700, 1024, 1500, 3000, vocab // 3, vocab // 2, vocab - 1030, vocab - 1})
+
+
+def check_rows(ctx, pkg, x, rows, top):
+    """`x` in batches of `rows` rows (which decides how a row is shared): ids, and where there is a distribution the numbers."""
+    tokens = np.full(len(x), 3)
+    with np.errstate(all="ignore"):
+        want = ref.token_logprobs(x, tokens, top)
+        bound = [allowed(x, np.where(np.isfinite(want[j]), want[j], 0.0)) for j in (0, 1, 3)]
+    for first in range(0, len(x), min(rows, len(x))):
+        pick = (first + np.arange(rows)) % len(x)
+        got = pkg.ops.token_logprobs(ctx, x[pick], tokens[pick], top)
+        wrong = np.argwhere((got[2] != want[2][pick]).any(1)).ravel()
+        assert not len(wrong), (pick[wrong[0]], got[2][wrong[0]], want[2][pick[wrong[0]]])
+        for j, limit in zip((0, 1, 3), bound):
+            w = want[j][pick]
+            assert np.array_equal(np.isnan(got[j]), np.isnan(w)) and np.array_equal(np.isinf(got[j]), np.isinf(w))
+            fine = np.isfinite(w)
+            assert np.all(np.abs(got[j][fine].astype(np.float64) - w[fine]) <= limit[pick][fine])
+
+
+WAYS = pytest.mark.parametrize("rows,vocab", [(1, 131077), (300, 9001), (300, 20021), (100, 90001)], ids=["shared", "alone", "alone, streamed", "shared, streamed"])
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
+@WAYS
+@pytest.mark.parametrize("top", [1, 5, 32])
+def test_one_step_above_many_equal_logits(ctx, pkg, dtype, rows, vocab, top):
+    """Rows of one value with a few that are the next larger number of the type, anywhere: these are the best, not the equal ones in front of them."""
+    lines = []
+    for base in (1.0, -1.5, 0.0, -0.0):
+        base = dtype(base)
+        above = np.nextafter(base, dtype(np.inf), dtype=dtype)
+        for p in places(vocab):
+            x = np.full(vocab, base, dtype)
+            x[p] = above
+            lines.append(x)
+        x = np.full(vocab, base, dtype)
+        x[places(vocab)] = above
+        lines.append(x)
+    x = lines[0].copy()
+    x[::977] = np.nextafter(x[0], dtype(np.inf), dtype=dtype)
+    x[vocab - 5] = np.nextafter(x[977], dtype(np.inf), dtype=dtype)      # two steps
+    check_rows(ctx, pkg, np.stack(lines + [x]), rows, top)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
+@WAYS
+@pytest.mark.parametrize("top", [1, 5, 32])
+def test_banned_logits_beside_the_lowest_number(ctx, pkg, dtype, rows, vocab, top):
+    """-inf and the type's lowest value (another way to ban): the lowest value is the larger one, also where few are."""
+    rng = np.random.default_rng(vocab)
+    lowest, lines = np.finfo(dtype).min, []
+    for some in (1, 3, 40, 300):
+        x = np.full(vocab, -np.inf, dtype)
+        x[rng.choice(vocab, some, replace=False)] = lowest
+        lines.append(x.copy())
+        x[rng.choice(vocab, 2, replace=False)] = 1.0
+        lines.append(x)
+    for p in places(vocab):
+        x = np.full(vocab, -np.inf, dtype)
+        x[p] = lowest
+        lines.append(x)
+    check_rows(ctx, pkg, np.stack(lines), rows, top)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
+@WAYS
+@pytest.mark.parametrize("top", [1, 5, 32])
+def test_nan_in_front_of_banned_logits(ctx, pkg, dtype, rows, vocab, top):
+    """Rows that begin (or go on for a while) with NaN: the ids are those of what compares, -inf too."""
+    lines = []
+    for n in (1, 63, 1024, 1030, 4096, vocab - 3):
+        x = np.full(vocab, -np.inf, dtype)
+        x[:n] = np.nan
+        lines.append(x.copy())
+        x[n // 2::1500] = -np.inf
+        x[min(n + 2000, vocab - 1)] = 2.0
+        lines.append(x)
+    x = np.full(vocab, np.nan, dtype)
+    x[::700] = -np.inf
+    lines.append(x)
+    check_rows(ctx, pkg, np.stack(lines), rows, top)

@@ -489,7 +489,8 @@ int hipc_kv4_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_at
 
 /*
  * Beside the greedy pick of the decode step (ArgMax, shaders/reduction.rs:76-191): for every row of logits
- * [rows, vocab] (f16 or f32, rows row_stride elements apart), with lse = log sum_v exp(x_v) in f32,
+ * [rows, vocab] (f16 or f32, rows row_stride elements apart), with lse = log sum_v exp(x_v), all in f32 and relative to the row's
+ * largest logit (so a row that is shifted as a whole gives the same numbers, and none above 0),
  *   logprob [rows] f32       x_t - lse for the row's given token t = tokens[row] (i32): -1 gives 0 (padding), any other number
  *                            outside [0, vocab) gives NaN; tokens and logprob are given together or not at all (NULL)
  *   entropy [rows] f32       lse - sum_v p_v x_v (a logit of -inf adds nothing), or NULL

@@ -279,15 +279,17 @@ __device__ __forceinline__ LogSum log_join(const LogSum &a, const LogSum &b) {
 // `token` is the row's given one and `given` its logit
 __device__ __forceinline__ void log_finish(const LogprobArgs &a, int64_t row, int token, float given, const LogSum &s, uint64_t list) {
     const int lane = threadIdx.x & 63;
-    // no finite largest value: no distribution (a NaN among the logits has made l one; +inf too, by inf - inf)
-    const float log_l = logf(s.l), lse = s.m == -INFINITY ? NAN : s.m + log_l;
+    // No finite largest value: no distribution (a NaN among the logits has made l one; +inf too, by inf - inf). The
+    // largest logit is taken off first: m + log l would be rounded at the size of m, and what is left could lie above 0.
+    const float log_l = logf(s.l);
+    auto below = [&](float x) { return (x - s.m) - log_l; };
     if (lane == 0) {
-        if (a.logprob) a.logprob[row] = token == -1 ? 0.f : token < 0 || token >= a.vocab ? NAN : given - lse;
+        if (a.logprob) a.logprob[row] = token == -1 ? 0.f : token < 0 || token >= a.vocab || s.m == -INFINITY ? NAN : below(given);
         if (a.entropy) a.entropy[row] = s.m == -INFINITY ? NAN : log_l - kLn2 * (s.w / s.l);
     }
     if (lane < a.top) {
         a.top_ids[row * a.top + lane] = list ? key_id(list) : -1;
-        a.top_logprobs[row * a.top + lane] = list ? key_value(list) - lse : NAN;
+        a.top_logprobs[row * a.top + lane] = list && s.m != -INFINITY ? below(key_value(list)) : NAN;
     }
 }
 

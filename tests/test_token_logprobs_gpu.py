@@ -266,3 +266,28 @@ def test_nan_in_front_of_banned_logits(ctx, pkg, dtype, rows, vocab, top):
     x[::700] = -np.inf
     lines.append(x)
     check_rows(ctx, pkg, np.stack(lines), rows, top)
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 131077), (300, 9001), (300, 20021), (100, 90001)], ids=["shared", "alone", "alone, streamed", "shared, streamed"])
+@pytest.mark.parametrize("dtype,step,shift", [(np.float32, 2.0 ** -8, 2.0 ** 14), (np.float32, 2.0 ** -4, -2.0 ** 18), (np.float16, 2.0 ** -5, 32.0), (np.float16, 8.0, -8192.0)])
+def test_rows_far_from_zero(ctx, pkg, dtype, step, shift, rows, vocab):
+    """A distribution does not know by how much its logits are shifted: where the type holds the shifted logits exactly, the same bits come out. The
+    numbers are off by x - m (one rounding), the logarithm of the sum (8 roundings with its own) and what the exponentials' arguments lose (as above):
+    nothing at the size of the logits. No log-probability is above 0: x - m is not, and the sum has the largest logit's own 1 in it."""
+    rng = np.random.default_rng(vocab)
+    x = (np.round(3 * rng.standard_normal((min(rows, 4), vocab)) / step) * step).astype(dtype)
+    x[:, 77] = x.max(1) + dtype(40 * step)
+    pick = np.arange(rows) % len(x)
+    far = (x.astype(np.float64) + shift).astype(dtype)
+    assert np.array_equal(far.astype(np.float64) - shift, x.astype(np.float64))
+    tokens = np.where(pick % 2, 77, 5)
+    near = pkg.ops.token_logprobs(ctx, x[pick], tokens, 5)
+    got = pkg.ops.token_logprobs(ctx, far[pick], tokens, 5)
+    for a, b in zip(got, near):
+        assert np.array_equal(a.view(np.uint32), b.view(np.uint32))
+    want = ref.token_logprobs(x, tokens[:len(x)], 5)
+    size = 8 + 2 * (np.log(vocab) + 20)
+    for j in (0, 1, 3):
+        w = want[j][pick]
+        assert np.all(np.abs(got[j].astype(np.float64) - w) <= 2.0 ** -23 * (size + np.abs(w)))
+    assert np.array_equal(got[2], want[2][pick]) and np.all(got[0] <= 0) and np.all(got[3] <= 0)

@@ -318,8 +318,9 @@ __global__ void __launch_bounds__(64 * W, HD <= 128 ? 2 : 1) kv4_attend_kernel(c
                 for (int j = 0; j < 8; j++) qx[w][j] *= sign, most = fmaxf(most, fabsf(qx[w][j]));
             if (QT == 2) {
                 most = groups_max(most);
-                // the row's largest value into [2^14, 2^15); an infinity stays where it is
-                const int up = most > 0.f && most < INFINITY ? 14 - ilogbf(most) : 0;
+                // The row's largest value into [2^14, 2^15); an infinity stays where it is. And no further up than leaves the scores' factor an ordinary
+                // number: at 0 it would make NaN of what is hidden (scores of -inf). Rows that this stops have scores of 0 to working precision.
+                const int up = most > 0.f && most < INFINITY ? min(14 - ilogbf(most), 126 + ilogbf(fminf(c2, 0x1p126f))) : 0;
                 c2 = ldexpf(c2, -up);
 #pragma unroll
                 for (int w = 0; w < WPL; w++)

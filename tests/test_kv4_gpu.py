@@ -407,3 +407,23 @@ def test_refusals(ctx, pkg):
     assert b"hipc_kv4_attention" in ctx.lib.hipc_last_error(ctx.handle)
     assert attend(n_seqs=0) == 0
     d.free(), p.gpu.free()
+
+
+@pytest.mark.parametrize("dim,heads,kv", [(64, 4, 2), (128, 8, 1), (256, 4, 1)])
+@pytest.mark.parametrize("scale", [0.0, 1.0, 1e-30, -1e-38, 3e-45])
+@pytest.mark.parametrize("tokens,window", [(1, 0), (3, 20)])
+def test_queries_and_scales_of_next_to_nothing(ctx, pkg, dim, heads, kv, scale, tokens, window):
+    """f32 queries down to the least number there is, with scales as small: scores of 0 to working precision, so a row is the mean of what it sees.
+    Rows of every size stand beside each other."""
+    p = Pair(ctx, pkg, np.random.default_rng(dim + tokens), 3, 5, 32, kv, dim)
+    p.append([130, 65, 7])
+    q = p.rng.standard_normal((3 * tokens, heads, dim))
+    sizes = np.array([0.0, 1e-45, 1e-42, 1e-39, 1e-35, 1e-20, 1.0])
+    q = (q * sizes[np.arange(q.shape[0] * heads) % len(sizes)].reshape(q.shape[0], heads, 1)).astype(np.float32)
+    got = p.gpu.attention(q, tokens, window, scale)
+    want, weight, size = p.ref.attention(q, p.lengths, tokens, window, scale or None)
+    k_most = 2 * float(np.nanmax(np.abs(p.ref.params[0].astype(np.float64)))) * 16
+    factor = abs(scale) * np.sqrt(dim) if scale else 1.0            # (the tolerance has the scale 1 / sqrt(dim) in it)
+    off = np.abs(got.astype(np.float64) - want) - tolerance(np.float32, q.astype(np.float64) * max(factor, 1e-30), int(p.lengths.max()), want, weight, size, k_most)
+    assert np.all(off <= 0), (float(off.max()), np.unravel_index(np.argmax(off), off.shape))
+    p.gpu.free()

@@ -26,6 +26,10 @@ constexpr int kScratchPrompt = 3;   // scratch slot of the parts
 
 constexpr int kScratchPadded = 8;   // ... and of the operands in rows of the matrix cores' kind
 
+// A factor of what a row sees is above 0, however small: where the type has no number for it, the least one stands in, so that an infinity times it
+// stays one. (A NaN stays a NaN.)
+__device__ __forceinline__ float above_zero(float w) { return w == 0.f ? 0x1p-149f : w; }
+
 // Heads too wide for the matrix cores, and calls without scratch memory for aligned rows: one wavefront per query row and head, a lane a channel of every
 // 64, KEYS keys on their way at once. Bound by the trips to memory: 1000 rows of 4 / 2 heads of 264 in f16 726 us, 1145 with one key at a time.
 template <typename T, int C>
@@ -69,7 +73,7 @@ __global__ void __launch_bounds__(64) prompt_rows_kernel(const PromptArgs a) {
             s[e] = lean_wave_sum(sum);
             if (t0 + e < to) grown = fmaxf(grown, s[e]);
         }
-        const float keep = m == -INFINITY ? 0.f : expf(m - grown);
+        const float keep = m == -INFINITY ? 0.f : above_zero(expf(m - grown));
         m = grown, l *= keep;
 #pragma unroll
         for (int i = 0; i < C; i++) acc[i] *= keep;
@@ -77,7 +81,7 @@ __global__ void __launch_bounds__(64) prompt_rows_kernel(const PromptArgs a) {
         for (int e = 0; e < KEYS; e++) {
             if (t0 + e >= to) break;
             // (a score of -inf has no weight, also before any other has one)
-            const float p = s[e] == -INFINITY ? 0.f : expf(s[e] - grown);
+            const float p = s[e] == -INFINITY ? 0.f : above_zero(expf(s[e] - grown));
             l += p;
 #pragma unroll
             for (int i = 0; i < C; i++) acc[i] = __builtin_fmaf(p, (float)v[e][i], acc[i]);
@@ -373,7 +377,7 @@ struct PromptRows {
             for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[b][r]);
         mx = halves_max(mx) * c2;
         if (__any(mx > m + kRescaleAt)) {
-            const float grown = mx > m + kRescaleAt ? mx : m, keep = grown == m ? 1.f : __builtin_amdgcn_exp2f(m - grown);   // (a row goes by its own scores)
+            const float grown = mx > m + kRescaleAt ? mx : m, keep = grown == m ? 1.f : above_zero(__builtin_amdgcn_exp2f(m - grown));   // (a row goes by its own scores)
             m = grown, l *= keep;
 #pragma unroll
             for (int i = 0; i < HC / 32; i++)
@@ -439,6 +443,59 @@ struct PromptRows {
         for (int ot = 0; ot < HC / 32; ot++)
 #pragma unroll
             for (int u = 0; u < KT / 16; u++) o[ot] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_part(vs, ot, u), p[u], o[ot], 0, 0, 0);
+    }
+    // Tiles that all rows see whole are not looked through, and an infinity under a weight that f16 rounded to zero has made NaN of its channel there. Where a
+    // row's sums (not its weights) are NaN, the values under them are read once more, and infinities of one sign stand for the sum. (Each wavefront by itself, behind
+    // the tiles: going over these again with every one looked through cost 2 % of 8192 rows' time and a microsecond of a short call's, this less than half of
+    // that. 8192 rows of 32 / 8 heads of 128 that all see a key whose values are NaN take 2.1 ms beside 0.6.)
+    __device__ __forceinline__ void settle(const PromptArgs &a, const PromptTile &pt, const PromptRow &pr, const PromptSpan &sp, int kvh, int c0) {
+        float most = 0.f;   // a NaN wins
+#pragma unroll
+        for (int i = 0; i < HC / 32; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) most = __builtin_elementwise_maximum(most, o[i][r]);
+        const bool odd = pr.mine && l == l && most != most;
+        if (__builtin_expect(!__any(odd), 1)) return;
+        // a bit for each of the lane's sums: it is NaN, and there is an infinity of that sign under it, or a NaN (both)
+        static_assert(HC / 2 <= 64, "of 64");
+        uint64_t left = 0, up = 0, down = 0;
+#pragma unroll
+        for (int i = 0; i < HC / 32; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                if (odd && o[i][r] != o[i][r]) left |= (uint64_t)1 << (16 * i + r);
+        const int from = max(pr.lane_begin, sp.t0 * KT), to = min(pr.lane_end, sp.t1 * KT);
+        while (left) {   // four channels at a time, eight keys on their way at once
+            const int at = __builtin_ctzll(left) & ~3, c = c0 + 32 * (at / 16) + 8 * (at / 4 % 4) + 4 * h;
+            const uint32_t sums = (uint32_t)(left >> at) & 15u;
+            const _Float16 *v = static_cast<const _Float16 *>(a.v) + a.v_stride * pt.k0 + (int64_t)kvh * a.dim + c;
+            uint32_t u = 0, d = 0;
+            for (int key = from; key < to && (u & d & sums) != sums && c < a.dim; key += 8) {
+                uint64_t w[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) w[e] = *reinterpret_cast<const uint64_t *>(v + a.v_stride * min(key + e, to - 1));
+#pragma unroll 1
+                for (int e = 0; e < 8; e++) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t bits = (uint32_t)(w[0] >> (16 * j)) & 0xffffu;
+                        if (bits > 0xfc00u || (bits >= 0x7c00u && bits < 0x8000u)) u |= 1u << j;                          // +inf, NaN
+                        if (bits >= 0xfc00u || (bits > 0x7c00u && bits < 0x8000u)) d |= 1u << j;                          // -inf, NaN
+                    }
+#pragma unroll
+                    for (int f = 0; f < 7; f++) w[f] = w[f + 1];
+                }
+            }
+            up |= (uint64_t)u << at, down |= (uint64_t)d << at;
+            left &= ~((uint64_t)15 << at);
+        }
+#pragma unroll
+        for (int i = 0; i < HC / 32; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const bool p = up >> (16 * i + r) & 1, n = down >> (16 * i + r) & 1;
+                if (odd && p != n && o[i][r] != o[i][r]) o[i][r] = p ? INFINITY : -INFINITY;
+            }
     }
 };
 
@@ -527,6 +584,7 @@ __global__ void __launch_bounds__(64 * W, 2) prompt_tiles_kernel(const PromptArg
         rows.weights(s, t * KT, masked, pr, p);
         rows.values(ks + TILE, t * KT, masked, pr, p);
     }
+    rows.settle(a, pt, pr, sp, kvh, c0);
     prompt_rows_out<_Float16, HC>(a, pt, pr, rows.h, c0, rows.m, rows.l, rows.o);
 }
 
@@ -569,6 +627,7 @@ __global__ void __launch_bounds__(64 * W, 2) prompt_few_kernel(const PromptArgs 
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (more) from.values_of(t + W, lds + TILE);
     }
+    rows.settle(a, pt, pr, sp, kvh, 0);   // (the keys of the workgroup's other wavefronts too: these add up)
     if (W == 1) {
         prompt_rows_out<_Float16, HD>(a, pt, pr, rows.h, 0, rows.m, rows.l, rows.o);
         return;
@@ -583,7 +642,7 @@ __global__ void __launch_bounds__(64 * W, 2) prompt_few_kernel(const PromptArgs 
     for (int w = 0; w < W; w++) best = fmaxf(best, ml[w][0][n]);
 #pragma unroll
     for (int w = 0; w < W; w++) sum += ml[w][1][n] == 0.f ? 0.f : ml[w][1][n] * __builtin_amdgcn_exp2f(ml[w][0][n] - best);
-    const float keep = rows.l == 0.f ? 0.f : __builtin_amdgcn_exp2f(rows.m - best);
+    const float keep = rows.l == 0.f ? 0.f : above_zero(__builtin_amdgcn_exp2f(rows.m - best));
     float4 *sums = reinterpret_cast<float4 *>(smem);   // [wavefront][four results of a lane][lane]
 #pragma unroll
     for (int i = 0; i < HD / 8; i++) {
@@ -767,7 +826,7 @@ __global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) prompt_ter
         for (int r = 1; r < 16; r++) mx = fmaxf(mx, s[r]);
         mx = halves_max(mx);
         if (__any(mx > m + kRescaleAt)) {
-            const float grown = mx > m + kRescaleAt ? mx : m, keep = grown == m ? 1.f : __builtin_amdgcn_exp2f(m - grown);
+            const float grown = mx > m + kRescaleAt ? mx : m, keep = grown == m ? 1.f : above_zero(__builtin_amdgcn_exp2f(m - grown));
             m = grown, l *= keep;
 #pragma unroll
             for (int i = 0; i < HC / 32; i++)
@@ -861,13 +920,13 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs a) {
 #pragma unroll
         for (int e = 0; e < AT_ONCE; e++)
             if (z0 + e < a.splits && ml[e].y != 0.f) most = fmaxf(most, ml[e].x);
-        const float before = m == most ? 1.f : __builtin_amdgcn_exp2f(m - most);
+        const float before = m == most ? 1.f : above_zero(__builtin_amdgcn_exp2f(m - most));
         m = most;
         if (l != 0.f) l *= before, acc.x *= before, acc.y *= before, acc.z *= before, acc.w *= before;
 #pragma unroll
         for (int e = 0; e < AT_ONCE; e++) {
             if (z0 + e >= a.splits || ml[e].y == 0.f) continue;   // (the range has nothing the row sees, and its part may hold anything)
-            const float keep = ml[e].x == m ? 1.f : __builtin_amdgcn_exp2f(ml[e].x - m);
+            const float keep = ml[e].x == m ? 1.f : above_zero(__builtin_amdgcn_exp2f(ml[e].x - m));
             l = __builtin_fmaf(ml[e].y, keep, l);
             acc.x = __builtin_fmaf(keep, o[e].x, acc.x), acc.y = __builtin_fmaf(keep, o[e].y, acc.y);
             acc.z = __builtin_fmaf(keep, o[e].z, acc.z), acc.w = __builtin_fmaf(keep, o[e].w, acc.w);

@@ -243,3 +243,31 @@ def test_many_keys_far_below_one(ctx, pkg, waves, split, dim, at):
     tol = tolerance(np.float16, dim, keys, want, weight, size) + keys * 2.0 ** -32 * (2.0 + np.abs(want))
     off = np.abs(got.astype(np.float64) - want) - tol
     assert np.all(off <= 0), (float(off.max()), float(got[0, 0, 1]), want[0, 0, 1])
+
+
+@pytest.mark.parametrize("dtype,waves,split,dim", [(np.float16, w, s, d) for w in (1, 2, 4, 8) for s in (1, 3) for d in (64, 256)] +
+                         [(np.float32, w, s, d) for w in (4, 8) for s in (1, 3) for d in (64, 256)] + [(np.float16, -1, -1, 264), (np.float32, -1, -1, 264), (np.float16, -1, -1, 100)])
+@pytest.mark.parametrize("kind", ["light", "outweighed later", "outweighed before"])
+def test_an_infinity_that_is_seen_reaches_the_row(ctx, pkg, dtype, waves, split, dim, kind):
+    """Whatever its key weighs: e^-30 of the others in a tile that all rows see, or e^-150 of one that comes later, or before. The channels it is not in are
+    as without."""
+    rng = np.random.default_rng(dim)
+    rows, keys, heads = 5, 700, 2
+    q, k, v = np.zeros((rows, heads, dim), dtype), np.zeros((keys, 1, dim), dtype), rng.standard_normal((keys, 1, dim)).astype(dtype)
+    q[:, :, 0] = np.sqrt(dim).astype(dtype)
+    k[:, 0, 0] = rng.uniform(-0.5, 0.5, keys)
+    odd = np.array([10, 11, 12, 13, 14]) + (500 if kind == "outweighed before" else 0)
+    if kind == "light":
+        k[odd, 0, 0] = -30.0
+    else:
+        k[20 if kind == "outweighed before" else 600, 0, 0] = 150.0
+    v[odd[0], 0, 0], v[odd[1], 0, 1] = np.inf, -np.inf
+    v[odd[2], 0, 2], v[odd[3], 0, 2] = np.inf, -np.inf
+    v[odd[4], 0, dim - 1] = np.nan
+    with ctx.options(HIPC_PROMPT_WAVES=waves, HIPC_PROMPT_SPLIT=split):
+        got = pkg.ops.prompt_attention(ctx, q, k, v, [rows], [keys]).astype(np.float64)
+    assert np.all(got[..., 0] == np.inf) and np.all(got[..., 1] == -np.inf) and np.isnan(got[..., 2]).all() and np.isnan(got[..., dim - 1]).all()
+    v[odd, 0, :3], v[odd, 0, dim - 1] = 0, 0
+    want, weight, size = ref.prompt(q, k, v, [rows], [keys])
+    off = np.abs(got - want) - tolerance(q.dtype, dim, keys, want, weight, size)
+    assert np.all(off[..., 3:dim - 1] <= 0), float(off[..., 3:dim - 1].max())

@@ -325,7 +325,7 @@ template <int HC, int KT, int PITCH>
 struct PromptRows {
     ph8 qf[HC / 16];
     pf16 o[HC / 32];
-    float m = -INFINITY, l = 0.f, c2;
+    float m = -INFINITY, l = 0.f, c2, down = -kWeightUp;   // down: what is taken off a score before the exponential
     uint32_t k_at[4], v_at[2];
     int h;
 
@@ -378,20 +378,19 @@ struct PromptRows {
         mx = halves_max(mx) * c2;
         if (__any(mx > m + kRescaleAt)) {
             const float grown = mx > m + kRescaleAt ? mx : m, keep = grown == m ? 1.f : above_zero(__builtin_amdgcn_exp2f(m - grown));   // (a row goes by its own scores)
-            m = grown, l *= keep;
+            m = grown, l *= keep, down = (m == -INFINITY ? 0.f : m) - kWeightUp;
 #pragma unroll
             for (int i = 0; i < HC / 32; i++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) o[i][r] *= keep;
         }
-        const float shift = (m == -INFINITY ? 0.f : m) - kWeightUp;
 #pragma unroll
         for (int u = 0; u < KT / 16; u++)
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
                 typedef float f2 __attribute__((ext_vector_type(2)));
-                const f2 w = {__builtin_amdgcn_exp2f(__builtin_fmaf(s[u / 2][8 * (u & 1) + j], c2, -shift)),
-                              __builtin_amdgcn_exp2f(__builtin_fmaf(s[u / 2][8 * (u & 1) + j + 1], c2, -shift))};
+                const f2 w = {__builtin_amdgcn_exp2f(__builtin_fmaf(s[u / 2][8 * (u & 1) + j], c2, -down)),
+                              __builtin_amdgcn_exp2f(__builtin_fmaf(s[u / 2][8 * (u & 1) + j + 1], c2, -down))};
                 const ph2 w16 = __builtin_convertvector(w, ph2);   // the second product's operand; the sum is that of the same rounded weights
                 p[u][j] = w16.x, p[u][j + 1] = w16.y;
                 l = __builtin_amdgcn_fdot2(w16, ph2{(_Float16)1.f, (_Float16)1.f}, l, false);
@@ -479,8 +478,8 @@ struct PromptRows {
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const uint32_t bits = (uint32_t)(w[0] >> (16 * j)) & 0xffffu;
-                        if (bits > 0xfc00u || (bits >= 0x7c00u && bits < 0x8000u)) u |= 1u << j;                          // +inf, NaN
-                        if (bits >= 0xfc00u || (bits > 0x7c00u && bits < 0x8000u)) d |= 1u << j;                          // -inf, NaN
+                        if (bits > 0xfc00u || (bits >= 0x7c00u && bits < 0x8000u)) u |= 1u << j;   // +inf, NaN
+                        if (bits >= 0xfc00u || (bits > 0x7c00u && bits < 0x8000u)) d |= 1u << j;   // -inf, NaN
                     }
 #pragma unroll
                     for (int f = 0; f < 7; f++) w[f] = w[f + 1];

@@ -431,7 +431,8 @@ typedef struct {
  * to 2^23 elements) are on 16 bytes, else through copies in scratch memory. Wider heads run on a kernel that computes in f32
  * on the vector units.
  * n_seqs <= 2^20; totals <= 2^30. Q, K and V may not overlap Y. With few rows, keys are shared by several workgroups whose
- * parts lie in scratch memory; a call recorded before any like it ran does without either (slower; another order of the sums).
+ * parts lie in scratch memory. A call recorded before any like it ran, or on a device without room for them, does without
+ * parts and copies (slower; another order of the sums).
  */
 int hipc_prompt_attention(hipc_ctx *ctx, const hipc_attention_heads *heads, int dtype, const void *Q, int64_t q_stride,
                           const void *K, int64_t k_stride, const void *V, int64_t v_stride, const void *q_starts,

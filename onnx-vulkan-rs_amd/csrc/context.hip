@@ -30,7 +30,11 @@ int scratch_get(hipc_ctx *ctx, int slot, size_t bytes, void **out) {
         s.ptr = nullptr;
         s.bytes = 0;
         size_t want = (bytes + 0xfffff) & ~(size_t)0xfffff;
-        HIPC_TRY(ctx, hipMalloc(&s.ptr, want));
+        if (const hipError_t e = hipMalloc(&s.ptr, want); e != hipSuccess) {
+            (void)hipGetLastError();   // (or the next launch would report it)
+            s.ptr = nullptr;
+            return fail(ctx, HIPC_ERR_BACKEND, "%zu bytes of scratch memory: %s", want, hipGetErrorString(e));
+        }
         s.bytes = want;
     }
     *out = s.ptr;

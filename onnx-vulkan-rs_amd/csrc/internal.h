@@ -326,6 +326,8 @@ __global__ void fill_words(uint32_t *dst, size_t words, uint32_t value);
 // whether it would: inside a capture only what the slot has grown to before. A call that was never run eagerly takes a route
 // that needs no scratch memory there, where it has one
 inline bool scratch_fits(const hipc_ctx *ctx, int slot, size_t bytes) { return !ctx->capturing || ctx->scratch[slot].bytes >= bytes; }
+// the block itself, or false where the slot does not hold it and it is not to be had: for calls that have a route without
+inline bool scratch_have(hipc_ctx *ctx, int slot, size_t bytes, void **out) { return scratch_fits(ctx, slot, bytes) && scratch_get(ctx, slot, bytes, out) == HIPC_OK; }
 // host bytes -> device through the context's pinned staging ring; records only (see StageRing)
 int stage_upload(hipc_ctx *ctx, void *dst, const void *host, size_t bytes);
 // looks up this device's address of the static range-partials array of the DynamicQuantizeLinear

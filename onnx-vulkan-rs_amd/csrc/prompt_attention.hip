@@ -30,7 +30,7 @@ constexpr int kScratchPadded = 8;   // ... and of the operands in rows of the ma
 // stays one. (A NaN stays a NaN.)
 __device__ __forceinline__ float above_zero(float w) { return w == 0.f ? 0x1p-149f : w; }
 
-// Heads too wide for the matrix cores, and calls without scratch memory for aligned rows: one wavefront per query row and head, a lane a channel of every
+// Heads too wide for the matrix cores, and calls without scratch memory for aligned rows (in a recording, or where the device has no more): one wavefront per query row and head, a lane a channel of every
 // 64, KEYS keys on their way at once. Bound by the trips to memory: 1000 rows of 4 / 2 heads of 264 in f16 726 us, 1145 with one key at a time.
 template <typename T, int C>
 __global__ void __launch_bounds__(64) prompt_rows_kernel(const PromptArgs a) {
@@ -965,16 +965,13 @@ size_t prompt_parts_bytes(const PromptArgs &a, int splits) { return splits > 1 ?
 
 // W == 1: the kernel for few rows; 2: the same with a wavefront by itself
 template <typename T, int HD, int W>
-int prompt_launch(hipc_ctx *ctx, PromptArgs a, int splits) {
+int prompt_launch(hipc_ctx *ctx, PromptArgs a, int splits, void *parts) {
     const int64_t tiles = ceil_div((int64_t)a.total_q * a.group, W <= 2 ? 32 : 32 * W / (HD > 128 ? 2 : 1)) + a.n_seqs;   // (at most: a sequence may leave one unfinished)
     a.tiles = (int)tiles, a.splits = splits;
     // (where all tiles run at once, their order is not worth the microsecond that it takes to find it)
     a.by_keys = W > 2 && a.causal && a.window == 0 && a.n_seqs > 1 && a.n_seqs <= 64 && tiles * (a.n_q_heads / a.group) > 2 * ctx->cu_count;
     if (splits > 1) {
-        const size_t rows = (size_t)splits * a.total_q * a.n_q_heads;
-        void *s = nullptr;
-        if (int rc = scratch_get(ctx, kScratchPrompt, prompt_parts_bytes(a, splits), &s)) return rc;
-        a.part_o = static_cast<float *>(s), a.part_ml = a.part_o + rows * a.dim;
+        a.part_o = static_cast<float *>(parts), a.part_ml = a.part_o + (size_t)splits * a.total_q * a.n_q_heads * a.dim;
     }
     const dim3 grid((unsigned)(tiles * (a.n_q_heads / a.group)), splits);
     if constexpr (sizeof(T) == 2 && W <= 2) hipLaunchKernelGGL((prompt_few_kernel<HD, W == 1 ? 4 : 1>), grid, W == 1 ? 256 : 64, 0, ctx->stream, a);
@@ -1028,15 +1025,16 @@ int prompt_matrix(hipc_ctx *ctx, const PromptArgs &a) {
         if (time < best) best = time, splits = s;
     }
     if (ctx->tune.prompt_split > 0) splits = std::min(ctx->tune.prompt_split, 256);
-    if (!scratch_fits(ctx, kScratchPrompt, prompt_parts_bytes(a, splits))) splits = 1;
+    void *parts = nullptr;
+    if (splits > 1 && !scratch_have(ctx, kScratchPrompt, prompt_parts_bytes(a, splits), &parts)) splits = 1;
     auto launch = [&](auto width) -> int {
         constexpr int HD = decltype(width)::value;
-        if (waves >= 8) return prompt_launch<T, HD, 8>(ctx, a, splits);
+        if (waves >= 8) return prompt_launch<T, HD, 8>(ctx, a, splits, parts);
         if constexpr (sizeof(T) == 2 && HD <= 128) {
-            if (waves == 1) return prompt_launch<T, HD, 1>(ctx, a, splits);
-            if (waves < 4) return prompt_launch<T, HD, 2>(ctx, a, splits);
+            if (waves == 1) return prompt_launch<T, HD, 1>(ctx, a, splits, parts);
+            if (waves < 4) return prompt_launch<T, HD, 2>(ctx, a, splits, parts);
         }
-        return prompt_launch<T, HD, 4>(ctx, a, splits);
+        return prompt_launch<T, HD, 4>(ctx, a, splits, parts);
     };
     // (96 beside 128: 6000 rows of 16 / 8 heads of 96 in f16 147 us, as heads of 128 166; two prompts of up to 1500 in f32 135 and 194. A wavefront of
     // its own for 160 channels spills: 119 us where 256 shared by two take 88.)
@@ -1091,9 +1089,8 @@ int hipc_prompt_attention(hipc_ctx *ctx, const hipc_attention_heads *heads, int 
                 at[i] = bytes;
                 if (pad[i]) bytes += (size_t)count[i] * of_heads[i] * dim8 * size;
             }
-            if (scratch_fits(ctx, kScratchPadded, bytes)) {
-                void *block = nullptr;
-                if (int rc = scratch_get(ctx, kScratchPadded, bytes, &block)) return rc;
+            void *block = nullptr;
+            if (scratch_have(ctx, kScratchPadded, bytes, &block)) {
                 PromptPadded in{{}, {}, {q_stride, k_stride, v_stride}, {a.q_starts, a.k_starts, a.k_starts}, {a.total_q, a.total_k, a.total_k}, {of_heads[0], of_heads[1], of_heads[2]}, a.n_seqs, a.dim, dim8 / 8};
                 PromptPadded out{{Y}, {static_cast<char *>(block) + at[3]}, {y_stride}, {a.q_starts}, {a.total_q}, {of_heads[3]}, a.n_seqs, a.dim, dim8 / 8};
                 PromptArgs m = a;

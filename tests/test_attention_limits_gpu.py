@@ -270,3 +270,20 @@ def test_rows_outside_the_sequences_when_keys_are_shared(ctx, pkg, dtype, split,
     check(y[3:51], q[3:51], k[:480], v[:480], [17, 0, 31], [300, 0, 180])
     for b in (dQ, dK, dV, dY, qs, ks):
         b.free()
+
+
+def test_copies_that_the_device_has_no_room_for(pkg):
+    """Operands that pass through scratch memory, declared so large (the rows behind the sequences are never touched) that it is not to be had: the call takes the way
+    without, and the ones behind it know nothing of that."""
+    rng = np.random.default_rng(6)
+    heads, dim, keys, total = 16, 250, 40, (1 << 26) - 4
+    q, k, v = operands(rng, np.float32, keys, keys, heads, heads, dim)
+    with pkg.Context(0) as ctx:
+        dQ, dK, dV, dY, dS = (ctx.upload(x) for x in (q, k, v, np.zeros_like(q), np.array([0, 7, keys], np.int32)))
+        h, w = pkg.AttentionHeads(heads, heads, dim, 1, 0, 0.0), heads * dim
+        for most in (total, keys, total):
+            ctx.fill(dY, 0, dY.nbytes, 0)
+            pkg.ops.prompt_attention_device(ctx, h, pkg.F32, dQ, w, dK, w, dV, w, dS, dS, 2, keys, most, dY, w)
+            check(ctx.download(dY, np.float32, q.shape), q, k, v, [7, keys - 7], [7, keys - 7])
+        for b in (dQ, dK, dV, dY, dS):
+            b.free()

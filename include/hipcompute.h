@@ -422,7 +422,8 @@ typedef struct {
  * A row that sees no key (a position below 0) is zero. Rows of Q and Y in front of the first and behind the last sequence are
  * neither read nor written. Starts ascend; they are held to [0, total], and a sequence that would end before it starts has no rows.
  * Keys and values that a row does not see do not enter its result, whatever they hold (infinities and NaN too). A row that sees an
- * infinity or a NaN gets what these make of it; in f32 an infinite query or key that a row sees makes it NaN.
+ * infinity or a NaN gets what these make of it; in f32 (up to 256 channels) an infinite query or key that a row sees makes it
+ * NaN. A row that sees keys but whose scores are all -inf has no weights: it is zero too.
  * f16: products of the f16 values as they are, sums in f32, softmax in f32, its weights rounded to f16 for the second
  * product and for the sum it is divided by: each is off by at most 2^-11 of itself or, below 2^-21 of the row's heaviest,
  * 2^-32 of that. f32: every factor as three bf16 terms (24 bits), sums in f32. Weighted values are summed before they are
@@ -480,8 +481,9 @@ int hipc_kv4_read(hipc_ctx *ctx, const hipc_kv4_cache *cache, int dtype, const v
  * lengths[s] - tokens + i. heads->causal has to be set; heads->n_kv_heads and head_dim are the cache's. A row that sees
  * nothing (an empty sequence, a position below 0) is zero. The cache's values enter exactly, f16 queries too, f32 queries
  * with 22 bits of a row's largest value; weights with 22 bits; sums in f32. tokens * n_q_heads / n_kv_heads <= 1024.
- * The order of the sums is fixed by the shapes, the lengths and the device: results repeat bit for bit. The call needs a scratch block of
- * fixed size: run one on the context before recording one.
+ * An infinite query makes its row NaN, or, in f16 where all its scores are -inf, zero. The order of the sums is fixed by the
+ * shapes, the lengths and the device: results repeat bit for bit. The call needs a scratch block whose size goes by the device alone
+ * (258 KiB a CU, 65 MiB for 256), allocated by the first one: run one on the context before recording one.
  */
 int hipc_kv4_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_attention_heads *heads, int dtype, int64_t tokens,
                        const void *Q, int64_t q_stride, void *Y, int64_t y_stride);
@@ -498,8 +500,8 @@ int hipc_kv4_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_at
  *   top_ids [rows, top] i32, top_logprobs [rows, top] f32: the `top` (0 to HIPC_TOP_MAX) largest logits, largest first, the lower id
  *                            first among equals; NaN never counts; where fewer than `top` logits compare the rest is -1 and NaN
  * A row without a finite largest logit (all -inf, a +inf or a NaN in it) has no distribution: its logprob, entropy and
- * top_logprobs are NaN. The logits are read once. vocab <= 2^30. Few rows are shared by several workgroups, which need a scratch block of fixed
- * size; a call recorded before any other ran does without (another order of the sums).
+ * top_logprobs are NaN. The logits are read once. vocab <= 2^30. Few rows are shared by several workgroups, which need a scratch
+ * block of 1 MiB; a call recorded before any other ran does without (another order of the sums).
  */
 #define HIPC_TOP_MAX 32
 int hipc_token_logprobs(hipc_ctx *ctx, int dtype, const void *logits, int64_t row_stride, int64_t rows, int64_t vocab,

@@ -427,3 +427,25 @@ def test_queries_and_scales_of_next_to_nothing(ctx, pkg, dim, heads, kv, scale, 
     off = np.abs(got.astype(np.float64) - want) - tolerance(np.float32, q.astype(np.float64) * max(factor, 1e-30), int(p.lengths.max()), want, weight, size, k_most)
     assert np.all(off <= 0), (float(off.max()), np.unravel_index(np.argmax(off), off.shape))
     p.gpu.free()
+
+
+def test_an_infinite_query(ctx, pkg):
+    """f16: NaN, or zero where all its scores are -inf; f32: NaN. The rows beside it are as without."""
+    p = Pair(ctx, pkg, np.random.default_rng(31), 2, 4, 16, 1, 64)
+
+    def change(k, v):
+        k[..., 0] = -1 - np.abs(k[..., 0])
+
+    p.append([50, 20], np.float16, change)
+    for dtype in (np.float16, np.float32):
+        q = p.rng.standard_normal((2, 3, 64)).astype(dtype)
+        want = p.gpu.attention(q)
+        q[0, 1] = 0
+        q[0, 1, 0] = np.inf
+        got = p.gpu.attention(q)
+        assert not got[0, 1].any() if dtype == np.float16 else np.isnan(got[0, 1]).all()
+        q[0, 1, 0] = -np.inf
+        assert np.isnan(p.gpu.attention(q)[0, 1]).all()
+        got[0, 1] = want[0, 1]
+        assert np.array_equal(bits(got), bits(want))
+    p.gpu.free()

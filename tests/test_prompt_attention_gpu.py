@@ -271,3 +271,26 @@ def test_an_infinity_that_is_seen_reaches_the_row(ctx, pkg, dtype, waves, split,
     want, weight, size = ref.prompt(q, k, v, [rows], [keys])
     off = np.abs(got - want) - tolerance(q.dtype, dim, keys, want, weight, size)
     assert np.all(off[..., 3:dim - 1] <= 0), float(off[..., 3:dim - 1].max())
+
+
+@pytest.mark.parametrize("dtype,waves,split,dim", [(np.float16, w, s, 64) for w in (1, 2, 4, 8) for s in (1, 3)] + [(np.float16, 4, 1, 256), (np.float16, -1, -1, 264),
+                                                   (np.float32, -1, -1, 264), (np.float32, -1, -1, 64)])
+def test_rows_whose_scores_are_all_minus_infinity(ctx, pkg, dtype, waves, split, dim):
+    """They have no weights and are zero (f32 on the matrix cores: NaN, as whatever sees an infinite query); a NaN among the scores makes NaN."""
+    rng = np.random.default_rng(dim)
+    q, k, v = operands(rng, dtype, 9, 200, 2, 1, dim)
+    q[3], k[:, 0, 0] = 0, -1 - rng.random(200).astype(dtype)
+    q[3, :, 0] = np.inf                                       # against -1 .. -2
+    q[5] = q[3]
+    q[5, :, 1] = np.nan
+    with ctx.options(HIPC_PROMPT_WAVES=waves, HIPC_PROMPT_SPLIT=split):
+        got = pkg.ops.prompt_attention(ctx, q, k, v, [9], [200])
+    if dtype == np.float32 and dim == 64:
+        assert np.isnan(got[3]).all()
+    else:
+        assert not got[3].any()
+    assert np.isnan(got[5]).all()
+    q[[3, 5]], got[[3, 5]] = 0, 0
+    keep = [0, 1, 2, 4, 6, 7, 8]
+    want, weight, size = ref.prompt(q, k, v, [9], [200])
+    assert np.all(np.abs(got.astype(np.float64) - want)[keep] <= tolerance(q.dtype, dim, 200, want, weight, size)[keep])

@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(256) prompt_pad_kernel(const PromptPadded a) {
 // The running maximum is let grow by up to 2^8 before sums are rescaled, and weights are kept 2^7 times as large: up to 2^15 in f16, whose ordinary
 // numbers then reach down to 2^-21 of the heaviest weight and whose subnormal ones, off by up to 2^-32 of it, to 2^-31. (Around 1, f16 loses weights below
 // 2^-25: of 60000 keys that together weigh 2^-10 of one more, all.) That weights are rounded to f16 at all is a choice: as two terms each they would take half as
-// many products again of a kernel that these bound, to bring errors of 1.2 to 1.35 times what rounding the results alone makes down to that.
+// many products again of a kernel that these bound, to bring errors of 1.1 to 1.35 times what rounding the results alone makes down to that.
 // Tiles of K and V go from memory to LDS without a register, one tile ahead; 16-byte chunks of a row lie at chunk ^ f(row), so
 // that the eight (K) and four (V) rows a read takes per cycle lie in different banks. Chunks behind head_dim and rows behind the
 // sequence are zeros (the buffer's range check).

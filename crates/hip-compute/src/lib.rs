@@ -20,7 +20,7 @@ use std::ffi::{CStr, CString};
 use std::os::raw::{c_int, c_void};
 use std::ptr;
 
-pub use sys::{hipc_attention_heads as AttentionHeads, hipc_conv_geom as ConvGeom, hipc_decoder_config as DecoderConfig, hipc_kv4_cache as Kv4Cache, HIPC_TOP_MAX};
+pub use sys::{hipc_attention_heads as AttentionHeads, hipc_conv_geom as ConvGeom, hipc_decoder_config as DecoderConfig, hipc_kv4_cache as Kv4Cache, hipc_rotary_heads as RotaryHeads, hipc_rotary_scaling as RotaryScaling, HIPC_TOP_MAX};
 
 /// What went wrong, in the interpreter's terms.
 #[derive(Clone, Copy, Debug, PartialEq, Eq)]
@@ -586,6 +586,32 @@ impl HipContext {
         })
     }
 
+    // --------------------------- norms and positions of queries and keys
+
+    /// Query and key heads of `rows` rows normed and turned by `positions` [rows] i32 (on the device); `q_out` and `k_out` may be `q` and `k`.
+    pub fn rotary(
+        &self, heads: &RotaryHeads, dtype: DType, positions: BufferSlice<'_>, rows: i64, q: Rows<'_>, k: Rows<'_>, q_out: Rows<'_>, k_out: Rows<'_>,
+    ) -> Result<()> {
+        self.check(unsafe {
+            sys::hipc_rotary(
+                self.raw, heads, dtype.raw(), positions.ptr(), rows, q.at.ptr(), q.stride, k.at.ptr(), k.stride, q_out.at.ptr(), q_out.stride,
+                k_out.at.ptr(), k_out.stride,
+            )
+        })
+    }
+    /// `rotary` and `kv4_append` in one pass: queries to `q_out`, keys and values into the cache.
+    pub fn kv4_append_rotary(
+        &self, cache: &Kv4Cache, heads: &RotaryHeads, dtype: DType, starts: BufferSlice<'_>, total: i64, q: Rows<'_>, k: Rows<'_>, v: Rows<'_>,
+        q_out: Rows<'_>,
+    ) -> Result<()> {
+        self.check(unsafe {
+            sys::hipc_kv4_append_rotary(
+                self.raw, cache, heads, dtype.raw(), starts.ptr(), total, q.at.ptr(), q.stride, k.at.ptr(), k.stride, v.at.ptr(), v.stride,
+                q_out.at.ptr(), q_out.stride,
+            )
+        })
+    }
+
     // ------------------------- attention over prompts and a cache in 4 bits
 
     /// Prompts of different lengths packed one behind the other (`GroupQueryAttention`'s prompt form, interp.rs:7514-7949):
@@ -694,6 +720,16 @@ pub fn read_initializer(tensor: &[u8], base_dir: Option<&std::path::Path>) -> Re
     }
     let name = unsafe { CStr::from_ptr(info.name.as_ptr()) }.to_string_lossy().into_owned();
     Ok(Initializer { name, dtype: info.data_type, shape: info.dims[..info.n_dims as usize].to_vec(), data })
+}
+
+/// The frequencies of a rotation of `rotary_dim` channels, stretched for longer contexts or (`None`) as they are.
+pub fn rotary_frequencies(theta: f64, rotary_dim: i32, scaling: Option<&RotaryScaling>) -> Result<Vec<f32>> {
+    let mut out = vec![0f32; rotary_dim.max(0) as usize / 2];
+    let rc = unsafe { sys::hipc_rotary_frequencies(theta, rotary_dim, scaling.map_or(ptr::null(), |s| s), out.as_mut_ptr()) };
+    if rc != sys::HIPC_OK {
+        return Err(host_error(rc));
+    }
+    Ok(out)
 }
 
 /// Every initializer of a serialized `ModelProto`, in file order (`model_to_ir`, `convert.rs:51-76`):

@@ -60,6 +60,37 @@ pub struct hipc_attention_heads {
     pub scale: f32,
 }
 
+/// how query and key heads are normed and turned by their positions
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct hipc_rotary_heads {
+    pub n_q_heads: i32,
+    pub n_kv_heads: i32,
+    pub head_dim: i32,
+    pub rotary_dim: i32,
+    pub interleaved: i32,
+    pub norm_eps: f32,
+    pub amplitude: f32,
+    pub frequencies: *const c_void,
+    pub q_norm: *const c_void,
+    pub k_norm: *const c_void,
+}
+
+pub const HIPC_ROTARY_LINEAR: i32 = 1;
+pub const HIPC_ROTARY_BASE: i32 = 2;
+pub const HIPC_ROTARY_BY_PARTS: i32 = 3;
+
+/// how frequencies are stretched for longer contexts
+#[repr(C)]
+#[derive(Clone, Copy, Debug, Default, PartialEq)]
+pub struct hipc_rotary_scaling {
+    pub kind: i32,
+    pub factor: f32,
+    pub trained: f32,
+    pub slow: f32,
+    pub fast: f32,
+}
+
 /// a paged cache of keys and values in 4 bits, and whose pages are whose
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
@@ -242,6 +273,13 @@ unsafe extern "C" {
     ) -> c_int;
     pub fn hipc_host_error() -> *const c_char;
 
+    // ---- norms and positions of queries and keys
+    pub fn hipc_rotary_frequencies(theta: f64, rotary_dim: i32, scaling: *const hipc_rotary_scaling, frequencies: *mut f32) -> c_int;
+    pub fn hipc_rotary(
+        ctx: *mut hipc_ctx, heads: *const hipc_rotary_heads, dtype: c_int, positions: *const c_void, rows: i64, q: *const c_void,
+        q_stride: i64, k: *const c_void, k_stride: i64, q_out: *mut c_void, q_out_stride: i64, k_out: *mut c_void, k_out_stride: i64,
+    ) -> c_int;
+
     // ---- attention over prompts and a cache in 4 bits
     pub fn hipc_prompt_attention(
         ctx: *mut hipc_ctx, heads: *const hipc_attention_heads, dtype: c_int, q: *const c_void, q_stride: i64, k: *const c_void,
@@ -251,6 +289,10 @@ unsafe extern "C" {
     pub fn hipc_kv4_append(
         ctx: *mut hipc_ctx, cache: *const hipc_kv4_cache, dtype: c_int, starts: *const c_void, total: i64, k: *const c_void,
         k_stride: i64, v: *const c_void, v_stride: i64,
+    ) -> c_int;
+    pub fn hipc_kv4_append_rotary(
+        ctx: *mut hipc_ctx, cache: *const hipc_kv4_cache, heads: *const hipc_rotary_heads, dtype: c_int, starts: *const c_void, total: i64,
+        q: *const c_void, q_stride: i64, k: *const c_void, k_stride: i64, v: *const c_void, v_stride: i64, q_out: *mut c_void, q_out_stride: i64,
     ) -> c_int;
     pub fn hipc_kv4_read(
         ctx: *mut hipc_ctx, cache: *const hipc_kv4_cache, dtype: c_int, starts: *const c_void, total: i64, k: *mut c_void,

@@ -392,8 +392,56 @@ int hipc_initializer_read(const void *tensor, size_t len, const char *base_dir, 
  * graph is HIPC_ERR_INVALID, one with sparse initializers HIPC_ERR_UNSUPPORTED, as in the reference. */
 int hipc_model_initializers(const void *model, size_t len, size_t *offsets, size_t *sizes, int64_t cap,
                             int64_t *count);
-/* message of the last failed host-only call (the two above) on the calling thread */
+/* message of the last failed host-only call (the two above, hipc_rotary_frequencies) on the calling thread */
 const char *hipc_host_error(void);
+
+/* -------------------------------------------- norms and positions of queries and keys */
+
+/*
+ * What stands between a projection and attention: query and key heads are normed, each by itself, and turned by their row's position
+ * (SimplifiedLayerNormalization over a head, shaders/normalization.rs:109-181, and the rotary embedding of GroupQueryAttention,
+ * shaders/attention.rs:128-317, which the decode step does inside its launch):
+ *   x^ = x / sqrt(mean(x^2) + norm_eps) * w                             where there are weights w (q_norm, k_norm), else x
+ *   y_a = A (x^_a cos t - x^_b sin t),  y_b = A (x^_b cos t + x^_a sin t),  t = position * frequencies[i], A the amplitude
+ * for the pairs i = 0 .. rotary_dim / 2 - 1 of a head: channels (a, b) = (i, i + rotary_dim / 2), or (2i, 2i + 1) where interleaved.
+ * Channels from rotary_dim on do not turn.
+ */
+typedef struct {
+    int32_t n_q_heads, n_kv_heads, head_dim; /* either count may be 0 (hipc_rotary); head_dim up to 512 */
+    int32_t rotary_dim;                      /* even, 0 to head_dim */
+    int32_t interleaved;
+    float norm_eps;
+    float amplitude;                         /* 0 => 1 */
+    const void *frequencies;                 /* [rotary_dim / 2] f32 on the device, radians a position */
+    const void *q_norm, *k_norm;             /* [head_dim] f32 on the device, or NULL: not normed */
+} hipc_rotary_heads;
+
+/* The frequencies theta^(-2i / rotary_dim), formed in 64 bits and rounded once; `scaling` NULL, or how they are stretched for
+ * contexts `factor` (1 or more) times as long as the model was trained on:
+ *   LINEAR    every frequency divided by factor (positions divided by it)
+ *   BASE      theta times factor^(rotary_dim / (rotary_dim - 2)): the slowest pair as LINEAR has it, the fastest as it was
+ *   BY_PARTS  with r turns over `trained` positions: pairs of fewer than `slow` turns as LINEAR, of more than `fast` as they were,
+ *             between them both, weighed by (r - slow) / (fast - slow)
+ * (What a model multiplies its cosines with goes to `amplitude`: 0.1 ln factor + 1 is usual with BY_PARTS.)
+ * Host code only (no context): writes rotary_dim / 2 numbers; a failed call leaves its message in hipc_host_error. */
+#define HIPC_ROTARY_LINEAR 1
+#define HIPC_ROTARY_BASE 2
+#define HIPC_ROTARY_BY_PARTS 3
+typedef struct {
+    int32_t kind;
+    float factor, trained, slow, fast;   /* the last three: BY_PARTS */
+} hipc_rotary_scaling;
+int hipc_rotary_frequencies(double theta, int32_t rotary_dim, const hipc_rotary_scaling *scaling, float *frequencies);
+
+/*
+ * Q [rows, n_q_heads, head_dim] and K [rows, n_kv_heads, head_dim], f16 or f32, rows *_stride elements apart (parts of one projection's
+ * rows, for instance), to Q_out and K_out; these may be Q and K themselves (same address and stride) and else overlap nothing.
+ * positions [rows] i32 on the device, of any sign (a key that is to stand n positions earlier is turned by -n). Angles are
+ * formed in 64 bits, a position's product with the f32 frequency off by less than 2^-51 of itself; queries are computed in f32 and rounded once;
+ * keys in 64 bits and rounded once, so that what a cache quantizes does not hang on the order of a sum.
+ */
+int hipc_rotary(hipc_ctx *ctx, const hipc_rotary_heads *heads, int dtype, const void *positions, int64_t rows, const void *Q, int64_t q_stride,
+                const void *K, int64_t k_stride, void *Q_out, int64_t q_out_stride, void *K_out, int64_t k_out_stride);
 
 /* ------------------------------------------ attention over prompts and a cache in 4 bits */
 
@@ -471,7 +519,15 @@ typedef struct {
  */
 int hipc_kv4_append(hipc_ctx *ctx, const hipc_kv4_cache *cache, int dtype, const void *starts, int64_t total, const void *K,
                     int64_t k_stride, const void *V, int64_t v_stride);
-/* Read the rows back as the values they stand for (exact in f16, widened in f32): the same arguments, K / V are written.
+/*
+ * hipc_rotary and hipc_kv4_append in one pass: the rows' queries go to Q_out (which may be Q itself), keys and values into the cache, bit for
+ * bit what hipc_rotary at the positions that hipc_kv4_append gives the rows leaves behind. Rows outside every sequence are left as they
+ * are; keys and values of rows without a place are not stored, their queries are turned all the same. heads->n_kv_heads and head_dim are the cache's.
+ */
+int hipc_kv4_append_rotary(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_rotary_heads *heads, int dtype, const void *starts, int64_t total,
+                           const void *Q, int64_t q_stride, const void *K, int64_t k_stride, const void *V, int64_t v_stride, void *Q_out,
+                           int64_t q_out_stride);
+/* Read rows back as the values they stand for (exact in f16, widened in f32): the arguments of hipc_kv4_append, K / V are written.
  * A row at a position below 0, or on no page, is zero; rows outside every sequence are left as they are. */
 int hipc_kv4_read(hipc_ctx *ctx, const hipc_kv4_cache *cache, int dtype, const void *starts, int64_t total, void *K,
                   int64_t k_stride, void *V, int64_t v_stride);

@@ -16,6 +16,8 @@ from .runtime import (  # noqa: F401
     DecoderConfig,
     AttentionHeads,
     Kv4Cache,
+    RotaryHeads,
+    RotaryScaling,
     library_path,
     load_library,
     F32, F16, U8, I8, I32,

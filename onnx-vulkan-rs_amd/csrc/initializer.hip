@@ -26,9 +26,11 @@
 #include "../../include/hipcompute.h"
 
 namespace {
-
 thread_local std::string g_host_error;
+}
 
+namespace hipc {
+// (declared in internal.h, for the other calls without a context)
 int host_fail(int code, const char *fmt, ...) {
     char buf[512];
     va_list ap;
@@ -38,6 +40,11 @@ int host_fail(int code, const char *fmt, ...) {
     g_host_error = buf;
     return code;
 }
+}  // namespace hipc
+
+namespace {
+
+using hipc::host_fail;
 
 // TensorProto.DataType
 enum : int32_t {

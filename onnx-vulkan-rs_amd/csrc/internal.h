@@ -199,6 +199,9 @@ inline int fail(hipc_ctx *ctx, int code, const char *fmt, ...) {
     return code;
 }
 
+// the same for calls without a context: the message goes to hipc_host_error (initializer.hip)
+int host_fail(int code, const char *fmt, ...);
+
 // RAII: serialise the call and make the context's device current.
 struct Guard {
     std::unique_lock<std::mutex> lock;

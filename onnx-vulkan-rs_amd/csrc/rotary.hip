@@ -1,0 +1,414 @@
+// Norms of query and key heads and their rotation by position (hipc_rotary), and the same on the way into the 4-bit cache
+// (hipc_kv4_append_rotary).
+//
+//   x^ = x / sqrt(mean(x^2) + eps) * w                                (per head, where there is a weight w)
+//   y_a = x^_a cos - x^_b sin,  y_b = x^_b cos + x^_a sin              (a, b) = (i, i + n) or (2i, 2i + 1), angle = position * frequency[i]
+//
+// A position's angles are one row's and all its heads'. They are formed in 64 bits: in 32 an angle of a million is off by a sixteenth. A product of
+// 31 and 24 bits, in turns; what is left behind whole turns goes to sine and cosine. Queries are then computed in 32 bits. Keys are computed in 64 up to their
+// one rounding, because a cache stores what they are quantized to: a key next to the border between two codes, or that is the lowest of
+// its group, would fall on either side by the order of a sum.
+//
+// Memory bounds it. A wavefront has a row, or some heads of one where rows are few, and takes 64 / L heads at a time, L lanes a head; a lane has a
+// vector of V channels and the V channels they turn with, the same channels of every head it sees, so that its cosines and sines stay in registers.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "kv4.h"
+#include "lanes.h"
+
+namespace hipc {
+
+namespace {
+
+constexpr int kRotaryMaxHead = 512;
+
+struct RotaryArgs {
+    hipc_kv4_cache cache;              // storing
+    const int *starts, *positions;     // ... and its rows; or the rows' positions
+    const void *q, *k, *v;
+    void *q_out, *k_out;
+    int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
+    const float *frequencies, *q_norm, *k_norm;
+    int rows, n_q, n_kv, dim, half, interleaved;
+    int lg_lanes, chunks, per;         // lanes of a head (a power of two); wavefronts of a row, and what each takes of it
+    float eps;
+    double amplitude;
+};
+
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, true), hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, true);
+    return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) { return v + lean_dpp<CTRL>(v); }
+// the sum over 2^lg neighbouring lanes, in all of them (lg is uniform)
+template <typename F>
+__device__ __forceinline__ F lanes_sum(F v, int lg) {
+    if (lg > 0) v = dpp_add<0xB1>(v);    // quad_perm [1,0,3,2]
+    if (lg > 1) v = dpp_add<0x4E>(v);    // quad_perm [2,3,0,1]
+    if (lg > 2) v = dpp_add<0x141>(v);   // the other four of eight (mirrored)
+    if (lg > 3) v = dpp_add<0x140>(v);   // the other eight of sixteen
+    if (lg > 4) v += __shfl_xor(v, 16);
+    if (lg > 5) v += __shfl_xor(v, 32);
+    return v;
+}
+
+// one rounding to the rows' type
+__device__ __forceinline__ void rounded(double d, float *out) { *out = (float)d; }
+__device__ __forceinline__ void rounded(double d, _Float16 *out) {
+    // through f32 rounded to odd: what lies between two f32 numbers takes the odd one, so that the second rounding sees on which side of a tie it was
+    float f = (float)d;
+    uint32_t bits = __float_as_uint(f);
+    const double back = (double)f;
+    if (back != d && d - d == 0.0 && !(bits & 1)) bits += __builtin_fabs(d) > __builtin_fabs(back) ? 1 : -1;
+    *out = (_Float16)__uint_as_float(bits);
+}
+__device__ __forceinline__ void rounded(float f, float *out) { *out = f; }
+__device__ __forceinline__ void rounded(float f, _Float16 *out) { *out = (_Float16)f; }
+
+__device__ __forceinline__ float one_over_root(float v) { return 1.f / sqrtf(v); }
+__device__ __forceinline__ double one_over_root(double v) { return 1.0 / sqrt(v); }
+__device__ __forceinline__ float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
+
+// V values side by side; rows and strides lie on 16 bytes (V values, where these are less) or V is 1
+template <typename T, int V>
+struct RotaryVector {
+    typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T) * V < 16 ? sizeof(T) * V : 16)));
+};
+template <typename T>
+struct RotaryVector<T, 1> {
+    typedef T type;
+};
+template <typename T, int V>
+__device__ __forceinline__ void rotary_load(const T *p, T (&x)[V]) {
+    const auto v = *reinterpret_cast<const typename RotaryVector<T, V>::type *>(p);
+    __builtin_memcpy(x, &v, sizeof x);
+}
+template <typename T, int V>
+__device__ __forceinline__ void rotary_store(T *p, const T (&x)[V]) {
+    typename RotaryVector<T, V>::type v;
+    __builtin_memcpy(&v, x, sizeof x);
+    *reinterpret_cast<typename RotaryVector<T, V>::type *>(p) = v;
+}
+
+// what this wavefront has stored to its LDS is there for its other lanes
+__device__ __forceinline__ void wave_meets() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <typename T, int V, bool STORE>
+__global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
+    constexpr int E = V == 1 ? 4 : 1;            // items of a lane: V channels and the V they turn with, or 2 V behind those that turn
+    constexpr int N = 2 * V * E, UNITS = N / 8;   // a lane's values at a time; as units of eight side by side
+    __shared__ double2 turns[4][kRotaryMaxHead / 2];
+    __shared__ float keys[STORE ? 4 : 1][STORE ? 64 * N : 1];
+    const int w = kv4_wave(), lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = w / a.chunks, chunk = w - row * a.chunks;
+    if (row >= a.rows) return;
+    int position;
+    Kv4Place place = {0, false};
+    if (STORE) {
+        int seq, first, end;
+        if (!packed_sequence(a.starts, a.cache.n_seqs, a.rows, row, &seq, &first, &end)) return;
+        position = kv4_length(a.cache, seq) - end + row;
+        place = kv4_place(a.cache, seq, position);
+    } else {
+        position = a.half > 0 ? a.positions[row] : 0;
+    }
+
+    // what this wavefront takes: the query heads, then the key heads, then (storing) units of the values
+    const int lanes = 1 << a.lg_lanes, together = 64 >> a.lg_lanes, l = lane & (lanes - 1), head0 = lane >> a.lg_lanes;
+    const int q_passes = (a.n_q + together - 1) >> (6 - a.lg_lanes), k_passes = (a.n_kv + together - 1) >> (6 - a.lg_lanes);
+    const int v_units = STORE ? a.n_kv * (a.dim >> 3) : 0, v_passes = STORE ? (v_units + 64 * UNITS - 1) / (64 * UNITS) : 0;
+    const int passes = STORE && !place.there ? q_passes : q_passes + k_passes + v_passes;
+    const int pass0 = chunk * a.per, pass1 = min(pass0 + a.per, passes);
+    if (pass0 >= pass1) return;
+
+    // the lane's channels of a head: at c[e][0] and c[e][1], V each (none: -1); the pairs they turn with
+    int c[E][2], pair[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int item = l + (e << a.lg_lanes), turning = a.half / V;
+        pair[e] = item < turning ? item * V : -1;
+        c[e][0] = item < turning && !a.interleaved ? item * V : 2 * item * V;   // (behind the pairs, 2 V an item as well)
+        c[e][1] = item < turning && !a.interleaved ? a.half + item * V : 2 * item * V + V;
+        if (c[e][0] >= a.dim) c[e][0] = -1;
+        if (c[e][1] >= a.dim) c[e][1] = -1;
+    }
+    auto load = [&](int pass, T (&x)[N]) {
+        if (STORE && pass >= q_passes + k_passes) {
+#pragma unroll
+            for (int i = 0; i < N; i += V) {
+                const int u = ((pass - q_passes - k_passes) * UNITS + i / 8) * 64 + lane;
+                T v[V] = {};
+                if (u < v_units) rotary_load<T, V>(static_cast<const T *>(a.v) + a.v_stride * row + (int64_t)u * 8 + i % 8, v);
+#pragma unroll
+                for (int j = 0; j < V; j++) x[i + j] = v[j];
+            }
+            return;
+        }
+        const bool key = pass >= q_passes;
+        const int head = (key ? pass - q_passes : pass) * together + head0;
+        const T *from = static_cast<const T *>(key ? a.k : a.q) + (key ? a.k_stride : a.q_stride) * row + (int64_t)head * a.dim;
+#pragma unroll
+        for (int i = 0; i < 2 * E; i++) {
+            T v[V] = {};
+            if (head < (key ? a.n_kv : a.n_q) && c[i / 2][i % 2] >= 0) rotary_load<T, V>(from + c[i / 2][i % 2], v);
+#pragma unroll
+            for (int j = 0; j < V; j++) x[i * V + j] = v[j];
+        }
+    };
+    T next[N];
+    load(pass0, next);
+
+    // the angles, a pair a lane, while the first heads are on their way
+    for (int p = lane; p < a.half; p += 64) {
+        const double turn = (double)position * (double)a.frequencies[p] * 0.15915494309189533577;   // 1 / (2 pi)
+        double s, co;
+        sincospi(2.0 * (turn - __builtin_rint(turn)), &s, &co);
+        turns[wave][p] = make_double2(co * a.amplitude, s * a.amplitude);
+    }
+    wave_meets();
+    float cos32[E][V], sin32[E][V];
+#pragma unroll
+    for (int e = 0; e < E; e++)
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const double2 t = pair[e] >= 0 ? turns[wave][pair[e] + j] : make_double2(1.0, 0.0);
+            cos32[e][j] = (float)t.x, sin32[e][j] = (float)t.y;
+        }
+
+    // the lane's values of a head, normed and turned in F: the same steps for queries (32 bits) and keys (64)
+    auto turned = [&](auto zero, const T (&x)[N], const float *weight, auto cosine, auto sine, T (&y)[N]) {
+        typedef decltype(zero) F;
+        F v[N];
+        F sum = zero;
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = (F)(float)x[i], sum = fused(v[i], v[i], sum);
+        if (weight) {
+            const F by = one_over_root(lanes_sum(sum, a.lg_lanes) / (F)a.dim + (F)a.eps);
+#pragma unroll
+            for (int i = 0; i < 2 * E; i++)
+#pragma unroll
+                for (int j = 0; j < V; j++)
+                    if (c[i / 2][i % 2] >= 0) v[i * V + j] = v[i * V + j] * by * (F)weight[c[i / 2][i % 2] + j];
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++)
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                // (one of an item's halves and the other's, or its neighbours)
+                const F half_a = v[2 * e * V + j], half_b = v[(2 * e + 1) * V + j], near_a = v[2 * e * V + 2 * j], near_b = v[2 * e * V + 2 * j + 1];
+                const F p = a.interleaved ? near_a : half_a, q = a.interleaved ? near_b : half_b, co = cosine(e, j), s = sine(e, j);
+                const F first = fused(p, co, -(q * s)), second = fused(q, co, p * s);
+                if (a.interleaved) {
+                    rounded(pair[e] >= 0 ? first : near_a, &y[2 * e * V + 2 * j]);
+                    rounded(pair[e] >= 0 ? second : near_b, &y[2 * e * V + 2 * j + 1]);
+                } else {
+                    rounded(pair[e] >= 0 ? first : half_a, &y[2 * e * V + j]);
+                    rounded(pair[e] >= 0 ? second : half_b, &y[(2 * e + 1) * V + j]);
+                }
+            }
+    };
+    auto put = [&](T *to, const T (&y)[N]) {
+#pragma unroll
+        for (int i = 0; i < 2 * E; i++) {
+            T v[V];
+#pragma unroll
+            for (int j = 0; j < V; j++) v[j] = y[i * V + j];
+            if (c[i / 2][i % 2] >= 0) rotary_store<T, V>(to + c[i / 2][i % 2], v);
+        }
+    };
+    // unit u of the row's heads, of keys or of values, into the cache
+    auto quantize = [&](int u, bool mine, float (&x)[8], void *codes, void *params) {
+        uint32_t bits;
+        const uint32_t param = kv4_quantize(x, &bits);
+        if (!mine) return;
+        const int per_head = a.dim >> 3, head = u / per_head, channel = (u - head * per_head) * 8;
+        const int64_t r = place.slot + (int64_t)head * a.cache.page_size;
+        *reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(codes) + r * (a.dim / 2) + channel / 2) = bits;
+        if ((lane & 3) == 0) static_cast<uint32_t *>(params)[r * (a.dim / kKv4Group) + channel / kKv4Group] = param;
+    };
+    for (int pass = pass0; pass < pass1; pass++) {
+        T x[N], y[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = next[i];
+        if (pass + 1 < pass1) load(pass + 1, next);
+        if (pass < q_passes) {
+            const int head = pass * together + head0;
+            turned(0.f, x, a.q_norm, [&](int e, int j) { return cos32[e][j]; }, [&](int e, int j) { return sin32[e][j]; }, y);
+            if (head < a.n_q) put(static_cast<T *>(a.q_out) + a.q_out_stride * row + (int64_t)head * a.dim, y);
+        } else if (pass < q_passes + k_passes) {
+            const int first = (pass - q_passes) * together, head = first + head0;
+            turned(0.0, x, a.k_norm, [&](int e, int j) { return turns[wave][max(pair[e], 0) + j].x; }, [&](int e, int j) { return turns[wave][max(pair[e], 0) + j].y; }, y);
+            if (!STORE) {
+                if (head < a.n_kv) put(static_cast<T *>(a.k_out) + a.k_out_stride * row + (int64_t)head * a.dim, y);
+                continue;
+            }
+            // the heads' channels in their order, through LDS
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (c[i / V / 2][i / V % 2] >= 0) keys[wave][head0 * a.dim + c[i / V / 2][i / V % 2] + i % V] = (float)y[i];
+            wave_meets();
+            const int units = min(together, a.n_kv - first) * (a.dim >> 3);
+#pragma unroll
+            for (int i = 0; i < UNITS; i++) {
+                const int u = i * 64 + lane;
+                float unit[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) unit[j] = u < units ? keys[wave][u * 8 + j] : 0.f;
+                quantize(first * (a.dim >> 3) + u, u < units, unit, a.cache.k_codes, a.cache.k_params);
+            }
+            wave_meets();   // (the next heads' channels go where these were)
+        } else if (STORE) {
+#pragma unroll
+            for (int i = 0; i < UNITS; i++) {
+                const int u = ((pass - q_passes - k_passes) * UNITS + i) * 64 + lane;
+                float unit[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) unit[j] = (float)x[i * 8 + j];
+                quantize(u, u < v_units, unit, a.cache.v_codes, a.cache.v_params);
+            }
+        }
+    }
+}
+
+int rotary_check(hipc_ctx *ctx, const char *who, const hipc_rotary_heads *h, int dtype, int64_t rows, RotaryArgs *a) {
+    HIPC_REQUIRE(ctx, h, "%s: null heads", who);
+    HIPC_REFUSE(ctx, dtype != HIPC_F16 && dtype != HIPC_F32, "%s: element type %d (f16 and f32 are taken)", who, dtype);
+    HIPC_REQUIRE(ctx, h->n_q_heads >= 0 && h->n_q_heads <= 65535 && h->n_kv_heads >= 0 && h->n_kv_heads <= 65535, "%s: %d query heads, %d key heads", who, h->n_q_heads, h->n_kv_heads);
+    HIPC_REQUIRE(ctx, h->head_dim > 0, "%s: head_dim %d", who, h->head_dim);
+    HIPC_REFUSE(ctx, h->head_dim > kRotaryMaxHead, "%s: head_dim %d (up to %d is taken)", who, h->head_dim, kRotaryMaxHead);
+    HIPC_REQUIRE(ctx, h->rotary_dim >= 0 && h->rotary_dim <= h->head_dim && h->rotary_dim % 2 == 0, "%s: %d channels of %d turn in pairs", who, h->rotary_dim, h->head_dim);
+    HIPC_REQUIRE(ctx, h->norm_eps >= 0.f && h->norm_eps - h->norm_eps == 0.f && h->amplitude - h->amplitude == 0.f, "%s: norm_eps and amplitude are finite numbers", who);
+    HIPC_REQUIRE(ctx, (h->rotary_dim == 0 || h->frequencies) && aligned(h->frequencies, 4) && aligned(h->q_norm, 4) && aligned(h->k_norm, 4), "%s: frequencies and norm weights", who);
+    HIPC_REQUIRE(ctx, rows >= 0 && rows <= 0x7fffffff, "%s: %lld rows", who, (long long)rows);
+    a->frequencies = static_cast<const float *>(h->frequencies), a->q_norm = static_cast<const float *>(h->q_norm), a->k_norm = static_cast<const float *>(h->k_norm);
+    a->rows = (int)rows, a->n_q = h->n_q_heads, a->n_kv = h->n_kv_heads, a->dim = h->head_dim, a->half = h->rotary_dim / 2, a->interleaved = h->interleaved != 0;
+    a->eps = h->norm_eps, a->amplitude = h->amplitude != 0.f ? h->amplitude : 1.0;
+    return HIPC_OK;
+}
+// rows of `heads` heads, `stride` apart
+int rotary_rows(hipc_ctx *ctx, const char *who, const char *what, const RotaryArgs &a, int heads, size_t size, const void *p, int64_t stride) {
+    if (heads == 0) return HIPC_OK;
+    HIPC_REQUIRE(ctx, p && aligned(p, size), "%s: %s", who, what);
+    HIPC_REQUIRE(ctx, stride >= (int64_t)heads * a.dim && stride <= (int64_t)1 << 40, "%s: rows of %s %lld apart, of %lld values", who, what, (long long)stride, (long long)heads * a.dim);
+    return HIPC_OK;
+}
+
+template <typename T, bool STORE>
+int rotary_launch(hipc_ctx *ctx, const char *who, RotaryArgs a) {
+    const int64_t strides[5] = {a.q_stride, a.k_stride, a.v_stride, a.q_out_stride, a.k_out_stride};
+    const void *rows[5] = {a.q, a.k, a.v, a.q_out, a.k_out};
+    const int heads[5] = {a.n_q, a.n_kv, STORE ? a.n_kv : 0, a.n_q, STORE ? 0 : a.n_kv};
+    // vectors of eight where pairs and rows allow, of four, or single values
+    auto fits = [&](int v) {
+        const int64_t bytes = std::min<int64_t>(v * sizeof(T), 16);
+        bool ok = a.dim % v == 0 && a.half % v == 0;
+        for (int i = 0; i < 5; i++)
+            if (heads[i]) ok &= aligned(rows[i], bytes) && strides[i] * (int64_t)sizeof(T) % bytes == 0;
+        return ok;
+    };
+    auto launch = [&](auto width) -> int {
+        constexpr int V = decltype(width)::value, N = 2 * V * (V == 1 ? 4 : 1);
+        const int items = (int)(a.half / V + ceil_div(a.dim - 2 * a.half, 2 * V));
+        while (a.lg_lanes < 6 && 1 << a.lg_lanes < items) a.lg_lanes++;
+        const int together = 64 >> a.lg_lanes;
+        const int64_t passes = ceil_div(a.n_q, together) + ceil_div(a.n_kv, together) + (STORE ? ceil_div((int64_t)a.n_kv * a.dim, 64 * N) : 0);
+        if (passes == 0) return HIPC_OK;
+        // rows that do not fill the device are shared by wavefronts (eight a CU)
+        a.chunks = (int)std::max<int64_t>(1, std::min(passes, 8 * (int64_t)ctx->cu_count / a.rows));
+        a.per = (int)ceil_div(passes, a.chunks), a.chunks = (int)ceil_div(passes, a.per);
+        const int64_t groups = ceil_div((int64_t)a.rows * a.chunks, 4);
+        HIPC_REFUSE(ctx, !grid_fits(groups, 256), "%s: %d rows: too many for one call", who, a.rows);
+        hipLaunchKernelGGL((rotary_kernel<T, V, STORE>), (unsigned)groups, 256, 0, ctx->stream, a);
+        HIPC_LAUNCHED(ctx);
+        return HIPC_OK;
+    };
+    if (fits(8)) return launch(std::integral_constant<int, 8>());
+    if (fits(4)) return launch(std::integral_constant<int, 4>());
+    return launch(std::integral_constant<int, 1>());
+}
+
+}  // namespace
+
+}  // namespace hipc
+
+using namespace hipc;
+
+extern "C" {
+
+int hipc_rotary_frequencies(double theta, int32_t rotary_dim, const hipc_rotary_scaling *scaling, float *frequencies) {
+    const char *who = "hipc_rotary_frequencies";
+    if (!(theta > 0.0) || !std::isfinite(theta)) return host_fail(HIPC_ERR_INVALID, "%s: a base of %g", who, theta);
+    if (rotary_dim < 0 || rotary_dim % 2 != 0) return host_fail(HIPC_ERR_INVALID, "%s: %d channels", who, rotary_dim);
+    if (rotary_dim > 0 && !frequencies) return host_fail(HIPC_ERR_INVALID, "%s: null pointer", who);
+    const double d = rotary_dim;
+    if (scaling) {
+        if (scaling->kind != HIPC_ROTARY_LINEAR && scaling->kind != HIPC_ROTARY_BASE && scaling->kind != HIPC_ROTARY_BY_PARTS)
+            return host_fail(HIPC_ERR_UNSUPPORTED, "%s: scaling of kind %d", who, scaling->kind);
+        if (!(scaling->factor >= 1.f) || !std::isfinite(scaling->factor)) return host_fail(HIPC_ERR_INVALID, "%s: a factor of %g", who, scaling->factor);
+        if (scaling->kind == HIPC_ROTARY_BY_PARTS && (!(scaling->trained > 0.f) || !std::isfinite(scaling->trained) || !(scaling->slow >= 0.f) || !(scaling->fast > scaling->slow) || !std::isfinite(scaling->fast)))
+            return host_fail(HIPC_ERR_INVALID, "%s: %g positions, %g to %g turns", who, scaling->trained, scaling->slow, scaling->fast);
+        if (scaling->kind == HIPC_ROTARY_BASE && rotary_dim > 2) theta *= std::pow((double)scaling->factor, d / (d - 2.0));
+    }
+    for (int i = 0; i < rotary_dim / 2; i++) {
+        double f = std::pow(theta, -2.0 * i / d);
+        if (scaling && scaling->kind == HIPC_ROTARY_LINEAR) f /= scaling->factor;
+        if (scaling && scaling->kind == HIPC_ROTARY_BY_PARTS) {
+            const double turns = scaling->trained * f / 6.283185307179586477;
+            const double keep = std::min(std::max((turns - scaling->slow) / ((double)scaling->fast - scaling->slow), 0.0), 1.0);
+            f = f / scaling->factor * (1.0 - keep) + f * keep;
+        }
+        frequencies[i] = (float)f;
+    }
+    return HIPC_OK;
+}
+
+int hipc_rotary(hipc_ctx *ctx, const hipc_rotary_heads *heads, int dtype, const void *positions, int64_t rows, const void *Q, int64_t q_stride,
+                const void *K, int64_t k_stride, void *Q_out, int64_t q_out_stride, void *K_out, int64_t k_out_stride) {
+    return entry(ctx, [&]() -> int {
+        const char *who = "hipc_rotary";
+        RotaryArgs a{};
+        if (int rc = rotary_check(ctx, who, heads, dtype, rows, &a)) return rc;
+        if (rows == 0) return HIPC_OK;
+        HIPC_REQUIRE(ctx, (a.half == 0 || positions) && aligned(positions, 4), "%s: positions", who);
+        const size_t size = dtype == HIPC_F16 ? 2 : 4;
+        if (int rc = rotary_rows(ctx, who, "Q", a, a.n_q, size, Q, q_stride)) return rc;
+        if (int rc = rotary_rows(ctx, who, "K", a, a.n_kv, size, K, k_stride)) return rc;
+        if (int rc = rotary_rows(ctx, who, "Q_out", a, a.n_q, size, Q_out, q_out_stride)) return rc;
+        if (int rc = rotary_rows(ctx, who, "K_out", a, a.n_kv, size, K_out, k_out_stride)) return rc;
+        a.positions = static_cast<const int *>(positions);
+        a.q = Q, a.k = K, a.q_out = Q_out, a.k_out = K_out, a.q_stride = q_stride, a.k_stride = k_stride, a.q_out_stride = q_out_stride, a.k_out_stride = k_out_stride;
+        return dtype == HIPC_F16 ? rotary_launch<_Float16, false>(ctx, who, a) : rotary_launch<float, false>(ctx, who, a);
+    });
+}
+
+int hipc_kv4_append_rotary(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_rotary_heads *heads, int dtype, const void *starts, int64_t total,
+                           const void *Q, int64_t q_stride, const void *K, int64_t k_stride, const void *V, int64_t v_stride, void *Q_out, int64_t q_out_stride) {
+    return entry(ctx, [&]() -> int {
+        const char *who = "hipc_kv4_append_rotary";
+        RotaryArgs a{};
+        if (int rc = kv4_check(ctx, who, cache)) return rc;
+        if (int rc = rotary_check(ctx, who, heads, dtype, total, &a)) return rc;
+        HIPC_REQUIRE(ctx, heads->n_kv_heads == cache->n_kv_heads && heads->head_dim == cache->head_dim, "%s: %d kv heads of %d channels, the cache has %d of %d", who, heads->n_kv_heads,
+                     heads->head_dim, cache->n_kv_heads, cache->head_dim);
+        if (total == 0 || cache->n_seqs == 0) return HIPC_OK;
+        const size_t size = dtype == HIPC_F16 ? 2 : 4;
+        HIPC_REQUIRE(ctx, starts && aligned(starts, 4), "%s: starts", who);
+        if (int rc = rotary_rows(ctx, who, "Q", a, a.n_q, size, Q, q_stride)) return rc;
+        if (int rc = rotary_rows(ctx, who, "K", a, a.n_kv, size, K, k_stride)) return rc;
+        if (int rc = rotary_rows(ctx, who, "V", a, a.n_kv, size, V, v_stride)) return rc;
+        if (int rc = rotary_rows(ctx, who, "Q_out", a, a.n_q, size, Q_out, q_out_stride)) return rc;
+        a.cache = *cache, a.starts = static_cast<const int *>(starts);
+        a.q = Q, a.k = K, a.v = V, a.q_out = Q_out, a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.q_out_stride = q_out_stride;
+        return dtype == HIPC_F16 ? rotary_launch<_Float16, true>(ctx, who, a) : rotary_launch<float, true>(ctx, who, a);
+    });
+}
+
+}  // extern "C"

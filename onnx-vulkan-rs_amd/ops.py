@@ -10,7 +10,8 @@ import ctypes as C
 
 import numpy as np
 
-from .runtime import AttentionHeads, Buffer, Context, ConvGeom, F16, F32, I8, Kv4Cache, U8, _ptr, hipc_dtype
+from .runtime import (AttentionHeads, Buffer, Context, ConvGeom, F16, F32, HipComputeError, I8, Kv4Cache, RotaryHeads, RotaryScaling, U8, _ptr,
+                      hipc_dtype, load_library)
 
 _vp = C.c_void_p
 
@@ -387,6 +388,70 @@ def qlinear_conv(ctx: Context, X, x_scale, x_zp, W, w_scale, w_zp, y_scale, y_zp
     return Y
 
 
+# ------------------------------------------ norms and positions of queries and keys
+
+ROTARY_LINEAR, ROTARY_BASE, ROTARY_BY_PARTS = 1, 2, 3
+
+
+def rotary_frequencies(theta, rotary_dim, kind=None, factor=1.0, trained=0.0, slow=1.0, fast=32.0):
+    """The frequencies of a rotation, ``[rotary_dim / 2]`` float32 on the host, stretched ``factor``-fold in one of the kinds above
+    (``hipc_rotary_frequencies``)."""
+    lib, out = load_library(), np.zeros(max(int(rotary_dim), 0) // 2, np.float32)
+    scaling = None if kind is None else C.byref(RotaryScaling(kind, factor, trained, slow, fast))
+    rc = lib.hipc_rotary_frequencies(theta, rotary_dim, scaling, out.ctypes.data)
+    if rc != 0:
+        raise HipComputeError(rc, lib.hipc_host_error().decode())
+    return out
+
+
+def rotary_device(ctx, heads: RotaryHeads, dtype, positions, rows, Q, q_stride, K, k_stride, Q_out, q_out_stride, K_out, k_out_stride):
+    ctx._check(ctx.lib.hipc_rotary(ctx.handle, heads, dtype, _ptr(positions), rows, _ptr(Q), q_stride, _ptr(K), k_stride, _ptr(Q_out), q_out_stride,
+                                   _ptr(K_out), k_out_stride))
+
+
+def kv4_append_rotary_device(ctx, cache: Kv4Cache, heads: RotaryHeads, dtype, starts, total, Q, q_stride, K, k_stride, V, v_stride, Q_out, q_out_stride):
+    ctx._check(ctx.lib.hipc_kv4_append_rotary(ctx.handle, cache, heads, dtype, _ptr(starts), total, _ptr(Q), q_stride, _ptr(K), k_stride, _ptr(V), v_stride,
+                                              _ptr(Q_out), q_out_stride))
+
+
+class Rotary:
+    """Norms and rotation of a layer's heads as a program keeps them: frequencies and norm weights on the device."""
+
+    def __init__(self, ctx: Context, n_q_heads, n_kv_heads, head_dim, frequencies, q_norm=None, k_norm=None, eps=1e-6, interleaved=False, amplitude=0.0):
+        frequencies = np.ascontiguousarray(frequencies, np.float32)
+        if frequencies.ndim != 1:
+            raise ValueError(f"Rotary: frequencies of shape {frequencies.shape}")
+        norms = [None if w is None else np.ascontiguousarray(w, np.float32) for w in (q_norm, k_norm)]
+        for w in norms:
+            if w is not None:
+                _rows_match("Rotary", (w,), ((head_dim,),), np.float32)
+        self.ctx, self.n_q_heads, self.n_kv_heads, self.head_dim = ctx, n_q_heads, n_kv_heads, head_dim
+        self.buffers = [None if x is None else ctx.upload(x) for x in (frequencies, *norms)]
+        self.heads = RotaryHeads(n_q_heads, n_kv_heads, head_dim, 2 * frequencies.size, int(interleaved), eps, amplitude,
+                                 *(None if b is None else b.ptr for b in self.buffers))
+
+    def rows_match(self, what, q, k):
+        _rows_match(what, (q, k), ((q.shape[0], self.n_q_heads, self.head_dim), (q.shape[0], self.n_kv_heads, self.head_dim)), q.dtype)
+
+    def __call__(self, q, k, positions):
+        """``q [rows, heads, dim]`` and ``k [rows, kv heads, dim]`` at ``positions [rows]``: both normed and turned."""
+        q, k, positions = np.ascontiguousarray(q), np.ascontiguousarray(k), np.ascontiguousarray(positions, np.int32)
+        self.rows_match("Rotary", q, k)
+        _rows_match("Rotary", (positions,), ((q.shape[0],),), np.int32)
+        dQ, dK, dP = (self.ctx.upload(x) for x in (q, k, positions))
+        qw, kw = self.n_q_heads * self.head_dim, self.n_kv_heads * self.head_dim
+        rotary_device(self.ctx, self.heads, hipc_dtype(q.dtype), dP, q.shape[0], dQ, qw, dK, kw, dQ, qw, dK, kw)
+        out = self.ctx.download(dQ, q.dtype, q.shape), self.ctx.download(dK, k.dtype, k.shape)
+        for b in (dQ, dK, dP):
+            b.free()
+        return out
+
+    def free(self):
+        for b in self.buffers:
+            if b is not None:
+                b.free()
+
+
 # ------------------------------------------ attention over prompts and a cache in 4 bits
 
 KV4_GROUP = 32   # channels that share a scale and a lowest value
@@ -481,6 +546,20 @@ class Kv4Pages:
         kv4_append_device(self.ctx, self.cache, hipc_dtype(k.dtype), ds, k.shape[0], dK, row, dV, row)
         for b in (dK, dV, ds):
             b.free()
+
+    def append_rotary(self, rotary: Rotary, q, k, v, new):
+        """``append`` of keys that ``rotary`` norms and turns on their way; returns the queries, turned by the same positions."""
+        q, k, v = (np.ascontiguousarray(x) for x in (q, k, v))
+        rotary.rows_match("append_rotary", q, k)
+        _rows_match("append_rotary", (k, v), ((q.shape[0], self.n_kv_heads, self.head_dim),) * 2, q.dtype)
+        starts = _starts("append_rotary", new, self.n_seqs, k.shape[0])
+        dQ, dK, dV, ds = (self.ctx.upload(x) for x in (q, k, v, starts))
+        qw, row = q.shape[1] * q.shape[2], self.n_kv_heads * self.head_dim
+        kv4_append_rotary_device(self.ctx, self.cache, rotary.heads, hipc_dtype(k.dtype), ds, k.shape[0], dQ, qw, dK, row, dV, row, dQ, qw)
+        out = self.ctx.download(dQ, q.dtype, q.shape)
+        for b in (dQ, dK, dV, ds):
+            b.free()
+        return out
 
     def read(self, count, dtype=np.float16):
         """The last ``count[s]`` positions of every sequence, packed: (keys, values)."""

@@ -70,6 +70,17 @@ class Kv4Cache(C.Structure):
                [("lengths", C.c_void_p), ("table", C.c_void_p), ("table_width", C.c_int64)]
 
 
+class RotaryHeads(C.Structure):
+    """``hipc_rotary_heads``: how query and key heads are normed and turned (device addresses of frequencies and weights)."""
+    _fields_ = [(n, C.c_int32) for n in ("n_q_heads", "n_kv_heads", "head_dim", "rotary_dim", "interleaved")] + \
+               [("norm_eps", C.c_float), ("amplitude", C.c_float)] + [(n, C.c_void_p) for n in ("frequencies", "q_norm", "k_norm")]
+
+
+class RotaryScaling(C.Structure):
+    """``hipc_rotary_scaling``."""
+    _fields_ = [("kind", C.c_int32)] + [(n, C.c_float) for n in ("factor", "trained", "slow", "fast")]
+
+
 class InitializerInfo(C.Structure):
     """``hipc_initializer_info``."""
     _fields_ = [("data_type", C.c_int32), ("n_dims", C.c_int32), ("dims", C.c_int64 * 8), ("bytes", C.c_size_t),
@@ -149,6 +160,10 @@ SIGNATURES = {
                                  C.c_int32, _int, _vp, C.POINTER(ConvGeom), _vp]),
     "hipc_prompt_attention": (_int, [_vp, C.POINTER(AttentionHeads), _int, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64,
                                      _i64, _vp, _i64]),
+    "hipc_rotary_frequencies": (_int, [C.c_double, C.c_int32, C.POINTER(RotaryScaling), _vp]),
+    "hipc_rotary": (_int, [_vp, C.POINTER(RotaryHeads), _int, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64]),
+    "hipc_kv4_append_rotary": (_int, [_vp, C.POINTER(Kv4Cache), C.POINTER(RotaryHeads), _int, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64,
+                                      _vp, _i64]),
     "hipc_kv4_append": (_int, [_vp, C.POINTER(Kv4Cache), _int, _vp, _i64, _vp, _i64, _vp, _i64]),
     "hipc_kv4_read": (_int, [_vp, C.POINTER(Kv4Cache), _int, _vp, _i64, _vp, _i64, _vp, _i64]),
     "hipc_kv4_attention": (_int, [_vp, C.POINTER(Kv4Cache), C.POINTER(AttentionHeads), _int, _i64, _vp, _i64, _vp, _i64]),

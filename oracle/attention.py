@@ -46,6 +46,23 @@ def prompt(q, k, v, q_lengths, k_lengths, causal=True, window=0, scale=None):
     return y, weight, size
 
 
+def rotary(x, positions, frequencies, norm=None, eps=1e-6, interleaved=False, amplitude=1.0):
+    """[rows, heads, dim] normed (``norm`` [dim] or None) and turned: (y, the sizes |x^_a cos| + |x^_b sin| of its two products), in 64 bits."""
+    y = x.astype(f64)
+    if norm is not None:
+        y = y / np.sqrt(np.mean(y * y, -1, keepdims=True) + f64(np.float32(eps))) * norm.astype(f64)
+    size = np.abs(y)
+    n = len(frequencies)
+    for i in range(n):
+        a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + n)
+        t = positions.astype(f64) * f64(frequencies[i])
+        c, s = (f64(np.float32(amplitude)) * f(t)[:, None] for f in (np.cos, np.sin))
+        p, q = y[..., a].copy(), y[..., b].copy()
+        y[..., a], y[..., b] = p * c - q * s, q * c + p * s
+        size[..., a], size[..., b] = abs(p * c) + abs(q * s), abs(q * c) + abs(p * s)
+    return y, size
+
+
 def quantize(x):
     """[..., dim] as (codes, scale f16, lowest f16), groups of 32 channels, every decision in 64 bits."""
     g = np.clip(x.astype(f64), -65408, 65408).reshape(x.shape[:-1] + (-1, GROUP))

@@ -210,6 +210,7 @@ inline float rsqrtf(float v) { return 1.f / std::sqrt(v); }
 inline float __fmul_rn(float a, float b) { return a * b; }
 inline float __fdiv_rn(float a, float b) { return a / b; }
 inline float __fadd_rn(float a, float b) { return a + b; }
+inline void sincospi(double x, double *s, double *c) { *s = std::sin(3.14159265358979323846 * x), *c = std::cos(3.14159265358979323846 * x); }
 using std::max;
 using std::min;
 

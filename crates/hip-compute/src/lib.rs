@@ -641,6 +641,15 @@ impl HipContext {
         self.check(unsafe { sys::hipc_kv4_attention(self.raw, cache, heads, dtype.raw(), tokens, q.at.ptr(), q.stride, y.at.ptr(), y.stride) })
     }
 
+    /// Attention of packed new rows, as many of each sequence as `starts` says, over the cache; with a window the first `sinks` positions stay visible.
+    pub fn kv4_prompt_attention(
+        &self, cache: &Kv4Cache, heads: &AttentionHeads, sinks: i32, dtype: DType, starts: BufferSlice<'_>, total: i64, q: Rows<'_>, y: Rows<'_>,
+    ) -> Result<()> {
+        self.check(unsafe {
+            sys::hipc_kv4_prompt_attention(self.raw, cache, heads, sinks, dtype.raw(), starts.ptr(), total, q.at.ptr(), q.stride, y.at.ptr(), y.stride)
+        })
+    }
+
     // ----------------------------------------- probabilities of the answers
 
     /// Log-probabilities of given tokens, entropies and the most likely alternatives of rows of logits (f16 or f32).

@@ -302,6 +302,10 @@ unsafe extern "C" {
         ctx: *mut hipc_ctx, cache: *const hipc_kv4_cache, heads: *const hipc_attention_heads, dtype: c_int, tokens: i64,
         q: *const c_void, q_stride: i64, y: *mut c_void, y_stride: i64,
     ) -> c_int;
+    pub fn hipc_kv4_prompt_attention(
+        ctx: *mut hipc_ctx, cache: *const hipc_kv4_cache, heads: *const hipc_attention_heads, sinks: i32, dtype: c_int, starts: *const c_void,
+        total: i64, q: *const c_void, q_stride: i64, y: *mut c_void, y_stride: i64,
+    ) -> c_int;
 
     // ---- probabilities of the answers
     pub fn hipc_token_logprobs(

@@ -149,7 +149,7 @@ const Entry kEntries[] = {
     BIND(hipc_matmul_integer_scale_bias), BIND(hipc_requantize), BIND(hipc_qlinear_matmul), BIND(hipc_conv_integer),
     BIND(hipc_qlinear_conv), BIND(hipc_decoder_reset), BIND(hipc_decoder_step), BIND(hipc_prompt_attention),
     BIND(hipc_kv4_append), BIND(hipc_kv4_read), BIND(hipc_kv4_attention), BIND(hipc_token_logprobs),
-    BIND(hipc_rotary), BIND(hipc_kv4_append_rotary),
+    BIND(hipc_rotary), BIND(hipc_kv4_append_rotary), BIND(hipc_kv4_prompt_attention),
 };
 #undef BIND
 

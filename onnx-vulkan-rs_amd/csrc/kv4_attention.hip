@@ -16,6 +16,8 @@ struct Kv4Attend {
     int64_t q_stride, y_stride;
     int tokens, n_q_heads, group, window, row_blocks, wide;   // wide: rows of Q and Y on 16 bytes
     float scale;
+    const int *starts;   // rows packed by sequence: whose are which of the `total`
+    int total, sinks, most;   // ... positions that stay visible in front of the window; a sequence of more query rows (tokens times group) is not this kernel's
     float *parts;        // [workgroup][2] parts of a unit: rows x channels sums, then (maximum, sum) pairs
     uint32_t *arrived;   // [workgroup]: parts of the unit that began here and went on; all zero between calls
 };
@@ -48,88 +50,144 @@ __device__ __forceinline__ float groups_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// The key tiles a sequence's newest tokens see: [first, first + count).
+// The key tiles a sequence's newest tokens see: the first `sink_tiles` of the sequence, then those from tile first + sink_tiles on, `count` in all; and
+// where the tokens' rows are.
 struct Kv4Span {
-    int length, first, count;
+    int length, first, count, tokens, row0, sink_tiles;
 };
-__device__ __forceinline__ Kv4Span kv4_span_of(const Kv4Attend &a, int length) {
-    const int held = kv4_held(a.cache, length);
-    const int begin = a.window > 0 ? max(length - a.tokens - a.window + 1, 0) : 0;
-    return {length, begin / kKv4Tile, held > begin ? (held + kKv4Tile - 1) / kKv4Tile - begin / kKv4Tile : 0};
+__device__ __forceinline__ int kv4_key_tile(const Kv4Span &s, int tile) { return tile < s.sink_tiles ? tile : s.first + tile; }
+// what memory says of a sequence. PACKED: sequences bring tokens of another number each (the starts say); else all bring a.tokens.
+struct Kv4Asked {
+    int length, from, to;
+};
+template <bool PACKED>
+__device__ __forceinline__ Kv4Asked kv4_ask(const Kv4Attend &a, int seq) {
+    const int s = min(seq, a.cache.n_seqs - 1);
+    return {a.cache.n_pages > 0 ? kv4_length(a.cache, s) : 0, PACKED ? a.starts[s] : 0, PACKED ? a.starts[s + 1] : 0};
 }
-
-__device__ __forceinline__ int kv4_span_length(const Kv4Attend &a, int seq) { return a.cache.n_pages > 0 ? kv4_length(a.cache, min(seq, a.cache.n_seqs - 1)) : 0; }
-__device__ __forceinline__ Kv4Span kv4_span(const Kv4Attend &a, int seq) { return kv4_span_of(a, kv4_span_length(a, seq)); }
+template <bool PACKED>
+__device__ __forceinline__ Kv4Span kv4_span_of(const Kv4Attend &a, const Kv4Asked &q) {
+    const int held = kv4_held(a.cache, q.length);
+    if (!PACKED) {
+        const int begin = a.window > 0 ? max(q.length - a.tokens - a.window + 1, 0) : 0;
+        return {q.length, begin / kKv4Tile, held > begin ? (held + kKv4Tile - 1) / kKv4Tile - begin / kKv4Tile : 0, a.tokens, 0, 0};
+    }
+    const int row0 = max(q.from, 0), end = min(q.to, a.total), brought = end > row0 ? end - row0 : 0;
+    const int tokens = (int64_t)brought * a.group <= a.most ? brought : 0;
+    const int begin = a.window > 0 ? max(q.length - tokens - a.window + 1, 0) : 0, first = begin / kKv4Tile;
+    const int sink_tiles = a.window > 0 ? min((min(a.sinks, held) + kKv4Tile - 1) / kKv4Tile, first) : 0;
+    const int count = sink_tiles + (held > begin ? (held + kKv4Tile - 1) / kKv4Tile - first : 0);
+    return {q.length, first - sink_tiles, tokens > 0 ? count : 0, tokens, row0, sink_tiles};
+}
+template <bool PACKED>
+__device__ __forceinline__ Kv4Span kv4_span(const Kv4Attend &a, int seq) { return kv4_span_of<PACKED>(a, kv4_ask<PACKED>(a, seq)); }
+// its blocks of 16 query rows
+template <bool PACKED>
+__device__ __forceinline__ int kv4_blocks(const Kv4Attend &a, const Kv4Span &s) { return PACKED ? (s.tokens * a.group + kKv4Rows - 1) / kKv4Rows : a.row_blocks; }
 // body(base, spans) for the sequences in chunks of 64, a lane's is base + lane (the last one's, behind it): the first 64 are there, of
 // the others four chunks' lengths are on their way at once. Ends where body is true.
-template <typename Body>
+template <bool PACKED, typename Body>
 __device__ __forceinline__ void kv4_sequences(const Kv4Attend &a, const Kv4Span &early, Body body) {
     if (body(0, early)) return;
     const int lane = threadIdx.x & 63;
     for (int base = 64; base < a.cache.n_seqs; base += 256) {
-        int length[4];
+        Kv4Asked asked[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) length[e] = kv4_span_length(a, base + 64 * e + lane);
+        for (int e = 0; e < 4; e++) asked[e] = kv4_ask<PACKED>(a, base + 64 * e + lane);
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            if (base + 64 * e < a.cache.n_seqs && body(base + 64 * e, kv4_span_of(a, length[e]))) return;
+            if (base + 64 * e < a.cache.n_seqs && body(base + 64 * e, kv4_span_of<PACKED>(a, asked[e]))) return;
     }
 }
 
 // A unit: (sequence, kv head, block of 16 query rows), counted in this order.
 struct Kv4Unit {
     Kv4Span span;
-    int seq, inner;       // inner = kv head * row_blocks + block
-    int64_t before;       // steps of all units in front of it
+    int seq, inner, blocks;   // inner = kv head * blocks + block
+    int64_t before;           // steps of all units in front of it
 };
 // a division of whole numbers that are hardly ever beyond 32 bits (one of 64 bits is some 100 instructions)
 __device__ __forceinline__ int64_t kv4_div(int64_t x, int64_t y) { return ((uint64_t)(x | y) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y; }
+__device__ __forceinline__ int64_t kv4_lane(int64_t v, int l) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l));
+}
+// inclusive sums over the lanes of n * times (times below 2^23, n at most 2^24): in two parts that 32 bits hold
+__device__ __forceinline__ int64_t kv4_scan(int n, int times) {
+    const int64_t v = (int64_t)n * times;
+    return ((int64_t)wave_scan((int)(v >> 24)) << 24) + wave_scan((int)(v & 0xffffff));
+}
 // Steps of a unit: its tiles, or (cut > 0) its parts of up to `cut` tiles. The unit that step number `at` of all units' belongs to.
 __device__ __forceinline__ int kv4_steps(int tiles, int cut) { return cut > 0 ? (tiles + cut - 1) / cut : tiles; }
-__device__ __forceinline__ bool kv4_find(const Kv4Attend &a, const Kv4Span &early, int per_seq, int64_t at, int cut, Kv4Unit *u) {
+__device__ __forceinline__ void kv4_take(const Kv4Span &s, int l, Kv4Unit *u) {
+    u->span = {__builtin_amdgcn_readlane(s.length, l), __builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.count, l), __builtin_amdgcn_readlane(s.tokens, l),
+               __builtin_amdgcn_readlane(s.row0, l), __builtin_amdgcn_readlane(s.sink_tiles, l)};
+}
+template <bool PACKED>
+__device__ __forceinline__ bool kv4_find(const Kv4Attend &a, const Kv4Span &early, int64_t at, int cut, Kv4Unit *u) {
     const int lane = threadIdx.x & 63;
     int64_t before = 0;
     bool found = false;
-    kv4_sequences(a, early, [&](int base, const Kv4Span &s) {
+    kv4_sequences<PACKED>(a, early, [&](int base, const Kv4Span &s) {
         const int n = base + lane < a.cache.n_seqs ? kv4_steps(s.count, cut) : 0;
-        const int sum = wave_scan(n);
-        const uint64_t over = __ballot(before + (int64_t)sum * per_seq > at);
-        if (over) {
-            const int l = __builtin_ctzll(over), steps = __builtin_amdgcn_readlane(n, l);
-            u->span = {__builtin_amdgcn_readlane(s.length, l), __builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.count, l)};
-            const int64_t first = before + (int64_t)(__builtin_amdgcn_readlane(sum, l) - steps) * per_seq;
-            u->seq = base + l;
-            u->inner = (int)kv4_div(at - first, steps);
-            u->before = first + (int64_t)u->inner * steps;
-            found = true;
+        if constexpr (PACKED) {
+            const int units = a.cache.n_kv_heads * kv4_blocks<PACKED>(a, s);
+            const int64_t sum = kv4_scan(n, units);
+            const uint64_t over = __ballot(before + sum > at);
+            if (over) {
+                const int l = __builtin_ctzll(over), steps = __builtin_amdgcn_readlane(n, l);
+                kv4_take(s, l, u);
+                const int64_t first = before + kv4_lane(sum - (int64_t)n * units, l);
+                u->seq = base + l, u->blocks = kv4_blocks<PACKED>(a, u->span);
+                u->inner = (int)kv4_div(at - first, steps);
+                u->before = first + (int64_t)u->inner * steps;
+                found = true;
+            }
+            before += kv4_lane(sum, 63);
+            return over != 0;
+        } else {
+            const int per_seq = a.cache.n_kv_heads * a.row_blocks;
+            const int sum = wave_scan(n);
+            const uint64_t over = __ballot(before + (int64_t)sum * per_seq > at);
+            if (over) {
+                const int l = __builtin_ctzll(over), steps = __builtin_amdgcn_readlane(n, l);
+                kv4_take(s, l, u);
+                const int64_t first = before + (int64_t)(__builtin_amdgcn_readlane(sum, l) - steps) * per_seq;
+                u->seq = base + l, u->blocks = a.row_blocks;
+                u->inner = (int)kv4_div(at - first, steps);
+                u->before = first + (int64_t)u->inner * steps;
+                found = true;
+            }
+            before += (int64_t)__builtin_amdgcn_readlane(sum, 63) * per_seq;
+            return over != 0;
         }
-        before += (int64_t)__builtin_amdgcn_readlane(sum, 63) * per_seq;
-        return over != 0;
     });
     return found;
 }
 // the unit behind the last one of its sequence, which ended at step `at`
+template <bool PACKED>
 __device__ __forceinline__ bool kv4_next(const Kv4Attend &a, int64_t at, int cut, Kv4Unit *u) {
     const int lane = threadIdx.x & 63;
     for (int base = u->seq + 1; base < a.cache.n_seqs; base += 64) {
-        const Kv4Span s = kv4_span(a, base + lane);
+        const Kv4Span s = kv4_span<PACKED>(a, base + lane);
         const uint64_t has = __ballot(base + lane < a.cache.n_seqs && kv4_steps(s.count, cut) > 0);
         if (!has) continue;
         const int l = __builtin_ctzll(has);
-        u->span = {__builtin_amdgcn_readlane(s.length, l), __builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.count, l)};
-        u->seq = base + l, u->inner = 0, u->before = at;
+        kv4_take(s, l, u);
+        u->seq = base + l, u->inner = 0, u->before = at, u->blocks = kv4_blocks<PACKED>(a, u->span);
         return true;
     }
     return false;
 }
 // steps of all units
-__device__ __forceinline__ int64_t kv4_total(const Kv4Attend &a, const Kv4Span &early, int per_seq, int cut, float *longest) {
+template <bool PACKED>
+__device__ __forceinline__ int64_t kv4_total(const Kv4Attend &a, const Kv4Span &early, int cut, float *longest) {
     const int lane = threadIdx.x & 63;
     int64_t total = 0;
     float most = 0.f;
-    kv4_sequences(a, early, [&](int base, const Kv4Span &s) {
+    kv4_sequences<PACKED>(a, early, [&](int base, const Kv4Span &s) {
         const int c = base + lane < a.cache.n_seqs ? s.count : 0;
-        total += (int64_t)__builtin_amdgcn_readlane(wave_scan(kv4_steps(c, cut)), 63) * per_seq;
+        if constexpr (PACKED) total += kv4_lane(kv4_scan(kv4_steps(c, cut), a.cache.n_kv_heads * kv4_blocks<PACKED>(a, s)), 63);
+        else total += (int64_t)__builtin_amdgcn_readlane(wave_scan(kv4_steps(c, cut)), 63) * (a.cache.n_kv_heads * a.row_blocks);
         most = fmaxf(most, lean_wave_max((float)c));
         return false;
     });
@@ -138,14 +196,15 @@ __device__ __forceinline__ int64_t kv4_total(const Kv4Attend &a, const Kv4Span &
 }
 
 // rows that see nothing for want of keys
-template <typename T, int HD>
+template <typename T, int HD, bool PACKED>
 __device__ void kv4_zero_rows(const Kv4Attend &a, const Kv4Span &early) {
     const int lane = threadIdx.x & 63;
-    kv4_sequences(a, early, [&](int base, const Kv4Span &span) {
-        for (uint64_t none = __ballot(base + lane < a.cache.n_seqs && span.count == 0); none; none &= none - 1) {
-            const int64_t s = base + __builtin_ctzll(none);
-            for (int r = 0; r < a.tokens; r++)
-                for (int i = threadIdx.x; i < a.n_q_heads * HD; i += blockDim.x) static_cast<T *>(a.y)[(s * a.tokens + r) * a.y_stride + i] = (T)0.f;
+    kv4_sequences<PACKED>(a, early, [&](int base, const Kv4Span &span) {
+        for (uint64_t none = __ballot(base + lane < a.cache.n_seqs && span.count == 0 && span.tokens > 0); none; none &= none - 1) {
+            const int l = __builtin_ctzll(none), tokens = __builtin_amdgcn_readlane(span.tokens, l);
+            const int64_t row0 = PACKED ? __builtin_amdgcn_readlane(span.row0, l) : (int64_t)(base + l) * a.tokens;
+            for (int r = 0; r < tokens; r++)
+                for (int i = threadIdx.x; i < a.n_q_heads * HD; i += blockDim.x) static_cast<T *>(a.y)[(row0 + r) * a.y_stride + i] = (T)0.f;
         }
         return false;
     });
@@ -168,7 +227,9 @@ __device__ void kv4_zero_rows(const Kv4Attend &a, const Kv4Span &early) {
 // The codes become f16 values on their way into the operands (exactly what the cache stands for), weights are two f16 terms, f32 queries
 // two terms of the row times a power of two. Keys come straight from memory into operand registers, a tile ahead; values (codes, and
 // the parameters of the keys that are seen, zeros for the others) pass through the wavefront's own LDS, without a barrier.
-template <int HD, int QT, int W>
+//
+// PACKED: every sequence brings as many tokens as its starts say, and with a window the first `sinks` positions stay visible.
+template <int HD, int QT, int W, bool PACKED>
 __global__ void __launch_bounds__(64 * W, HD <= 128 ? 2 : 1) kv4_attend_kernel(const Kv4Attend a) {
     constexpr int WPL = HD / 32;                              // words of codes of a key per lane; also groups of a row
     constexpr int UNITS = HD <= 32 ? 2 : HD <= 64 ? 4 : HD <= 128 ? 8 : 16;   // 8-byte units of an LDS row of codes
@@ -186,26 +247,25 @@ __global__ void __launch_bounds__(64 * W, HD <= 128 ? 2 : 1) kv4_attend_kernel(c
     const int n = lane & 15, q4 = lane >> 4;
     char *codes = smem + wave * (CODES + PARAMS), *params = codes + CODES;
     const int shift = 31 - __builtin_clz((unsigned)a.cache.page_size), page_mask = a.cache.page_size - 1;
-    const int per_seq = a.cache.n_kv_heads * a.row_blocks;
     const Kv4Unpack unpack;
 
     // at least a tile for each wavefront, and long units in few enough parts that joining them is not the longer half
     const int groups = (int)gridDim.x;
-    const Kv4Span early = kv4_span(a, min(lane, a.cache.n_seqs - 1));   // of the first 64 sequences, which mostly are all
+    const Kv4Span early = kv4_span<PACKED>(a, min(lane, a.cache.n_seqs - 1));   // of the first 64 sequences, which mostly are all
     float longest, same;
-    const int64_t tiles = kv4_total(a, early, per_seq, 0, &longest);
+    const int64_t tiles = kv4_total<PACKED>(a, early, 0, &longest);
     if (tiles == 0) {
-        if (blockIdx.x == gridDim.x - 1) kv4_zero_rows<T, HD>(a, early);
+        if (blockIdx.x == gridDim.x - 1) kv4_zero_rows<T, HD, PACKED>(a, early);
         return;
     }
     const int64_t even = kv4_div(tiles + groups - 1, groups);
     const int least = max(W, (int)sqrtf(longest * (1.f / 7.f)));
     int64_t share = even > least ? even : least;
     int cut = 0;
-    if (kv4_total(a, early, per_seq, 1 << 30, &same) <= groups) {
+    if (kv4_total<PACKED>(a, early, 1 << 30, &same) <= groups) {
         cut = (int)share;
         for (;;) {   // (longer parts make fewer of them; with one a unit it ends)
-            const int64_t parts = kv4_total(a, early, per_seq, cut, &same);
+            const int64_t parts = kv4_total<PACKED>(a, early, cut, &same);
             if (parts <= groups) break;
             cut = max(cut + 1, (int)min((float)cut * (float)parts / (float)groups, longest));
         }
@@ -213,12 +273,14 @@ __global__ void __launch_bounds__(64 * W, HD <= 128 ? 2 : 1) kv4_attend_kernel(c
     }
     int64_t at = share * blockIdx.x;
     Kv4Unit u;
-    if (blockIdx.x == gridDim.x - 1) kv4_zero_rows<T, HD>(a, early);
-    if (!kv4_find(a, early, per_seq, at, cut, &u)) return;
+    if (blockIdx.x == gridDim.x - 1) kv4_zero_rows<T, HD, PACKED>(a, early);
+    if (!kv4_find<PACKED>(a, early, at, cut, &u)) return;
     const int64_t run1 = at + share;
     for (;;) {
         const Kv4Span span = u.span;
-        const int kvh = u.inner / a.row_blocks, block = u.inner - kvh * a.row_blocks;
+        const int kvh = u.inner / u.blocks, block = u.inner - kvh * u.blocks;
+        const int tokens = PACKED ? span.tokens : a.tokens;
+        const int64_t row0 = PACKED ? span.row0 : (int64_t)u.seq * a.tokens;
         // its tiles of this workgroup
         const int steps = kv4_steps(span.count, cut);
         int from = (int)(at - u.before), to = run1 - u.before < steps ? (int)(run1 - u.before) : steps;
@@ -228,18 +290,18 @@ __global__ void __launch_bounds__(64 * W, HD <= 128 ? 2 : 1) kv4_attend_kernel(c
         }
 
         // the lane's query row
-        const int rows = min(a.tokens * a.group - block * kKv4Rows, kKv4Rows);
-        const int row = block * kKv4Rows + n, token = min(row, a.tokens * a.group - 1) / a.group, g = row - token * a.group;
+        const int rows = min(tokens * a.group - block * kKv4Rows, kKv4Rows);
+        const int row = block * kKv4Rows + n, token = min(row, tokens * a.group - 1) / a.group, g = row - token * a.group;
         const bool mine = n < rows;
-        const int pos = span.length - a.tokens + token;
+        const int pos = span.length - tokens + token;
         const int lane_begin = a.window > 0 ? max(pos - a.window + 1, 0) : 0, lane_end = mine ? pos + 1 : 0;
-        const int pos0 = span.length - a.tokens + block * kKv4Rows / a.group;                       // the first row's and the last's
-        const int pos1 = span.length - a.tokens + (block * kKv4Rows + rows - 1) / a.group;
+        const int pos0 = span.length - tokens + block * kKv4Rows / a.group;                       // the first row's and the last's
+        const int pos1 = span.length - tokens + (block * kKv4Rows + rows - 1) / a.group;
         const int any_begin = a.window > 0 ? max(pos0 - a.window + 1, 0) : 0, all_begin = a.window > 0 ? max(pos1 - a.window + 1, 0) : 0;
 
         float qx[WPL][8];
         {
-            const T *q = static_cast<const T *>(a.q) + ((int64_t)u.seq * a.tokens + (mine ? token : 0)) * a.q_stride + (int64_t)(kvh * a.group + (mine ? g : 0)) * HD;
+            const T *q = static_cast<const T *>(a.q) + (row0 + (mine ? token : 0)) * a.q_stride + (int64_t)(kvh * a.group + (mine ? g : 0)) * HD;
 #pragma unroll
             for (int w = 0; w < WPL; w++) kv4_load8(q + 8 * (q4 * WPL + w), a.wide, qx[w]);
         }
@@ -255,7 +317,7 @@ __global__ void __launch_bounds__(64 * W, HD <= 128 ? 2 : 1) kv4_attend_kernel(c
         uint32_t k_codes[4][WPL], k_params[4][NP], v_codes[WPL][4], v_params[WPL];
         const int *table = static_cast<const int *>(a.cache.table) + (int64_t)u.seq * a.cache.table_width;
         auto page_at = [&](int tile, int block) {
-            const int entry = ((span.first + tile) * kKv4Tile + 16 * block) >> shift, last = (int)a.cache.table_width - 1, page = table[min(entry, last)];
+            const int entry = (kv4_key_tile(span, tile) * kKv4Tile + 16 * block) >> shift, last = (int)a.cache.table_width - 1, page = table[min(entry, last)];
             return entry <= last ? page : -1;
         };
         auto is_page = [&](int page) { return page >= 0 && page < a.cache.n_pages; };
@@ -263,7 +325,7 @@ __global__ void __launch_bounds__(64 * W, HD <= 128 ? 2 : 1) kv4_attend_kernel(c
             return (((int64_t)(is_page(page) ? page : 0) * a.cache.n_kv_heads + kvh) << shift) + (key & page_mask);
         };
         auto load_values = [&](int tile, int page) {   // page: of block q4
-            const int key0 = (span.first + tile) * kKv4Tile;
+            const int key0 = kv4_key_tile(span, tile) * kKv4Tile;
             const int64_t row = row_of(page, key0 + lane);
             const uint32_t *vp = static_cast<const uint32_t *>(a.cache.v_params) + row * WPL;
 #pragma unroll
@@ -291,7 +353,7 @@ __global__ void __launch_bounds__(64 * W, HD <= 128 ? 2 : 1) kv4_attend_kernel(c
             }
         };
         auto load_keys = [&](int tile, int page) {   // page: of block n / 4
-            const int64_t row = row_of(page, (span.first + tile) * kKv4Tile + 16 * (n >> 2) + (n & 3));
+            const int64_t row = row_of(page, kv4_key_tile(span, tile) * kKv4Tile + 16 * (n >> 2) + (n & 3));
             const uint32_t *kc = reinterpret_cast<const uint32_t *>(static_cast<const char *>(a.cache.k_codes) + row * (HD / 2)) + q4 * WPL;
             const uint32_t *kp = static_cast<const uint32_t *>(a.cache.k_params) + row * WPL;
 #pragma unroll
@@ -339,8 +401,9 @@ __global__ void __launch_bounds__(64 * W, HD <= 128 ? 2 : 1) kv4_attend_kernel(c
         }
         for (; tile < to; tile += W) {
             const bool more = tile + W < to;
-            const int key0 = (span.first + tile) * kKv4Tile;
-            const bool v_there = is_page(v_page), masked = key0 + kKv4Tile > pos0 + 1 || key0 < all_begin || !__all(v_there);
+            const int key0 = kv4_key_tile(span, tile) * kKv4Tile;
+            const bool v_there = is_page(v_page);
+            const bool masked = key0 + kKv4Tile > pos0 + 1 || (key0 < all_begin && (!PACKED || key0 + kKv4Tile > a.sinks)) || !__all(v_there);
             int v_page2 = 0, k_page2 = 0;
             if (tile + 2 * W < to) v_page2 = page_at(tile + 2 * W, q4), k_page2 = page_at(tile + 2 * W, n >> 2);
             // values to LDS: codes in 8-byte units, unit x of row r at x ^ (r / PER), so that the 16 rows of a transposing load lie in different banks
@@ -355,8 +418,8 @@ __global__ void __launch_bounds__(64 * W, HD <= 128 ? 2 : 1) kv4_attend_kernel(c
             uint32_t odd_groups = 0;   // (several tokens) groups of the lane's key whose parameters are not finite
             if (masked) {
                 const int key = key0 + lane;
-                seen = key < span.length && key >= any_begin && v_there;
-                if (a.tokens > 1) {
+                seen = key < span.length && (key >= any_begin || (PACKED && key < a.sinks)) && v_there;
+                if (tokens > 1) {
 #pragma unroll
                     for (int i = 0; i < WPL; i++)
                         if (((((v_params[i] & 0x7c007c00u) + 0x04000400u) & 0x80008000u) != 0) && seen) odd_groups |= 1u << i;
@@ -394,7 +457,7 @@ __global__ void __launch_bounds__(64 * W, HD <= 128 ? 2 : 1) kv4_attend_kernel(c
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const int k = key0 + 16 * q4 + 4 * t + r;
-                        s[t][r] = block_there && k >= lane_begin && k < lane_end ? s[t][r] : -INFINITY;
+                        s[t][r] = block_there && (k >= lane_begin || (PACKED && k < a.sinks)) && k < lane_end ? s[t][r] : -INFINITY;
                     }
             }
             float mx = s[0][0];
@@ -440,12 +503,12 @@ __global__ void __launch_bounds__(64 * W, HD <= 128 ? 2 : 1) kv4_attend_kernel(c
                     o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p[h][0], o[i], 0, 0, 0);
                 }
             }
-            if (masked && a.tokens > 1) {
+            if (masked && tokens > 1) {
                 // a key with parameters that are not finite was left out above: what rows that see it get is NaN, the other tokens' rows nothing
                 for (uint64_t left = __ballot(odd_groups != 0); left; left &= left - 1) {
                     const int b = __builtin_ctzll(left), k = key0 + b;
                     const uint32_t odd = __builtin_amdgcn_readlane(odd_groups, b);
-                    const bool sees = k >= lane_begin && k < lane_end;
+                    const bool sees = (k >= lane_begin || (PACKED && k < a.sinks)) && k < lane_end;
 #pragma unroll
                     for (int i = 0; i < MT; i++)
                         if ((odd >> (i / 2) & 1) && sees) o[i] += kvf4{NAN, NAN, NAN, NAN};
@@ -474,7 +537,7 @@ __global__ void __launch_bounds__(64 * W, HD <= 128 ? 2 : 1) kv4_attend_kernel(c
         const bool whole = from == 0 && to == u.span.count;
         auto store_row = [&](int r, int c, const float4 &v, float inv) {
             const int rr = block * kKv4Rows + r, tk = rr / a.group;
-            T *y = static_cast<T *>(a.y) + ((int64_t)u.seq * a.tokens + tk) * a.y_stride + (int64_t)(kvh * a.group + rr - tk * a.group) * HD + c;
+            T *y = static_cast<T *>(a.y) + (row0 + tk) * a.y_stride + (int64_t)(kvh * a.group + rr - tk * a.group) * HD + c;
             typedef T T4 __attribute__((ext_vector_type(4)));
             const T4 out = {(T)(v.x * inv), (T)(v.y * inv), (T)(v.z * inv), (T)(v.w * inv)};
             if (a.wide) {
@@ -558,21 +621,75 @@ __global__ void __launch_bounds__(64 * W, HD <= 128 ? 2 : 1) kv4_attend_kernel(c
 
         at = u.before + steps;
         if (at >= run1) break;
-        if (++u.inner < per_seq) u.before = at;
-        else if (!kv4_next(a, at, cut, &u)) break;
+        if (++u.inner < a.cache.n_kv_heads * u.blocks) u.before = at;
+        else if (!kv4_next<PACKED>(a, at, cut, &u)) break;
     }
 }
 
-template <int HD>
+template <int HD, bool PACKED>
 void kv4_launch(hipc_ctx *ctx, const Kv4Attend &a, int dtype, bool alone) {
     auto launch = [&](auto waves) {
         constexpr int W = decltype(waves)::value;
         const unsigned grid = kKv4PerCu * ctx->cu_count / W;
-        if (dtype == HIPC_F16) hipLaunchKernelGGL((kv4_attend_kernel<HD, 1, W>), grid, 64 * W, 0, ctx->stream, a);
-        else hipLaunchKernelGGL((kv4_attend_kernel<HD, 2, W>), grid, 64 * W, 0, ctx->stream, a);
+        if (dtype == HIPC_F16) hipLaunchKernelGGL((kv4_attend_kernel<HD, 1, W, PACKED>), grid, 64 * W, 0, ctx->stream, a);
+        else hipLaunchKernelGGL((kv4_attend_kernel<HD, 2, W, PACKED>), grid, 64 * W, 0, ctx->stream, a);
     };
     if (alone) launch(std::integral_constant<int, 1>());
     else launch(std::integral_constant<int, 4>());
+}
+
+// what every attention over the cache checks beside its heads and its cache
+int kv4_attention_check(hipc_ctx *ctx, const char *who, const hipc_kv4_cache *cache, const hipc_attention_heads *heads) {
+    HIPC_REQUIRE(ctx, heads->causal, "%s: a cache is attended to causally", who);
+    HIPC_REQUIRE(ctx, heads->n_kv_heads == cache->n_kv_heads && heads->head_dim == cache->head_dim, "%s: %d kv heads of %d channels, the cache has %d of %d", who,
+                 heads->n_kv_heads, heads->head_dim, cache->n_kv_heads, cache->head_dim);
+    return HIPC_OK;
+}
+int kv4_attention_rows(hipc_ctx *ctx, const char *who, const hipc_attention_heads *heads, int dtype, const void *Q, int64_t q_stride, const void *Y, int64_t y_stride) {
+    const size_t size = dtype == HIPC_F16 ? 2 : 4;
+    const int64_t width = (int64_t)heads->n_q_heads * heads->head_dim;
+    HIPC_REQUIRE(ctx, Q && Y && aligned(Q, size) && aligned(Y, size), "%s: Q and Y", who);
+    HIPC_REQUIRE(ctx, q_stride >= width && y_stride >= width && q_stride <= (int64_t)1 << 40 && y_stride <= (int64_t)1 << 40,
+                 "%s: rows %lld and %lld apart, of %lld values", who, (long long)q_stride, (long long)y_stride, (long long)width);
+    return HIPC_OK;
+}
+void kv4_attend_args(const hipc_kv4_cache *cache, const hipc_attention_heads *heads, int dtype, const void *Q, int64_t q_stride, void *Y, int64_t y_stride, Kv4Attend *a) {
+    a->cache = *cache, a->q = Q, a->y = Y, a->q_stride = q_stride, a->y_stride = y_stride;
+    a->n_q_heads = heads->n_q_heads, a->group = heads->n_q_heads / heads->n_kv_heads, a->window = std::min(heads->window, kKv4MaxPositions);
+    const int64_t unit = dtype == HIPC_F16 ? 8 : 4;
+    a->wide = aligned(Q, 16) && aligned(Y, 16) && q_stride % unit == 0 && y_stride % unit == 0;
+}
+// what workgroups exchange, and the words they count in, in a scratch slot of these operators' own: the words are zero
+// between calls, so a new block is cleared once
+int kv4_attend_scratch(hipc_ctx *ctx, Kv4Attend *a) {
+    const unsigned grid = kKv4PerCu * ctx->cu_count;   // at most
+    const size_t count_bytes = (grid * 4 + 255) & ~(size_t)255;
+    const void *before = ctx->scratch[kScratchKv4].ptr;
+    void *block = nullptr;
+    if (int rc = scratch_get(ctx, kScratchKv4, count_bytes + (size_t)grid * 2 * kKv4Rows * (kKv4MaxHead + 2) * 4, &block)) return rc;
+    a->arrived = static_cast<uint32_t *>(block), a->parts = reinterpret_cast<float *>(static_cast<char *>(block) + count_bytes);
+    if (block != before) {
+        hipLaunchKernelGGL((fill_words), 1, 256, 0, ctx->stream, a->arrived, count_bytes / 4, 0u);
+        HIPC_LAUNCHED(ctx);
+    }
+    return HIPC_OK;
+}
+// units: how many there are, or about as many
+template <bool PACKED>
+int kv4_attend(hipc_ctx *ctx, const Kv4Attend &a, int dtype, int64_t units) {
+    const bool alone = units * 2 >= 3 * (int64_t)ctx->cu_count;
+    switch (a.cache.head_dim / 32) {
+        case 1: kv4_launch<32, PACKED>(ctx, a, dtype, alone); break;
+        case 2: kv4_launch<64, PACKED>(ctx, a, dtype, alone); break;
+        case 3: kv4_launch<96, PACKED>(ctx, a, dtype, alone); break;
+        case 4: kv4_launch<128, PACKED>(ctx, a, dtype, alone); break;
+        case 5: kv4_launch<160, PACKED>(ctx, a, dtype, alone); break;
+        case 6: kv4_launch<192, PACKED>(ctx, a, dtype, alone); break;
+        case 7: kv4_launch<224, PACKED>(ctx, a, dtype, alone); break;
+        default: kv4_launch<256, PACKED>(ctx, a, dtype, alone); break;
+    }
+    HIPC_LAUNCHED(ctx);
+    return HIPC_OK;
 }
 
 }  // namespace
@@ -602,49 +719,39 @@ int hipc_kv4_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_at
         Kv4Attend a{};
         if (int rc = kv4_check(ctx, who, cache)) return rc;
         if (int rc = attention_check(ctx, who, heads, dtype, &a.scale)) return rc;
-        HIPC_REQUIRE(ctx, heads->causal, "%s: a cache is attended to causally", who);
-        HIPC_REQUIRE(ctx, heads->n_kv_heads == cache->n_kv_heads && heads->head_dim == cache->head_dim, "%s: %d kv heads of %d channels, the cache has %d of %d", who,
-                     heads->n_kv_heads, heads->head_dim, cache->n_kv_heads, cache->head_dim);
+        if (int rc = kv4_attention_check(ctx, who, cache, heads)) return rc;
         const int64_t group = heads->n_q_heads / heads->n_kv_heads;
         HIPC_REQUIRE(ctx, tokens > 0, "%s: %lld tokens a sequence", who, (long long)tokens);
         HIPC_REFUSE(ctx, tokens > 1024 || tokens * group > 1024, "%s: %lld tokens of %lld heads to a kv head: more than 1024 query rows", who, (long long)tokens, (long long)group);
         if (cache->n_seqs == 0) return HIPC_OK;
-        const size_t size = dtype == HIPC_F16 ? 2 : 4;
-        const int64_t width = (int64_t)heads->n_q_heads * heads->head_dim;
-        HIPC_REQUIRE(ctx, Q && Y && aligned(Q, size) && aligned(Y, size), "%s: Q and Y", who);
-        HIPC_REQUIRE(ctx, q_stride >= width && y_stride >= width && q_stride <= (int64_t)1 << 40 && y_stride <= (int64_t)1 << 40,
-                     "%s: rows %lld and %lld apart, of %lld values", who, (long long)q_stride, (long long)y_stride, (long long)width);
-        a.cache = *cache, a.q = Q, a.y = Y, a.q_stride = q_stride, a.y_stride = y_stride;
-        a.tokens = (int)tokens, a.n_q_heads = heads->n_q_heads, a.group = (int)group, a.window = std::min(heads->window, kKv4MaxPositions);
-        a.row_blocks = (int)ceil_div(tokens * group, kKv4Rows);
-        const int64_t unit = dtype == HIPC_F16 ? 8 : 4;
-        a.wide = aligned(Q, 16) && aligned(Y, 16) && q_stride % unit == 0 && y_stride % unit == 0;
-        // what workgroups exchange, and the words they count in, in a scratch slot of this operator's own: the words are zero
-        // between calls, so a new block is cleared once
-        const unsigned grid = kKv4PerCu * ctx->cu_count;   // at most
-        const size_t count_bytes = (grid * 4 + 255) & ~(size_t)255;
-        const void *before = ctx->scratch[kScratchKv4].ptr;
-        void *block = nullptr;
-        if (int rc = scratch_get(ctx, kScratchKv4, count_bytes + (size_t)grid * 2 * kKv4Rows * (kKv4MaxHead + 2) * 4, &block)) return rc;
-        a.arrived = static_cast<uint32_t *>(block), a.parts = reinterpret_cast<float *>(static_cast<char *>(block) + count_bytes);
-        if (block != before) {
-            hipLaunchKernelGGL((fill_words), 1, 256, 0, ctx->stream, a.arrived, count_bytes / 4, 0u);
-            HIPC_LAUNCHED(ctx);
-        }
+        if (int rc = kv4_attention_rows(ctx, who, heads, dtype, Q, q_stride, Y, y_stride)) return rc;
+        kv4_attend_args(cache, heads, dtype, Q, q_stride, Y, y_stride, &a);
+        a.tokens = (int)tokens, a.row_blocks = (int)ceil_div(tokens * group, kKv4Rows);
+        if (int rc = kv4_attend_scratch(ctx, &a)) return rc;
         const int64_t units = (int64_t)cache->n_seqs * cache->n_kv_heads * a.row_blocks;
-        const bool alone = units * 2 >= 3 * (int64_t)ctx->cu_count;
-        switch (heads->head_dim / 32) {
-            case 1: kv4_launch<32>(ctx, a, dtype, alone); break;
-            case 2: kv4_launch<64>(ctx, a, dtype, alone); break;
-            case 3: kv4_launch<96>(ctx, a, dtype, alone); break;
-            case 4: kv4_launch<128>(ctx, a, dtype, alone); break;
-            case 5: kv4_launch<160>(ctx, a, dtype, alone); break;
-            case 6: kv4_launch<192>(ctx, a, dtype, alone); break;
-            case 7: kv4_launch<224>(ctx, a, dtype, alone); break;
-            default: kv4_launch<256>(ctx, a, dtype, alone); break;
-        }
-        HIPC_LAUNCHED(ctx);
-        return HIPC_OK;
+        return kv4_attend<false>(ctx, a, dtype, units);
+    });
+}
+
+int hipc_kv4_prompt_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_attention_heads *heads, int32_t sinks, int dtype, const void *starts,
+                              int64_t total, const void *Q, int64_t q_stride, void *Y, int64_t y_stride) {
+    return entry(ctx, [&]() -> int {
+        const char *who = "hipc_kv4_prompt_attention";
+        Kv4Attend a{};
+        if (int rc = kv4_check(ctx, who, cache)) return rc;
+        if (int rc = attention_check(ctx, who, heads, dtype, &a.scale)) return rc;
+        if (int rc = kv4_attention_check(ctx, who, cache, heads)) return rc;
+        HIPC_REQUIRE(ctx, sinks >= 0, "%s: %d first positions that stay visible", who, sinks);
+        HIPC_REQUIRE(ctx, total >= 0 && total <= 1 << 30, "%s: %lld rows", who, (long long)total);
+        if (total == 0 || cache->n_seqs == 0) return HIPC_OK;
+        HIPC_REQUIRE(ctx, starts && aligned(starts, 4), "%s: starts", who);
+        if (int rc = kv4_attention_rows(ctx, who, heads, dtype, Q, q_stride, Y, y_stride)) return rc;
+        kv4_attend_args(cache, heads, dtype, Q, q_stride, Y, y_stride, &a);
+        const int64_t blocks = ceil_div(total * a.group, kKv4Rows) + cache->n_seqs, units = blocks * cache->n_kv_heads;
+        HIPC_REFUSE(ctx, units > 1 << 22, "%s: %lld rows: too many for one call", who, (long long)total);
+        a.starts = static_cast<const int *>(starts), a.total = (int)total, a.sinks = std::min(sinks, kKv4MaxPositions), a.most = 1 << 30;
+        if (int rc = kv4_attend_scratch(ctx, &a)) return rc;
+        return kv4_attend<true>(ctx, a, dtype, units);
     });
 }
 

@@ -475,6 +475,10 @@ def kv4_attention_device(ctx, cache: Kv4Cache, heads: AttentionHeads, dtype, tok
     ctx._check(ctx.lib.hipc_kv4_attention(ctx.handle, cache, heads, dtype, tokens, _ptr(Q), q_stride, _ptr(Y), y_stride))
 
 
+def kv4_prompt_attention_device(ctx, cache: Kv4Cache, heads: AttentionHeads, sinks, dtype, starts, total, Q, q_stride, Y, y_stride):
+    ctx._check(ctx.lib.hipc_kv4_prompt_attention(ctx.handle, cache, heads, sinks, dtype, _ptr(starts), total, _ptr(Q), q_stride, _ptr(Y), y_stride))
+
+
 def _rows_match(what, arrays, shapes, dtype):
     """The device reads every operand by the first one's type and shape."""
     for x, shape in zip(arrays, shapes):
@@ -583,6 +587,21 @@ class Kv4Pages:
         kv4_attention_device(self.ctx, self.cache, heads, hipc_dtype(q.dtype), tokens, dQ, row, dY, row)
         y = self.ctx.download(dY, q.dtype, q.shape)
         dQ.free(), dY.free()
+        return y
+
+    def prompt_attention(self, q, new, window=0, sinks=0, scale=0.0):
+        """Packed rows ``q [sum(new), heads, dim]``, the last ``new[s]`` positions of sequence s, over its cache; with a window the first ``sinks``
+        positions stay visible."""
+        q = np.ascontiguousarray(q)
+        _rows_match("prompt_attention", (q,), ((q.shape[0], q.shape[1], self.head_dim),), q.dtype)
+        starts = _starts("prompt_attention", new, self.n_seqs, q.shape[0])
+        heads = AttentionHeads(q.shape[1], self.n_kv_heads, self.head_dim, 1, window, scale)
+        dQ, dY, ds = self.ctx.upload(q), self.ctx.upload(np.zeros_like(q)), self.ctx.upload(starts)
+        row = q.shape[1] * q.shape[2]
+        kv4_prompt_attention_device(self.ctx, self.cache, heads, sinks, hipc_dtype(q.dtype), ds, q.shape[0], dQ, row, dY, row)
+        y = self.ctx.download(dY, q.dtype, q.shape)
+        for b in (dQ, dY, ds):
+            b.free()
         return y
 
     def free(self):

@@ -167,6 +167,7 @@ SIGNATURES = {
     "hipc_kv4_append": (_int, [_vp, C.POINTER(Kv4Cache), _int, _vp, _i64, _vp, _i64, _vp, _i64]),
     "hipc_kv4_read": (_int, [_vp, C.POINTER(Kv4Cache), _int, _vp, _i64, _vp, _i64, _vp, _i64]),
     "hipc_kv4_attention": (_int, [_vp, C.POINTER(Kv4Cache), C.POINTER(AttentionHeads), _int, _i64, _vp, _i64, _vp, _i64]),
+    "hipc_kv4_prompt_attention": (_int, [_vp, C.POINTER(Kv4Cache), C.POINTER(AttentionHeads), C.c_int32, _int, _vp, _i64, _vp, _i64, _vp, _i64]),
     "hipc_token_logprobs": (_int, [_vp, _int, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _int, _vp, _vp]),
     "hipc_decoder_create": (_int, [_vp, C.POINTER(DecoderConfig), C.POINTER(_vp)]),
     "hipc_decoder_destroy": (None, [_vp, _vp]),

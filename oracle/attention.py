@@ -138,6 +138,30 @@ class Cache:
         return y, weight, size
 
 
+    def prompt_attention(self, q, starts, lengths, window=0, sinks=0, scale=None):
+        """Packed rows: (y, sum w |v|, score sizes, largest |v| seen [rows, heads, 1]); rows of no sequence are NaN."""
+        heads, n_kv = q.shape[1], self.codes[0].shape[1]
+        scale = scale or 1.0 / math.sqrt(q.shape[2])
+        y, weight = np.full(q.shape, np.nan), np.zeros(q.shape)
+        size, most = np.zeros(q.shape[:2] + (1,)), np.zeros(q.shape[:2] + (1,))
+        for s, length in enumerate(lengths):
+            length, first, end = max(0, int(length)), max(0, int(starts[s])), min(q.shape[0], int(starts[s + 1]))
+            held = [t for t in range(min(length, self.table.shape[1] * self.page)) if self.place(s, t) is not None] if first < end else []
+            k, v = (np.stack([self.load(w, s, t) for t in held], 1) if held else None for w in (0, 1))
+            held = np.array(held, np.int64)
+            for r in range(first, end):
+                pos = length - end + r
+                see = (held <= pos) & ((held > pos - window) | (held < sinks) if window else True)
+                y[r] = 0
+                if not see.any():
+                    continue
+                for h in range(heads):
+                    g = h // (heads // n_kv)
+                    y[r, h], weight[r, h], size[r, h] = attend_row(q[r, h], k[g][see], v[g][see], int(see.sum()) - 1, scale)
+                    most[r, h] = np.abs(v[g][see].astype(f64)).max()
+        return y, weight, size, most
+
+
 def token_logprobs(x, tokens, top):
     """(logprob, entropy, ids, logprobs of the best) in 64 bits."""
     rows, vocab = x.shape

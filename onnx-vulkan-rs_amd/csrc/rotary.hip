@@ -5,9 +5,9 @@
 //   y_a = x^_a cos - x^_b sin,  y_b = x^_b cos + x^_a sin              (a, b) = (i, i + n) or (2i, 2i + 1), angle = position * frequency[i]
 //
 // A position's angles are one row's and all its heads'. They are formed in 64 bits: in 32 an angle of a million is off by a sixteenth. A product of
-// 31 and 24 bits, in turns; what is left behind whole turns goes to sine and cosine. Queries are then computed in 32 bits. Keys are computed in 64 up to their
-// one rounding, because a cache stores what they are quantized to: a key next to the border between two codes, or that is the lowest of
-// its group, would fall on either side by the order of a sum.
+// 31 and 24 bits, in turns; what is left behind whole turns goes to sine and cosine. Everything else is f32, as in the decode step's norm and rotation,
+// every step rounded by itself (this file is compiled without contraction): a cache stores what keys are quantized to, and one that stands next to the border
+// between two codes, or is the lowest of its group, is to fall on the side where these steps put it, whatever kernel or layout takes them.
 //
 // Memory bounds it. A wavefront has a row, or some heads of one where rows are few, and takes 64 / L heads at a time, L lanes a head; a lane has a
 // vector of V channels and the V channels they turn with, the same channels of every head it sees, so that its cosines and sines stay in registers.
@@ -33,47 +33,19 @@ struct RotaryArgs {
     const float *frequencies, *q_norm, *k_norm;
     int rows, n_q, n_kv, dim, half, interleaved;
     int lg_lanes, chunks, per;         // lanes of a head (a power of two); wavefronts of a row, and what each takes of it
-    float eps;
-    double amplitude;
+    float eps, amplitude;
 };
 
-template <int CTRL>
-__device__ __forceinline__ double dpp_add(double v) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, true), hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, true);
-    return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-template <int CTRL>
-__device__ __forceinline__ float dpp_add(float v) { return v + lean_dpp<CTRL>(v); }
 // the sum over 2^lg neighbouring lanes, in all of them (lg is uniform)
-template <typename F>
-__device__ __forceinline__ F lanes_sum(F v, int lg) {
-    if (lg > 0) v = dpp_add<0xB1>(v);    // quad_perm [1,0,3,2]
-    if (lg > 1) v = dpp_add<0x4E>(v);    // quad_perm [2,3,0,1]
-    if (lg > 2) v = dpp_add<0x141>(v);   // the other four of eight (mirrored)
-    if (lg > 3) v = dpp_add<0x140>(v);   // the other eight of sixteen
+__device__ __forceinline__ float lanes_sum(float v, int lg) {
+    if (lg > 0) v += lean_dpp<0xB1>(v);    // quad_perm [1,0,3,2]
+    if (lg > 1) v += lean_dpp<0x4E>(v);    // quad_perm [2,3,0,1]
+    if (lg > 2) v += lean_dpp<0x141>(v);   // the other four of eight (mirrored)
+    if (lg > 3) v += lean_dpp<0x140>(v);   // the other eight of sixteen
     if (lg > 4) v += __shfl_xor(v, 16);
     if (lg > 5) v += __shfl_xor(v, 32);
     return v;
 }
-
-// one rounding to the rows' type
-__device__ __forceinline__ void rounded(double d, float *out) { *out = (float)d; }
-__device__ __forceinline__ void rounded(double d, _Float16 *out) {
-    // through f32 rounded to odd: what lies between two f32 numbers takes the odd one, so that the second rounding sees on which side of a tie it was
-    float f = (float)d;
-    uint32_t bits = __float_as_uint(f);
-    const double back = (double)f;
-    if (back != d && d - d == 0.0 && !(bits & 1)) bits += __builtin_fabs(d) > __builtin_fabs(back) ? 1 : -1;
-    *out = (_Float16)__uint_as_float(bits);
-}
-__device__ __forceinline__ void rounded(float f, float *out) { *out = f; }
-__device__ __forceinline__ void rounded(float f, _Float16 *out) { *out = (_Float16)f; }
-
-__device__ __forceinline__ float one_over_root(float v) { return 1.f / sqrtf(v); }
-__device__ __forceinline__ double one_over_root(double v) { return 1.0 / sqrt(v); }
-__device__ __forceinline__ float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
-__device__ __forceinline__ double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
 
 // V values side by side; rows and strides lie on 16 bytes (V values, where these are less) or V is 1
 template <typename T, int V>
@@ -106,7 +78,7 @@ template <typename T, int V, bool STORE>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     constexpr int E = V == 1 ? 4 : 1;            // items of a lane: V channels and the V they turn with, or 2 V behind those that turn
     constexpr int N = 2 * V * E, UNITS = N / 8;   // a lane's values at a time; as units of eight side by side
-    __shared__ double2 turns[4][kRotaryMaxHead / 2];
+    __shared__ float2 turns[4][kRotaryMaxHead / 2];
     __shared__ float keys[STORE ? 4 : 1][STORE ? 64 * N : 1];
     const int w = kv4_wave(), lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = w / a.chunks, chunk = w - row * a.chunks;
     if (row >= a.rows) return;
@@ -166,52 +138,57 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     T next[N];
     load(pass0, next);
 
+    // norm weights of the lane's channels: the queries', then the keys'
+    float weight[N];
+    auto load_weights = [&](const float *w) {
+#pragma unroll
+        for (int i = 0; i < 2 * E; i++)
+#pragma unroll
+            for (int j = 0; j < V; j++) weight[i * V + j] = w && c[i / 2][i % 2] >= 0 ? w[c[i / 2][i % 2] + j] : 1.f;
+    };
+    load_weights(pass0 < q_passes ? a.q_norm : a.k_norm);
+
     // the angles, a pair a lane, while the first heads are on their way
     for (int p = lane; p < a.half; p += 64) {
         const double turn = (double)position * (double)a.frequencies[p] * 0.15915494309189533577;   // 1 / (2 pi)
         double s, co;
         sincospi(2.0 * (turn - __builtin_rint(turn)), &s, &co);
-        turns[wave][p] = make_double2(co * a.amplitude, s * a.amplitude);
+        turns[wave][p] = make_float2((float)co * a.amplitude, (float)s * a.amplitude);
     }
     wave_meets();
-    float cos32[E][V], sin32[E][V];
+    float cosine[E][V], sine[E][V];
 #pragma unroll
     for (int e = 0; e < E; e++)
 #pragma unroll
         for (int j = 0; j < V; j++) {
-            const double2 t = pair[e] >= 0 ? turns[wave][pair[e] + j] : make_double2(1.0, 0.0);
-            cos32[e][j] = (float)t.x, sin32[e][j] = (float)t.y;
+            const float2 t = pair[e] >= 0 ? turns[wave][pair[e] + j] : make_float2(1.f, 0.f);
+            cosine[e][j] = t.x, sine[e][j] = t.y;
         }
 
-    // the lane's values of a head, normed and turned in F: the same steps for queries (32 bits) and keys (64)
-    auto turned = [&](auto zero, const T (&x)[N], const float *weight, auto cosine, auto sine, T (&y)[N]) {
-        typedef decltype(zero) F;
-        F v[N];
-        F sum = zero;
+    // the lane's values of a head, normed and turned
+    auto turned = [&](const T (&x)[N], bool norm, T (&y)[N]) {
+        float v[N], sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = (F)(float)x[i], sum = fused(v[i], v[i], sum);
-        if (weight) {
-            const F by = one_over_root(lanes_sum(sum, a.lg_lanes) / (F)a.dim + (F)a.eps);
+        for (int i = 0; i < N; i++) v[i] = (float)x[i], sum += v[i] * v[i];
+        if (norm) {
+            const float by = rsqrtf(lanes_sum(sum, a.lg_lanes) / (float)a.dim + a.eps);
 #pragma unroll
-            for (int i = 0; i < 2 * E; i++)
-#pragma unroll
-                for (int j = 0; j < V; j++)
-                    if (c[i / 2][i % 2] >= 0) v[i * V + j] = v[i * V + j] * by * (F)weight[c[i / 2][i % 2] + j];
+            for (int i = 0; i < N; i++) v[i] = v[i] * by * weight[i];
         }
 #pragma unroll
         for (int e = 0; e < E; e++)
 #pragma unroll
             for (int j = 0; j < V; j++) {
                 // (one of an item's halves and the other's, or its neighbours)
-                const F half_a = v[2 * e * V + j], half_b = v[(2 * e + 1) * V + j], near_a = v[2 * e * V + 2 * j], near_b = v[2 * e * V + 2 * j + 1];
-                const F p = a.interleaved ? near_a : half_a, q = a.interleaved ? near_b : half_b, co = cosine(e, j), s = sine(e, j);
-                const F first = fused(p, co, -(q * s)), second = fused(q, co, p * s);
+                const float half_a = v[2 * e * V + j], half_b = v[(2 * e + 1) * V + j], near_a = v[2 * e * V + 2 * j], near_b = v[2 * e * V + 2 * j + 1];
+                const float p = a.interleaved ? near_a : half_a, q = a.interleaved ? near_b : half_b;
+                const float first = p * cosine[e][j] - q * sine[e][j], second = q * cosine[e][j] + p * sine[e][j];
                 if (a.interleaved) {
-                    rounded(pair[e] >= 0 ? first : near_a, &y[2 * e * V + 2 * j]);
-                    rounded(pair[e] >= 0 ? second : near_b, &y[2 * e * V + 2 * j + 1]);
+                    y[2 * e * V + 2 * j] = (T)(pair[e] >= 0 ? first : near_a);
+                    y[2 * e * V + 2 * j + 1] = (T)(pair[e] >= 0 ? second : near_b);
                 } else {
-                    rounded(pair[e] >= 0 ? first : half_a, &y[2 * e * V + j]);
-                    rounded(pair[e] >= 0 ? second : half_b, &y[(2 * e + 1) * V + j]);
+                    y[2 * e * V + j] = (T)(pair[e] >= 0 ? first : half_a);
+                    y[(2 * e + 1) * V + j] = (T)(pair[e] >= 0 ? second : half_b);
                 }
             }
     };
@@ -241,11 +218,12 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
         if (pass + 1 < pass1) load(pass + 1, next);
         if (pass < q_passes) {
             const int head = pass * together + head0;
-            turned(0.f, x, a.q_norm, [&](int e, int j) { return cos32[e][j]; }, [&](int e, int j) { return sin32[e][j]; }, y);
+            turned(x, a.q_norm != nullptr, y);
             if (head < a.n_q) put(static_cast<T *>(a.q_out) + a.q_out_stride * row + (int64_t)head * a.dim, y);
         } else if (pass < q_passes + k_passes) {
             const int first = (pass - q_passes) * together, head = first + head0;
-            turned(0.0, x, a.k_norm, [&](int e, int j) { return turns[wave][max(pair[e], 0) + j].x; }, [&](int e, int j) { return turns[wave][max(pair[e], 0) + j].y; }, y);
+            if (pass == q_passes && pass > pass0) load_weights(a.k_norm);
+            turned(x, a.k_norm != nullptr, y);
             if (!STORE) {
                 if (head < a.n_kv) put(static_cast<T *>(a.k_out) + a.k_out_stride * row + (int64_t)head * a.dim, y);
                 continue;
@@ -290,7 +268,7 @@ int rotary_check(hipc_ctx *ctx, const char *who, const hipc_rotary_heads *h, int
     HIPC_REQUIRE(ctx, rows >= 0 && rows <= 0x7fffffff, "%s: %lld rows", who, (long long)rows);
     a->frequencies = static_cast<const float *>(h->frequencies), a->q_norm = static_cast<const float *>(h->q_norm), a->k_norm = static_cast<const float *>(h->k_norm);
     a->rows = (int)rows, a->n_q = h->n_q_heads, a->n_kv = h->n_kv_heads, a->dim = h->head_dim, a->half = h->rotary_dim / 2, a->interleaved = h->interleaved != 0;
-    a->eps = h->norm_eps, a->amplitude = h->amplitude != 0.f ? h->amplitude : 1.0;
+    a->eps = h->norm_eps, a->amplitude = h->amplitude != 0.f ? h->amplitude : 1.f;
     return HIPC_OK;
 }
 // rows of `heads` heads, `stride` apart

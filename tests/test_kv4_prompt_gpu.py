@@ -12,6 +12,7 @@ import pytest
 
 from oracle import attention as ref
 from test_kv4_gpu import Pair, bits
+from test_rotary_gpu import check
 
 pytestmark = pytest.mark.gpu
 
@@ -295,7 +296,7 @@ def test_recorded_on_a_context_that_has_run_none(pkg):
 @pytest.mark.parametrize("window,sinks", [(0, 0), (48, 4)], ids=str)
 def test_a_layer_of_prompts_in_pieces_and_tokens(ctx, pkg, dtype, window, sinks):
     """The calls as a program makes them: rows of a projection are normed, turned and stored, then attended with, piece by piece and token by token, beside
-    other sequences; every step against the definition on the oracle's cache, filled by the oracle's keys."""
+    other sequences; every step against the definition: queries and keys by the formulas, the cache by the oracle's from these keys, and attention on that."""
     rng = np.random.default_rng(11)
     heads, kv, dim, page = 8, 2, 64, 16
     f = pkg.ops.rotary_frequencies(1e4, dim, pkg.ops.ROTARY_BY_PARTS, 4.0, 64, 1, 8)
@@ -310,10 +311,9 @@ def test_a_layer_of_prompts_in_pieces_and_tokens(ctx, pkg, dtype, window, sinks)
         turned = c.gpu.append_rotary(turning, q, k, v, new)
         got = c.gpu.prompt_attention(turned, new, window, sinks)
         at = np.concatenate([np.arange(int(n) - m, int(n)) for m, n in zip(new, c.lengths)])
-        want_q, size = ref.rotary(q, at, f, norms[0], 1e-6, False, 1.1)
-        step = 2.0 ** -11 if dtype == np.float16 else 2.0 ** -24
-        assert np.all(np.abs(turned.astype(np.float64) - want_q) <= np.abs(want_q) * step + (dim / 2 + 12) * 2.0 ** -24 * 2 * size + 1e-6 * (dtype == np.float16))
-        key = ref.rotary(k, at, f, norms[1], 1e-6, False, 1.1)[0].astype(dtype)
+        again, key = turning(q, k, at)
+        assert np.array_equal(bits(again), bits(turned))
+        check(turned, q, at, f, norms[0], amplitude=1.1), check(key, k, at, f, norms[1], amplitude=1.1)
         i = 0
         for s, m in enumerate(new):
             for p in range(int(c.lengths[s]) - m, int(c.lengths[s])):

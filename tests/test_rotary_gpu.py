@@ -4,9 +4,8 @@ it stands for.
 Tolerances, of a result y with |x^_a cos| + |x^_b sin| = S (the oracle's second result):
   angles   position * frequency is off by 2^-51 of itself (stated), sine and cosine by a few steps of 64 bits more: A (|x^_a| + |x^_b|) (2^-51 angle + 2^-50);
            |x^_a| + |x^_b| is at most 2 S A^-1 / max(|cos|, |sin|) <= 2 sqrt(2) S_pair / A, S_pair the larger of the pair's two S
-  keys     64 bits (S dim 2^-52 is more than all their steps), one rounding: half a step of y, and of the type's least numbers
-  queries  f32: the sum of dim squares and the mean, off by (dim + 2) 2^-24 and halved by the root, which rounds with its reciprocal (3 steps); two products, cosine
-           and sine, two products and a sum: (dim / 2 + 12) 2^-24 S, then the rounding
+  values   f32: the sum of dim squares and the mean, off by (dim + 2) 2^-24 and halved by the root, which rounds with its reciprocal (3 steps); two products, cosine
+           and sine times the amplitude, two products and a sum: (dim / 2 + 12) 2^-24 S, then the rounding to the type
 """
 import numpy as np
 import pytest
@@ -23,7 +22,7 @@ def table(dim, base=1e4):
     return (base ** (-2.0 * np.arange(dim // 2) / max(dim, 1))).astype(np.float32)
 
 
-def check(got, x, positions, frequencies, norm, key, eps=1e-6, interleaved=False, amplitude=1.0):
+def check(got, x, positions, frequencies, norm, eps=1e-6, interleaved=False, amplitude=1.0):
     want, size = ref.rotary(x, positions, frequencies, norm, eps, interleaved, amplitude)
     n, dim = len(frequencies), x.shape[2]
     pair = size.copy()
@@ -33,7 +32,7 @@ def check(got, x, positions, frequencies, norm, key, eps=1e-6, interleaved=False
         pair[..., a] = pair[..., b] = np.maximum(size[..., a], size[..., b])
         angle[..., a] = angle[..., b] = np.abs(positions.astype(np.float64) * np.float64(frequencies[i]))[:, None]
     step, least = HALF_STEP[x.dtype]
-    allowed = 2 * 2 ** 0.5 * pair * (angle * 2.0 ** -51 + 2.0 ** -50) + (dim * 2.0 ** -52 if key else (dim / 2 + 12) * 2.0 ** -24) * size
+    allowed = 2 * 2 ** 0.5 * pair * (angle * 2.0 ** -51 + 2.0 ** -50) + (dim / 2 + 12) * 2.0 ** -24 * size
     allowed = allowed * (1 + step) + np.abs(want) * step + least
     off = np.abs(got.astype(np.float64) - want) - allowed
     assert got.dtype == x.dtype and np.all(off <= 0), (float(off.max()), np.unravel_index(np.argmax(off), off.shape))
@@ -54,8 +53,8 @@ def test_against_the_formulas(ctx, pkg, dtype, interleaved, heads, kv, dim, turn
         turning = pkg.ops.Rotary(ctx, heads, kv, dim, f, qn, kn, 1e-6, interleaved, amplitude)
         got_q, got_k = turning(q, k, at)
         turning.free()
-        check(got_q, q, at, f, qn, False, 1e-6, interleaved, amplitude)
-        check(got_k, k, at, f, kn, True, 1e-6, interleaved, amplitude)
+        check(got_q, q, at, f, qn, 1e-6, interleaved, amplitude)
+        check(got_k, k, at, f, kn, 1e-6, interleaved, amplitude)
 
 
 def test_positions_far_out(ctx, pkg):
@@ -67,8 +66,8 @@ def test_positions_far_out(ctx, pkg):
     turning = pkg.ops.Rotary(ctx, 2, 1, 128, f)
     got_q, got_k = turning(q, k, at)
     turning.free()
-    check(got_q, q, at, f, None, False)
-    check(got_k, k, at, f, None, True)
+    check(got_q, q, at, f, None)
+    check(got_k, k, at, f, None)
     assert np.array_equal(bits(got_q[0]), bits(q[0])) and np.array_equal(bits(got_k[0]), bits(k[0]))   # position 0 turns nothing
 
 
@@ -82,8 +81,8 @@ def test_many_rows(ctx, pkg):
     turning = pkg.ops.Rotary(ctx, 10, 3, 64, f, w, w)
     got_q, got_k = turning(q, k, at)
     turning.free()
-    check(got_q, q, at, f, w, False)
-    check(got_k, k, at, f, w, True)
+    check(got_q, q, at, f, w)
+    check(got_k, k, at, f, w)
 
 
 def test_unusual_values(ctx, pkg):
@@ -99,7 +98,7 @@ def test_unusual_values(ctx, pkg):
         turning = pkg.ops.Rotary(ctx, 6, 6, 64, f, norm, norm, 1e-6)
         q, k = turning(x, x, at)
         turning.free()
-        for got, key in ((q, False), (k, True)):
+        for got in (q, k):
             assert not got[0, 0].any()
             nan = np.isnan(got.astype(np.float32))
             if norm is None:
@@ -108,7 +107,7 @@ def test_unusual_values(ctx, pkg):
             else:
                 assert nan[0, 1].all() and nan[0, 2, 40] and not got[0, 2, 0]        # an infinite mean
             assert np.isfinite(got[0, 5].astype(np.float32)).all()
-            check(got[:, [0, 4, 5]], x[:, [0, 4, 5]], at, f, norm, key)
+            check(got[:, [0, 4, 5]], x[:, [0, 4, 5]], at, f, norm)
 
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
@@ -131,7 +130,7 @@ def test_rows_of_a_projection_in_place(ctx, pkg, dtype, off, pad):
     want_q, want_k = turning(q, k, at)
     out = got[off:].reshape(rows, width)
     close = [np.ascontiguousarray(out[:, a * dim:b * dim]).reshape(rows, -1, dim) for a, b in ((0, heads), (heads, heads + kv))]
-    check(close[0], q, at, f, w, False)
+    check(close[0], q, at, f, w)
     assert np.array_equal(bits(close[1]), bits(want_k))
     assert np.array_equal(bits(out[:, (heads + kv) * dim:]), bits(rowed[:, (heads + kv) * dim:])) and np.array_equal(bits(got[:off]), bits(flat[:off]))
     for b in (d, dP):
@@ -193,17 +192,15 @@ def test_into_the_cache_is_the_two_calls(ctx, pkg, dtype, interleaved, heads, kv
     for a, b in zip(one.gpu.buffers, two.gpu.buffers):
         a, b = (ctx.download(x, np.uint8, (x.nbytes,)) for x in (a, b))
         assert np.array_equal(a, b) and a.any()
-    # ... and what is stored is the definition's: the same keys, formed in 64 bits
-    key = ref.rotary(k, at, table(turn), w[1], 1e-5, interleaved)[0]
-    if dtype == np.float16:
-        three = ref.Cache(one.ref.codes[0].shape[0], page, kv, dim, lost)
-        i = 0
-        for s, (m, n) in enumerate(zip(new, lengths)):
-            for p in range(n - m, n):
-                three.store(s, p, (key[i].astype(dtype), v[i]))
-                i += 1
-        for b, want in zip(one.gpu.buffers, (three.codes[0], three.params[0], three.codes[1], three.params[1])):
-            assert np.array_equal(ctx.download(b, want.dtype, want.shape).view(np.uint8), want.view(np.uint8))
+    # ... and what is stored is the definition's, of the turned keys
+    three = ref.Cache(one.ref.codes[0].shape[0], page, kv, dim, lost)
+    i = 0
+    for s, (m, n) in enumerate(zip(new, lengths)):
+        for p in range(n - m, n):
+            three.store(s, p, (want_k[i], v[i]))
+            i += 1
+    for b, want in zip(one.gpu.buffers, (three.codes[0], three.params[0], three.codes[1], three.params[1])):
+        assert np.array_equal(ctx.download(b, want.dtype, want.shape).view(np.uint8), want.view(np.uint8))
     one.gpu.free(), two.gpu.free(), turning.free()
 
 

@@ -31,7 +31,7 @@ struct RotaryArgs {
     void *q_out, *k_out;
     int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
     const float *frequencies, *q_norm, *k_norm;
-    int rows, n_q, n_kv, dim, half, interleaved;
+    int rows, n_q, n_kv, dim, half;
     int lg_lanes, chunks, per;         // lanes of a head (a power of two); wavefronts of a row, and what each takes of it
     float eps, amplitude;
 };
@@ -74,7 +74,7 @@ __device__ __forceinline__ void wave_meets() {
     __builtin_amdgcn_wave_barrier();
 }
 
-template <typename T, int V, bool STORE>
+template <typename T, int V, bool NEAR, bool STORE>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     constexpr int E = V == 1 ? 4 : 1;            // items of a lane: V channels and the V they turn with, or 2 V behind those that turn
     constexpr int N = 2 * V * E, UNITS = N / 8;   // a lane's values at a time; as units of eight side by side
@@ -101,39 +101,34 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     const int pass0 = chunk * a.per, pass1 = min(pass0 + a.per, passes);
     if (pass0 >= pass1) return;
 
-    // the lane's channels of a head: at c[e][0] and c[e][1], V each (none: -1); the pairs they turn with
+    // The lane's channels of a head: V each from c[e][0] and c[e][1] on, where there[e][.] (else the head's first stand in), and the pairs that they
+    // turn with. NEAR: neighbours turn with each other, and the two lie side by side.
     int c[E][2], pair[E];
+    bool there[E][2];
 #pragma unroll
     for (int e = 0; e < E; e++) {
         const int item = l + (e << a.lg_lanes), turning = a.half / V;
-        pair[e] = item < turning ? item * V : -1;
-        c[e][0] = item < turning && !a.interleaved ? item * V : 2 * item * V;   // (behind the pairs, 2 V an item as well)
-        c[e][1] = item < turning && !a.interleaved ? a.half + item * V : 2 * item * V + V;
-        if (c[e][0] >= a.dim) c[e][0] = -1;
-        if (c[e][1] >= a.dim) c[e][1] = -1;
+        const bool turns_here = item < turning;
+        pair[e] = turns_here ? item * V : -1;
+        c[e][0] = turns_here && !NEAR ? item * V : 2 * item * V;   // (behind the pairs, 2 V an item as well)
+        c[e][1] = turns_here && !NEAR ? a.half + item * V : 2 * item * V + V;
+#pragma unroll
+        for (int h = 0; h < 2; h++) there[e][h] = c[e][h] < a.dim, c[e][h] = there[e][h] ? c[e][h] : 0;
     }
     auto load = [&](int pass, T (&x)[N]) {
         if (STORE && pass >= q_passes + k_passes) {
 #pragma unroll
             for (int i = 0; i < N; i += V) {
                 const int u = ((pass - q_passes - k_passes) * UNITS + i / 8) * 64 + lane;
-                T v[V] = {};
-                if (u < v_units) rotary_load<T, V>(static_cast<const T *>(a.v) + a.v_stride * row + (int64_t)u * 8 + i % 8, v);
-#pragma unroll
-                for (int j = 0; j < V; j++) x[i + j] = v[j];
+                rotary_load<T, V>(static_cast<const T *>(a.v) + a.v_stride * row + (int64_t)min(u, v_units - 1) * 8 + i % 8, *reinterpret_cast<T(*)[V]>(x + i));
             }
             return;
         }
         const bool key = pass >= q_passes;
-        const int head = (key ? pass - q_passes : pass) * together + head0;
+        const int head = min((key ? pass - q_passes : pass) * together + head0, (key ? a.n_kv : a.n_q) - 1);
         const T *from = static_cast<const T *>(key ? a.k : a.q) + (key ? a.k_stride : a.q_stride) * row + (int64_t)head * a.dim;
 #pragma unroll
-        for (int i = 0; i < 2 * E; i++) {
-            T v[V] = {};
-            if (head < (key ? a.n_kv : a.n_q) && c[i / 2][i % 2] >= 0) rotary_load<T, V>(from + c[i / 2][i % 2], v);
-#pragma unroll
-            for (int j = 0; j < V; j++) x[i * V + j] = v[j];
-        }
+        for (int i = 0; i < 2 * E; i++) rotary_load<T, V>(from + c[i / 2][i % 2], *reinterpret_cast<T(*)[V]>(x + i * V));
     };
     T next[N];
     load(pass0, next);
@@ -141,10 +136,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     // norm weights of the lane's channels: the queries', then the keys'
     float weight[N];
     auto load_weights = [&](const float *w) {
+        if (!w) return;
 #pragma unroll
-        for (int i = 0; i < 2 * E; i++)
-#pragma unroll
-            for (int j = 0; j < V; j++) weight[i * V + j] = w && c[i / 2][i % 2] >= 0 ? w[c[i / 2][i % 2] + j] : 1.f;
+        for (int i = 0; i < 2 * E; i++) __builtin_memcpy(weight + i * V, w + c[i / 2][i % 2], V * sizeof(float));
     };
     load_weights(pass0 < q_passes ? a.q_norm : a.k_norm);
 
@@ -167,10 +161,18 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
 
     // the lane's values of a head, normed and turned
     auto turned = [&](const T (&x)[N], bool norm, T (&y)[N]) {
-        float v[N], sum = 0.f;
+        float v[N];
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = (float)x[i], sum += v[i] * v[i];
+        for (int i = 0; i < N; i++) v[i] = (float)x[i];
         if (norm) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2 * E; i++) {
+                float part = v[i * V] * v[i * V];
+#pragma unroll
+                for (int j = 1; j < V; j++) part += v[i * V + j] * v[i * V + j];
+                sum += there[i / 2][i % 2] ? part : 0.f;
+            }
             const float by = rsqrtf(lanes_sum(sum, a.lg_lanes) / (float)a.dim + a.eps);
 #pragma unroll
             for (int i = 0; i < N; i++) v[i] = v[i] * by * weight[i];
@@ -179,27 +181,16 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
         for (int e = 0; e < E; e++)
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                // (one of an item's halves and the other's, or its neighbours)
-                const float half_a = v[2 * e * V + j], half_b = v[(2 * e + 1) * V + j], near_a = v[2 * e * V + 2 * j], near_b = v[2 * e * V + 2 * j + 1];
-                const float p = a.interleaved ? near_a : half_a, q = a.interleaved ? near_b : half_b;
-                const float first = p * cosine[e][j] - q * sine[e][j], second = q * cosine[e][j] + p * sine[e][j];
-                if (a.interleaved) {
-                    y[2 * e * V + 2 * j] = (T)(pair[e] >= 0 ? first : near_a);
-                    y[2 * e * V + 2 * j + 1] = (T)(pair[e] >= 0 ? second : near_b);
-                } else {
-                    y[2 * e * V + j] = (T)(pair[e] >= 0 ? first : half_a);
-                    y[(2 * e + 1) * V + j] = (T)(pair[e] >= 0 ? second : half_b);
-                }
+                const int ia = 2 * e * V + (NEAR ? 2 * j : j), ib = NEAR ? ia + 1 : ia + V;
+                const float first = v[ia] * cosine[e][j] - v[ib] * sine[e][j], second = v[ib] * cosine[e][j] + v[ia] * sine[e][j];
+                y[ia] = (T)(pair[e] >= 0 ? first : v[ia]);
+                y[ib] = (T)(pair[e] >= 0 ? second : v[ib]);
             }
     };
     auto put = [&](T *to, const T (&y)[N]) {
 #pragma unroll
-        for (int i = 0; i < 2 * E; i++) {
-            T v[V];
-#pragma unroll
-            for (int j = 0; j < V; j++) v[j] = y[i * V + j];
-            if (c[i / 2][i % 2] >= 0) rotary_store<T, V>(to + c[i / 2][i % 2], v);
-        }
+        for (int i = 0; i < 2 * E; i++)
+            if (there[i / 2][i % 2]) rotary_store<T, V>(to + c[i / 2][i % 2], *reinterpret_cast<const T(*)[V]>(y + i * V));
     };
     // unit u of the row's heads, of keys or of values, into the cache
     auto quantize = [&](int u, bool mine, float (&x)[8], void *codes, void *params) {
@@ -231,7 +222,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
             // the heads' channels in their order, through LDS
 #pragma unroll
             for (int i = 0; i < N; i++)
-                if (c[i / V / 2][i / V % 2] >= 0) keys[wave][head0 * a.dim + c[i / V / 2][i / V % 2] + i % V] = (float)y[i];
+                if (there[i / V / 2][i / V % 2]) keys[wave][head0 * a.dim + c[i / V / 2][i / V % 2] + i % V] = (float)y[i];
             wave_meets();
             const int units = min(together, a.n_kv - first) * (a.dim >> 3);
 #pragma unroll
@@ -267,7 +258,7 @@ int rotary_check(hipc_ctx *ctx, const char *who, const hipc_rotary_heads *h, int
     HIPC_REQUIRE(ctx, (h->rotary_dim == 0 || h->frequencies) && aligned(h->frequencies, 4) && aligned(h->q_norm, 4) && aligned(h->k_norm, 4), "%s: frequencies and norm weights", who);
     HIPC_REQUIRE(ctx, rows >= 0 && rows <= 0x7fffffff, "%s: %lld rows", who, (long long)rows);
     a->frequencies = static_cast<const float *>(h->frequencies), a->q_norm = static_cast<const float *>(h->q_norm), a->k_norm = static_cast<const float *>(h->k_norm);
-    a->rows = (int)rows, a->n_q = h->n_q_heads, a->n_kv = h->n_kv_heads, a->dim = h->head_dim, a->half = h->rotary_dim / 2, a->interleaved = h->interleaved != 0;
+    a->rows = (int)rows, a->n_q = h->n_q_heads, a->n_kv = h->n_kv_heads, a->dim = h->head_dim, a->half = h->rotary_dim / 2;
     a->eps = h->norm_eps, a->amplitude = h->amplitude != 0.f ? h->amplitude : 1.f;
     return HIPC_OK;
 }
@@ -280,7 +271,7 @@ int rotary_rows(hipc_ctx *ctx, const char *who, const char *what, const RotaryAr
 }
 
 template <typename T, bool STORE>
-int rotary_launch(hipc_ctx *ctx, const char *who, RotaryArgs a) {
+int rotary_launch(hipc_ctx *ctx, const char *who, RotaryArgs a, bool near) {
     const int64_t strides[5] = {a.q_stride, a.k_stride, a.v_stride, a.q_out_stride, a.k_out_stride};
     const void *rows[5] = {a.q, a.k, a.v, a.q_out, a.k_out};
     const int heads[5] = {a.n_q, a.n_kv, STORE ? a.n_kv : 0, a.n_q, STORE ? 0 : a.n_kv};
@@ -304,7 +295,8 @@ int rotary_launch(hipc_ctx *ctx, const char *who, RotaryArgs a) {
         a.per = (int)ceil_div(passes, a.chunks), a.chunks = (int)ceil_div(passes, a.per);
         const int64_t groups = ceil_div((int64_t)a.rows * a.chunks, 4);
         HIPC_REFUSE(ctx, !grid_fits(groups, 256), "%s: %d rows: too many for one call", who, a.rows);
-        hipLaunchKernelGGL((rotary_kernel<T, V, STORE>), (unsigned)groups, 256, 0, ctx->stream, a);
+        if (near) hipLaunchKernelGGL((rotary_kernel<T, V, true, STORE>), (unsigned)groups, 256, 0, ctx->stream, a);
+        else hipLaunchKernelGGL((rotary_kernel<T, V, false, STORE>), (unsigned)groups, 256, 0, ctx->stream, a);
         HIPC_LAUNCHED(ctx);
         return HIPC_OK;
     };
@@ -363,7 +355,7 @@ int hipc_rotary(hipc_ctx *ctx, const hipc_rotary_heads *heads, int dtype, const 
         if (int rc = rotary_rows(ctx, who, "K_out", a, a.n_kv, size, K_out, k_out_stride)) return rc;
         a.positions = static_cast<const int *>(positions);
         a.q = Q, a.k = K, a.q_out = Q_out, a.k_out = K_out, a.q_stride = q_stride, a.k_stride = k_stride, a.q_out_stride = q_out_stride, a.k_out_stride = k_out_stride;
-        return dtype == HIPC_F16 ? rotary_launch<_Float16, false>(ctx, who, a) : rotary_launch<float, false>(ctx, who, a);
+        return dtype == HIPC_F16 ? rotary_launch<_Float16, false>(ctx, who, a, heads->interleaved) : rotary_launch<float, false>(ctx, who, a, heads->interleaved);
     });
 }
 
@@ -385,7 +377,7 @@ int hipc_kv4_append_rotary(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hip
         if (int rc = rotary_rows(ctx, who, "Q_out", a, a.n_q, size, Q_out, q_out_stride)) return rc;
         a.cache = *cache, a.starts = static_cast<const int *>(starts);
         a.q = Q, a.k = K, a.v = V, a.q_out = Q_out, a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.q_out_stride = q_out_stride;
-        return dtype == HIPC_F16 ? rotary_launch<_Float16, true>(ctx, who, a) : rotary_launch<float, true>(ctx, who, a);
+        return dtype == HIPC_F16 ? rotary_launch<_Float16, true>(ctx, who, a, heads->interleaved) : rotary_launch<float, true>(ctx, who, a, heads->interleaved);
     });
 }
 

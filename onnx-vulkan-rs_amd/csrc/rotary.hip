@@ -61,11 +61,13 @@ __device__ __forceinline__ void rotary_load(const T *p, T (&x)[V]) {
     const auto v = *reinterpret_cast<const typename RotaryVector<T, V>::type *>(p);
     __builtin_memcpy(x, &v, sizeof x);
 }
-template <typename T, int V>
+template <typename T, int V, bool PAST>
 __device__ __forceinline__ void rotary_store(T *p, const T (&x)[V]) {
     typename RotaryVector<T, V>::type v;
-    __builtin_memcpy(&v, x, sizeof x);
-    *reinterpret_cast<typename RotaryVector<T, V>::type *>(p) = v;
+    __builtin_memcpy(&v, x, sizeof v);
+    auto *to = reinterpret_cast<typename RotaryVector<T, V>::type *>(p);
+    if constexpr (PAST) __builtin_nontemporal_store(v, to);
+    else *to = v;
 }
 
 // what this wavefront has stored to its LDS is there for its other lanes
@@ -74,7 +76,8 @@ __device__ __forceinline__ void wave_meets() {
     __builtin_amdgcn_wave_barrier();
 }
 
-template <typename T, int V, bool NEAR, bool STORE>
+// NEAR: interleaved pairs; STORE: into a cache; PAST: results leave past the caches
+template <typename T, int V, bool NEAR, bool STORE, bool PAST>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     constexpr int E = V == 1 ? 4 : 1;            // items of a lane: V channels and the V they turn with, or 2 V behind those that turn
     constexpr int N = 2 * V * E, UNITS = N / 8;   // a lane's values at a time; as units of eight side by side
@@ -190,7 +193,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     auto put = [&](T *to, const T (&y)[N]) {
 #pragma unroll
         for (int i = 0; i < 2 * E; i++)
-            if (there[i / 2][i % 2]) rotary_store<T, V>(to + c[i / 2][i % 2], *reinterpret_cast<const T(*)[V]>(y + i * V));
+            if (there[i / 2][i % 2]) rotary_store<T, V, PAST>(to + c[i / 2][i % 2], *reinterpret_cast<const T(*)[V]>(y + i * V));
     };
     // unit u of the row's heads, of keys or of values, into the cache
     auto quantize = [&](int u, bool mine, float (&x)[8], void *codes, void *params) {
@@ -295,8 +298,16 @@ int rotary_launch(hipc_ctx *ctx, const char *who, RotaryArgs a, bool near) {
         a.per = (int)ceil_div(passes, a.chunks), a.chunks = (int)ceil_div(passes, a.per);
         const int64_t groups = ceil_div((int64_t)a.rows * a.chunks, 4);
         HIPC_REFUSE(ctx, !grid_fits(groups, 256), "%s: %d rows: too many for one call", who, a.rows);
-        if (near) hipLaunchKernelGGL((rotary_kernel<T, V, true, STORE>), (unsigned)groups, 256, 0, ctx->stream, a);
-        else hipLaunchKernelGGL((rotary_kernel<T, V, false, STORE>), (unsigned)groups, 256, 0, ctx->stream, a);
+        auto run = [&](auto neighbours, auto past) {
+            hipLaunchKernelGGL((rotary_kernel<T, V, decltype(neighbours)::value, STORE, decltype(past)::value>), (unsigned)groups, 256, 0, ctx->stream, a);
+        };
+        // Many rows -- more than the caches near the CUs hold -- leave past these where neighbouring lanes store side by side, whole lines: 8192 rows of 32 / 8 heads of
+        // 128 in f16 33.4 us, through the caches 40.3; 48 rows 6.9 and 6.4. (In f32 a lane's values are two stores apart, and lines in parts cost: 1500 rows of 16 / 16
+        // heads of 96 18.9 us past the caches, 11.4 through them.)
+        constexpr bool LINES = sizeof(T) * V == 16 && sizeof(T) == 2;
+        if (near) run(std::true_type(), std::false_type());
+        else if (LINES && a.chunks == 1 && a.half * sizeof(T) % 128 == 0) run(std::false_type(), std::integral_constant<bool, LINES>());
+        else run(std::false_type(), std::false_type());
         HIPC_LAUNCHED(ctx);
         return HIPC_OK;
     };

@@ -3,6 +3,7 @@
 #include <type_traits>
 
 #include "kv4.h"
+#include "kv4_prompt.h"
 #include "lanes.h"
 
 namespace hipc {
@@ -32,6 +33,7 @@ constexpr int kScratchKv4 = 6;     // scratch slot of this operator alone
 constexpr int kKv4Rows = 16;       // query rows of a unit
 constexpr int kKv4Tile = 64;       // keys a wavefront takes at a time
 constexpr int kKv4PerCu = 8;       // wavefronts
+constexpr int kKv4FewRows = 64;    // query rows of a sequence that this file's kernel takes (hipc_kv4_prompt_attention)
 constexpr float kKv4Log2e = 1.4426950408889634f;
 constexpr float kKv4RescaleAt = 8.f;   // the running maximum may fall behind by 2^8 before sums are rescaled ...
 constexpr float kKv4Up = 7.f;          // ... and weights are kept 2^7 times as large: up to 2^15, so that two f16 terms hold 22 bits of more of them
@@ -659,14 +661,16 @@ void kv4_attend_args(const hipc_kv4_cache *cache, const hipc_attention_heads *he
     const int64_t unit = dtype == HIPC_F16 ? 8 : 4;
     a->wide = aligned(Q, 16) && aligned(Y, 16) && q_stride % unit == 0 && y_stride % unit == 0;
 }
+// a word and two parts for every workgroup there can be (of kv4_tiles fewer: it counts in the same words)
+size_t kv4_count_bytes(const hipc_ctx *ctx) { return ((size_t)kKv4PerCu * ctx->cu_count * 4 + 255) & ~(size_t)255; }
+size_t kv4_part_bytes(const hipc_ctx *ctx) { return (size_t)kKv4PerCu * ctx->cu_count * 2 * kKv4Rows * (kKv4MaxHead + 2) * 4; }
 // what workgroups exchange, and the words they count in, in a scratch slot of these operators' own: the words are zero
 // between calls, so a new block is cleared once
 int kv4_attend_scratch(hipc_ctx *ctx, Kv4Attend *a) {
-    const unsigned grid = kKv4PerCu * ctx->cu_count;   // at most
-    const size_t count_bytes = (grid * 4 + 255) & ~(size_t)255;
+    const size_t count_bytes = kv4_count_bytes(ctx);
     const void *before = ctx->scratch[kScratchKv4].ptr;
     void *block = nullptr;
-    if (int rc = scratch_get(ctx, kScratchKv4, count_bytes + (size_t)grid * 2 * kKv4Rows * (kKv4MaxHead + 2) * 4, &block)) return rc;
+    if (int rc = scratch_get(ctx, kScratchKv4, count_bytes + kv4_part_bytes(ctx), &block)) return rc;
     a->arrived = static_cast<uint32_t *>(block), a->parts = reinterpret_cast<float *>(static_cast<char *>(block) + count_bytes);
     if (block != before) {
         hipLaunchKernelGGL((fill_words), 1, 256, 0, ctx->stream, a->arrived, count_bytes / 4, 0u);
@@ -747,11 +751,19 @@ int hipc_kv4_prompt_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const 
         HIPC_REQUIRE(ctx, starts && aligned(starts, 4), "%s: starts", who);
         if (int rc = kv4_attention_rows(ctx, who, heads, dtype, Q, q_stride, Y, y_stride)) return rc;
         kv4_attend_args(cache, heads, dtype, Q, q_stride, Y, y_stride, &a);
-        const int64_t blocks = ceil_div(total * a.group, kKv4Rows) + cache->n_seqs, units = blocks * cache->n_kv_heads;
-        HIPC_REFUSE(ctx, units > 1 << 22, "%s: %lld rows: too many for one call", who, (long long)total);
-        a.starts = static_cast<const int *>(starts), a.total = (int)total, a.sinks = std::min(sinks, kKv4MaxPositions), a.most = 1 << 30;
+        a.starts = static_cast<const int *>(starts), a.total = (int)total, a.sinks = std::min(sinks, kKv4MaxPositions);
+        HIPC_REFUSE(ctx, total * a.group > 1 << 30, "%s: %lld rows of %d heads to a kv head: too many for one call", who, (long long)total, a.group);
         if (int rc = kv4_attend_scratch(ctx, &a)) return rc;
-        return kv4_attend<true>(ctx, a, dtype, units);
+        // Who brings how many is known on the device: where some sequence can bring many rows, both parts are launched, and each leaves the other's alone.
+        a.most = kKv4FewRows;
+        const bool many = total * a.group > a.most;
+        const int64_t blocks = std::min(ceil_div(total * a.group, kKv4Rows) + std::min<int64_t>(cache->n_seqs, total), (int64_t)cache->n_seqs * ceil_div(a.most, kKv4Rows));
+        if (int rc = kv4_attend<true>(ctx, a, dtype, blocks * cache->n_kv_heads)) return rc;
+        if (!many) return HIPC_OK;
+        Kv4Tiles t{};
+        t.cache = a.cache, t.q = a.q, t.y = a.y, t.q_stride = a.q_stride, t.y_stride = a.y_stride, t.starts = a.starts, t.total = a.total, t.n_q_heads = a.n_q_heads;
+        t.group = a.group, t.window = a.window, t.sinks = a.sinks, t.wide = a.wide, t.most = a.most, t.scale = a.scale, t.parts = a.parts, t.arrived = a.arrived;
+        return kv4_tiles(ctx, t, dtype, kv4_part_bytes(ctx));
     });
 }
 

@@ -1,0 +1,551 @@
+// Attention of packed new rows over the paged 4-bit cache (hipc_kv4_prompt_attention): the sequences that bring many. Those that bring few are
+// kv4_attention.hip's.
+#include <algorithm>
+#include <type_traits>
+
+#include "kv4.h"
+#include "kv4_prompt.h"
+#include "lanes.h"
+
+namespace hipc {
+
+namespace {
+
+typedef _Float16 th8 __attribute__((ext_vector_type(8)));
+typedef _Float16 th2 __attribute__((ext_vector_type(2)));
+typedef short ts4 __attribute__((ext_vector_type(4)));
+typedef float tf16 __attribute__((ext_vector_type(16)));
+typedef uint32_t tu4 __attribute__((ext_vector_type(4)));
+
+constexpr float kTileLog2e = 1.4426950408889634f;
+constexpr float kTileRescaleAt = 8.f;   // in powers of two (see Kv4TileRows)
+constexpr float kTileUp = 7.f;
+
+__device__ __forceinline__ float tile_halves_max(float v) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float tile_halves_sum(float v) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// What a lane knows of a sequence: its rows (none, where it brings few), how many tiles of ROWS (row, head of the group) pairs they make.
+struct TileSequence {
+    int row0, tokens, length, tiles;
+    __device__ __forceinline__ TileSequence(const Kv4Tiles &a, int seq, int rows) {
+        const int s = min(seq, a.cache.n_seqs - 1), from = a.starts[s], to = a.starts[s + 1];
+        length = a.cache.n_pages > 0 ? kv4_length(a.cache, s) : 0;
+        row0 = max(from, 0);
+        const int end = min(to, a.total), brought = end > row0 && seq < a.cache.n_seqs ? end - row0 : 0;
+        tokens = (int64_t)brought * a.group > a.most ? brought : 0;
+        tiles = (int)(((int64_t)tokens * a.group + rows - 1) / rows);
+    }
+};
+// Which rows of one kv head a workgroup has, and which key tiles of KT: the first `sink_tiles`, then those from first + sink_tiles on, `count` in all.
+struct Tile {
+    int seq, row0, tokens, length, r0, rows;   // rows: of the sequence (tokens times group)
+    int first, count, sink_tiles;
+};
+template <int ROWS, int KT>
+__device__ __forceinline__ void tile_keys(const Kv4Tiles &a, Tile *t) {
+    const int past = t->length - t->tokens, held = kv4_held(a.cache, t->length);
+    const int last = (min(t->r0 + ROWS, t->rows) - 1) / a.group, end = min(past + last + 1, held);
+    const int begin = a.window > 0 ? max(past + t->r0 / a.group - a.window + 1, 0) : 0, first = begin / KT;
+    t->sink_tiles = a.window > 0 && end > 0 ? min((min(a.sinks, end) + KT - 1) / KT, first) : 0;
+    t->first = first - t->sink_tiles;
+    t->count = t->sink_tiles + (end > begin ? (end + KT - 1) / KT - first : 0);
+}
+// all tiles, and the longest sequence that has any
+template <int ROWS>
+__device__ __forceinline__ int tile_total(const Kv4Tiles &a, const TileSequence &early, int *longest) {
+    const int lane = threadIdx.x & 63;
+    int total = __builtin_amdgcn_readlane(wave_scan(early.tiles), 63);
+    float most = lean_wave_max(early.tiles > 0 ? (float)early.length : 0.f);
+    for (int base = 64; base < a.cache.n_seqs; base += 64) {
+        const TileSequence s(a, base + lane, ROWS);
+        total += __builtin_amdgcn_readlane(wave_scan(s.tiles), 63);
+        most = fmaxf(most, lean_wave_max(s.tiles > 0 ? (float)s.length : 0.f));
+    }
+    *longest = (int)fminf(most, 1.5e9f);
+    return total;
+}
+// tile number `at`, the sequences' in their order
+template <int ROWS>
+__device__ __forceinline__ void tile_find(const Kv4Tiles &a, const TileSequence &early, int at, Tile *t) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    TileSequence s = early;
+    for (int base = 0;; base += 64) {
+        if (base > 0) s = TileSequence(a, base + lane, ROWS);
+        const int sum = wave_scan(s.tiles);
+        const uint64_t over = __ballot(before + sum > at);
+        if (over) {
+            const int l = __builtin_ctzll(over);
+            t->seq = base + l;
+            t->row0 = __builtin_amdgcn_readlane(s.row0, l), t->tokens = __builtin_amdgcn_readlane(s.tokens, l), t->length = __builtin_amdgcn_readlane(s.length, l);
+            t->rows = t->tokens * a.group;
+            t->r0 = (at - (before + __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(s.tiles, l))) * ROWS;
+            return;
+        }
+        before += __builtin_amdgcn_readlane(sum, 63);
+    }
+}
+
+// A lane's query row and what it sees: keys below `end` that are not below `begin`, or are below a.sinks; and what some and what all of its wavefront's rows see.
+struct TileRow {
+    bool mine, any;
+    int token, head, lane_begin, lane_end, begin, end, all_begin, all_end;
+    __device__ __forceinline__ TileRow(const Kv4Tiles &a, const Tile &t, int first, int n, int kvh) {
+        const int past = t.length - t.tokens, held = kv4_held(a.cache, t.length), row = first + n;
+        any = first < t.rows, mine = row < t.rows;
+        token = row / a.group, head = kvh * a.group + (row - token * a.group);
+        const int p0 = past + first / a.group, p1 = past + min(first + 31, t.rows - 1) / a.group;
+        auto ends = [&](int pos) { return min(pos + 1, held); };
+        auto begins = [&](int pos) { return a.window > 0 ? max(pos - a.window + 1, 0) : 0; };
+        lane_begin = begins(past + token), lane_end = ends(past + token);
+        begin = begins(p0), end = ends(p1), all_begin = begins(p1), all_end = ends(p0);
+    }
+    __device__ __forceinline__ bool sees(const Kv4Tiles &a, int key) const { return key < lane_end && (key >= lane_begin || key < a.sinks); }
+};
+
+// A wavefront's 32 query rows, HC channels of them from channel c0 on, over key tiles of KT rows of PITCH halfs in LDS, both products turned around:
+//   S^T = K Q^T      32x32x16: a lane's 16 results are one query's scores (query = lane % 32) of keys 8 (r / 4) + 4 (lane / 32) + r % 4
+//   O^T = V^T P^T    the lane's weights are the second operand as they lie; V^T is read from row-major LDS rows by the transposing loads
+// so maximum, sum and rescale of the softmax are numbers of one lane, exchanged once between the two halves of the wavefront.
+// The running maximum may grow by 2^8 before sums are rescaled, and weights are kept 2^7 times as large: f16's ordinary numbers then reach down to 2^-21 of the
+// heaviest weight, its subnormal ones to 2^-31. QT = 1, f16 rows: queries as they are, weights rounded to f16 (as two terms they would be half as many
+// products again of a kernel that these bound; the result's own rounding is as large). QT = 2, f32 rows: two f16 terms each, of the row times a power of two, and of the weight.
+// The eight channels of a word of codes lie in the order in which it unpacks, 0 4 1 5 2 6 3 7, in K's rows, V's and the queries alike.
+template <int HC, int KT, int PITCH, int QT>
+struct Kv4TileRows {
+    th8 qf[HC / 16][QT];
+    tf16 o[HC / 32];
+    float m = -INFINITY, l = 0.f, c2, down = -kTileUp;
+    uint32_t k_at[4], v_at[2];
+    int h;
+
+    __device__ __forceinline__ Kv4TileRows(const Kv4Tiles &a, int lane, int c0) {
+        const int n = lane & 31, i16 = lane & 15;
+        h = lane >> 5;
+        c2 = fabsf(a.scale) * kTileLog2e;
+#pragma unroll
+        for (int c = 0; c < 4; c++) k_at[c] = n * PITCH * 2 + (((2 * c + h) ^ (n & 7)) * 16) + 2 * c0;
+#pragma unroll
+        for (int i = 0; i < 2; i++) v_at[i] = (4 * h + (i16 >> 2)) * PITCH * 2 + (((4 * i + 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1)) ^ ((i16 >> 2) << 1)) * 16) + (i16 & 1) * 8 + 2 * c0;
+#pragma unroll
+        for (int i = 0; i < HC / 32; i++) o[i] = tf16{};
+    }
+    template <typename T>
+    __device__ __forceinline__ void queries(const Kv4Tiles &a, const Tile &t, const TileRow &r, int c0) {
+        const T *q = static_cast<const T *>(a.q) + a.q_stride * (t.row0 + (r.mine ? r.token : 0)) + (int64_t)(r.mine ? r.head : 0) * a.cache.head_dim;
+        const int dim = a.cache.head_dim;
+        float sign = a.scale < 0.f ? -1.f : 1.f;
+        int up = 0;
+        if (QT == 2) {
+            // The row's largest value into [2^14, 2^15); an infinity stays where it is. And no further up than leaves the scores' factor an ordinary number: at 0 it
+            // would make NaN of what is hidden. (A wavefront with half of the channels looks at the whole row.)
+            float most = 0.f;
+            for (int c = 8 * h; c < dim; c += 16) {
+                float x[8];
+                kv4_load8(q + c, a.wide, x);
+#pragma unroll
+                for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(x[j]));
+            }
+            most = tile_halves_max(most);
+            up = most > 0.f && most < INFINITY ? min(14 - ilogbf(most), 126 + ilogbf(fminf(c2, 0x1p126f))) : 0;
+            c2 = ldexpf(c2, -up);
+        }
+#pragma unroll
+        for (int c = 0; c < HC / 16; c++) {
+            const int at = c0 + 16 * c + 8 * h;
+            float x[8] = {};
+            if (at < dim) kv4_load8(q + at, a.wide, x);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                float v = x[(j & 1) * 4 + (j >> 1)] * sign;
+                if (QT == 2) v = ldexpf(v, up);
+                const _Float16 hi = (_Float16)v;
+                qf[c][0][j] = r.mine ? hi : (_Float16)0;
+                if (QT == 2) qf[c][QT - 1][j] = r.mine ? (_Float16)(v - (float)hi) : (_Float16)0;
+            }
+        }
+    }
+    __device__ __forceinline__ void scores(const char *ks, tf16 (&s)[KT / 32]) const {
+#pragma unroll
+        for (int b = 0; b < KT / 32; b++) {
+            s[b] = tf16{};
+#pragma unroll
+            for (int c = 0; c < HC / 16; c++) {
+                const th8 k = *reinterpret_cast<const th8 *>(ks + k_at[c & 3] + (c >> 2) * 128 + b * 64 * PITCH);
+#pragma unroll
+                for (int e = QT - 1; e >= 0; e--) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[c][e], s[b], 0, 0, 0);
+            }
+        }
+    }
+    // the scores of keys key0 .. become weights; `there`: which blocks of 16 keys lie on pages
+    __device__ __forceinline__ void weights(const Kv4Tiles &a, tf16 (&s)[KT / 32], int key0, bool masked, uint32_t there, const TileRow &row, th8 (&p)[KT / 16][QT]) {
+        if (masked) {
+#pragma unroll
+            for (int b = 0; b < KT / 32; b++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int key = key0 + 32 * b + 8 * (r / 4) + 4 * h + r % 4;
+                    s[b][r] = (there >> (2 * b + r / 8) & 1) && row.sees(a, key) ? s[b][r] : -INFINITY;
+                }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int b = 0; b < KT / 32; b++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[b][r]);
+        mx = tile_halves_max(mx) * c2;
+        if (__any(mx > m + kTileRescaleAt)) {
+            const float grown = mx > m + kTileRescaleAt ? mx : m, keep = grown == m ? 1.f : __builtin_amdgcn_exp2f(m - grown);   // (a row goes by its own scores)
+            m = grown, l *= keep, down = (m == -INFINITY ? 0.f : m) - kTileUp;
+#pragma unroll
+            for (int i = 0; i < HC / 32; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[i][r] *= keep;
+        }
+#pragma unroll
+        for (int u = 0; u < KT / 16; u++)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                typedef float f2 __attribute__((ext_vector_type(2)));
+                const f2 w = {__builtin_amdgcn_exp2f(__builtin_fmaf(s[u / 2][8 * (u & 1) + j], c2, -down)),
+                              __builtin_amdgcn_exp2f(__builtin_fmaf(s[u / 2][8 * (u & 1) + j + 1], c2, -down))};
+                const th2 hi = __builtin_convertvector(w, th2);
+                p[u][0][j] = hi.x, p[u][0][j + 1] = hi.y;
+                if (QT == 1) {   // the sum is that of the same rounded weights
+                    l = __builtin_amdgcn_fdot2(hi, th2{(_Float16)1.f, (_Float16)1.f}, l, false);
+                } else {
+                    l += w.x + w.y;
+                    p[u][QT - 1][j] = (_Float16)(w.x - (float)hi.x), p[u][QT - 1][j + 1] = (_Float16)(w.y - (float)hi.y);
+                }
+            }
+    }
+    __device__ __forceinline__ th8 v_part(const char *vs, int ot, int u) const {
+        const char *at = vs + v_at[ot & 1] + (ot >> 1) * 128 + u * 32 * PITCH;
+        const ts4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ts4 *)(at));
+        const ts4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ts4 *)(at + 16 * PITCH));
+        return __builtin_bit_cast(th8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    __device__ __forceinline__ void values(const Kv4Tiles &a, const char *vs, int key0, bool masked, const TileRow &row, const th8 (&p)[KT / 16][QT]) {
+        if (masked) {
+            // A hidden key's weight is zero, but zero times what is not finite is not: where the tile has such values, the product takes zeros in
+            // their places, and a second one finds the rows that see them.
+            uint32_t bad = 0;
+#pragma unroll
+            for (int ot = 0; ot < HC / 32; ot++)
+#pragma unroll
+                for (int u = 0; u < KT / 16; u++) {
+                    const tu4 w = __builtin_bit_cast(tu4, v_part(vs, ot, u));
+#pragma unroll
+                    for (int j = 0; j < 4; j++) bad |= ((w[j] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+                }
+            if (__any(bad != 0)) {
+#pragma unroll
+                for (int ot = 0; ot < HC / 32; ot++) {
+                    tf16 seen = tf16{};
+#pragma unroll
+                    for (int u = 0; u < KT / 16; u++) {
+                        th8 v = v_part(vs, ot, u), kind = {}, sees = {};
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            if ((__builtin_bit_cast(uint16_t, (_Float16)v[j]) & 0x7c00) == 0x7c00) kind[j] = (_Float16)1.f, v[j] = (_Float16)0.f;
+                            sees[j] = (_Float16)(row.sees(a, key0 + 16 * u + 8 * (j / 4) + 4 * h + j % 4) ? 1.f : 0.f);
+                        }
+#pragma unroll
+                        for (int e = QT - 1; e >= 0; e--) o[ot] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u][e], o[ot], 0, 0, 0);
+                        seen = __builtin_amdgcn_mfma_f32_32x32x16_f16(kind, sees, seen, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (seen[r] != 0.f) o[ot][r] = NAN;
+                }
+                return;
+            }
+        }
+#pragma unroll
+        for (int ot = 0; ot < HC / 32; ot++)
+#pragma unroll
+            for (int u = 0; u < KT / 16; u++) {
+                const th8 v = v_part(vs, ot, u);
+#pragma unroll
+                for (int e = QT - 1; e >= 0; e--) o[ot] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u][e], o[ot], 0, 0, 0);
+            }
+    }
+    // sums ot, r .. r + 3 (r a multiple of 4) as the channels 32 ot + 8 (r / 4) + 4 h .. + 3: the halves of the wavefront hold 0 4 1 5 and 2 6 3 7 of eight
+    __device__ __forceinline__ float4 channels(int ot, int r) const {
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[ot][r]), __float_as_uint(o[ot][r + 1]), false, false);
+        const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[ot][r + 2]), __float_as_uint(o[ot][r + 3]), false, false);
+        return make_float4(__uint_as_float(x[0]), __uint_as_float(y[0]), __uint_as_float(x[1]), __uint_as_float(y[1]));
+    }
+};
+
+// The codes of a key tile on their way from pages to f16 rows in LDS, by all threads of a workgroup: a thread takes 32 channels of a key or a value (16 bytes of codes and
+// their parameters), EACH of them. Page numbers are asked for two tiles ahead, codes one. Keys behind the sequence and on no page are zeros.
+template <int HD, int KT, int PITCH, int W>
+struct Kv4TileFetch {
+    static constexpr int GP = HD <= 64 ? 2 : HD <= 128 ? 4 : 8;    // groups of a row, rounded up to a power of two
+    static constexpr int UNITS = 2 * KT * GP, EACH = (UNITS + 64 * W - 1) / (64 * W);
+    static constexpr int TILE = KT * PITCH * 2;                    // bytes of a tile of K, or of V
+    tu4 codes[EACH];
+    uint32_t params[EACH];
+    int page[EACH], block_page;   // of the tile whose codes are asked for next
+    const int *table;
+    int shift, groups, held, kvh, tid;
+
+    __device__ __forceinline__ Kv4TileFetch(const Kv4Tiles &a, const Tile &t, int kvh_, int tid_) : kvh(kvh_), tid(tid_) {
+        table = static_cast<const int *>(a.cache.table) + (int64_t)t.seq * a.cache.table_width;
+        shift = 31 - __builtin_clz((unsigned)a.cache.page_size), groups = a.cache.head_dim / kKv4Group, held = kv4_held(a.cache, t.length);
+    }
+    __device__ __forceinline__ int page_of(const Kv4Tiles &a, int key) const {
+        const int entry = key >> shift, last = (int)a.cache.table_width - 1, p = table[min(entry, last)];
+        return entry <= last ? p : -1;
+    }
+    __device__ __forceinline__ bool is_page(const Kv4Tiles &a, int p) const { return p >= 0 && p < a.cache.n_pages; }
+    __device__ __forceinline__ void ask_pages(const Kv4Tiles &a, int tile) {
+#pragma unroll
+        for (int e = 0; e < EACH; e++) page[e] = page_of(a, tile * KT + ((tid + e * 64 * W) / GP) % KT);
+        block_page = page_of(a, tile * KT + 16 * (tid % (KT / 16)));
+    }
+    // which blocks of 16 keys of the tile asked for lie on pages
+    __device__ __forceinline__ uint32_t blocks_there(const Kv4Tiles &a) const { return (uint32_t)__ballot(is_page(a, block_page)) & ((1u << (KT / 16)) - 1); }
+    __device__ __forceinline__ void ask_codes(const Kv4Tiles &a, int tile) {
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const int unit = tid + e * 64 * W, g = unit % GP, key = tile * KT + (unit / GP) % KT;
+            const bool value = unit >= KT * GP, there = is_page(a, page[e]) && key < held && g < groups && unit < UNITS;
+            const int64_t row = (((int64_t)(there ? page[e] : 0) * a.cache.n_kv_heads + kvh) << shift) + (key & (a.cache.page_size - 1));
+            const int gg = g < groups ? g : 0;
+            codes[e] = *reinterpret_cast<const tu4 *>(static_cast<const char *>(value ? a.cache.v_codes : a.cache.k_codes) + row * (a.cache.head_dim / 2) + gg * 16);
+            const uint32_t p = static_cast<const uint32_t *>(value ? a.cache.v_params : a.cache.k_params)[row * groups + gg];
+            params[e] = there ? p : 0u;
+        }
+    }
+    __device__ __forceinline__ void unpack(char *k, char *v) const {
+        const Kv4Unpack take;
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const int unit = tid + e * 64 * W, g = unit % GP, r = (unit / GP) % KT;
+            if (UNITS % (64 * W) != 0 && unit >= UNITS) break;
+            if (32 * g >= HD) continue;   // (heads of 96 in rows of 128)
+            const bool value = unit >= KT * GP;
+            const kvh2 p = __builtin_bit_cast(kvh2, params[e]);
+            char *row = (value ? v : k) + r * PITCH * 2;
+            const int turn = value ? (r & 3) << 1 : r & 7;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                kvh2 x[4];
+                take(codes[e][j], kvh2{p.x, p.x}, kvh2{p.y, p.y}, x);
+                *reinterpret_cast<th8 *>(row + ((4 * g + j) ^ turn) * 16) = th8{x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};
+            }
+        }
+    }
+};
+
+template <int HD, int QT, int W>
+__global__ void __launch_bounds__(64 * W, 2) kv4_tiles_kernel(const Kv4Tiles a) {
+    constexpr int C = HD > 128 ? 2 : 1, HC = HD / C;               // wavefronts of a row, channels of each
+    constexpr int KT = HD > 128 ? 32 : 64;
+    constexpr int PITCH = HD <= 64 ? 64 : HD <= 128 ? 128 : 256;   // halfs of an LDS row
+    constexpr int TILE = KT * PITCH * 2, ROWS = 32 * W / C;
+    typedef typename std::conditional<QT == 1, _Float16, float>::type T;
+    __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];   // [buffer][K, V]
+    __shared__ float4 scores[C > 1 ? W : 1][KT / 8][64];             // a wavefront's own, for the other
+    __shared__ int last_here;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+    // Where tiles are fewer than workgroups, the keys of each are shared by as many as there are, no fewer than four key tiles each.
+    const int heads = a.cache.n_kv_heads, kvh = (int)(blockIdx.x % heads);
+    const TileSequence early(a, lane, ROWS);
+    int longest;
+    const int tiles = tile_total<ROWS>(a, early, &longest);
+    if (tiles == 0) return;
+    const int splits = max(1, min(a.slots / max(1, tiles * heads), (longest + 4 * KT - 1) / (4 * KT)));
+    const int item = (int)(blockIdx.x / heads), at = item / splits, split = item - at * splits;
+    if (at >= tiles) return;
+    Tile t;
+    tile_find<ROWS>(a, early, tiles - 1 - at, &t);   // the last tiles of a sequence are the heaviest
+    tile_keys<ROWS, KT>(a, &t);
+    const int per = max(1, (t.count + splits - 1) / splits), parts = max(1, (t.count + per - 1) / per);
+    if (split >= parts) return;
+    const int i0 = split * per, i1 = min(i0 + per, t.count);
+
+    const TileRow row(a, t, t.r0 + 32 * (wave / C), lane & 31, kvh);
+    const int c0 = C > 1 ? (wave & 1) * HC : 0;   // the wavefront's first channel
+    auto key_tile = [&](int i) { return i < t.sink_tiles ? i : t.first + i; };
+    Kv4TileFetch<HD, KT, PITCH, W> from(a, t, kvh, tid);
+    Kv4TileRows<HC, KT, PITCH, QT> rows(a, lane, c0);
+    auto buffer = [&](int i) { return smem + ((i - i0) & 1) * 2 * TILE; };
+    uint32_t there = 0, there1 = 0;
+    if (i0 < i1) {
+        from.ask_pages(a, key_tile(i0));
+        there = from.blocks_there(a);
+        from.ask_codes(a, key_tile(i0));
+        if (i0 + 1 < i1) from.ask_pages(a, key_tile(i0 + 1));
+    }
+    rows.template queries<T>(a, t, row, c0);
+    if (i0 < i1) {
+        from.unpack(buffer(i0), buffer(i0) + TILE);
+        if (i0 + 1 < i1) {
+            there1 = from.blocks_there(a);
+            from.ask_codes(a, key_tile(i0 + 1));
+            if (i0 + 2 < i1) from.ask_pages(a, key_tile(i0 + 2));
+        }
+    }
+    for (int i = i0; i < i1; i++) {
+        __syncthreads();   // this tile is there, and every wavefront is done with the other buffer
+        const uint32_t here = there;
+        if (i + 1 < i1) {
+            from.unpack(buffer(i + 1), buffer(i + 1) + TILE);
+            there = there1;
+            if (i + 2 < i1) {
+                there1 = from.blocks_there(a);
+                from.ask_codes(a, key_tile(i + 2));
+                if (i + 3 < i1) from.ask_pages(a, key_tile(i + 3));
+            }
+        }
+        const int key0 = key_tile(i) * KT;
+        const bool active = row.any && key0 < row.end && (key0 + KT > row.begin || key0 < a.sinks);
+        if (C == 1 && !active) continue;
+        const char *ks = buffer(i);
+        tf16 s[KT / 32];
+        rows.scores(ks, s);
+        if (C > 1) {
+#pragma unroll
+            for (int j = 0; j < KT / 8; j++) scores[wave][j][lane] = make_float4(s[j / 4][j % 4 * 4], s[j / 4][j % 4 * 4 + 1], s[j / 4][j % 4 * 4 + 2], s[j / 4][j % 4 * 4 + 3]);
+            __syncthreads();
+            if (!active) continue;
+#pragma unroll
+            for (int j = 0; j < KT / 8; j++) {
+                const float4 v = scores[wave ^ 1][j][lane];
+                s[j / 4][j % 4 * 4] += v.x, s[j / 4][j % 4 * 4 + 1] += v.y, s[j / 4][j % 4 * 4 + 2] += v.z, s[j / 4][j % 4 * 4 + 3] += v.w;
+            }
+        }
+        const bool masked = key0 + KT > row.all_end || (key0 < row.all_begin && key0 + KT > a.sinks) || here != (1u << (KT / 16)) - 1;
+        th8 p[KT / 16][QT];
+        rows.weights(a, s, key0, masked, here, row, p);
+        rows.values(a, ks + TILE, key0, masked, row, p);
+    }
+
+    const float l = tile_halves_sum(rows.l);
+    const int dim = a.cache.head_dim, h = lane >> 5;
+    auto store = [&](int token, int head, int c, const float4 &v, float inv) {
+        T *y = static_cast<T *>(a.y) + a.y_stride * (t.row0 + token) + (int64_t)head * dim + c;
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        const T4 out = {(T)(v.x * inv), (T)(v.y * inv), (T)(v.z * inv), (T)(v.w * inv)};
+        if (a.wide) {
+            *reinterpret_cast<T4 *>(y) = out;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[j] = out[j];
+        }
+    };
+    if (parts == 1) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int ot = 0; ot < HC / 32; ot++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const float4 v = rows.channels(ot, r);
+                const int c = c0 + 32 * ot + 8 * (r / 4) + 4 * h;
+                if (row.mine && c < dim) store(row.token, row.head, c, v, inv);
+            }
+        return;
+    }
+    // Of several workgroups the one that comes last joins the parts, in their order: [row][channel] sums, then (maximum, sum) pairs
+    const int64_t unit = (int64_t)at * heads + kvh;
+    auto part_of = [&](int z) { return a.parts + (unit * splits + z) * (int64_t)(ROWS * (dim + 2)); };
+    // two floats at a time, stored where (and read from where) every workgroup sees them
+    auto put = [](float *to_pair, float x, float y) {
+        __hip_atomic_store(reinterpret_cast<uint64_t *>(to_pair), (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
+    auto get = [](const float *pair) {
+        const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t *>(pair), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+    };
+    {
+        float *part = part_of(split);
+        const int n = 32 * (wave / C) + (lane & 31);
+#pragma unroll
+        for (int ot = 0; ot < HC / 32; ot++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const float4 v = rows.channels(ot, r);
+                const int c = c0 + 32 * ot + 8 * (r / 4) + 4 * h;
+                if (row.mine && c < dim) put(part + (int64_t)n * dim + c, v.x, v.y), put(part + (int64_t)n * dim + c + 2, v.z, v.w);
+            }
+        if (row.mine && h == 0 && c0 == 0) put(part + (int64_t)ROWS * dim + 2 * n, rows.m, l);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's stores are where everyone sees them
+    __syncthreads();
+    if (tid == 0) {
+        const uint32_t others = __hip_atomic_fetch_add(a.arrived + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last_here = others == (uint32_t)(parts - 1);
+        if (last_here) __hip_atomic_store(a.arrived + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next call
+    }
+    __syncthreads();
+    if (!last_here) return;
+    const int quads = dim / 4, mine = min(ROWS, t.rows - t.r0);
+    for (int i = tid; i < mine * quads; i += 64 * W) {
+        const int n = i / quads, c = (i - n * quads) * 4;
+        float top = -INFINITY, all = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr int N = 4;   // parts on their way together
+        for (int z = 0; z < parts; z += N) {
+            float2 ml[N], x01[N], x23[N];
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const float *x = part_of(min(z + e, parts - 1));
+                ml[e] = get(x + (int64_t)ROWS * dim + 2 * n), x01[e] = get(x + (int64_t)n * dim + c), x23[e] = get(x + (int64_t)n * dim + c + 2);
+                if (z + e >= parts) ml[e] = make_float2(-INFINITY, 0.f);
+            }
+            float higher = top;
+#pragma unroll
+            for (int e = 0; e < N; e++) higher = fmaxf(higher, ml[e].x);
+            const float back = all == 0.f ? 0.f : __builtin_amdgcn_exp2f(top - higher);
+            top = higher, all *= back, v.x *= back, v.y *= back, v.z *= back, v.w *= back;
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                if (ml[e].y == 0.f) continue;   // nothing the row sees
+                const float keep = __builtin_amdgcn_exp2f(ml[e].x - top);
+                all += ml[e].y * keep, v.x += x01[e].x * keep, v.y += x01[e].y * keep, v.z += x23[e].x * keep, v.w += x23[e].y * keep;
+            }
+        }
+        const int r = t.r0 + n, token = r / a.group;
+        store(token, kvh * a.group + (r - token * a.group), c, v, all == 0.f ? 0.f : 1.f / all);
+    }
+}
+
+template <int HD, int QT, int W>
+int tiles_launch(hipc_ctx *ctx, Kv4Tiles a, size_t part_bytes) {
+    constexpr int ROWS = 32 * W / (HD > 128 ? 2 : 1);
+    const int64_t rows = (int64_t)a.total * a.group, kv = a.cache.n_kv_heads;
+    // tiles there can be: a sequence has some only if it brings more than a.most rows
+    const int64_t tiles = rows / ROWS + std::min<int64_t>(a.cache.n_seqs, rows / (a.most + 1));
+    a.slots = (int)std::min<int64_t>(2 * (int64_t)ctx->cu_count * (W == 8 ? 1 : 2), part_bytes / ((size_t)ROWS * (a.cache.head_dim + 2) * 4));
+    const int64_t groups = std::max<int64_t>(tiles * kv, ceil_div(a.slots, kv) * kv);
+    HIPC_REFUSE(ctx, !grid_fits(groups, 64 * W), "hipc_kv4_prompt_attention: %d rows: too many for one call", a.total);
+    hipLaunchKernelGGL((kv4_tiles_kernel<HD, QT, W>), (unsigned)groups, 64 * W, 0, ctx->stream, a);
+    HIPC_LAUNCHED(ctx);
+    return HIPC_OK;
+}
+
+}  // namespace
+
+int kv4_tiles(hipc_ctx *ctx, const Kv4Tiles &a, int dtype, size_t part_bytes) {
+    auto launch = [&](auto width) -> int {
+        constexpr int HD = decltype(width)::value;
+        return dtype == HIPC_F16 ? tiles_launch<HD, 1, 8>(ctx, a, part_bytes) : tiles_launch<HD, 2, 8>(ctx, a, part_bytes);
+    };
+    const int dim = a.cache.head_dim;
+    return dim <= 64    ? launch(std::integral_constant<int, 64>())
+           : dim <= 96  ? launch(std::integral_constant<int, 96>())
+           : dim <= 128 ? launch(std::integral_constant<int, 128>())
+                        : launch(std::integral_constant<int, 256>());
+}
+
+}  // namespace hipc

@@ -14,7 +14,9 @@ struct Kv4Tiles {
     const int *starts;
     int total, n_q_heads, group, window, sinks, wide;   // wide: rows of Q and Y on 16 bytes
     int most;        // query rows (tokens times group) that a sequence has to pass to be in this part
-    int slots;       // workgroups that may share keys
+    int slots;       // workgroups that run at once
+    int splits;      // workgroups that share a tile's keys, or (not above 0) as many as tile_us and part_us say
+    float tile_us, part_us;
     float scale;
     float *parts;    // what these exchange
     uint32_t *arrived;   // [slots]: parts of a unit that have come; all zero between calls

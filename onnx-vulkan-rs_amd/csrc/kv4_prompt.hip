@@ -56,18 +56,19 @@ __device__ __forceinline__ void tile_keys(const Kv4Tiles &a, Tile *t) {
     t->first = first - t->sink_tiles;
     t->count = t->sink_tiles + (end > begin ? (end + KT - 1) / KT - first : 0);
 }
-// all tiles, and the longest sequence that has any
-template <int ROWS>
+// all tiles, and how many key tiles the longest of them has
+template <int ROWS, int KT>
 __device__ __forceinline__ int tile_total(const Kv4Tiles &a, const TileSequence &early, int *longest) {
-    const int lane = threadIdx.x & 63;
-    int total = __builtin_amdgcn_readlane(wave_scan(early.tiles), 63);
-    float most = lean_wave_max(early.tiles > 0 ? (float)early.length : 0.f);
-    for (int base = 64; base < a.cache.n_seqs; base += 64) {
-        const TileSequence s(a, base + lane, ROWS);
+    int total = 0;
+    float most = 0.f;
+    auto add = [&](const TileSequence &s) {
         total += __builtin_amdgcn_readlane(wave_scan(s.tiles), 63);
-        most = fmaxf(most, lean_wave_max(s.tiles > 0 ? (float)s.length : 0.f));
-    }
-    *longest = (int)fminf(most, 1.5e9f);
+        const int keys = min(s.length, a.window > 0 ? min(a.window, 1 << 29) + ROWS / a.group + min(a.sinks, 1 << 29) : kKv4MaxPositions);
+        most = fmaxf(most, lean_wave_max(s.tiles > 0 ? (float)(keys / KT + 1) : 0.f));
+    };
+    add(early);
+    for (int base = 64; base < a.cache.n_seqs; base += 64) add(TileSequence(a, base + (threadIdx.x & 63), ROWS));
+    *longest = (int)most;
     return total;
 }
 // tile number `at`, the sequences' in their order
@@ -90,6 +91,20 @@ __device__ __forceinline__ void tile_find(const Kv4Tiles &a, const TileSequence 
         }
         before += __builtin_amdgcn_readlane(sum, 63);
     }
+}
+
+// How many workgroups share the keys of a tile where tiles are fewer than workgroups run at once: every part costs its way out and, one behind the other, back into the
+// workgroup that joins them (a.part_us), and pays while it takes more key tiles (a.tile_us) off the longest chain.
+__device__ __forceinline__ int tile_splits(const Kv4Tiles &a, int units, int longest) {
+    if (a.splits > 0) return min(a.splits, max(1, a.slots / units));
+    const int most = min(a.slots / units, longest);
+    int best = 1;
+    float time = a.tile_us * longest;
+    for (int s = 2; s <= most; s++) {
+        const float t = a.tile_us * ((longest + s - 1) / s) + a.part_us * (s + 2);
+        if (t < time) time = t, best = s;
+    }
+    return best;
 }
 
 // A lane's query row and what it sees: keys below `end` that are not below `begin`, or are below a.sinks; and what some and what all of its wavefront's rows see.
@@ -358,13 +373,12 @@ __global__ void __launch_bounds__(64 * W, 2) kv4_tiles_kernel(const Kv4Tiles a) 
     __shared__ int last_here;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-    // Where tiles are fewer than workgroups, the keys of each are shared by as many as there are, no fewer than four key tiles each.
     const int heads = a.cache.n_kv_heads, kvh = (int)(blockIdx.x % heads);
     const TileSequence early(a, lane, ROWS);
     int longest;
-    const int tiles = tile_total<ROWS>(a, early, &longest);
+    const int tiles = tile_total<ROWS, KT>(a, early, &longest);
     if (tiles == 0) return;
-    const int splits = max(1, min(a.slots / max(1, tiles * heads), (longest + 4 * KT - 1) / (4 * KT)));
+    const int splits = tile_splits(a, tiles * heads, longest);
     const int item = (int)(blockIdx.x / heads), at = item / splits, split = item - at * splits;
     if (at >= tiles) return;
     Tile t;
@@ -444,8 +458,8 @@ __global__ void __launch_bounds__(64 * W, 2) kv4_tiles_kernel(const Kv4Tiles a) 
             for (int j = 0; j < 4; j++) y[j] = out[j];
         }
     };
-    if (parts == 1) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+    auto out = [&](float sum) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
         for (int ot = 0; ot < HC / 32; ot++)
 #pragma unroll
@@ -454,31 +468,26 @@ __global__ void __launch_bounds__(64 * W, 2) kv4_tiles_kernel(const Kv4Tiles a) 
                 const int c = c0 + 32 * ot + 8 * (r / 4) + 4 * h;
                 if (row.mine && c < dim) store(row.token, row.head, c, v, inv);
             }
+    };
+    if (parts == 1) {
+        out(l);
         return;
     }
-    // Of several workgroups the one that comes last joins the parts, in their order: [row][channel] sums, then (maximum, sum) pairs
+    // Of several workgroups the one that comes last joins the parts, in their order: every thread stores what it has, two floats at a time, where every workgroup
+    // sees them, and the last one's threads read what the same threads of the others had.
+    constexpr int PAIRS = HC / 4 + 1;   // of a thread: its sums, then (maximum, sum)
     const int64_t unit = (int64_t)at * heads + kvh;
-    auto part_of = [&](int z) { return a.parts + (unit * splits + z) * (int64_t)(ROWS * (dim + 2)); };
-    // two floats at a time, stored where (and read from where) every workgroup sees them
-    auto put = [](float *to_pair, float x, float y) {
-        __hip_atomic_store(reinterpret_cast<uint64_t *>(to_pair), (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    };
-    auto get = [](const float *pair) {
-        const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t *>(pair), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
-    };
+    auto part_of = [&](int z) { return reinterpret_cast<uint64_t *>(a.parts) + (unit * splits + z) * (int64_t)(PAIRS * 64 * W) + tid; };
     {
-        float *part = part_of(split);
-        const int n = 32 * (wave / C) + (lane & 31);
+        uint64_t *part = part_of(split);
+        auto put = [&](int i, float x, float y) {
+            __hip_atomic_store(part + i * (64 * W), (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        };
+        if (row.mine) {
+            put(PAIRS - 1, rows.m, l);
 #pragma unroll
-        for (int ot = 0; ot < HC / 32; ot++)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const float4 v = rows.channels(ot, r);
-                const int c = c0 + 32 * ot + 8 * (r / 4) + 4 * h;
-                if (row.mine && c < dim) put(part + (int64_t)n * dim + c, v.x, v.y), put(part + (int64_t)n * dim + c + 2, v.z, v.w);
-            }
-        if (row.mine && h == 0 && c0 == 0) put(part + (int64_t)ROWS * dim + 2 * n, rows.m, l);
+            for (int i = 0; i < HC / 4; i++) put(i, rows.o[i / 8][i % 8 * 2], rows.o[i / 8][i % 8 * 2 + 1]);
+        }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's stores are where everyone sees them
     __syncthreads();
@@ -488,45 +497,46 @@ __global__ void __launch_bounds__(64 * W, 2) kv4_tiles_kernel(const Kv4Tiles a) 
         if (last_here) __hip_atomic_store(a.arrived + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next call
     }
     __syncthreads();
-    if (!last_here) return;
-    const int quads = dim / 4, mine = min(ROWS, t.rows - t.r0);
-    for (int i = tid; i < mine * quads; i += 64 * W) {
-        const int n = i / quads, c = (i - n * quads) * 4;
-        float top = -INFINITY, all = 0.f;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        constexpr int N = 4;   // parts on their way together
-        for (int z = 0; z < parts; z += N) {
-            float2 ml[N], x01[N], x23[N];
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const float *x = part_of(min(z + e, parts - 1));
-                ml[e] = get(x + (int64_t)ROWS * dim + 2 * n), x01[e] = get(x + (int64_t)n * dim + c), x23[e] = get(x + (int64_t)n * dim + c + 2);
-                if (z + e >= parts) ml[e] = make_float2(-INFINITY, 0.f);
-            }
-            float higher = top;
-#pragma unroll
-            for (int e = 0; e < N; e++) higher = fmaxf(higher, ml[e].x);
-            const float back = all == 0.f ? 0.f : __builtin_amdgcn_exp2f(top - higher);
-            top = higher, all *= back, v.x *= back, v.y *= back, v.z *= back, v.w *= back;
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                if (ml[e].y == 0.f) continue;   // nothing the row sees
-                const float keep = __builtin_amdgcn_exp2f(ml[e].x - top);
-                all += ml[e].y * keep, v.x += x01[e].x * keep, v.y += x01[e].y * keep, v.z += x23[e].x * keep, v.w += x23[e].y * keep;
-            }
-        }
-        const int r = t.r0 + n, token = r / a.group;
-        store(token, kvh * a.group + (r - token * a.group), c, v, all == 0.f ? 0.f : 1.f / all);
+    if (!last_here || !row.any) return;
+    auto get = [&](int z, int i) {
+        const uint64_t v = __hip_atomic_load(part_of(z) + i * (64 * W), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+    };
+    float top = -INFINITY, all = 0.f;
+    for (int z = 0; z < parts; z++) {
+        const float2 ml = row.mine ? get(z, PAIRS - 1) : make_float2(-INFINITY, 0.f);
+        if (ml.y != 0.f) top = fmaxf(top, ml.x);   // (else nothing that the row sees)
     }
+#pragma unroll
+    for (int i = 0; i < HC / 32; i++) rows.o[i] = tf16{};
+    for (int z = 0; z < parts; z++) {
+        if (!row.mine) break;
+        const float2 ml = get(z, PAIRS - 1);
+        float2 x[HC / 4];
+#pragma unroll
+        for (int i = 0; i < HC / 4; i++) x[i] = get(z, i);
+        const bool counts = ml.y != 0.f;
+        const float keep = counts ? __builtin_amdgcn_exp2f(ml.x - top) : 0.f;
+        all += counts ? ml.y * keep : 0.f;
+#pragma unroll
+        for (int i = 0; i < HC / 4; i++) {
+            float &x0 = reinterpret_cast<float *>(&rows.o[i / 8])[i % 8 * 2], &x1 = reinterpret_cast<float *>(&rows.o[i / 8])[i % 8 * 2 + 1];
+            x0 += counts ? x[i].x * keep : 0.f, x1 += counts ? x[i].y * keep : 0.f;
+        }
+    }
+    out(all);
 }
 
 template <int HD, int QT, int W>
 int tiles_launch(hipc_ctx *ctx, Kv4Tiles a, size_t part_bytes) {
-    constexpr int ROWS = 32 * W / (HD > 128 ? 2 : 1);
+    constexpr int C = HD > 128 ? 2 : 1, HC = HD / C, ROWS = 32 * W / C;
     const int64_t rows = (int64_t)a.total * a.group, kv = a.cache.n_kv_heads;
     // tiles there can be: a sequence has some only if it brings more than a.most rows
     const int64_t tiles = rows / ROWS + std::min<int64_t>(a.cache.n_seqs, rows / (a.most + 1));
-    a.slots = (int)std::min<int64_t>(2 * (int64_t)ctx->cu_count * (W == 8 ? 1 : 2), part_bytes / ((size_t)ROWS * (a.cache.head_dim + 2) * 4));
+    a.slots = (int)std::min<int64_t>((int64_t)ctx->cu_count * (8 / W), part_bytes / ((size_t)(HC / 4 + 1) * 64 * W * 8));
+    // us of a key tile (of half as many keys where heads are wider than 128), and of a part on its way through memory
+    a.tile_us = (W == 8 ? 2.6f : 1.8f) * QT * (HD <= 64 ? 0.6f : 1.f), a.part_us = 2.f;
+    a.splits = ctx->tune.prompt_split;
     const int64_t groups = std::max<int64_t>(tiles * kv, ceil_div(a.slots, kv) * kv);
     HIPC_REFUSE(ctx, !grid_fits(groups, 64 * W), "hipc_kv4_prompt_attention: %d rows: too many for one call", a.total);
     hipLaunchKernelGGL((kv4_tiles_kernel<HD, QT, W>), (unsigned)groups, 64 * W, 0, ctx->stream, a);
@@ -539,7 +549,11 @@ int tiles_launch(hipc_ctx *ctx, Kv4Tiles a, size_t part_bytes) {
 int kv4_tiles(hipc_ctx *ctx, const Kv4Tiles &a, int dtype, size_t part_bytes) {
     auto launch = [&](auto width) -> int {
         constexpr int HD = decltype(width)::value;
-        return dtype == HIPC_F16 ? tiles_launch<HD, 1, 8>(ctx, a, part_bytes) : tiles_launch<HD, 2, 8>(ctx, a, part_bytes);
+        const int64_t units = ceil_div((int64_t)a.total * a.group, HD > 128 ? 128 : 256) * a.cache.n_kv_heads;
+        int waves = units >= (int64_t)ctx->cu_count ? 8 : 4;
+        if (ctx->tune.prompt_waves >= 4) waves = ctx->tune.prompt_waves;
+        if (waves >= 8) return dtype == HIPC_F16 ? tiles_launch<HD, 1, 8>(ctx, a, part_bytes) : tiles_launch<HD, 2, 8>(ctx, a, part_bytes);
+        return dtype == HIPC_F16 ? tiles_launch<HD, 1, 4>(ctx, a, part_bytes) : tiles_launch<HD, 2, 4>(ctx, a, part_bytes);
     };
     const int dim = a.cache.head_dim;
     return dim <= 64    ? launch(std::integral_constant<int, 64>())

@@ -121,7 +121,14 @@ struct TileRow {
         lane_begin = begins(past + token), lane_end = ends(past + token);
         begin = begins(p0), end = ends(p1), all_begin = begins(p1), all_end = ends(p0);
     }
-    __device__ __forceinline__ bool sees(const Kv4Tiles &a, int key) const { return key < lane_end && (key >= lane_begin || key < a.sinks); }
+    // the keys key0 .. key0 + 63 that the lane's row sees, a bit each; `there`: blocks of 16 that lie on pages
+    __device__ __forceinline__ uint64_t seen(const Kv4Tiles &a, int key0, uint32_t there) const {
+        auto below = [&](int end) { return end <= key0 ? 0 : end - key0 >= 64 ? ~(uint64_t)0 : ((uint64_t)1 << (end - key0)) - 1; };
+        uint64_t pages = 0;
+#pragma unroll
+        for (int b = 0; b < 4; b++) pages |= there >> b & 1 ? (uint64_t)0xffff << (16 * b) : 0;
+        return below(lane_end) & (~below(lane_begin) | below(a.sinks)) & pages;
+    }
 };
 
 // A wavefront's 32 query rows, HC channels of them from channel c0 on, over key tiles of KT rows of PITCH halfs in LDS, both products turned around:
@@ -198,16 +205,18 @@ struct Kv4TileRows {
             }
         }
     }
-    // the scores of keys key0 .. become weights; `there`: which blocks of 16 keys lie on pages
-    __device__ __forceinline__ void weights(const Kv4Tiles &a, tf16 (&s)[KT / 32], int key0, bool masked, uint32_t there, const TileRow &row, th8 (&p)[KT / 16][QT]) {
+    // the scores of a tile become weights; `seen` (masked tiles): a bit for each of its keys that the lane's row sees
+    __device__ __forceinline__ void weights(tf16 (&s)[KT / 32], bool masked, uint64_t seen, th8 (&p)[KT / 16][QT]) {
         if (masked) {
 #pragma unroll
-            for (int b = 0; b < KT / 32; b++)
+            for (int b = 0; b < KT / 32; b++) {
+                const uint32_t hidden = ~(uint32_t)(seen >> (32 * b)) >> (4 * h);
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int key = key0 + 32 * b + 8 * (r / 4) + 4 * h + r % 4;
-                    s[b][r] = (there >> (2 * b + r / 8) & 1) && row.sees(a, key) ? s[b][r] : -INFINITY;
+                for (int r = 0; r < 16; r++) {   // (key 32 b + 8 (r / 4) + 4 h + r % 4)
+                    const uint32_t all = (uint32_t)((int32_t)(hidden << (31 - 8 * (r / 4) - r % 4)) >> 31);
+                    s[b][r] = __uint_as_float((all & 0xff800000u) | (~all & __float_as_uint(s[b][r])));
                 }
+            }
         }
         float mx = s[0][0];
 #pragma unroll
@@ -246,42 +255,7 @@ struct Kv4TileRows {
         const ts4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ts4 *)(at + 16 * PITCH));
         return __builtin_bit_cast(th8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
-    __device__ __forceinline__ void values(const Kv4Tiles &a, const char *vs, int key0, bool masked, const TileRow &row, const th8 (&p)[KT / 16][QT]) {
-        if (masked) {
-            // A hidden key's weight is zero, but zero times what is not finite is not: where the tile has such values, the product takes zeros in
-            // their places, and a second one finds the rows that see them.
-            uint32_t bad = 0;
-#pragma unroll
-            for (int ot = 0; ot < HC / 32; ot++)
-#pragma unroll
-                for (int u = 0; u < KT / 16; u++) {
-                    const tu4 w = __builtin_bit_cast(tu4, v_part(vs, ot, u));
-#pragma unroll
-                    for (int j = 0; j < 4; j++) bad |= ((w[j] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
-                }
-            if (__any(bad != 0)) {
-#pragma unroll
-                for (int ot = 0; ot < HC / 32; ot++) {
-                    tf16 seen = tf16{};
-#pragma unroll
-                    for (int u = 0; u < KT / 16; u++) {
-                        th8 v = v_part(vs, ot, u), kind = {}, sees = {};
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            if ((__builtin_bit_cast(uint16_t, (_Float16)v[j]) & 0x7c00) == 0x7c00) kind[j] = (_Float16)1.f, v[j] = (_Float16)0.f;
-                            sees[j] = (_Float16)(row.sees(a, key0 + 16 * u + 8 * (j / 4) + 4 * h + j % 4) ? 1.f : 0.f);
-                        }
-#pragma unroll
-                        for (int e = QT - 1; e >= 0; e--) o[ot] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u][e], o[ot], 0, 0, 0);
-                        seen = __builtin_amdgcn_mfma_f32_32x32x16_f16(kind, sees, seen, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        if (seen[r] != 0.f) o[ot][r] = NAN;
-                }
-                return;
-            }
-        }
+    __device__ __forceinline__ void values(const char *vs, const th8 (&p)[KT / 16][QT]) {
 #pragma unroll
         for (int ot = 0; ot < HC / 32; ot++)
 #pragma unroll
@@ -290,6 +264,23 @@ struct Kv4TileRows {
 #pragma unroll
                 for (int e = QT - 1; e >= 0; e--) o[ot] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u][e], o[ot], 0, 0, 0);
             }
+    }
+    // Groups of values that are not all numbers are zeros in the product (zero times a NaN is none): the sums of the rows that see them are NaN. Lane l has the marks of
+    // units 4 l .. + 3 of the tile, GP a key.
+    template <int GP>
+    __device__ __forceinline__ void odd_values(uint32_t marks, uint64_t seen, int c0) {
+        for (uint64_t left = __ballot(marks != 0); left; left &= left - 1) {
+            const int at = __builtin_ctzll(left);
+            const uint32_t word = __builtin_amdgcn_readlane(marks, at);
+            for (int j = 0; j < 4; j++) {
+                const int g = (4 * at + j) % GP, r = (4 * at + j) / GP;
+                if (!(word >> (8 * j) & 1)) continue;
+                const float more = seen >> r & 1 ? NAN : 0.f;
+#pragma unroll
+                for (int ot = 0; ot < HC / 32; ot++)
+                    if (c0 / 32 + ot == g) o[ot] += more;
+            }
+        }
     }
     // sums ot, r .. r + 3 (r a multiple of 4) as the channels 32 ot + 8 (r / 4) + 4 h .. + 3: the halves of the wavefront hold 0 4 1 5 and 2 6 3 7 of eight
     __device__ __forceinline__ float4 channels(int ot, int r) const {
@@ -304,65 +295,90 @@ struct Kv4TileRows {
 template <int HD, int KT, int PITCH, int W>
 struct Kv4TileFetch {
     static constexpr int GP = HD <= 64 ? 2 : HD <= 128 ? 4 : 8;    // groups of a row, rounded up to a power of two
-    static constexpr int UNITS = 2 * KT * GP, EACH = (UNITS + 64 * W - 1) / (64 * W);
-    static constexpr int TILE = KT * PITCH * 2;                    // bytes of a tile of K, or of V
+    static constexpr int UNITS = KT * GP;                          // of a tile of K, or of V
+    static constexpr int EACH = (2 * UNITS + 64 * W - 1) / (64 * W);
     tu4 codes[EACH];
     uint32_t params[EACH];
+    bool none[EACH];   // nothing there: zeros
     int page[EACH], block_page;   // of the tile whose codes are asked for next
+    const char *codes_at[EACH], *params_at[EACH];   // the unit's in page 0, place 0
     const int *table;
-    int shift, groups, held, kvh, tid;
+    uint64_t page_bytes;   // codes of a page; parameters are a quarter of that, wherever one looks
+    int shift, row_bytes, held, tid;
 
-    __device__ __forceinline__ Kv4TileFetch(const Kv4Tiles &a, const Tile &t, int kvh_, int tid_) : kvh(kvh_), tid(tid_) {
+    __device__ __forceinline__ Kv4TileFetch(const Kv4Tiles &a, const Tile &t, int kvh, int tid_) : tid(tid_) {
         table = static_cast<const int *>(a.cache.table) + (int64_t)t.seq * a.cache.table_width;
-        shift = 31 - __builtin_clz((unsigned)a.cache.page_size), groups = a.cache.head_dim / kKv4Group, held = kv4_held(a.cache, t.length);
+        shift = 31 - __builtin_clz((unsigned)a.cache.page_size), row_bytes = a.cache.head_dim / 2, held = kv4_held(a.cache, t.length);
+        page_bytes = (uint64_t)(a.cache.n_kv_heads * (int64_t)row_bytes) << shift;
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const Unit u = unit(e);
+            const int64_t at = ((int64_t)kvh * row_bytes << shift) + (u.g * 16 < row_bytes ? u.g * 16 : 0);
+            codes_at[e] = static_cast<const char *>(u.value ? a.cache.v_codes : a.cache.k_codes) + at;
+            params_at[e] = static_cast<const char *>(u.value ? a.cache.v_params : a.cache.k_params) + at / 4;
+        }
     }
-    __device__ __forceinline__ int page_of(const Kv4Tiles &a, int key) const {
-        const int entry = key >> shift, last = (int)a.cache.table_width - 1, p = table[min(entry, last)];
-        return entry <= last ? p : -1;
+    // the thread's units: of eight wavefronts the lower four have the keys', the upper ones the values'
+    struct Unit {
+        int g, r;
+        bool value, any;
+    };
+    __device__ __forceinline__ Unit unit(int e) const {
+        const int u = W == 8 ? tid & 255 : tid + e * 64 * W;
+        const bool value = W == 8 ? tid >= 256 : u >= UNITS;
+        return {u % GP, (u / GP) % KT, value, W == 8 ? u < UNITS : u < 2 * UNITS};
     }
-    __device__ __forceinline__ bool is_page(const Kv4Tiles &a, int p) const { return p >= 0 && p < a.cache.n_pages; }
+    // (what the table says is looked at a tile later: whether it is a page, too, so that nothing waits for it before)
+    __device__ __forceinline__ int page_of(const Kv4Tiles &a, int key) const { return table[min(key >> shift, (int)a.cache.table_width - 1)]; }
+    __device__ __forceinline__ bool is_page(const Kv4Tiles &a, int p, int key) const { return (uint32_t)p < (uint32_t)a.cache.n_pages && key < held; }
     __device__ __forceinline__ void ask_pages(const Kv4Tiles &a, int tile) {
 #pragma unroll
-        for (int e = 0; e < EACH; e++) page[e] = page_of(a, tile * KT + ((tid + e * 64 * W) / GP) % KT);
+        for (int e = 0; e < EACH; e++) page[e] = page_of(a, tile * KT + unit(e).r);
         block_page = page_of(a, tile * KT + 16 * (tid % (KT / 16)));
     }
     // which blocks of 16 keys of the tile asked for lie on pages
-    __device__ __forceinline__ uint32_t blocks_there(const Kv4Tiles &a) const { return (uint32_t)__ballot(is_page(a, block_page)) & ((1u << (KT / 16)) - 1); }
+    __device__ __forceinline__ uint32_t blocks_there(const Kv4Tiles &a, int tile) const {
+        return (uint32_t)__ballot(is_page(a, block_page, tile * KT + 16 * (tid % (KT / 16)))) & ((1u << (KT / 16)) - 1);
+    }
     __device__ __forceinline__ void ask_codes(const Kv4Tiles &a, int tile) {
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
-            const int unit = tid + e * 64 * W, g = unit % GP, key = tile * KT + (unit / GP) % KT;
-            const bool value = unit >= KT * GP, there = is_page(a, page[e]) && key < held && g < groups && unit < UNITS;
-            const int64_t row = (((int64_t)(there ? page[e] : 0) * a.cache.n_kv_heads + kvh) << shift) + (key & (a.cache.page_size - 1));
-            const int gg = g < groups ? g : 0;
-            codes[e] = *reinterpret_cast<const tu4 *>(static_cast<const char *>(value ? a.cache.v_codes : a.cache.k_codes) + row * (a.cache.head_dim / 2) + gg * 16);
-            const uint32_t p = static_cast<const uint32_t *>(value ? a.cache.v_params : a.cache.k_params)[row * groups + gg];
-            params[e] = there ? p : 0u;
+            const Unit u = unit(e);
+            const int key = tile * KT + u.r;
+            const bool there = is_page(a, page[e], key) && u.any && u.g * 16 < row_bytes;
+            const uint64_t at = (uint32_t)(there ? page[e] : 0) * page_bytes + (uint64_t)(uint32_t)(key & (a.cache.page_size - 1)) * (uint32_t)row_bytes;
+            codes[e] = *reinterpret_cast<const tu4 *>(codes_at[e] + at);
+            params[e] = *reinterpret_cast<const uint32_t *>(params_at[e] + at / 4);
+            none[e] = !there;
         }
     }
-    __device__ __forceinline__ void unpack(char *k, char *v) const {
+    // odd: marks of the tile's values, a byte a unit
+    __device__ __forceinline__ void unpack(char *k, char *v, uint8_t *odd) const {
         const Kv4Unpack take;
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
-            const int unit = tid + e * 64 * W, g = unit % GP, r = (unit / GP) % KT;
-            if (UNITS % (64 * W) != 0 && unit >= UNITS) break;
-            if (32 * g >= HD) continue;   // (heads of 96 in rows of 128)
-            const bool value = unit >= KT * GP;
-            const kvh2 p = __builtin_bit_cast(kvh2, params[e]);
-            char *row = (value ? v : k) + r * PITCH * 2;
-            const int turn = value ? (r & 3) << 1 : r & 7;
+            const Unit u = unit(e);
+            if (!u.any || 32 * u.g >= HD) continue;   // (heads of 96 in rows of 128)
+            kvh2 p = __builtin_bit_cast(kvh2, none[e] ? 0u : params[e]);
+            // a group that has a NaN, or numbers past f16's range (its values lie between code 0's and code 15's): keys are NaN, values zeros with a mark
+            const _Float16 top = __builtin_fmaf16((_Float16)15.f, p.x, p.y);
+            const bool bad = (__builtin_bit_cast(uint16_t, top) & 0x7c00) == 0x7c00;
+            if (bad) p = __builtin_bit_cast(kvh2, u.value ? 0u : 0x7e007e00u);
+            if (u.value) odd[u.r * GP + u.g] = bad;
+            char *row = (u.value ? v : k) + u.r * PITCH * 2;
+            const int turn = u.value ? (u.r & 3) << 1 : u.r & 7;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 kvh2 x[4];
                 take(codes[e][j], kvh2{p.x, p.x}, kvh2{p.y, p.y}, x);
-                *reinterpret_cast<th8 *>(row + ((4 * g + j) ^ turn) * 16) = th8{x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};
+                *reinterpret_cast<th8 *>(row + ((4 * u.g + j) ^ turn) * 16) = th8{x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};
             }
         }
     }
 };
 
 template <int HD, int QT, int W>
-__global__ void __launch_bounds__(64 * W, 2) kv4_tiles_kernel(const Kv4Tiles a) {
+__global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_kernel(const Kv4Tiles a) {
     constexpr int C = HD > 128 ? 2 : 1, HC = HD / C;               // wavefronts of a row, channels of each
     constexpr int KT = HD > 128 ? 32 : 64;
     constexpr int PITCH = HD <= 64 ? 64 : HD <= 128 ? 128 : 256;   // halfs of an LDS row
@@ -370,6 +386,9 @@ __global__ void __launch_bounds__(64 * W, 2) kv4_tiles_kernel(const Kv4Tiles a) 
     typedef typename std::conditional<QT == 1, _Float16, float>::type T;
     __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];   // [buffer][K, V]
     __shared__ float4 scores[C > 1 ? W : 1][KT / 8][64];             // a wavefront's own, for the other
+    constexpr int GP = HD <= 64 ? 2 : HD <= 128 ? 4 : 8;
+    __shared__ __attribute__((aligned(16))) uint8_t odd[2][256];     // [buffer][key][group]: values that are not all numbers
+    static_assert(KT * GP <= 256, "a byte a unit");
     __shared__ int last_here;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
@@ -393,56 +412,70 @@ __global__ void __launch_bounds__(64 * W, 2) kv4_tiles_kernel(const Kv4Tiles a) 
     auto key_tile = [&](int i) { return i < t.sink_tiles ? i : t.first + i; };
     Kv4TileFetch<HD, KT, PITCH, W> from(a, t, kvh, tid);
     Kv4TileRows<HC, KT, PITCH, QT> rows(a, lane, c0);
-    auto buffer = [&](int i) { return smem + ((i - i0) & 1) * 2 * TILE; };
+    auto k_buffer = [&](int i) { return smem + ((i - i0) & 1) * 2 * TILE; };
+    auto v_buffer = [&](int i) { return smem + ((i - i0) & 1) * 2 * TILE + TILE; };
+    auto odd_buffer = [&](int i) { return odd[(i - i0) & 1]; };
+    auto masked_at = [&](int key0, uint32_t here) { return key0 + KT > row.all_end || (key0 < row.all_begin && key0 + KT > a.sinks) || here != (1u << (KT / 16)) - 1; };
+    auto active_at = [&](int key0) { return row.any && key0 < row.end && (key0 + KT > row.begin || key0 < a.sinks); };
+    // what a wavefront of two that share a row has of the scores, and the other's
+    auto give = [&](const tf16 (&s)[KT / 32]) {
+#pragma unroll
+        for (int j = 0; j < KT / 8; j++) scores[wave][j][lane] = make_float4(s[j / 4][j % 4 * 4], s[j / 4][j % 4 * 4 + 1], s[j / 4][j % 4 * 4 + 2], s[j / 4][j % 4 * 4 + 3]);
+    };
+    auto take = [&](tf16 (&s)[KT / 32]) {
+#pragma unroll
+        for (int j = 0; j < KT / 8; j++) {
+            const float4 v = scores[wave ^ 1][j][lane];
+            s[j / 4][j % 4 * 4] += v.x, s[j / 4][j % 4 * 4 + 1] += v.y, s[j / 4][j % 4 * 4 + 2] += v.z, s[j / 4][j % 4 * 4 + 3] += v.w;
+        }
+    };
+    if (tid < 128) reinterpret_cast<uint32_t *>(odd)[tid] = 0;   // (units that heads of this width do not have stay so)
+    __syncthreads();
     uint32_t there = 0, there1 = 0;
     if (i0 < i1) {
         from.ask_pages(a, key_tile(i0));
-        there = from.blocks_there(a);
+        there = from.blocks_there(a, key_tile(i0));
         from.ask_codes(a, key_tile(i0));
         if (i0 + 1 < i1) from.ask_pages(a, key_tile(i0 + 1));
     }
     rows.template queries<T>(a, t, row, c0);
-    if (i0 < i1) {
-        from.unpack(buffer(i0), buffer(i0) + TILE);
-        if (i0 + 1 < i1) {
-            there1 = from.blocks_there(a);
-            from.ask_codes(a, key_tile(i0 + 1));
-            if (i0 + 2 < i1) from.ask_pages(a, key_tile(i0 + 2));
+    // a tile's codes to LDS, and the codes and pages behind it asked for
+    auto carry_on = [&](int i) {
+        from.unpack(k_buffer(i), v_buffer(i), odd_buffer(i));
+        if (i + 1 < i1) {
+            there1 = from.blocks_there(a, key_tile(i + 1));
+            from.ask_codes(a, key_tile(i + 1));
+            if (i + 2 < i1) from.ask_pages(a, key_tile(i + 2));
         }
-    }
+    };
+    if (i0 < i1) carry_on(i0);
     for (int i = i0; i < i1; i++) {
         __syncthreads();   // this tile is there, and every wavefront is done with the other buffer
         const uint32_t here = there;
-        if (i + 1 < i1) {
-            from.unpack(buffer(i + 1), buffer(i + 1) + TILE);
-            there = there1;
-            if (i + 2 < i1) {
-                there1 = from.blocks_there(a);
-                from.ask_codes(a, key_tile(i + 2));
-                if (i + 3 < i1) from.ask_pages(a, key_tile(i + 3));
-            }
-        }
+        there = there1;
         const int key0 = key_tile(i) * KT;
-        const bool active = row.any && key0 < row.end && (key0 + KT > row.begin || key0 < a.sinks);
-        if (C == 1 && !active) continue;
-        const char *ks = buffer(i);
+        const bool active = active_at(key0);
+        if (C == 1 && !active) {
+            if (i + 1 < i1) carry_on(i + 1);
+            continue;
+        }
         tf16 s[KT / 32];
-        rows.scores(ks, s);
+        rows.scores(k_buffer(i), s);
+        // (the next tile's codes are unpacked while the products are on their way)
+        if (i + 1 < i1) carry_on(i + 1);
         if (C > 1) {
-#pragma unroll
-            for (int j = 0; j < KT / 8; j++) scores[wave][j][lane] = make_float4(s[j / 4][j % 4 * 4], s[j / 4][j % 4 * 4 + 1], s[j / 4][j % 4 * 4 + 2], s[j / 4][j % 4 * 4 + 3]);
+            give(s);
             __syncthreads();
             if (!active) continue;
-#pragma unroll
-            for (int j = 0; j < KT / 8; j++) {
-                const float4 v = scores[wave ^ 1][j][lane];
-                s[j / 4][j % 4 * 4] += v.x, s[j / 4][j % 4 * 4 + 1] += v.y, s[j / 4][j % 4 * 4 + 2] += v.z, s[j / 4][j % 4 * 4 + 3] += v.w;
-            }
+            take(s);
         }
-        const bool masked = key0 + KT > row.all_end || (key0 < row.all_begin && key0 + KT > a.sinks) || here != (1u << (KT / 16)) - 1;
+        const bool masked = masked_at(key0, here);
         th8 p[KT / 16][QT];
-        rows.weights(a, s, key0, masked, here, row, p);
-        rows.values(a, ks + TILE, key0, masked, row, p);
+        const uint64_t seen = masked ? row.seen(a, key0, here) : ~(uint64_t)0;
+        rows.weights(s, masked, seen, p);
+        const uint32_t marks = *reinterpret_cast<const uint32_t *>(odd_buffer(i) + 4 * lane);
+        rows.values(v_buffer(i), p);
+        if (__builtin_expect(__any(marks != 0), 0)) rows.template odd_values<GP>(marks, seen, c0);
     }
 
     const float l = tile_halves_sum(rows.l);

@@ -77,8 +77,9 @@ struct Tuning {
     int dec_wide = -1;        // HIPC_DEC_WIDE       1: as where the workgroups of a group do not share an L2
     int dec_polls = -1;       // HIPC_DEC_POLLS      polls a thread may make before the step is given up
     int dql_wait = -1;        // HIPC_DQL_WAIT       0: DynamicQuantizeLinear never in one launch of several workgroups; n: how long these wait for each other, in 10 ns
-    int prompt_waves = -1;    // HIPC_PROMPT_WAVES   wavefronts of a workgroup of the prompt attention: 4 or 8 of 32 query rows each; f16: 1: four that share 32 rows, 2: one by itself
-    int prompt_split = -1;    // HIPC_PROMPT_SPLIT   n: workgroups that share the keys of its query tiles
+    int prompt_waves = -1;    // HIPC_PROMPT_WAVES   wavefronts of a workgroup of the prompt attention: 4 or 8 of 32 query rows each (also over the 4-bit cache, whose kernel for many rows is then
+                              //                     launched however few there are in all); f16: 1: four that share 32 rows, 2: one by itself
+    int prompt_split = -1;    // HIPC_PROMPT_SPLIT   n: workgroups that share the keys of its query tiles (over the 4-bit cache as far as they run at once)
     int dec_prefetch = -1;    // HIPC_DEC_PREFETCH   bits: which launches of a layer carry helper rows that read ahead for the next launch (0 none, 31 all; see hipc_decoder_step)
 };
 

@@ -33,7 +33,7 @@ constexpr int kScratchKv4 = 6;     // scratch slot of this operator alone
 constexpr int kKv4Rows = 16;       // query rows of a unit
 constexpr int kKv4Tile = 64;       // keys a wavefront takes at a time
 constexpr int kKv4PerCu = 8;       // wavefronts
-constexpr int kKv4FewRows = 64;    // query rows of a sequence that this file's kernel takes (hipc_kv4_prompt_attention)
+constexpr int kKv4FewRows = 64;    // query rows of a sequence that this file's kernel takes beside another one (hipc_kv4_prompt_attention)
 constexpr float kKv4Log2e = 1.4426950408889634f;
 constexpr float kKv4RescaleAt = 8.f;   // the running maximum may fall behind by 2^8 before sums are rescaled ...
 constexpr float kKv4Up = 7.f;          // ... and weights are kept 2^7 times as large: up to 2^15, so that two f16 terms hold 22 bits of more of them
@@ -681,7 +681,9 @@ int kv4_attend_scratch(hipc_ctx *ctx, Kv4Attend *a) {
 // units: how many there are, or about as many
 template <bool PACKED>
 int kv4_attend(hipc_ctx *ctx, const Kv4Attend &a, int dtype, int64_t units) {
-    const bool alone = units * 2 >= 3 * (int64_t)ctx->cu_count;
+    // (PACKED, lengths as even as a window makes them; us, four / one: a token of each of 40 contexts that see 4000 positions, 32 / 8 heads of 128 in f16, 320 units, 68 / 51, of 32
+    // 44 / 45, of 24 35 / 38; of 40 of up to 500 13 / 16)
+    const bool alone = PACKED ? units > ctx->cu_count : units * 2 >= 3 * (int64_t)ctx->cu_count;
     switch (a.cache.head_dim / 32) {
         case 1: kv4_launch<32, PACKED>(ctx, a, dtype, alone); break;
         case 2: kv4_launch<64, PACKED>(ctx, a, dtype, alone); break;
@@ -754,11 +756,16 @@ int hipc_kv4_prompt_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const 
         a.starts = static_cast<const int *>(starts), a.total = (int)total, a.sinks = std::min(sinks, kKv4MaxPositions);
         HIPC_REFUSE(ctx, total * a.group > 1 << 30, "%s: %lld rows of %d heads to a kv head: too many for one call", who, (long long)total, a.group);
         if (int rc = kv4_attend_scratch(ctx, &a)) return rc;
-        // Who brings how many is known on the device: where some sequence can bring many rows, both parts are launched, and each leaves the other's alone.
-        a.most = kKv4FewRows;
-        const bool many = total * a.group > a.most;
-        const int64_t blocks = std::min(ceil_div(total * a.group, kKv4Rows) + std::min<int64_t>(cache->n_seqs, total), (int64_t)cache->n_seqs * ceil_div(a.most, kKv4Rows));
-        if (int rc = kv4_attend<true>(ctx, a, dtype, blocks * cache->n_kv_heads)) return rc;
+        // Who brings how many is known on the device. While all rows together are few enough for the workgroups of this file's kernel it takes them all; beyond, both
+        // kernels are launched, sequences of more than kKv4FewRows rows are the other one's, and each leaves the other's alone (nothing to do takes one 4.5 us). One
+        // sequence, this kernel / the other, in us: 128 rows behind 4000 keys, 32 / 8 heads of 128 in f16 (512 of a kv head: 4096 in all) 47 / 45, behind 500 20 / 25,
+        // behind 30000 220 / 120; 256 rows 87 / 57, 39 / 25 and 437 / 185, in f32 88 / 73, 41 / 32 and 449 / 279. 256 rows of 4 / 1 heads of 256 behind 4000 57 / 59.
+        const int64_t all = total * a.group * cache->n_kv_heads;
+        const bool many = ctx->tune.prompt_waves >= 4 || all > (dtype == HIPC_F16 ? 4096 : 6144);
+        a.most = many ? kKv4FewRows : 1 << 30;
+        // (where there are both kinds, sequences of few rows are taken to bring one token)
+        const int64_t blocks = ceil_div((many ? 1 : ceil_div(total, cache->n_seqs)) * a.group, kKv4Rows);
+        if (int rc = kv4_attend<true>(ctx, a, dtype, std::min<int64_t>(cache->n_seqs, total) * blocks * cache->n_kv_heads)) return rc;
         if (!many) return HIPC_OK;
         Kv4Tiles t{};
         t.cache = a.cache, t.q = a.q, t.y = a.y, t.q_stride = a.q_stride, t.y_stride = a.y_stride, t.starts = a.starts, t.total = a.total, t.n_q_heads = a.n_q_heads;

@@ -17,6 +17,16 @@ from test_rotary_gpu import check
 pytestmark = pytest.mark.gpu
 
 
+ROUTES = {"by size": {}, "four wavefronts": dict(HIPC_PROMPT_WAVES=4), "eight wavefronts": dict(HIPC_PROMPT_WAVES=8), "shared": dict(HIPC_PROMPT_WAVES=4, HIPC_PROMPT_SPLIT=3)}
+
+
+@pytest.fixture(params=list(ROUTES))
+def route(request, ctx):
+    """Who takes sequences of more than 64 query rows: whoever the sizes ask for, or the kernel for many rows with so many wavefronts, its keys shared or not."""
+    with ctx.options(**ROUTES[request.param]):
+        yield request.param
+
+
 def starts_of(new):
     return np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
 
@@ -54,7 +64,7 @@ def case(ctx, pkg, lengths, page, kv, dim, seed=0, table=None):
 @pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
 @pytest.mark.parametrize("new,lengths", [([1], [1]), ([5], [5]), ([64], [64]), ([65, 1, 17], [65, 200, 80]), ([0, 3, 1, 0], [9, 3, 64, 0]), ([130], [131]), ([257, 1], [300, 513])], ids=str)
 @pytest.mark.parametrize("heads,kv,dim,page", [(4, 1, 256, 512), (8, 2, 128, 16), (3, 3, 64, 32)], ids=str)
-def test_pieces_prompts_and_tokens(ctx, pkg, dtype, new, lengths, heads, kv, dim, page):
+def test_pieces_prompts_and_tokens(ctx, pkg, route, dtype, new, lengths, heads, kv, dim, page):
     c = case(ctx, pkg, lengths, page, kv, dim)
     c.attend(heads, new, dtype)
     c.gpu.free()
@@ -62,7 +72,7 @@ def test_pieces_prompts_and_tokens(ctx, pkg, dtype, new, lengths, heads, kv, dim
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
 @pytest.mark.parametrize("heads,kv,dim", [(14, 2, 64), (4, 2, 96), (2, 2, 32), (5, 5, 160), (6, 1, 192), (3, 1, 224), (40, 1, 64), (7, 1, 128), (1, 1, 256)], ids=str)
-def test_head_layouts(ctx, pkg, dtype, heads, kv, dim):
+def test_head_layouts(ctx, pkg, route, dtype, heads, kv, dim):
     c = case(ctx, pkg, [150, 40, 70], 16, kv, dim)
     c.attend(heads, [90, 2, 70], dtype)
     c.gpu.free()
@@ -71,14 +81,14 @@ def test_head_layouts(ctx, pkg, dtype, heads, kv, dim):
 @pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (33, 0), (64, 1), (1, 1), (100, 4), (64, 64), (20, 70), (128, 200), (1000, 4), (7, 1 << 30), (1 << 30, 3)], ids=str)
 @pytest.mark.parametrize("new,lengths,heads,kv,dim", [([1, 1, 1], [400, 3, 70], 8, 2, 128), ([70, 5, 1], [380, 5, 66], 4, 1, 256), ([150, 40], [310, 41], 4, 4, 64)], ids=str)
-def test_windows_and_first_positions(ctx, pkg, dtype, window, sinks, new, lengths, heads, kv, dim):
+def test_windows_and_first_positions(ctx, pkg, route, dtype, window, sinks, new, lengths, heads, kv, dim):
     c = case(ctx, pkg, lengths, 32, kv, dim, window + sinks)
     c.attend(heads, new, dtype, window, sinks)
     c.gpu.free()
 
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
-def test_rows_that_see_nothing_and_rows_that_are_nobodys(ctx, pkg, dtype):
+def test_rows_that_see_nothing_and_rows_that_are_nobodys(ctx, pkg, route, dtype):
     """Rows in front of the first sequence and behind the last, positions below 0, sequences without keys, starts out of range."""
     c = case(ctx, pkg, [30, 90, 5, 1], 16, 2, 64)
     for starts, lengths, total in (([3, 20, 70, 80, 81], [10, 90, 0, 1], 90), ([-5, 10, 40, 40, 60], [30, 90, 5, 1], 50), ([0, 50, 30, 30, 35], [30, 90, 5, 1], 40), ([0, 200, 200, 200, 200], [30, 9, 5, 1], 200)):
@@ -102,7 +112,7 @@ def test_rows_that_see_nothing_and_rows_that_are_nobodys(ctx, pkg, dtype):
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
 @pytest.mark.parametrize("new", [[1, 1], [90, 70], [3, 150]], ids=str)
-def test_pages_that_are_no_pages(ctx, pkg, dtype, new):
+def test_pages_that_are_no_pages(ctx, pkg, route, dtype, new):
     table = np.array([[3, -1, 0, 1 << 30, 9, 4, 17, 15, 16, 11, 14], [-7, 5, 99, 6, 7, 8, 1, 2, 10, -1, 12]], np.int32)
     c = case(ctx, pkg, [160, 150], 16, 2, 128, table=table)
     for window, sinks in ((0, 0), (20, 0), (64, 30), (100, 4)):
@@ -111,7 +121,7 @@ def test_pages_that_are_no_pages(ctx, pkg, dtype, new):
 
 
 @pytest.mark.parametrize("new", [[3, 1], [100, 90]], ids=str)
-def test_lengths_past_the_table_and_below_zero(ctx, pkg, new):
+def test_lengths_past_the_table_and_below_zero(ctx, pkg, route, new):
     """Positions behind the table are not seen, though they count where a window does; a length below 0 counts as 0."""
     c = case(ctx, pkg, [100, 96], 32, 1, 64)
     held = c.ref.table.shape[1] * 32
@@ -131,7 +141,7 @@ def test_lengths_past_the_table_and_below_zero(ctx, pkg, new):
 @pytest.mark.parametrize("which", [0, 1], ids=["keys", "values"])
 @pytest.mark.parametrize("new", [[4], [120]], ids=str)
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
-def test_parameters_that_are_not_finite(ctx, pkg, dtype, which, new, value):
+def test_parameters_that_are_not_finite(ctx, pkg, route, dtype, which, new, value):
     """A position in the rows' midst: rows behind it are NaN (of a value: in its channels; infinite parameters make lowest + c * scale infinite for c > 0, and
     a weight times that is no NaN: there the result may be the infinity), rows in front of it are as without."""
     c = case(ctx, pkg, [150], 16, 2, 96)
@@ -161,7 +171,7 @@ def test_parameters_that_are_not_finite(ctx, pkg, dtype, which, new, value):
 @pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
 @pytest.mark.parametrize("new", [[5, 1], [80, 40]], ids=str)
 @pytest.mark.parametrize("off,pad", [(0, 8), (1, 0), (0, 3), (3, 5)], ids=str)
-def test_rows_anywhere(ctx, pkg, dtype, new, off, pad):
+def test_rows_anywhere(ctx, pkg, route, dtype, new, off, pad):
     """Rows apart by odd numbers of elements and off 16 bytes give what rows side by side give; what lies between them stays."""
     c = case(ctx, pkg, [130, 40], 32, 2, 64)
     rows, width = sum(new), 6 * 64 + pad
@@ -180,7 +190,7 @@ def test_rows_anywhere(ctx, pkg, dtype, new, off, pad):
 
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
-def test_many_sequences_of_every_kind(ctx, pkg, dtype):
+def test_many_sequences_of_every_kind(ctx, pkg, route, dtype):
     """More sequences than a wavefront has lanes: some bring nothing, most one token, a few whole prompts and pieces."""
     rng = np.random.default_rng(3)
     seqs = 150
@@ -195,7 +205,7 @@ def test_many_sequences_of_every_kind(ctx, pkg, dtype):
 @pytest.mark.parametrize("scale", [0.0, 0.02, -0.1])
 @pytest.mark.parametrize("new", [[3], [100]], ids=str)
 @pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
-def test_scales_and_heavy_weights(ctx, pkg, dtype, new, scale):
+def test_scales_and_heavy_weights(ctx, pkg, route, dtype, new, scale):
     """Scores of several hundred (one key has all the weight), of either sign, and next to none."""
     c = case(ctx, pkg, [160], 32, 1, 64)
     for gain in (0.001, 40.0):
@@ -209,7 +219,7 @@ def test_scales_and_heavy_weights(ctx, pkg, dtype, new, scale):
     c.gpu.free()
 
 
-def test_the_newest_tokens_call_agrees(ctx, pkg):
+def test_the_newest_tokens_call_agrees(ctx, pkg, route):
     """As many tokens of every sequence: hipc_kv4_attention's case, whatever the route."""
     c = case(ctx, pkg, [300, 64, 2, 0], 16, 2, 128)
     for tokens in (1, 2, 33):
@@ -219,7 +229,7 @@ def test_the_newest_tokens_call_agrees(ctx, pkg):
     c.gpu.free()
 
 
-def test_results_repeat_and_recorded_calls_follow_what_is_written(ctx, pkg):
+def test_results_repeat_and_recorded_calls_follow_what_is_written(ctx, pkg, route):
     """Starts, lengths and table are read when the kernels run: a recorded call, replayed with others of as many rows, gives what the call gives, bit for bit."""
     c = case(ctx, pkg, [400, 380, 300], 16, 2, 128)
     q = c.rng.standard_normal((300, 8, 128)).astype(np.float16)
@@ -294,7 +304,7 @@ def test_recorded_on_a_context_that_has_run_none(pkg):
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (48, 4)], ids=str)
-def test_a_layer_of_prompts_in_pieces_and_tokens(ctx, pkg, dtype, window, sinks):
+def test_a_layer_of_prompts_in_pieces_and_tokens(ctx, pkg, route, dtype, window, sinks):
     """The calls as a program makes them: rows of a projection are normed, turned and stored, then attended with, piece by piece and token by token, beside
     other sequences; every step against the definition: queries and keys by the formulas, the cache by the oracle's from these keys, and attention on that."""
     rng = np.random.default_rng(11)

@@ -762,10 +762,11 @@ int hipc_kv4_prompt_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const 
         // behind 30000 220 / 120; 256 rows 87 / 57, 39 / 25 and 437 / 185, in f32 88 / 73, 41 / 32 and 449 / 279. 256 rows of 4 / 1 heads of 256 behind 4000 57 / 59.
         const int64_t all = total * a.group * cache->n_kv_heads;
         const bool many = ctx->tune.prompt_waves >= 4 || all > (dtype == HIPC_F16 ? 4096 : 6144);
-        a.most = many ? kKv4FewRows : 1 << 30;
+        a.most = many ? (cache->n_seqs == 1 ? 0 : kKv4FewRows) : 1 << 30;   // (one sequence is one kernel's)
         // (where there are both kinds, sequences of few rows are taken to bring one token)
         const int64_t blocks = ceil_div((many ? 1 : ceil_div(total, cache->n_seqs)) * a.group, kKv4Rows);
-        if (int rc = kv4_attend<true>(ctx, a, dtype, std::min<int64_t>(cache->n_seqs, total) * blocks * cache->n_kv_heads)) return rc;
+        if (a.most > 0)
+            if (int rc = kv4_attend<true>(ctx, a, dtype, std::min<int64_t>(cache->n_seqs, total) * blocks * cache->n_kv_heads)) return rc;
         if (!many) return HIPC_OK;
         Kv4Tiles t{};
         t.cache = a.cache, t.q = a.q, t.y = a.y, t.q_stride = a.q_stride, t.y_stride = a.y_stride, t.starts = a.starts, t.total = a.total, t.n_q_heads = a.n_q_heads;

@@ -582,8 +582,12 @@ int tiles_launch(hipc_ctx *ctx, Kv4Tiles a, size_t part_bytes) {
 int kv4_tiles(hipc_ctx *ctx, const Kv4Tiles &a, int dtype, size_t part_bytes) {
     auto launch = [&](auto width) -> int {
         constexpr int HD = decltype(width)::value;
+        // Eight wavefronts unpack a key tile once for twice as many rows as four and are half as many workgroups. us, four / eight: 2048 rows behind 30000 keys, 32 / 8 heads of 128 in
+        // f16 1360 / 1207; 500 behind 8000 beside single tokens 148 / 139; prompts of up to 1024, 28 / 4 heads, 44 / 47; pieces of 1000 that see 512 keys, 4 / 1 heads of 256,
+        // 33 / 40. How long sequences are is known on the device only: the table's room stands for it.
         const int64_t units = ceil_div((int64_t)a.total * a.group, HD > 128 ? 128 : 256) * a.cache.n_kv_heads;
-        int waves = units >= (int64_t)ctx->cu_count ? 8 : 4;
+        const int64_t room = a.cache.table_width * a.cache.page_size, keys = a.window > 0 ? std::min<int64_t>(room, a.window) : room;
+        int waves = units >= (int64_t)ctx->cu_count || (keys >= 4096 && 4 * units >= (int64_t)ctx->cu_count) ? 8 : 4;
         if (ctx->tune.prompt_waves >= 4) waves = ctx->tune.prompt_waves;
         if (waves >= 8) return dtype == HIPC_F16 ? tiles_launch<HD, 1, 8>(ctx, a, part_bytes) : tiles_launch<HD, 2, 8>(ctx, a, part_bytes);
         return dtype == HIPC_F16 ? tiles_launch<HD, 1, 4>(ctx, a, part_bytes) : tiles_launch<HD, 2, 4>(ctx, a, part_bytes);

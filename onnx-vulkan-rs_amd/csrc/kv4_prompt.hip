@@ -131,7 +131,30 @@ struct TileRow {
     }
 };
 
-// A wavefront's 32 query rows, HC channels of them from channel c0 on, over key tiles of KT rows of PITCH halfs in LDS, both products turned around:
+// Where a lane reads operands in key tiles of KT rows of PITCH halfs in LDS. 16-byte chunks of a row lie at chunk ^ f(row), so that the rows a read takes at a time lie in
+// different banks.
+template <int KT, int PITCH>
+struct Kv4TileReads {
+    uint32_t k_at[4], v_at[2];
+    __device__ __forceinline__ Kv4TileReads(int lane, int c0) {
+        const int n = lane & 31, i16 = lane & 15, h = lane >> 5;
+#pragma unroll
+        for (int c = 0; c < 4; c++) k_at[c] = n * PITCH * 2 + (((2 * c + h) ^ (n & 7)) * 16) + 2 * c0;
+#pragma unroll
+        for (int i = 0; i < 2; i++) v_at[i] = (4 * h + (i16 >> 2)) * PITCH * 2 + (((4 * i + 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1)) ^ ((i16 >> 2) << 1)) * 16) + (i16 & 1) * 8 + 2 * c0;
+    }
+    // keys 32 b + lane % 32, channels 16 c + 8 (lane / 32) .. + 7
+    __device__ __forceinline__ th8 keys(const char *ks, int b, int c) const { return *reinterpret_cast<const th8 *>(ks + k_at[c & 3] + (c >> 2) * 128 + b * 64 * PITCH); }
+    // channels 32 ot + lane % 32 of the keys 16 u + 8 (j / 4) + 4 (lane / 32) + j % 4: the order in which scores come out
+    __device__ __forceinline__ th8 values(const char *vs, int ot, int u) const {
+        const char *at = vs + v_at[ot & 1] + (ot >> 1) * 128 + u * 32 * PITCH;
+        const ts4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ts4 *)(at));
+        const ts4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ts4 *)(at + 16 * PITCH));
+        return __builtin_bit_cast(th8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+};
+
+// 32 query rows of a wavefront, HC channels of them from channel c0 on, both products turned around:
 //   S^T = K Q^T      32x32x16: a lane's 16 results are one query's scores (query = lane % 32) of keys 8 (r / 4) + 4 (lane / 32) + r % 4
 //   O^T = V^T P^T    the lane's weights are the second operand as they lie; V^T is read from row-major LDS rows by the transposing loads
 // so maximum, sum and rescale of the softmax are numbers of one lane, exchanged once between the two halves of the wavefront.
@@ -139,31 +162,23 @@ struct TileRow {
 // heaviest weight, its subnormal ones to 2^-31. QT = 1, f16 rows: queries as they are, weights rounded to f16 (as two terms they would be half as many
 // products again of a kernel that these bound; the result's own rounding is as large). QT = 2, f32 rows: two f16 terms each, of the row times a power of two, and of the weight.
 // The eight channels of a word of codes lie in the order in which it unpacks, 0 4 1 5 2 6 3 7, in K's rows, V's and the queries alike.
-template <int HC, int KT, int PITCH, int QT>
+template <int HC, int KT, int QT>
 struct Kv4TileRows {
     th8 qf[HC / 16][QT];
     tf16 o[HC / 32];
     float m = -INFINITY, l = 0.f, c2, down = -kTileUp;
-    uint32_t k_at[4], v_at[2];
-    int h;
 
-    __device__ __forceinline__ Kv4TileRows(const Kv4Tiles &a, int lane, int c0) {
-        const int n = lane & 31, i16 = lane & 15;
-        h = lane >> 5;
-        c2 = fabsf(a.scale) * kTileLog2e;
-#pragma unroll
-        for (int c = 0; c < 4; c++) k_at[c] = n * PITCH * 2 + (((2 * c + h) ^ (n & 7)) * 16) + 2 * c0;
-#pragma unroll
-        for (int i = 0; i < 2; i++) v_at[i] = (4 * h + (i16 >> 2)) * PITCH * 2 + (((4 * i + 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1)) ^ ((i16 >> 2) << 1)) * 16) + (i16 & 1) * 8 + 2 * c0;
+    __device__ __forceinline__ Kv4TileRows() {
 #pragma unroll
         for (int i = 0; i < HC / 32; i++) o[i] = tf16{};
     }
     template <typename T>
-    __device__ __forceinline__ void queries(const Kv4Tiles &a, const Tile &t, const TileRow &r, int c0) {
+    __device__ __forceinline__ void queries(const Kv4Tiles &a, const Tile &t, const TileRow &r, int h, int c0) {
         const T *q = static_cast<const T *>(a.q) + a.q_stride * (t.row0 + (r.mine ? r.token : 0)) + (int64_t)(r.mine ? r.head : 0) * a.cache.head_dim;
         const int dim = a.cache.head_dim;
-        float sign = a.scale < 0.f ? -1.f : 1.f;
+        const float sign = a.scale < 0.f ? -1.f : 1.f;
         int up = 0;
+        c2 = fabsf(a.scale) * kTileLog2e;
         if (QT == 2) {
             // The row's largest value into [2^14, 2^15); an infinity stays where it is. And no further up than leaves the scores' factor an ordinary number: at 0 it
             // would make NaN of what is hidden. (A wavefront with half of the channels looks at the whole row.)
@@ -193,31 +208,19 @@ struct Kv4TileRows {
             }
         }
     }
-    __device__ __forceinline__ void scores(const char *ks, tf16 (&s)[KT / 32]) const {
+    // scores of keys that the lane's row does not see are -inf; `seen`: a bit for each key of the tile
+    static __device__ __forceinline__ void hide(tf16 (&s)[KT / 32], uint64_t seen, int h) {
 #pragma unroll
         for (int b = 0; b < KT / 32; b++) {
-            s[b] = tf16{};
+            const uint32_t hidden = ~(uint32_t)(seen >> (32 * b)) >> (4 * h);
 #pragma unroll
-            for (int c = 0; c < HC / 16; c++) {
-                const th8 k = *reinterpret_cast<const th8 *>(ks + k_at[c & 3] + (c >> 2) * 128 + b * 64 * PITCH);
-#pragma unroll
-                for (int e = QT - 1; e >= 0; e--) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[c][e], s[b], 0, 0, 0);
+            for (int r = 0; r < 16; r++) {   // (key 32 b + 8 (r / 4) + 4 h + r % 4)
+                const uint32_t all = (uint32_t)((int32_t)(hidden << (31 - 8 * (r / 4) - r % 4)) >> 31);
+                s[b][r] = __uint_as_float((all & 0xff800000u) | (~all & __float_as_uint(s[b][r])));
             }
         }
     }
-    // the scores of a tile become weights; `seen` (masked tiles): a bit for each of its keys that the lane's row sees
-    __device__ __forceinline__ void weights(tf16 (&s)[KT / 32], bool masked, uint64_t seen, th8 (&p)[KT / 16][QT]) {
-        if (masked) {
-#pragma unroll
-            for (int b = 0; b < KT / 32; b++) {
-                const uint32_t hidden = ~(uint32_t)(seen >> (32 * b)) >> (4 * h);
-#pragma unroll
-                for (int r = 0; r < 16; r++) {   // (key 32 b + 8 (r / 4) + 4 h + r % 4)
-                    const uint32_t all = (uint32_t)((int32_t)(hidden << (31 - 8 * (r / 4) - r % 4)) >> 31);
-                    s[b][r] = __uint_as_float((all & 0xff800000u) | (~all & __float_as_uint(s[b][r])));
-                }
-            }
-        }
+    __device__ __forceinline__ void rise(const tf16 (&s)[KT / 32]) {
         float mx = s[0][0];
 #pragma unroll
         for (int b = 0; b < KT / 32; b++)
@@ -232,6 +235,8 @@ struct Kv4TileRows {
 #pragma unroll
                 for (int r = 0; r < 16; r++) o[i][r] *= keep;
         }
+    }
+    __device__ __forceinline__ void weights(const tf16 (&s)[KT / 32], th8 (&p)[KT / 16][QT]) {
 #pragma unroll
         for (int u = 0; u < KT / 16; u++)
 #pragma unroll
@@ -247,22 +252,6 @@ struct Kv4TileRows {
                     l += w.x + w.y;
                     p[u][QT - 1][j] = (_Float16)(w.x - (float)hi.x), p[u][QT - 1][j + 1] = (_Float16)(w.y - (float)hi.y);
                 }
-            }
-    }
-    __device__ __forceinline__ th8 v_part(const char *vs, int ot, int u) const {
-        const char *at = vs + v_at[ot & 1] + (ot >> 1) * 128 + u * 32 * PITCH;
-        const ts4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ts4 *)(at));
-        const ts4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ts4 *)(at + 16 * PITCH));
-        return __builtin_bit_cast(th8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-    }
-    __device__ __forceinline__ void values(const char *vs, const th8 (&p)[KT / 16][QT]) {
-#pragma unroll
-        for (int ot = 0; ot < HC / 32; ot++)
-#pragma unroll
-            for (int u = 0; u < KT / 16; u++) {
-                const th8 v = v_part(vs, ot, u);
-#pragma unroll
-                for (int e = QT - 1; e >= 0; e--) o[ot] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u][e], o[ot], 0, 0, 0);
             }
     }
     // Groups of values that are not all numbers are zeros in the product (zero times a NaN is none): the sums of the rows that see them are NaN. Lane l has the marks of
@@ -291,16 +280,17 @@ struct Kv4TileRows {
 };
 
 // The codes of a key tile on their way from pages to f16 rows in LDS, by all threads of a workgroup: a thread takes 32 channels of a key or a value (16 bytes of codes and
-// their parameters), EACH of them. Page numbers are asked for two tiles ahead, codes one. Keys behind the sequence and on no page are zeros.
+// their parameters), EACH of them. Codes are asked for a tile before they are unpacked, page numbers another. Keys behind the sequence and on no page are zeros.
 template <int HD, int KT, int PITCH, int W>
 struct Kv4TileFetch {
     static constexpr int GP = HD <= 64 ? 2 : HD <= 128 ? 4 : 8;    // groups of a row, rounded up to a power of two
     static constexpr int UNITS = KT * GP;                          // of a tile of K, or of V
-    static constexpr int EACH = (2 * UNITS + 64 * W - 1) / (64 * W);
+    static constexpr int EACH = W == 8 ? 1 : 2;
+    static_assert(UNITS <= 256 && (W == 4 || W == 8), "one of each for 256 threads");
     tu4 codes[EACH];
     uint32_t params[EACH];
     bool none[EACH];   // nothing there: zeros
-    int page[EACH], block_page;   // of the tile whose codes are asked for next
+    int page[EACH], block_page;   // of the tiles asked for next
     const char *codes_at[EACH], *params_at[EACH];   // the unit's in page 0, place 0
     const int *table;
     uint64_t page_bytes;   // codes of a page; parameters are a quarter of that, wherever one looks
@@ -318,79 +308,77 @@ struct Kv4TileFetch {
             params_at[e] = static_cast<const char *>(u.value ? a.cache.v_params : a.cache.k_params) + at / 4;
         }
     }
-    // the thread's units: of eight wavefronts the lower four have the keys', the upper ones the values'
+    // the thread's units: of eight wavefronts the lower four have the keys', the upper ones the values'; of four all have one of each
     struct Unit {
         int g, r;
         bool value, any;
     };
     __device__ __forceinline__ Unit unit(int e) const {
-        const int u = W == 8 ? tid & 255 : tid + e * 64 * W;
-        const bool value = W == 8 ? tid >= 256 : u >= UNITS;
-        return {u % GP, (u / GP) % KT, value, W == 8 ? u < UNITS : u < 2 * UNITS};
+        const int u = tid & 255;
+        return {u % GP, (u / GP) % KT, W == 8 ? tid >= 256 : e == 1, u < UNITS};
     }
     // (what the table says is looked at a tile later: whether it is a page, too, so that nothing waits for it before)
     __device__ __forceinline__ int page_of(const Kv4Tiles &a, int key) const { return table[min(key >> shift, (int)a.cache.table_width - 1)]; }
     __device__ __forceinline__ bool is_page(const Kv4Tiles &a, int p, int key) const { return (uint32_t)p < (uint32_t)a.cache.n_pages && key < held; }
-    __device__ __forceinline__ void ask_pages(const Kv4Tiles &a, int tile) {
-#pragma unroll
-        for (int e = 0; e < EACH; e++) page[e] = page_of(a, tile * KT + unit(e).r);
-        block_page = page_of(a, tile * KT + 16 * (tid % (KT / 16)));
-    }
+    // (of unit e's tile)
+    __device__ __forceinline__ void ask_page(const Kv4Tiles &a, int e, int tile) { page[e] = page_of(a, tile * KT + unit(e).r); }
+    __device__ __forceinline__ void ask_blocks(const Kv4Tiles &a, int tile) { block_page = page_of(a, tile * KT + 16 * (tid % (KT / 16))); }
     // which blocks of 16 keys of the tile asked for lie on pages
     __device__ __forceinline__ uint32_t blocks_there(const Kv4Tiles &a, int tile) const {
         return (uint32_t)__ballot(is_page(a, block_page, tile * KT + 16 * (tid % (KT / 16)))) & ((1u << (KT / 16)) - 1);
     }
-    __device__ __forceinline__ void ask_codes(const Kv4Tiles &a, int tile) {
-#pragma unroll
-        for (int e = 0; e < EACH; e++) {
-            const Unit u = unit(e);
-            const int key = tile * KT + u.r;
-            const bool there = is_page(a, page[e], key) && u.any && u.g * 16 < row_bytes;
-            const uint64_t at = (uint32_t)(there ? page[e] : 0) * page_bytes + (uint64_t)(uint32_t)(key & (a.cache.page_size - 1)) * (uint32_t)row_bytes;
-            codes[e] = *reinterpret_cast<const tu4 *>(codes_at[e] + at);
-            params[e] = *reinterpret_cast<const uint32_t *>(params_at[e] + at / 4);
-            none[e] = !there;
-        }
+    __device__ __forceinline__ void ask_codes(const Kv4Tiles &a, int e, int tile) {
+        const Unit u = unit(e);
+        const int key = tile * KT + u.r;
+        const bool there = is_page(a, page[e], key) && u.any && u.g * 16 < row_bytes;
+        const uint64_t at = (uint32_t)(there ? page[e] : 0) * page_bytes + (uint64_t)(uint32_t)(key & (a.cache.page_size - 1)) * (uint32_t)row_bytes;
+        codes[e] = *reinterpret_cast<const tu4 *>(codes_at[e] + at);
+        params[e] = *reinterpret_cast<const uint32_t *>(params_at[e] + at / 4);
+        none[e] = !there;
     }
-    // odd: marks of the tile's values, a byte a unit
-    __device__ __forceinline__ void unpack(char *k, char *v, uint8_t *odd) const {
+    // into a tile of K or of V; odd: marks of the tile's values, a byte a unit
+    __device__ __forceinline__ void unpack(int e, char *to, uint8_t *odd) const {
         const Kv4Unpack take;
+        const Unit u = unit(e);
+        if (UNITS % (64 * W) != 0 && W != 8 && !u.any) return;
+        if (HD % (32 * GP) != 0 && 32 * u.g >= HD) return;   // (heads of 96 in rows of 128)
+        if (W == 8 && UNITS < 256 && !u.any) return;
+        kvh2 p = __builtin_bit_cast(kvh2, none[e] ? 0u : params[e]);
+        // a group that has a NaN, or numbers past f16's range (its values lie between code 0's and code 15's): keys are NaN, values zeros with a mark
+        const _Float16 top = __builtin_fmaf16((_Float16)15.f, p.x, p.y);
+        const bool bad = (__builtin_bit_cast(uint16_t, top) & 0x7c00) == 0x7c00;
+        p = __builtin_bit_cast(kvh2, bad ? (u.value ? 0u : 0x7e007e00u) : __builtin_bit_cast(uint32_t, p));
+        if (u.value) odd[u.r * GP + u.g] = bad;
+        char *row = to + u.r * PITCH * 2;
+        const int turn = u.value ? (u.r & 3) << 1 : u.r & 7;
 #pragma unroll
-        for (int e = 0; e < EACH; e++) {
-            const Unit u = unit(e);
-            if (!u.any || 32 * u.g >= HD) continue;   // (heads of 96 in rows of 128)
-            kvh2 p = __builtin_bit_cast(kvh2, none[e] ? 0u : params[e]);
-            // a group that has a NaN, or numbers past f16's range (its values lie between code 0's and code 15's): keys are NaN, values zeros with a mark
-            const _Float16 top = __builtin_fmaf16((_Float16)15.f, p.x, p.y);
-            const bool bad = (__builtin_bit_cast(uint16_t, top) & 0x7c00) == 0x7c00;
-            if (bad) p = __builtin_bit_cast(kvh2, u.value ? 0u : 0x7e007e00u);
-            if (u.value) odd[u.r * GP + u.g] = bad;
-            char *row = (u.value ? v : k) + u.r * PITCH * 2;
-            const int turn = u.value ? (u.r & 3) << 1 : u.r & 7;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                kvh2 x[4];
-                take(codes[e][j], kvh2{p.x, p.x}, kvh2{p.y, p.y}, x);
-                *reinterpret_cast<th8 *>(row + ((4 * u.g + j) ^ turn) * 16) = th8{x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};
-            }
+        for (int j = 0; j < 4; j++) {
+            kvh2 x[4];
+            take(codes[e][j], kvh2{p.x, p.x}, kvh2{p.y, p.y}, x);
+            *reinterpret_cast<th8 *>(row + ((4 * u.g + j) ^ turn) * 16) = th8{x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};
         }
     }
 };
 
+// AHEAD: the scores of the next tile are multiplied while those of this one become weights, so that products and softmax of one wavefront overlap; it has registers for
+// that with four wavefronts a workgroup (f16). With eight, which have a SIMD by twos, it did not pay: 2048 rows behind 30000 keys, 32 / 8 heads of 128, 1236 us, and 1207
+// in turn; with four, six prompts of up to 1024, 28 / 4 heads of 128, 40.5 us, and 44 in turn. (Nor did it pay that the two wavefronts of a SIMD took turns at multiplying, with
+// barriers in between: 1208 us; nor 64 rows a wavefront with a SIMD to itself: 1690.)
 template <int HD, int QT, int W>
 __global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_kernel(const Kv4Tiles a) {
     constexpr int C = HD > 128 ? 2 : 1, HC = HD / C;               // wavefronts of a row, channels of each
     constexpr int KT = HD > 128 ? 32 : 64;
     constexpr int PITCH = HD <= 64 ? 64 : HD <= 128 ? 128 : 256;   // halfs of an LDS row
     constexpr int TILE = KT * PITCH * 2, ROWS = 32 * W / C;
-    typedef typename std::conditional<QT == 1, _Float16, float>::type T;
-    __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];   // [buffer][K, V]
-    __shared__ float4 scores[C > 1 ? W : 1][KT / 8][64];             // a wavefront's own, for the other
     constexpr int GP = HD <= 64 ? 2 : HD <= 128 ? 4 : 8;
+    constexpr bool AHEAD = W == 4 && QT == 1;
+    typedef typename std::conditional<QT == 1, _Float16, float>::type T;
+    __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];   // [K, V][buffer]
+    __shared__ float4 scores[C > 1 ? W : 1][KT / 8][64];             // a wavefront's own, for the other
     __shared__ __attribute__((aligned(16))) uint8_t odd[2][256];     // [buffer][key][group]: values that are not all numbers
     static_assert(KT * GP <= 256, "a byte a unit");
     __shared__ int last_here;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
 
     const int heads = a.cache.n_kv_heads, kvh = (int)(blockIdx.x % heads);
     const TileSequence early(a, lane, ROWS);
@@ -409,14 +397,30 @@ __global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_
 
     const TileRow row(a, t, t.r0 + 32 * (wave / C), lane & 31, kvh);
     const int c0 = C > 1 ? (wave & 1) * HC : 0;   // the wavefront's first channel
-    auto key_tile = [&](int i) { return i < t.sink_tiles ? i : t.first + i; };
+    // (behind the last tile of this workgroup that one stands in: it is unpacked once more, and not looked at)
+    auto key_tile = [&](int i) {
+        const int j = min(i, i1 - 1);
+        return j < t.sink_tiles ? j : t.first + j;
+    };
     Kv4TileFetch<HD, KT, PITCH, W> from(a, t, kvh, tid);
-    Kv4TileRows<HC, KT, PITCH, QT> rows(a, lane, c0);
-    auto k_buffer = [&](int i) { return smem + ((i - i0) & 1) * 2 * TILE; };
-    auto v_buffer = [&](int i) { return smem + ((i - i0) & 1) * 2 * TILE + TILE; };
+    constexpr int EACH = Kv4TileFetch<HD, KT, PITCH, W>::EACH;
+    const Kv4TileReads<KT, PITCH> read(lane, c0);
+    Kv4TileRows<HC, KT, QT> rows;
+    auto k_buffer = [&](int i) { return smem + ((i - i0) & 1) * TILE; };
+    auto v_buffer = [&](int i) { return smem + 2 * TILE + ((i - i0) & 1) * TILE; };
     auto odd_buffer = [&](int i) { return odd[(i - i0) & 1]; };
-    auto masked_at = [&](int key0, uint32_t here) { return key0 + KT > row.all_end || (key0 < row.all_begin && key0 + KT > a.sinks) || here != (1u << (KT / 16)) - 1; };
-    auto active_at = [&](int key0) { return row.any && key0 < row.end && (key0 + KT > row.begin || key0 < a.sinks); };
+    auto score = [&](const char *ks, tf16 (&s)[KT / 32]) {
+#pragma unroll
+        for (int b = 0; b < KT / 32; b++) {
+            s[b] = tf16{};
+#pragma unroll
+            for (int c = 0; c < HC / 16; c++) {
+                const th8 k = read.keys(ks, b, c);
+#pragma unroll
+                for (int e = QT - 1; e >= 0; e--) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, rows.qf[c][e], s[b], 0, 0, 0);
+            }
+        }
+    };
     // what a wavefront of two that share a row has of the scores, and the other's
     auto give = [&](const tf16 (&s)[KT / 32]) {
 #pragma unroll
@@ -429,57 +433,93 @@ __global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_
             s[j / 4][j % 4 * 4] += v.x, s[j / 4][j % 4 * 4 + 1] += v.y, s[j / 4][j % 4 * 4 + 2] += v.z, s[j / 4][j % 4 * 4 + 3] += v.w;
         }
     };
-    if (tid < 128) reinterpret_cast<uint32_t *>(odd)[tid] = 0;   // (units that heads of this width do not have stay so)
-    __syncthreads();
-    uint32_t there = 0, there1 = 0;
-    if (i0 < i1) {
-        from.ask_pages(a, key_tile(i0));
-        there = from.blocks_there(a, key_tile(i0));
-        from.ask_codes(a, key_tile(i0));
-        if (i0 + 1 < i1) from.ask_pages(a, key_tile(i0 + 1));
-    }
-    rows.template queries<T>(a, t, row, c0);
-    // a tile's codes to LDS, and the codes and pages behind it asked for
-    auto carry_on = [&](int i) {
-        from.unpack(k_buffer(i), v_buffer(i), odd_buffer(i));
-        if (i + 1 < i1) {
-            there1 = from.blocks_there(a, key_tile(i + 1));
-            from.ask_codes(a, key_tile(i + 1));
-            if (i + 2 < i1) from.ask_pages(a, key_tile(i + 2));
-        }
+    // unit e's tile i to LDS, and what is behind it asked for
+    auto unpack = [&](int e, int i) {
+        from.unpack(e, from.unit(e).value ? v_buffer(i) : k_buffer(i), odd_buffer(i));
+        from.ask_codes(a, e, key_tile(i + 1));
+        from.ask_page(a, e, key_tile(i + 2));
     };
-    if (i0 < i1) carry_on(i0);
-    for (int i = i0; i < i1; i++) {
-        __syncthreads();   // this tile is there, and every wavefront is done with the other buffer
-        const uint32_t here = there;
-        there = there1;
-        const int key0 = key_tile(i) * KT;
-        const bool active = active_at(key0);
-        if (C == 1 && !active) {
-            if (i + 1 < i1) carry_on(i + 1);
-            continue;
-        }
+    // In turn i values of tile i + 1 are unpacked, and keys of tile i + 1 or (AHEAD) i + 2: into buffers whose tiles were last read in turn i - 1.
+    auto unpack_all = [&](int i) {
+#pragma unroll
+        for (int e = 0; e < EACH; e++) unpack(e, i + (AHEAD && !from.unit(e).value ? 2 : 1));
+    };
+    // keys and values that this turn reads are there, and everybody is done with the other buffers (codes on their way are not waited for)
+    auto meet = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    if (tid < 128) reinterpret_cast<uint32_t *>(odd)[tid] = 0;   // (units that heads of this width do not have stay so)
+    if (i0 < i1) {
+        from.ask_blocks(a, key_tile(i0));
+#pragma unroll
+        for (int e = 0; e < EACH; e++) from.ask_page(a, e, key_tile(i0));
+#pragma unroll
+        for (int e = 0; e < EACH; e++) from.ask_codes(a, e, key_tile(i0)), from.ask_page(a, e, key_tile(i0 + 1));
+    }
+    rows.template queries<T>(a, t, row, h, c0);
+    if (i0 < i1) {
+        meet();   // (the marks are cleared)
         tf16 s[KT / 32];
-        rows.scores(k_buffer(i), s);
-        // (the next tile's codes are unpacked while the products are on their way)
-        if (i + 1 < i1) carry_on(i + 1);
-        if (C > 1) {
-            give(s);
-            __syncthreads();
-            if (!active) continue;
-            take(s);
+#pragma unroll
+        for (int e = 0; e < EACH; e++) unpack(e, i0);
+        if (AHEAD) {
+            meet();
+            score(k_buffer(i0), s);
+            if (C > 1) give(s);
+#pragma unroll
+            for (int e = 0; e < EACH; e++)
+                if (!from.unit(e).value) unpack(e, i0 + 1);
         }
-        const bool masked = masked_at(key0, here);
-        th8 p[KT / 16][QT];
-        const uint64_t seen = masked ? row.seen(a, key0, here) : ~(uint64_t)0;
-        rows.weights(s, masked, seen, p);
-        const uint32_t marks = *reinterpret_cast<const uint32_t *>(odd_buffer(i) + 4 * lane);
-        rows.values(v_buffer(i), p);
-        if (__builtin_expect(__any(marks != 0), 0)) rows.template odd_values<GP>(marks, seen, c0);
+        for (int i = i0; i < i1; i++) {
+            const int tile = key_tile(i), key0 = tile * KT;
+            const uint32_t here = from.blocks_there(a, tile);
+            from.ask_blocks(a, key_tile(i + 1));
+            meet();
+            const bool active = row.any && key0 < row.end && (key0 + KT > row.begin || key0 < a.sinks);
+            if (!AHEAD) {
+                if (C == 1 && !active) {
+                    unpack_all(i);
+                    continue;
+                }
+                score(k_buffer(i), s);
+                unpack_all(i);   // (while the products are on their way)
+                if (C > 1) {
+                    give(s);
+                    meet();
+                    if (!active) continue;
+                }
+            }
+            if (C > 1) take(s);
+            const bool masked = key0 + KT > row.all_end || (key0 < row.all_begin && key0 + KT > a.sinks) || here != (1u << (KT / 16)) - 1;
+            uint64_t seen = ~(uint64_t)0;
+            if (masked) {
+                seen = row.seen(a, key0, here);
+                rows.hide(s, seen, h);
+            }
+            rows.rise(s);
+            th8 p[KT / 16][QT];
+            const uint32_t marks = *reinterpret_cast<const uint32_t *>(odd_buffer(i) + 4 * lane);
+            tf16 next[KT / 32];
+            if (AHEAD) score(k_buffer(i + 1), next);
+            rows.weights(s, p);
+            if (AHEAD) unpack_all(i);
+#pragma unroll
+            for (int ot = 0; ot < HC / 32; ot++)
+#pragma unroll
+                for (int u = 0; u < KT / 16; u++) {
+                    const th8 v = read.values(v_buffer(i), ot, u);
+#pragma unroll
+                    for (int e = QT - 1; e >= 0; e--) rows.o[ot] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u][e], rows.o[ot], 0, 0, 0);
+                }
+            if (__builtin_expect(__any(marks != 0), 0)) rows.template odd_values<GP>(marks, seen, c0);
+            if (AHEAD) {
+                if (C > 1) give(next);
+#pragma unroll
+                for (int b = 0; b < KT / 32; b++) s[b] = next[b];
+            }
+        }
     }
 
     const float l = tile_halves_sum(rows.l);
-    const int dim = a.cache.head_dim, h = lane >> 5;
+    const int dim = a.cache.head_dim;
     auto store = [&](int token, int head, int c, const float4 &v, float inv) {
         T *y = static_cast<T *>(a.y) + a.y_stride * (t.row0 + token) + (int64_t)head * dim + c;
         typedef T T4 __attribute__((ext_vector_type(4)));

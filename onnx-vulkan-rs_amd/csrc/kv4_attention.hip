@@ -769,7 +769,7 @@ int hipc_kv4_prompt_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const 
             if (int rc = kv4_attend<true>(ctx, a, dtype, std::min<int64_t>(cache->n_seqs, total) * blocks * cache->n_kv_heads)) return rc;
         if (!many) return HIPC_OK;
         Kv4Tiles t{};
-        t.cache = a.cache, t.q = a.q, t.y = a.y, t.q_stride = a.q_stride, t.y_stride = a.y_stride, t.starts = a.starts, t.total = a.total, t.n_q_heads = a.n_q_heads;
+        t.cache = a.cache, t.q = a.q, t.y = a.y, t.q_stride = a.q_stride, t.y_stride = a.y_stride, t.starts = a.starts, t.total = a.total;
         t.group = a.group, t.window = a.window, t.sinks = a.sinks, t.wide = a.wide, t.most = a.most, t.scale = a.scale, t.parts = a.parts, t.arrived = a.arrived;
         return kv4_tiles(ctx, t, dtype, kv4_part_bytes(ctx));
     });

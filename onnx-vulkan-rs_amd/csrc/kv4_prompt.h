@@ -12,7 +12,7 @@ struct Kv4Tiles {
     void *y;
     int64_t q_stride, y_stride;
     const int *starts;
-    int total, n_q_heads, group, window, sinks, wide;   // wide: rows of Q and Y on 16 bytes
+    int total, group, window, sinks, wide;   // wide: rows of Q and Y on 16 bytes
     int most;        // query rows (tokens times group) that a sequence has to pass to be in this part
     int slots;       // workgroups that run at once
     int splits;      // workgroups that share a tile's keys, or (not above 0) as many as tile_us and part_us say

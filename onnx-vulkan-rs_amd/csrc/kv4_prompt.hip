@@ -340,9 +340,8 @@ struct Kv4TileFetch {
     __device__ __forceinline__ void unpack(int e, char *to, uint8_t *odd) const {
         const Kv4Unpack take;
         const Unit u = unit(e);
-        if (UNITS % (64 * W) != 0 && W != 8 && !u.any) return;
+        if (UNITS < 256 && !u.any) return;
         if (HD % (32 * GP) != 0 && 32 * u.g >= HD) return;   // (heads of 96 in rows of 128)
-        if (W == 8 && UNITS < 256 && !u.any) return;
         kvh2 p = __builtin_bit_cast(kvh2, none[e] ? 0u : params[e]);
         // a group that has a NaN, or numbers past f16's range (its values lie between code 0's and code 15's): keys are NaN, values zeros with a mark
         const _Float16 top = __builtin_fmaf16((_Float16)15.f, p.x, p.y);
@@ -374,7 +373,7 @@ __global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_
     constexpr bool AHEAD = W == 4 && QT == 1;
     typedef typename std::conditional<QT == 1, _Float16, float>::type T;
     __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];   // [K, V][buffer]
-    __shared__ float4 scores[C > 1 ? W : 1][KT / 8][64];             // a wavefront's own, for the other
+    __shared__ float4 scores[C > 1 && AHEAD ? 2 : 1][C > 1 ? W : 1][KT / 8][64];   // a wavefront's own, for the other
     __shared__ __attribute__((aligned(16))) uint8_t odd[2][256];     // [buffer][key][group]: values that are not all numbers
     static_assert(KT * GP <= 256, "a byte a unit");
     __shared__ int last_here;
@@ -421,15 +420,16 @@ __global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_
             }
         }
     };
-    // what a wavefront of two that share a row has of the scores, and the other's
-    auto give = [&](const tf16 (&s)[KT / 32]) {
+    // What a wavefront of two that share a row has of tile i's scores, and the other's. (AHEAD, there is one barrier between giving and taking and none behind: the other
+    // may still take a tile's while the next one's are given.)
+    auto give = [&](int i, const tf16 (&s)[KT / 32]) {
 #pragma unroll
-        for (int j = 0; j < KT / 8; j++) scores[wave][j][lane] = make_float4(s[j / 4][j % 4 * 4], s[j / 4][j % 4 * 4 + 1], s[j / 4][j % 4 * 4 + 2], s[j / 4][j % 4 * 4 + 3]);
+        for (int j = 0; j < KT / 8; j++) scores[AHEAD ? (i - i0) & 1 : 0][wave][j][lane] = make_float4(s[j / 4][j % 4 * 4], s[j / 4][j % 4 * 4 + 1], s[j / 4][j % 4 * 4 + 2], s[j / 4][j % 4 * 4 + 3]);
     };
-    auto take = [&](tf16 (&s)[KT / 32]) {
+    auto take = [&](int i, tf16 (&s)[KT / 32]) {
 #pragma unroll
         for (int j = 0; j < KT / 8; j++) {
-            const float4 v = scores[wave ^ 1][j][lane];
+            const float4 v = scores[AHEAD ? (i - i0) & 1 : 0][wave ^ 1][j][lane];
             s[j / 4][j % 4 * 4] += v.x, s[j / 4][j % 4 * 4 + 1] += v.y, s[j / 4][j % 4 * 4 + 2] += v.z, s[j / 4][j % 4 * 4 + 3] += v.w;
         }
     };
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_
         if (AHEAD) {
             meet();
             score(k_buffer(i0), s);
-            if (C > 1) give(s);
+            if (C > 1) give(i0, s);
 #pragma unroll
             for (int e = 0; e < EACH; e++)
                 if (!from.unit(e).value) unpack(e, i0 + 1);
@@ -482,12 +482,12 @@ __global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_
                 score(k_buffer(i), s);
                 unpack_all(i);   // (while the products are on their way)
                 if (C > 1) {
-                    give(s);
+                    give(i, s);
                     meet();
                     if (!active) continue;
                 }
             }
-            if (C > 1) take(s);
+            if (C > 1) take(i, s);
             const bool masked = key0 + KT > row.all_end || (key0 < row.all_begin && key0 + KT > a.sinks) || here != (1u << (KT / 16)) - 1;
             uint64_t seen = ~(uint64_t)0;
             if (masked) {
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_
                 }
             if (__builtin_expect(__any(marks != 0), 0)) rows.template odd_values<GP>(marks, seen, c0);
             if (AHEAD) {
-                if (C > 1) give(next);
+                if (C > 1) give(i + 1, next);
 #pragma unroll
                 for (int b = 0; b < KT / 32; b++) s[b] = next[b];
             }

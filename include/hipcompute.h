@@ -546,15 +546,16 @@ int hipc_kv4_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_at
 
 /*
  * Attention of new rows of every kind over the cache: starts [n_seqs + 1] i32 on the device says which rows of Q / Y [total, n_q_heads, head_dim] (f16
- * or f32) are whose, as in hipc_kv4_append (they ascend, and are held to [0, total]): the rows of a sequence are its LAST positions, row i of n at position lengths[s] - n + i. So a
- * piece of a prompt, a whole prompt and a single token are rows of one call. A row at position p sees the keys j <= p; with heads->window > 0 of those
- * only the last `window`, its own included, and the first `sinks` of the sequence (j < sinks; 0: none). heads->causal has to be set; heads->n_kv_heads and
- * head_dim are the cache's. A row that sees nothing (a position below 0, pages that are none) is zero; rows outside every sequence are left as they are.
- * A NaN in the cache (a group that had one is stored so) makes NaN of the rows that see it and of no others; infinite parameters, which nothing stores, make
- * these NaN or infinite. The cache's values enter exactly, f16 queries
- * too, f32 queries with 22 bits of a row's largest value; weights with 22 bits; sums in f32. An infinite query makes its row NaN, or, in f16 where
- * all its scores are -inf, zero.
- * Results repeat bit for bit, with scratch memory as in hipc_kv4_attention.
+ * or f32) are whose, as in hipc_kv4_append (they ascend, and are held to [0, total]): the rows of a sequence are its LAST positions, row i of n at position
+ * lengths[s] - n + i. So a piece of a prompt, a whole prompt and a single token are rows of one call. A row at position p sees the keys j <= p; with
+ * heads->window > 0 of those only the last `window`, its own included, and the first `sinks` of the sequence (j < sinks; 0: none). heads->causal has to be
+ * set; heads->n_kv_heads and head_dim are the cache's. A row that sees nothing (a position below 0, pages that are none) is zero; rows outside every sequence
+ * are left as they are. A NaN in the cache (a group that had one is stored so) makes NaN of the rows that see it and of no others; infinite parameters, which
+ * nothing stores, make these NaN or infinite. An infinite query makes its row NaN, or, in f16 where all its scores are -inf, zero.
+ * The cache's values enter exactly, f16 queries too, f32 queries with 22 bits of a row's largest value; sums are f32. Weights, for f32 rows, have 22 bits; for f16
+ * rows, of sequences that bring many, they are rounded to f16: a weight is off by at most 2^-11 of itself, as the result is, or by 2^-32 of the row's heaviest.
+ * total * n_q_heads / n_kv_heads <= 2^30. Results repeat bit for bit for the same shapes, lengths and device, but which sequences a row stands beside may change the
+ * order of its sums. The call needs the scratch block of hipc_kv4_attention: run one of either on the context before recording one.
  */
 int hipc_kv4_prompt_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_attention_heads *heads, int32_t sinks, int dtype,
                               const void *starts, int64_t total, const void *Q, int64_t q_stride, void *Y, int64_t y_stride);

@@ -762,11 +762,19 @@ int hipc_kv4_prompt_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const 
         // behind 30000 220 / 120; 256 rows 87 / 57, 39 / 25 and 437 / 185, in f32 88 / 73, 41 / 32 and 449 / 279. 256 rows of 4 / 1 heads of 256 behind 4000 57 / 59.
         const int64_t all = total * a.group * cache->n_kv_heads;
         const bool many = ctx->tune.prompt_waves >= 4 || all > (dtype == HIPC_F16 ? 4096 : 6144);
-        a.most = many ? (cache->n_seqs == 1 ? 0 : kKv4FewRows) : 1 << 30;   // (one sequence is one kernel's)
+        // One sequence is one kernel's. So are several, where those that bring few rows cannot make the other kernel much longer: their key tiles, taken by as many workgroups
+        // as run at once, are less than the launch that finds nothing to do, and none has many more than the tiles of a prompt of a thousand. us, two kernels / one: six
+        // prompts of up to 1024, 28 / 4 heads of 128 in f16, 40 / 38; pieces of 1000 that see 512 keys, 4 / 1 heads of 256, 33 / 31; a prompt of 500 beside seven tokens
+        // behind 1200, 32 / 8 heads of 128, 33 / 30; five of 700 beside three of 5 72 / 59; four pieces of 300 beside twenty tokens that see 512, 4 / 1 heads of 256, 45 / 47.
+        const int64_t seqs = std::min<int64_t>(cache->n_seqs, total);
+        const int64_t seen = a.window > 0 ? std::min<int64_t>(cache->table_width * cache->page_size, (int64_t)a.window + a.sinks + kKv4FewRows) : cache->table_width * cache->page_size;
+        const int64_t tiles = ceil_div(seen, cache->head_dim > 128 ? 32 : 64) + 1;
+        const bool together = cache->n_seqs == 1 || (tiles <= 24 && seqs * cache->n_kv_heads * tiles <= 5 * (int64_t)ctx->cu_count);
+        a.most = many ? (together ? 0 : kKv4FewRows) : 1 << 30;
         // (where there are both kinds, sequences of few rows are taken to bring one token)
         const int64_t blocks = ceil_div((many ? 1 : ceil_div(total, cache->n_seqs)) * a.group, kKv4Rows);
         if (a.most > 0)
-            if (int rc = kv4_attend<true>(ctx, a, dtype, std::min<int64_t>(cache->n_seqs, total) * blocks * cache->n_kv_heads)) return rc;
+            if (int rc = kv4_attend<true>(ctx, a, dtype, seqs * blocks * cache->n_kv_heads)) return rc;
         if (!many) return HIPC_OK;
         Kv4Tiles t{};
         t.cache = a.cache, t.q = a.q, t.y = a.y, t.q_stride = a.q_stride, t.y_stride = a.y_stride, t.starts = a.starts, t.total = a.total;

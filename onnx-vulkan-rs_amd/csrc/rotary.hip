@@ -9,8 +9,9 @@
 // every step rounded by itself (this file is compiled without contraction): a cache stores what keys are quantized to, and one that stands next to the border
 // between two codes, or is the lowest of its group, is to fall on the side where these steps put it, whatever kernel or layout takes them.
 //
-// Memory bounds it. A wavefront has a row, or some heads of one where rows are few, and takes 64 / L heads at a time, L lanes a head; a lane has a
-// vector of V channels and the V channels they turn with, the same channels of every head it sees, so that its cosines and sines stay in registers.
+// Memory bounds it. A wavefront has a row, or some heads of one where rows are few or long, and takes 64 / L heads at a time, L lanes a head; a lane has
+// two vectors of V channels, half a rotation apart (the channels that turn with each other, or pairs that lie in one vector), the same channels of every head it sees, so that its
+// cosines and sines stay in registers. 8192 rows of 32 / 8 heads of 128: f16 33.6 us, 5.0 TB/s, f32 65.7, 5.1 (a 1 GiB copy: 4.96); 1500 of 16 / 16 heads of 96 in f32 8.0; 48 rows 4.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -23,6 +24,7 @@ namespace hipc {
 namespace {
 
 constexpr int kRotaryMaxHead = 512;
+constexpr int64_t kRotaryCaches = 32 << 20;   // bytes: the L2 caches
 
 struct RotaryArgs {
     hipc_kv4_cache cache;              // storing
@@ -104,17 +106,18 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     const int pass0 = chunk * a.per, pass1 = min(pass0 + a.per, passes);
     if (pass0 >= pass1) return;
 
-    // The lane's channels of a head: V each from c[e][0] and c[e][1] on, where there[e][.] (else the head's first stand in), and the pairs that they
-    // turn with. NEAR: neighbours turn with each other, and the two lie side by side.
-    int c[E][2], pair[E];
+    // The lane's channels of a head: V each from c[e][0] and c[e][1] on, where there[e][.] (else the head's first stand in), half a rotation apart, so that lanes side by
+    // side have vectors side by side; and whether they turn. (NEAR single channels: neighbours.)
+    constexpr bool BESIDE = NEAR && V == 1;
+    int c[E][2];
+    bool turns_here[E];
     bool there[E][2];
 #pragma unroll
     for (int e = 0; e < E; e++) {
         const int item = l + (e << a.lg_lanes), turning = a.half / V;
-        const bool turns_here = item < turning;
-        pair[e] = turns_here ? item * V : -1;
-        c[e][0] = turns_here && !NEAR ? item * V : 2 * item * V;   // (behind the pairs, 2 V an item as well)
-        c[e][1] = turns_here && !NEAR ? a.half + item * V : 2 * item * V + V;
+        turns_here[e] = item < turning;
+        c[e][0] = turns_here[e] && !BESIDE ? item * V : 2 * item * V;   // (behind the pairs, 2 V an item as well)
+        c[e][1] = turns_here[e] && !BESIDE ? a.half + item * V : 2 * item * V + V;
 #pragma unroll
         for (int h = 0; h < 2; h++) there[e][h] = c[e][h] < a.dim, c[e][h] = there[e][h] ? c[e][h] : 0;
     }
@@ -158,7 +161,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     for (int e = 0; e < E; e++)
 #pragma unroll
         for (int j = 0; j < V; j++) {
-            const float2 t = pair[e] >= 0 ? turns[wave][pair[e] + j] : make_float2(1.f, 0.f);
+            const int pair = !NEAR ? c[e][0] + j : V == 1 ? c[e][0] / 2 : j < V / 2 ? c[e][0] / 2 + j : c[e][1] / 2 + j - V / 2;
+            const float2 t = turns_here[e] ? turns[wave][pair] : make_float2(1.f, 0.f);
             cosine[e][j] = t.x, sine[e][j] = t.y;
         }
 
@@ -186,8 +190,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
             for (int j = 0; j < V; j++) {
                 const int ia = 2 * e * V + (NEAR ? 2 * j : j), ib = NEAR ? ia + 1 : ia + V;
                 const float first = v[ia] * cosine[e][j] - v[ib] * sine[e][j], second = v[ib] * cosine[e][j] + v[ia] * sine[e][j];
-                y[ia] = (T)(pair[e] >= 0 ? first : v[ia]);
-                y[ib] = (T)(pair[e] >= 0 ? second : v[ib]);
+                y[ia] = (T)(turns_here[e] ? first : v[ia]);
+                y[ib] = (T)(turns_here[e] ? second : v[ib]);
             }
     };
     auto put = [&](T *to, const T (&y)[N]) {
@@ -278,7 +282,7 @@ int rotary_launch(hipc_ctx *ctx, const char *who, RotaryArgs a, bool near) {
     const int64_t strides[5] = {a.q_stride, a.k_stride, a.v_stride, a.q_out_stride, a.k_out_stride};
     const void *rows[5] = {a.q, a.k, a.v, a.q_out, a.k_out};
     const int heads[5] = {a.n_q, a.n_kv, STORE ? a.n_kv : 0, a.n_q, STORE ? 0 : a.n_kv};
-    // vectors of eight where pairs and rows allow, of four, or single values
+    // vectors of 16 bytes where pairs and rows allow (of eight f32, two loads: 8192 rows of 32 / 8 heads of 128 69.7 us, of four 67.0), f16 ones of 8, or single values
     auto fits = [&](int v) {
         const int64_t bytes = std::min<int64_t>(v * sizeof(T), 16);
         bool ok = a.dim % v == 0 && a.half % v == 0;
@@ -293,25 +297,31 @@ int rotary_launch(hipc_ctx *ctx, const char *who, RotaryArgs a, bool near) {
         const int together = 64 >> a.lg_lanes;
         const int64_t passes = ceil_div(a.n_q, together) + ceil_div(a.n_kv, together) + (STORE ? ceil_div((int64_t)a.n_kv * a.dim, 64 * N) : 0);
         if (passes == 0) return HIPC_OK;
-        // rows that do not fill the device are shared by wavefronts (eight a CU)
-        a.chunks = (int)std::max<int64_t>(1, std::min(passes, 8 * (int64_t)ctx->cu_count / a.rows));
+        // Rows that do not fill the device are shared by wavefronts, 32 a CU (storing 16): 1500 rows of 16 / 16 heads of 96 in f32 9.0 us, by eight a CU 13.2; stored, of 32 / 8 heads
+        // of 128 in f16, 13.3, and 15.3. So are long rows of f32, in pairs of passes, however many: 8192 of 32 / 8 heads of 128 65.7 us, a wavefront each 86.8 (f16 35 and 30).
+        a.chunks = (int)std::max<int64_t>(1, std::min(passes, (STORE ? 16 : 32) * (int64_t)ctx->cu_count / a.rows));
+        if (sizeof(T) == 4 && passes > 8) a.chunks = std::max(a.chunks, (int)ceil_div(passes, 2));
         a.per = (int)ceil_div(passes, a.chunks), a.chunks = (int)ceil_div(passes, a.per);
         const int64_t groups = ceil_div((int64_t)a.rows * a.chunks, 4);
         HIPC_REFUSE(ctx, !grid_fits(groups, 256), "%s: %d rows: too many for one call", who, a.rows);
         auto run = [&](auto neighbours, auto past) {
             hipLaunchKernelGGL((rotary_kernel<T, V, decltype(neighbours)::value, STORE, decltype(past)::value>), (unsigned)groups, 256, 0, ctx->stream, a);
         };
-        // Many rows -- more than the caches near the CUs hold -- leave past these where neighbouring lanes store side by side, whole lines: 8192 rows of 32 / 8 heads of
-        // 128 in f16 33.4 us, through the caches 40.3; 48 rows 6.9 and 6.4. (In f32 a lane's values are two stores apart, and lines in parts cost: 1500 rows of 16 / 16
-        // heads of 96 18.9 us past the caches, 11.4 through them.)
-        constexpr bool LINES = sizeof(T) * V == 16 && sizeof(T) == 2;
-        if (near) run(std::true_type(), std::false_type());
-        else if (LINES && a.chunks == 1 && a.half * sizeof(T) % 128 == 0) run(std::false_type(), std::integral_constant<bool, LINES>());
-        else run(std::false_type(), std::false_type());
+        // Many rows -- more than the caches near the CUs hold -- leave past these where neighbouring lanes store side by side, whole lines: 8192 rows of 32 / 8 heads of 128 in f16
+        // 33.4 us (through the caches 40.3), in f32 86.8 (94.3); 48 rows 6.9 and 6.4.
+        constexpr bool LINES = sizeof(T) * V == 16;
+        const bool past = LINES && a.half * sizeof(T) % 128 == 0 && (int64_t)a.rows * (a.n_q + (STORE ? 0 : a.n_kv)) * a.dim * (int64_t)sizeof(T) >= kRotaryCaches;
+        auto kinds = [&](auto neighbours) {
+            if (past) run(neighbours, std::integral_constant<bool, LINES>());
+            else run(neighbours, std::false_type());
+        };
+        if (near) kinds(std::true_type());
+        else kinds(std::false_type());
         HIPC_LAUNCHED(ctx);
         return HIPC_OK;
     };
-    if (fits(8)) return launch(std::integral_constant<int, 8>());
+    if constexpr (sizeof(T) == 2)
+        if (fits(8)) return launch(std::integral_constant<int, 8>());
     if (fits(4)) return launch(std::integral_constant<int, 4>());
     return launch(std::integral_constant<int, 1>());
 }

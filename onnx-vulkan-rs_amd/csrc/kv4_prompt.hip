@@ -4,9 +4,9 @@
 //   y_i = sum_j w_ij v_j / sum_j w_ij,  w_ij = exp(scale q_i.k_j - m_i)      over the keys j that row i sees, m_i the running maximum
 //
 // The matrix cores bound it, and the vector instructions beside them: of a key tile of 64 a wavefront's 32 rows of 128 channels take 32 products of 32x32x16 and some 230 vector
-// instructions, an exponential and six others a score and a seventh of them to unpack codes. So codes become f16 once a workgroup, in LDS, not once a wavefront, and eight
-// wavefronts share them where there are rows for that. 2048 rows behind 30000 keys, 32 / 8 heads of 128 in f16: 1119 to 1207 us by card = 0.86 to 0.93 PFLOP/s (a product of
-// 8192^3: 1.21); matrix cores busy 43 % of the cycles, vector instructions 50 %, LDS 54 %. 500 rows behind 8000: 95 to 110 us. Short prompts are chains: 1.8 us a key tile, 5 to start.
+// instructions, an exponential and some five others a score and a quarter of them to unpack codes. So codes become f16 once a workgroup, in LDS, not once a wavefront, and eight
+// wavefronts share them where there are rows for that. 2048 rows behind 30000 keys, 32 / 8 heads of 128 in f16: 1110 to 1190 us by card = 0.87 to 0.94 PFLOP/s (a product of
+// 8192^3: 1.21); matrix cores busy 44 % of the cycles, vector instructions 50 %, LDS 56 %: a fragment read from LDS serves 32 rows, and takes as long as its product. 500 rows behind 8000: 95 to 110 us. Short prompts are chains: 1.8 us a key tile, 5 to start.
 #include <algorithm>
 #include <type_traits>
 
@@ -298,21 +298,22 @@ struct Kv4TileFetch {
     uint32_t params[EACH];
     bool none[EACH];   // nothing there: zeros
     int page[EACH], block_page;   // of the tiles asked for next
-    const char *codes_at[EACH], *params_at[EACH];   // the unit's in page 0, place 0
+    const tu4 *codes_at[EACH];         // the unit's in page 0, place 0
+    const uint32_t *params_at[EACH];   // ... a word beside every 16 bytes of codes, wherever one looks
     const int *table;
-    uint64_t page_bytes;   // codes of a page; parameters are a quarter of that, wherever one looks
-    int shift, row_bytes, held, tid;
+    uint32_t page_units, row_units;    // 16 bytes of codes; of a page (32 bits: where there is more than one, it holds less than 64 GB), of a row
+    int shift, held, tid;
 
     __device__ __forceinline__ Kv4TileFetch(const Kv4Tiles &a, const Tile &t, int kvh, int tid_) : tid(tid_) {
         table = static_cast<const int *>(a.cache.table) + (int64_t)t.seq * a.cache.table_width;
-        shift = 31 - __builtin_clz((unsigned)a.cache.page_size), row_bytes = a.cache.head_dim / 2, held = kv4_held(a.cache, t.length);
-        page_bytes = (uint64_t)(a.cache.n_kv_heads * (int64_t)row_bytes) << shift;
+        shift = 31 - __builtin_clz((unsigned)a.cache.page_size), row_units = a.cache.head_dim / 32, held = kv4_held(a.cache, t.length);
+        page_units = (uint32_t)((uint64_t)(a.cache.n_kv_heads * row_units) << shift);
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
             const Unit u = unit(e);
-            const int64_t at = ((int64_t)kvh * row_bytes << shift) + (u.g * 16 < row_bytes ? u.g * 16 : 0);
-            codes_at[e] = static_cast<const char *>(u.value ? a.cache.v_codes : a.cache.k_codes) + at;
-            params_at[e] = static_cast<const char *>(u.value ? a.cache.v_params : a.cache.k_params) + at / 4;
+            const int64_t at = ((int64_t)kvh * row_units << shift) + (u.g < (int)row_units ? u.g : 0);
+            codes_at[e] = static_cast<const tu4 *>(u.value ? a.cache.v_codes : a.cache.k_codes) + at;
+            params_at[e] = static_cast<const uint32_t *>(u.value ? a.cache.v_params : a.cache.k_params) + at;
         }
     }
     // the thread's units: of eight wavefronts the lower four have the keys', the upper ones the values'; of four all have one of each
@@ -325,7 +326,10 @@ struct Kv4TileFetch {
         return {u % GP, (u / GP) % KT, W == 8 ? tid >= 256 : e == 1, u < UNITS};
     }
     // (what the table says is looked at a tile later: whether it is a page, too, so that nothing waits for it before)
-    __device__ __forceinline__ int page_of(const Kv4Tiles &a, int key) const { return table[min(key >> shift, (int)a.cache.table_width - 1)]; }
+    __device__ __forceinline__ int page_of(const Kv4Tiles &a, int key) const {
+        const uint32_t at = (uint32_t)min(key >> shift, (int)a.cache.table_width - 1) * 4;   // (tables have up to 2^26 pages)
+        return *reinterpret_cast<const int *>(reinterpret_cast<const char *>(table) + at);
+    }
     __device__ __forceinline__ bool is_page(const Kv4Tiles &a, int p, int key) const { return (uint32_t)p < (uint32_t)a.cache.n_pages && key < held; }
     // (of unit e's tile)
     __device__ __forceinline__ void ask_page(const Kv4Tiles &a, int e, int tile) { page[e] = page_of(a, tile * KT + unit(e).r); }
@@ -337,10 +341,10 @@ struct Kv4TileFetch {
     __device__ __forceinline__ void ask_codes(const Kv4Tiles &a, int e, int tile) {
         const Unit u = unit(e);
         const int key = tile * KT + u.r;
-        const bool there = is_page(a, page[e], key) && u.any && u.g * 16 < row_bytes;
-        const uint64_t at = (uint32_t)(there ? page[e] : 0) * page_bytes + (uint64_t)(uint32_t)(key & (a.cache.page_size - 1)) * (uint32_t)row_bytes;
-        codes[e] = *reinterpret_cast<const tu4 *>(codes_at[e] + at);
-        params[e] = *reinterpret_cast<const uint32_t *>(params_at[e] + at / 4);
+        const bool there = is_page(a, page[e], key) && u.any && u.g < (int)row_units;
+        const uint64_t at = (uint64_t)(uint32_t)(there ? page[e] : 0) * page_units + (uint64_t)(uint32_t)(key & (a.cache.page_size - 1)) * row_units;
+        codes[e] = codes_at[e][at];
+        params[e] = params_at[e][at];
         none[e] = !there;
     }
     // into a tile of K or of V; odd: marks of the tile's values, a byte a unit

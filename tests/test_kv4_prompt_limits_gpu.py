@@ -189,3 +189,25 @@ def test_a_cache_without_pages(ctx, pkg):
     assert np.array_equal(bits(got[:43]), bits(want)) and np.all(got[43:] == 1)
     for b in (lengths, starts, dQ, dY):
         b.free()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
+@pytest.mark.parametrize("waves", [1, 4, 8])
+@pytest.mark.parametrize("q_heads,kv,dim", [(4, 2, 64), (2, 1, 128), (4, 1, 256)], ids=str)
+def test_queries_that_are_no_numbers(ctx, pkg, dtype, waves, q_heads, kv, dim):
+    """A head's row with a NaN or infinities is NaN (in f16, where every score is -inf, zero), a row that sees nothing is zero all the same, and every other row is as before."""
+    c = case(ctx, pkg, [140, 30], 16, kv, dim)
+    new = [90, 40]                                        # (the second sequence's first ten rows lie in front of it)
+    q = c.rng.standard_normal((130, q_heads, dim)).astype(dtype)
+    bad = q.copy()
+    odd = {(3, 0): np.nan, (17, 1): np.inf, (60, 0): -np.inf, (89, 1): np.nan, (93, 0): np.nan, (95, 1): np.inf, (129, 1): -np.inf}
+    for (row, head), x in odd.items():
+        bad[row, head, 5] = x
+    with ctx.options(HIPC_PROMPT_WAVES=waves):
+        clean, got = c.gpu.prompt_attention(q, new), c.gpu.prompt_attention(bad, new)
+    for row, head in odd:
+        y = got[row, head]
+        assert not y.any() if row in (93, 95) else np.isnan(y).all() or (dtype == np.float16 and not y.any())
+        got[row, head] = clean[row, head]
+    assert np.array_equal(bits(got), bits(clean)) and not clean[90:100].any()
+    c.gpu.free()

@@ -5,6 +5,7 @@ import threading
 import numpy as np
 import pytest
 
+from oracle import attention as ref
 from test_kv4_gpu import Pair, bits
 from test_kv4_prompt_gpu import case, starts_of
 from test_rotary_gpu import table as frequencies
@@ -210,4 +211,27 @@ def test_queries_that_are_no_numbers(ctx, pkg, dtype, waves, q_heads, kv, dim):
         assert not y.any() if row in (93, 95) else np.isnan(y).all() or (dtype == np.float16 and not y.any())
         got[row, head] = clean[row, head]
     assert np.array_equal(bits(got), bits(clean)) and not clean[90:100].any()
+    c.gpu.free()
+
+
+@pytest.mark.parametrize("waves", [1, 4, 8])
+@pytest.mark.parametrize("q_heads,kv,dim", [(4, 2, 64), (4, 1, 128), (2, 1, 256)], ids=str)
+@pytest.mark.parametrize("scale", [0.0, 1.0, 1e-30, -1e-38, 3e-45])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 3)], ids=str)
+def test_queries_and_scales_of_next_to_nothing(ctx, pkg, waves, q_heads, kv, dim, scale, window, sinks):
+    """f32 rows down to the least number there is beside ordinary ones, with scales as small: scores of 0 to working precision make a row the mean of what it sees. The tolerance is
+    test_kv4_prompt_gpu.py's for f32, with this scale in the place of 1 / sqrt(dim)."""
+    c = case(ctx, pkg, [130, 65, 7], 32, kv, dim)
+    new = [70, 33, 7]
+    q = c.rng.standard_normal((110, q_heads, dim))
+    sizes = np.array([0.0, 1e-45, 1e-42, 1e-39, 1e-35, 1e-20, 1.0])
+    q = (q * sizes[np.arange(110 * q_heads) % len(sizes)].reshape(110, q_heads, 1)).astype(np.float32)
+    with ctx.options(HIPC_PROMPT_WAVES=waves):
+        got = c.gpu.prompt_attention(q, new, window, sinks, scale)
+    want, weight, size, most = c.ref.prompt_attention(q, starts_of(new), c.lengths, window, sinks, scale or None)
+    k_most = max(float(np.abs(ref.values(np.full((1, 1, 1), code, np.uint8), p[..., :1], p[..., 1:])).max()) for p in (c.ref.params[0].reshape(-1, 1, 2),) for code in (0, 15))
+    relative = 2 * (dim + 2) * 2.0 ** -24 * size + (16 + 130) * 2.0 ** -24 + 2.0 ** -22
+    relative = relative + 2 * 2.0 ** -22 * np.abs(q.astype(np.float64)).max(-1, keepdims=True) * dim * k_most * (abs(scale) or 1 / np.sqrt(dim))
+    off = np.abs(got.astype(np.float64) - want) - (weight * relative + 130 * 2.0 ** -32 * most + 1e-37)
+    assert np.all(off <= 0), (float(off.max()), np.unravel_index(np.argmax(off), off.shape))
     c.gpu.free()

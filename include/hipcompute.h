@@ -438,7 +438,7 @@ int hipc_rotary_frequencies(double theta, int32_t rotary_dim, const hipc_rotary_
  * rows, for instance), to Q_out and K_out; these may be Q and K themselves (same address and stride) and else overlap nothing.
  * positions [rows] i32 on the device, of any sign (a key that is to stand n positions earlier is turned by -n). Angles are
  * formed in 64 bits, a position's product with the f32 frequency off by less than 2^-51 of itself; the rest is f32, every step rounded by itself
- * (sum of squares, mean, + norm_eps, reciprocal root; x times that, times w; A cos and A sin; two products and their sum), the result once to the rows' type.
+ * (sum of squares, mean, + norm_eps, reciprocal root to half a step; x times that, times w; A cos and A sin; two products and their sum), the result once to the rows' type.
  */
 int hipc_rotary(hipc_ctx *ctx, const hipc_rotary_heads *heads, int dtype, const void *positions, int64_t rows, const void *Q, int64_t q_stride,
                 const void *K, int64_t k_stride, void *Q_out, int64_t q_out_stride, void *K_out, int64_t k_out_stride);

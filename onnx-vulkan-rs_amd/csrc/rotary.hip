@@ -11,7 +11,7 @@
 //
 // Memory bounds it. A wavefront has a row, or some heads of one where rows are few or long, and takes 64 / L heads at a time, L lanes a head; a lane has
 // two vectors of V channels, half a rotation apart (the channels that turn with each other, or pairs that lie in one vector), the same channels of every head it sees, so that its
-// cosines and sines stay in registers. 8192 rows of 32 / 8 heads of 128: f16 33.6 us, 5.0 TB/s, f32 65.7, 5.1 (a 1 GiB copy: 4.96); 1500 of 16 / 16 heads of 96 in f32 8.0; 48 rows 4.
+// cosines and sines stay in registers. 8192 rows of 32 / 8 heads of 128: f16 34.7 us, 4.8 TB/s, f32 65.7, 5.1 (a 1 GiB copy: 4.96); 1500 of 16 / 16 heads of 96 in f32 8.0; 48 rows 4.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -47,6 +47,12 @@ __device__ __forceinline__ float lanes_sum(float v, int lg) {
     if (lg > 4) v += __shfl_xor(v, 16);
     if (lg > 5) v += __shfl_xor(v, 32);
     return v;
+}
+
+// 1 / sqrt(x) to half a step and a little: the function's step of error goes with one Newton step whose remainder, 1 - x y^2, is formed without rounding x y
+__device__ __forceinline__ float reciprocal_root(float x) {
+    const float y = rsqrtf(x), root = x * y, low = __builtin_fmaf(x, y, -root), rest = __builtin_fmaf(-low, y, __builtin_fmaf(-root, y, 1.f));
+    return x > 0.f && x < INFINITY ? __builtin_fmaf(0.5f * y, rest, y) : y;
 }
 
 // V values side by side; rows and strides lie on 16 bytes (V values, where these are less) or V is 1
@@ -172,15 +178,26 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] = (float)x[i];
         if (norm) {
-            float sum = 0.f;
+            // squares four side by side, then neighbours by twos: an error that grows with the logarithm, and (whole heads turn, V > 1) the same order whatever the vectors'
+            // width; a plain form in PyTorch has the same sums to the bit at 128 and 256 channels, so that it and a cache filled here agree in their codes
+            float part[2] = {0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 2 * E; i++) {
-                float part = v[i * V] * v[i * V];
+            for (int e = 0; e < E; e++) {
+                float p[2];
 #pragma unroll
-                for (int j = 1; j < V; j++) part += v[i * V + j] * v[i * V + j];
-                sum += there[i / 2][i % 2] ? part : 0.f;
+                for (int h = 0; h < 2; h++) {
+                    float quads[(V + 3) / 4];
+#pragma unroll
+                    for (int i = 0; i < V; i++) {
+                        const float x = v[(2 * e + h) * V + i], square = x * x;
+                        quads[i / 4] = i % 4 ? quads[i / 4] + square : square;
+                    }
+                    p[h] = there[e][h] ? (V == 8 ? quads[0] + quads[V / 8] : quads[0]) : 0.f;
+                }
+                part[0] += turns_here[e] ? p[0] : p[0] + p[1], part[1] += turns_here[e] ? p[1] : 0.f;
             }
-            const float by = rsqrtf(lanes_sum(sum, a.lg_lanes) / (float)a.dim + a.eps);
+            const float sum = lanes_sum(part[0], a.lg_lanes) + lanes_sum(part[1], a.lg_lanes);
+            const float by = reciprocal_root(sum / (float)a.dim + a.eps);
 #pragma unroll
             for (int i = 0; i < N; i++) v[i] = v[i] * by * weight[i];
         }

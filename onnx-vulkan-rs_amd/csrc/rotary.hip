@@ -11,7 +11,7 @@
 //
 // Memory bounds it. A wavefront has a row, or some heads of one where rows are few or long, and takes 64 / L heads at a time, L lanes a head; a lane has
 // two vectors of V channels, half a rotation apart (the channels that turn with each other, or pairs that lie in one vector), the same channels of every head it sees, so that its
-// cosines and sines stay in registers. 8192 rows of 32 / 8 heads of 128: f16 34.7 us, 4.8 TB/s, f32 65.7, 5.1 (a 1 GiB copy: 4.96); 1500 of 16 / 16 heads of 96 in f32 8.0; 48 rows 4.
+// cosines and sines stay in registers. 8192 rows of 32 / 8 heads of 128: f16 33.1 to 34.7 us by card, 5.0 TB/s, f32 65.7, 5.1 (a 1 GiB copy: 4.96); 1500 of 16 / 16 heads of 96 in f32 8.0; 48 rows 4.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -34,19 +34,28 @@ struct RotaryArgs {
     int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
     const float *frequencies, *q_norm, *k_norm;
     int rows, n_q, n_kv, dim, half;
-    int lg_lanes, chunks, per;         // lanes of a head (a power of two); wavefronts of a row, and what each takes of it
+    int lg_lanes, lg_turning, chunks, per;   // lanes of a head (a power of two) and of its channels that turn; wavefronts of a row, and what each takes of it
     float eps, amplitude;
 };
 
-// the sum over 2^lg neighbouring lanes, in all of them (lg is uniform)
-__device__ __forceinline__ float lanes_sum(float v, int lg) {
-    if (lg > 0) v += lean_dpp<0xB1>(v);    // quad_perm [1,0,3,2]
-    if (lg > 1) v += lean_dpp<0x4E>(v);    // quad_perm [2,3,0,1]
-    if (lg > 2) v += lean_dpp<0x141>(v);   // the other four of eight (mirrored)
-    if (lg > 3) v += lean_dpp<0x140>(v);   // the other eight of sixteen
-    if (lg > 4) v += __shfl_xor(v, 16);
-    if (lg > 5) v += __shfl_xor(v, 32);
-    return v;
+// The sum of x and y over 2^lanes neighbouring lanes, in all of them: over 2^part of x, over as many of y, these two, and then the others' (both numbers are uniform).
+__device__ __forceinline__ float lanes_sum(float x, float y, int part, int lanes) {
+    if (part > 0) x += lean_dpp<0xB1>(x), y += lean_dpp<0xB1>(y);      // quad_perm [1,0,3,2]
+    if (part > 1) x += lean_dpp<0x4E>(x), y += lean_dpp<0x4E>(y);      // quad_perm [2,3,0,1]
+    if (part > 2) x += lean_dpp<0x141>(x), y += lean_dpp<0x141>(y);    // the other four of eight (mirrored)
+    if (part > 3) x += lean_dpp<0x140>(x), y += lean_dpp<0x140>(y);    // the other eight of sixteen
+    if (part > 4) x += __shfl_xor(x, 16), y += __shfl_xor(y, 16);
+    if (part > 5) x += __shfl_xor(x, 32), y += __shfl_xor(y, 32);
+    x += y;
+    if (part < lanes) {
+        if (part < 1) x += lean_dpp<0xB1>(x);
+        if (part < 2 && lanes > 1) x += lean_dpp<0x4E>(x);
+        if (part < 3 && lanes > 2) x += lean_dpp<0x141>(x);
+        if (part < 4 && lanes > 3) x += lean_dpp<0x140>(x);
+        if (part < 5 && lanes > 4) x += __shfl_xor(x, 16);
+        if (lanes > 5) x += __shfl_xor(x, 32);
+    }
+    return x;
 }
 
 // 1 / sqrt(x) to half a step and a little: the function's step of error goes with one Newton step whose remainder, 1 - x y^2, is formed without rounding x y
@@ -178,8 +187,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] = (float)x[i];
         if (norm) {
-            // squares four side by side, then neighbours by twos: an error that grows with the logarithm, and (whole heads turn, V > 1) the same order whatever the vectors'
-            // width; a plain form in PyTorch has the same sums to the bit at 128 and 256 channels, so that it and a cache filled here agree in their codes
+            // squares four side by side, then neighbours by twos: an error that grows with the logarithm, and (V > 1, powers of two) the same order whatever the vectors'
+            // width and however many channels turn; a plain form in PyTorch has the same sums to the bit at 128 and 256 channels, so that it and a cache filled here agree in their codes
             float part[2] = {0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < E; e++) {
@@ -196,7 +205,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
                 }
                 part[0] += turns_here[e] ? p[0] : p[0] + p[1], part[1] += turns_here[e] ? p[1] : 0.f;
             }
-            const float sum = lanes_sum(part[0], a.lg_lanes) + lanes_sum(part[1], a.lg_lanes);
+            const float sum = lanes_sum(part[0], part[1], a.lg_turning, a.lg_lanes);
             const float by = reciprocal_root(sum / (float)a.dim + a.eps);
 #pragma unroll
             for (int i = 0; i < N; i++) v[i] = v[i] * by * weight[i];
@@ -311,6 +320,7 @@ int rotary_launch(hipc_ctx *ctx, const char *who, RotaryArgs a, bool near) {
         constexpr int V = decltype(width)::value, N = 2 * V * (V == 1 ? 4 : 1);
         const int items = (int)(a.half / V + ceil_div(a.dim - 2 * a.half, 2 * V));
         while (a.lg_lanes < 6 && 1 << a.lg_lanes < items) a.lg_lanes++;
+        while (a.lg_turning < a.lg_lanes && 1 << a.lg_turning < a.half / V) a.lg_turning++;
         const int together = 64 >> a.lg_lanes;
         const int64_t passes = ceil_div(a.n_q, together) + ceil_div(a.n_kv, together) + (STORE ? ceil_div((int64_t)a.n_kv * a.dim, 64 * N) : 0);
         if (passes == 0) return HIPC_OK;

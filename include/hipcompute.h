@@ -552,8 +552,8 @@ int hipc_kv4_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hipc_at
  * set; heads->n_kv_heads and head_dim are the cache's. A row that sees nothing (a position below 0, pages that are none) is zero; rows outside every sequence
  * are left as they are. A NaN in the cache (a group that had one is stored so) makes NaN of the rows that see it and of no others; infinite parameters, which
  * nothing stores, make these NaN or infinite. An infinite query makes its row NaN, or, in f16 where all its scores are -inf, zero.
- * The cache's values enter exactly, f16 queries too, f32 queries with 22 bits of a row's largest value; sums are f32. Weights, for f32 rows, have 22 bits; for f16
- * rows, of sequences that bring many, they are rounded to f16: a weight is off by at most 2^-11 of itself, as the result is, or by 2^-32 of the row's heaviest.
+ * The cache's values enter exactly, f16 queries too, f32 queries with 22 bits of a row's largest value; sums are f32. Weights have 22 bits, and no less than 2^-32 of the
+ * row's heaviest, whatever rows stand beside a row.
  * total * n_q_heads / n_kv_heads <= 2^30. Results repeat bit for bit for the same shapes, lengths and device, but which sequences a row stands beside may change the
  * order of its sums. The call needs the scratch block of hipc_kv4_attention: run one of either on the context before recording one.
  */

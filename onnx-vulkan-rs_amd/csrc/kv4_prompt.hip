@@ -3,10 +3,10 @@
 //
 //   y_i = sum_j w_ij v_j / sum_j w_ij,  w_ij = exp(scale q_i.k_j - m_i)      over the keys j that row i sees, m_i the running maximum
 //
-// The matrix cores bound it, and the vector instructions beside them: of a key tile of 64 a wavefront's 32 rows of 128 channels take 32 products of 32x32x16 and some 230 vector
-// instructions, an exponential and some five others a score and a quarter of them to unpack codes. So codes become f16 once a workgroup, in LDS, not once a wavefront, and eight
-// wavefronts share them where there are rows for that. 2048 rows behind 30000 keys, 32 / 8 heads of 128 in f16: 1110 to 1190 us by card = 0.87 to 0.94 PFLOP/s (a product of
-// 8192^3: 1.21); matrix cores busy 44 % of the cycles, vector instructions 50 %, LDS 56 %: a fragment read from LDS serves 32 rows, and takes as long as its product. 500 rows behind 8000: 95 to 110 us. Short prompts are chains: 1.8 us a key tile, 5 to start.
+// The matrix cores bound it: of a key tile of 64 a wavefront's 32 rows of 128 channels take 48 products of 32x32x16 -- weights enter as two terms each -- beside some 290 vector
+// instructions, an exponential and some six others a score and a quarter of them to unpack codes. So codes become f16 once a workgroup, in LDS, not once a wavefront, and eight
+// wavefronts share them where there are rows for that. 2048 rows behind 30000 keys, 32 / 8 heads of 128 in f16: 1500 us, 0.69 PFLOP/s of the operation's, 1.04 of the products that it takes
+// (a product of 8192^3: 1.21). 500 rows behind 8000: 120 us. Short prompts are chains: 2.4 us a key tile, 5 to start.
 #include <algorithm>
 #include <type_traits>
 
@@ -185,8 +185,9 @@ struct Kv4TileReads {
 //   O^T = V^T P^T    the lane's weights are the second operand as they lie; V^T is read from row-major LDS rows by the transposing loads
 // so maximum, sum and rescale of the softmax are numbers of one lane, exchanged once between the two halves of the wavefront.
 // The running maximum may grow by 2^8 before sums are rescaled, and weights are kept 2^7 times as large: f16's ordinary numbers then reach down to 2^-21 of the
-// heaviest weight, its subnormal ones to 2^-31. QT = 1, f16 rows: queries as they are, weights rounded to f16 (as two terms they would be half as many
-// products again of a kernel that these bound; the result's own rounding is as large). QT = 2, f32 rows: two f16 terms each, of the row times a power of two, and of the weight.
+// heaviest weight, its subnormal ones to 2^-31. A weight enters as two f16 terms, 22 bits, as it does in the kernel for few rows: which of the two takes a row is decided by
+// the rows beside it, and is not to be seen in the result. (One term a weight: errors 1.02 to 1.2 times those of the result's own rounding; 2048 rows behind 30000 keys 1128 us, two
+// 1500.) QT = 1, f16 rows: queries as they are. QT = 2, f32 rows: two f16 terms of the row times a power of two.
 // The eight channels of a word of codes lie in the order in which it unpacks, 0 4 1 5 2 6 3 7, in K's rows, V's and the queries alike.
 template <int HC, int KT, int QT>
 struct Kv4TileRows {
@@ -262,7 +263,9 @@ struct Kv4TileRows {
                 for (int r = 0; r < 16; r++) o[i][r] *= keep;
         }
     }
-    __device__ __forceinline__ void weights(const tf16 (&s)[KT / 32], th8 (&p)[KT / 16][QT]) {
+    __device__ __forceinline__ void weights(const tf16 (&s)[KT / 32], th8 (&p)[KT / 16][2]) {
+        float one = 1.f;
+        HIPC_PIN_SGPR(one);   // (a product with it, not a subtraction: one instruction takes the f16 term as it is)
 #pragma unroll
         for (int u = 0; u < KT / 16; u++)
 #pragma unroll
@@ -272,12 +275,8 @@ struct Kv4TileRows {
                               __builtin_amdgcn_exp2f(__builtin_fmaf(s[u / 2][8 * (u & 1) + j + 1], c2, -down))};
                 const th2 hi = __builtin_convertvector(w, th2);
                 p[u][0][j] = hi.x, p[u][0][j + 1] = hi.y;
-                if (QT == 1) {   // the sum is that of the same rounded weights
-                    l = __builtin_amdgcn_fdot2(hi, th2{(_Float16)1.f, (_Float16)1.f}, l, false);
-                } else {
-                    l += w.x + w.y;
-                    p[u][QT - 1][j] = (_Float16)(w.x - (float)hi.x), p[u][QT - 1][j + 1] = (_Float16)(w.y - (float)hi.y);
-                }
+                l += w.x + w.y;
+                p[u][1][j] = (_Float16)__builtin_fmaf(-(float)hi.x, one, w.x), p[u][1][j + 1] = (_Float16)__builtin_fmaf(-(float)hi.y, one, w.y);
             }
     }
     // Groups of values that are not all numbers are zeros in the product (zero times a NaN is none): the sums of the rows that see them are NaN. Lane l has the marks of
@@ -389,10 +388,8 @@ struct Kv4TileFetch {
     }
 };
 
-// AHEAD: the scores of the next tile are multiplied while those of this one become weights, so that products and softmax of one wavefront overlap; it has registers for
-// that with four wavefronts a workgroup (f16). With eight, which have a SIMD by twos, it did not pay: 2048 rows behind 30000 keys, 32 / 8 heads of 128, 1236 us, and 1207
-// in turn; with four, six prompts of up to 1024, 28 / 4 heads of 128, 40.5 us, and 44 in turn. (Nor did it pay that the two wavefronts of a SIMD took turns at multiplying, with
-// barriers in between: 1208 us; nor 64 rows a wavefront with a SIMD to itself: 1690.)
+// (Four wavefronts, the next tile's scores multiplied while this one's become weights: six prompts of up to 1024, 28 / 4 heads of 128 in f16, 46.0 us, in turn 43.8. Nor did it pay that
+// the two wavefronts of a SIMD took turns at multiplying, with barriers in between, or that one had 64 rows and a SIMD to itself.)
 template <int HD, int QT, int W>
 __global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_kernel(const Kv4Tiles a) {
     constexpr int C = HD > 128 ? 2 : 1, HC = HD / C;               // wavefronts of a row, channels of each
@@ -400,10 +397,9 @@ __global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_
     constexpr int PITCH = HD <= 64 ? 64 : HD <= 128 ? 128 : 256;   // halfs of an LDS row
     constexpr int TILE = KT * PITCH * 2, ROWS = 32 * W / C;
     constexpr int GP = HD <= 64 ? 2 : HD <= 128 ? 4 : 8;
-    constexpr bool AHEAD = W == 4 && QT == 1;
     typedef typename std::conditional<QT == 1, _Float16, float>::type T;
     __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];   // [K, V][buffer]
-    __shared__ float4 scores[C > 1 && AHEAD ? 2 : 1][C > 1 ? W : 1][KT / 8][64];   // a wavefront's own, for the other
+    __shared__ float4 scores[C > 1 ? W : 1][KT / 8][64];             // a wavefront's own, for the other
     __shared__ __attribute__((aligned(16))) uint8_t odd[2][256];     // [buffer][key][group]: values that are not all numbers
     static_assert(KT * GP <= 256, "a byte a unit");
     __shared__ int last_here;
@@ -450,16 +446,15 @@ __global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_
             }
         }
     };
-    // What a wavefront of two that share a row has of tile i's scores, and the other's. (AHEAD, there is one barrier between giving and taking and none behind: the other
-    // may still take a tile's while the next one's are given.)
-    auto give = [&](int i, const tf16 (&s)[KT / 32]) {
+    // what a wavefront of two that share a row has of a tile's scores, and the other's
+    auto give = [&](const tf16 (&s)[KT / 32]) {
 #pragma unroll
-        for (int j = 0; j < KT / 8; j++) scores[AHEAD ? (i - i0) & 1 : 0][wave][j][lane] = make_float4(s[j / 4][j % 4 * 4], s[j / 4][j % 4 * 4 + 1], s[j / 4][j % 4 * 4 + 2], s[j / 4][j % 4 * 4 + 3]);
+        for (int j = 0; j < KT / 8; j++) scores[wave][j][lane] = make_float4(s[j / 4][j % 4 * 4], s[j / 4][j % 4 * 4 + 1], s[j / 4][j % 4 * 4 + 2], s[j / 4][j % 4 * 4 + 3]);
     };
-    auto take = [&](int i, tf16 (&s)[KT / 32]) {
+    auto take = [&](tf16 (&s)[KT / 32]) {
 #pragma unroll
         for (int j = 0; j < KT / 8; j++) {
-            const float4 v = scores[AHEAD ? (i - i0) & 1 : 0][wave ^ 1][j][lane];
+            const float4 v = scores[wave ^ 1][j][lane];
             s[j / 4][j % 4 * 4] += v.x, s[j / 4][j % 4 * 4 + 1] += v.y, s[j / 4][j % 4 * 4 + 2] += v.z, s[j / 4][j % 4 * 4 + 3] += v.w;
         }
     };
@@ -469,10 +464,10 @@ __global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_
         from.ask_codes(a, e, key_tile(i + 1));
         from.ask_page(a, e, key_tile(i + 2));
     };
-    // In turn i values of tile i + 1 are unpacked, and keys of tile i + 1 or (AHEAD) i + 2: into buffers whose tiles were last read in turn i - 1.
+    // In turn i tile i + 1 is unpacked: into buffers whose tiles were last read in turn i - 1.
     auto unpack_all = [&](int i) {
 #pragma unroll
-        for (int e = 0; e < EACH; e++) unpack(e, i + (AHEAD && !from.unit(e).value ? 2 : 1));
+        for (int e = 0; e < EACH; e++) unpack(e, i + 1);
     };
     // keys and values that this turn reads are there, and everybody is done with the other buffers (codes on their way are not waited for)
     auto meet = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
@@ -487,37 +482,27 @@ __global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_
     rows.template queries<T>(a, t, row, h, c0);
     if (i0 < i1) {
         meet();   // (the marks are cleared)
-        tf16 s[KT / 32];
 #pragma unroll
         for (int e = 0; e < EACH; e++) unpack(e, i0);
-        if (AHEAD) {
-            meet();
-            score(k_buffer(i0), s);
-            if (C > 1) give(i0, s);
-#pragma unroll
-            for (int e = 0; e < EACH; e++)
-                if (!from.unit(e).value) unpack(e, i0 + 1);
-        }
         for (int i = i0; i < i1; i++) {
             const int tile = key_tile(i), key0 = tile * KT;
             const uint32_t here = from.blocks_there(a, tile);
             from.ask_blocks(a, key_tile(i + 1));
             meet();
             const bool active = row.any && key0 < row.end && (key0 + KT > row.begin || key0 < a.sinks);
-            if (!AHEAD) {
-                if (C == 1 && !active) {
-                    unpack_all(i);
-                    continue;
-                }
-                score(k_buffer(i), s);
-                unpack_all(i);   // (while the products are on their way)
-                if (C > 1) {
-                    give(i, s);
-                    meet();
-                    if (!active) continue;
-                }
+            if (C == 1 && !active) {
+                unpack_all(i);
+                continue;
             }
-            if (C > 1) take(i, s);
+            tf16 s[KT / 32];
+            score(k_buffer(i), s);
+            unpack_all(i);   // (while the products are on their way)
+            if (C > 1) {
+                give(s);
+                meet();   // (and the next turn's barrier keeps the next scores from being given before these are taken)
+                if (!active) continue;
+                take(s);
+            }
             const bool masked = key0 + KT > row.all_end || (key0 < row.all_begin && key0 + KT > a.sinks) || here != (1u << (KT / 16)) - 1;
             uint64_t seen = ~(uint64_t)0;
             if (masked) {
@@ -525,26 +510,18 @@ __global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_
                 rows.hide(s, seen, h);
             }
             rows.rise(s);
-            th8 p[KT / 16][QT];
+            th8 p[KT / 16][2];
             const uint32_t marks = *reinterpret_cast<const uint32_t *>(odd_buffer(i) + 4 * lane);
-            tf16 next[KT / 32];
-            if (AHEAD) score(k_buffer(i + 1), next);
             rows.weights(s, p);
-            if (AHEAD) unpack_all(i);
 #pragma unroll
             for (int ot = 0; ot < HC / 32; ot++)
 #pragma unroll
                 for (int u = 0; u < KT / 16; u++) {
                     const th8 v = read.values(v_buffer(i), ot, u);
 #pragma unroll
-                    for (int e = QT - 1; e >= 0; e--) rows.o[ot] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u][e], rows.o[ot], 0, 0, 0);
+                    for (int e = 1; e >= 0; e--) rows.o[ot] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u][e], rows.o[ot], 0, 0, 0);
                 }
             if (__builtin_expect(__any(marks != 0), 0)) rows.template odd_values<GP>(marks, seen, c0);
-            if (AHEAD) {
-                if (C > 1) give(i + 1, next);
-#pragma unroll
-                for (int b = 0; b < KT / 32; b++) s[b] = next[b];
-            }
         }
     }
 

@@ -390,8 +390,10 @@ struct Kv4TileFetch {
 
 // (Four wavefronts, the next tile's scores multiplied while this one's become weights: six prompts of up to 1024, 28 / 4 heads of 128 in f16, 46.0 us, in turn 43.8. Nor did it pay that
 // the two wavefronts of a SIMD took turns at multiplying, with barriers in between, or that one had 64 rows and a SIMD to itself.)
+// Workgroups that a CU runs at once: two wavefronts a SIMD, but one where heads are wider than 128 and four wavefronts have more than half of the LDS.
+constexpr int tiles_per_cu(int hd, int w) { return hd > 128 ? 1 : 8 / w; }
 template <int HD, int QT, int W>
-__global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_kernel(const Kv4Tiles a) {
+__global__ void __launch_bounds__(64 * W, tiles_per_cu(HD, W) * W / 4) kv4_tiles_kernel(const Kv4Tiles a) {
     constexpr int C = HD > 128 ? 2 : 1, HC = HD / C;               // wavefronts of a row, channels of each
     constexpr int KT = HD > 128 ? 32 : 64;
     constexpr int PITCH = HD <= 64 ? 64 : HD <= 128 ? 128 : 256;   // halfs of an LDS row
@@ -403,6 +405,7 @@ __global__ void __launch_bounds__(64 * W, HD > 128 && W == 4 ? 1 : 2) kv4_tiles_
     __shared__ __attribute__((aligned(16))) uint8_t odd[2][256];     // [buffer][key][group]: values that are not all numbers
     static_assert(KT * GP <= 256, "a byte a unit");
     __shared__ int last_here;
+    static_assert(tiles_per_cu(HD, W) * (sizeof smem + sizeof scores + sizeof odd + sizeof last_here) <= 160 * 1024, "a CU's LDS");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
 
     const int heads = a.cache.n_kv_heads, kvh = (int)(blockIdx.x % heads);
@@ -613,9 +616,9 @@ int tiles_launch(hipc_ctx *ctx, Kv4Tiles a, size_t part_bytes) {
     const int64_t rows = (int64_t)a.total * a.group, kv = a.cache.n_kv_heads;
     // tiles there can be: a sequence has some only if it brings more than a.most rows
     const int64_t tiles = rows / ROWS + std::min<int64_t>(a.cache.n_seqs, rows / (a.most + 1));
-    a.slots = (int)std::min<int64_t>((int64_t)ctx->cu_count * (8 / W), part_bytes / ((size_t)(HC / 4 + 1) * 64 * W * 8));
+    a.slots = (int)std::min<int64_t>((int64_t)ctx->cu_count * tiles_per_cu(HD, W), part_bytes / ((size_t)(HC / 4 + 1) * 64 * W * 8));
     // us of a key tile (of half as many keys where heads are wider than 128), and of a part on its way through memory
-    a.tile_us = (W == 8 ? 2.6f : 1.8f) * QT * (HD <= 64 ? 0.6f : 1.f), a.part_us = 2.f;
+    a.tile_us = (W == 8 ? (QT == 1 ? 3.1f : 5.2f) : QT == 1 ? 2.4f : 3.6f) * (HD <= 64 ? 0.6f : 1.f), a.part_us = 2.f;
     a.splits = ctx->tune.prompt_split;
     const int64_t groups = std::max<int64_t>(tiles * kv, ceil_div(a.slots, kv) * kv);
     HIPC_REFUSE(ctx, !grid_fits(groups, 64 * W), "hipc_kv4_prompt_attention: %d rows: too many for one call", a.total);

@@ -1,0 +1,34 @@
+"""Which kernel, and how many of its workgroups, packed rows over the 4-bit cache are given to. Sums are in another order by another route, so that bits tell them apart."""
+import numpy as np
+import pytest
+
+from test_kv4_gpu import bits
+
+pytestmark = pytest.mark.gpu
+
+
+def filled(ctx, pkg, kv, dim, length, page=64, seed=0):
+    """A cache of one sequence of `length` positions."""
+    rng = np.random.default_rng(dim + length + seed)
+    width = -(-length // page)
+    pages = pkg.ops.Kv4Pages(ctx, width, page, kv, dim, np.arange(width).reshape(1, width))
+    pages.set_lengths([length])
+    k, v = (rng.standard_normal((length, kv, dim)).astype(np.float16) for _ in range(2))
+    pages.append(k, v, [length])
+    return pages, rng
+
+
+@pytest.mark.parametrize("dim,waves,rows,per_cu", [(256, 4, 1600, 1), (160, 4, 1600, 1), (256, 8, 3200, 1), (128, 4, 3200, 2), (128, 8, 6400, 1), (64, 4, 3200, 2)], ids=str)
+def test_no_more_parts_than_run_at_once(ctx, pkg, dim, waves, rows, per_cu):
+    """100 query tiles leave room for 2 parts each on 256 CUs that run one workgroup at a time, and for 5 where they run two: more are not made, whatever is asked for."""
+    most = 256 * per_cu // 100
+    pages, rng = filled(ctx, pkg, 1, dim, rows)
+    q = rng.standard_normal((rows, 4, dim)).astype(np.float16)
+    got = {}
+    for split in (1, 2, 3, 5, 9):
+        with ctx.options(HIPC_PROMPT_WAVES=waves, HIPC_PROMPT_SPLIT=split):
+            got[split] = bits(pages.prompt_attention(q, [rows]))
+    assert not np.array_equal(got[1], got[2])
+    for split in (2, 3, 5, 9):
+        assert np.array_equal(got[split], got[min(split, most)]), split
+    pages.free()

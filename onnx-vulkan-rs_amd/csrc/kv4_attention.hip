@@ -1,5 +1,6 @@
 // Attention of the newest tokens of many sequences over the paged 4-bit cache (hipc_kv4_attention).
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "kv4.h"
@@ -758,16 +759,26 @@ int hipc_kv4_prompt_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const 
         if (int rc = kv4_attend_scratch(ctx, &a)) return rc;
         // Who brings how many is known on the device. While all rows together are few enough for the workgroups of this file's kernel it takes them all; beyond, both
         // kernels are launched, sequences of more than kKv4FewRows rows are the other one's, and each leaves the other's alone (nothing to do takes one 4.5 us). One
-        // sequence, this kernel / the other, in us: 128 rows behind 4000 keys, 32 / 8 heads of 128 in f16 (512 of a kv head: 4096 in all) 47 / 45, behind 500 20 / 25,
-        // behind 30000 220 / 120; 256 rows 87 / 57, 39 / 25 and 437 / 185, in f32 88 / 73, 41 / 32 and 449 / 279. 256 rows of 4 / 1 heads of 256 behind 4000 57 / 59.
+        // sequence, this kernel / the other, in us (by rows of all its heads; behind 200, 1000, 4000, 10000, 30000 keys):
+        //   32 / 8 heads of 128, f16   2048   14 / 18   20 / 29   30 / 43   54 / 64   129 / 127
+        //                              3072   17 / 18   24 / 29   45 / 54   87 / 81   223 / 134      (f32 19 / 24   26 / 33   49 / 59   93 / 90   227 / 153)
+        //                              4096   18 / 20   24 / 29   48 / 58   90 / 85   232 / 144      (f32 19 / 24   27 / 34   52 / 66   97 / 95   240 / 168)
+        //                              6144   31 / 22   41 / 30   77 / 59  142 / 86   356 / 183      (f32 33 / 26   43 / 34   79 / 68  152 / 100  370 / 218)
+        //   14 / 2 heads of 64, f16    3584   13 / 19   18 / 23   32 / 35   59 / 59   141 / 94
+        //   4 / 1 heads of 256, f16    1024   21 / 26   36 / 38   58 / 57   84 / 78   159 / 145
+        //                              1536   33 / 28   48 / 39   68 / 56  107 / 88   232 / 196
+        // Up to 4096 rows this kernel has a workgroup for each 16 of them; the longer their keys, the sooner it costs more that every 16 rows unpack these by themselves. Of several
+        // sequences: two pieces of 60 behind 30000, 32 / 8 heads of 128 in f16 208 / 147, 100 rows beside 23 tokens, 28 / 4 heads, 235 / 213; but heads of 256, 8 of 40 behind 200 14 / 22.
+        const int64_t seqs = std::min<int64_t>(cache->n_seqs, total), room = cache->table_width * cache->page_size;
+        const int64_t seen = a.window > 0 ? std::min<int64_t>(room, (int64_t)a.window + a.sinks + kKv4FewRows) : room;
         const int64_t all = total * a.group * cache->n_kv_heads;
-        const bool many = ctx->tune.prompt_waves >= 4 || all > (dtype == HIPC_F16 ? 4096 : 6144);
+        const double few = cache->head_dim > 128 ? (cache->n_seqs == 1 ? 1024. : 4096.) : 4096. * std::min(1., std::cbrt(5000. / (double)std::max<int64_t>(seen, 1)));
+        // (only if one sequence can bring more than kKv4FewRows where the others bring one each: up to 4096, f32 6144, single tokens stay one launch)
+        const bool many = ctx->tune.prompt_waves >= 4 || all > (dtype == HIPC_F16 ? 4096 : 6144) || (all > few && (total - cache->n_seqs + 1) * a.group > kKv4FewRows);
         // One sequence is one kernel's. So are several, where those that bring few rows cannot make the other kernel much longer: their key tiles, taken by as many workgroups
         // as run at once, are less than the launch that finds nothing to do, and none has many more than the tiles of a prompt of a thousand. us, two kernels / one: six
         // prompts of up to 1024, 28 / 4 heads of 128 in f16, 40 / 38; pieces of 1000 that see 512 keys, 4 / 1 heads of 256, 33 / 31; a prompt of 500 beside seven tokens
         // behind 1200, 32 / 8 heads of 128, 33 / 30; five of 700 beside three of 5 72 / 59; four pieces of 300 beside twenty tokens that see 512, 4 / 1 heads of 256, 45 / 47.
-        const int64_t seqs = std::min<int64_t>(cache->n_seqs, total);
-        const int64_t seen = a.window > 0 ? std::min<int64_t>(cache->table_width * cache->page_size, (int64_t)a.window + a.sinks + kKv4FewRows) : cache->table_width * cache->page_size;
         const int64_t tiles = ceil_div(seen, cache->head_dim > 128 ? 32 : 64) + 1;
         const bool together = cache->n_seqs == 1 || (tiles <= 24 && seqs * cache->n_kv_heads * tiles <= 5 * (int64_t)ctx->cu_count);
         a.most = many ? (together ? 0 : kKv4FewRows) : 1 << 30;

@@ -32,3 +32,17 @@ def test_no_more_parts_than_run_at_once(ctx, pkg, dim, waves, rows, per_cu):
     for split in (2, 3, 5, 9):
         assert np.array_equal(got[split], got[min(split, most)]), split
     pages.free()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32], ids=["f16", "f32"])
+@pytest.mark.parametrize("heads,kv,dim,new,behind,many", [(32, 8, 128, 128, 4000, False), (32, 8, 128, 160, 4000, True), (32, 8, 128, 60, 10000, False), (32, 8, 128, 128, 10000, True),
+                                                          (32, 8, 128, 60, 30000, False), (32, 8, 128, 96, 30000, True), (4, 1, 256, 256, 200, False), (4, 1, 256, 384, 200, True),
+                                                          (4, 1, 256, 384, 10000, True)], ids=str)
+def test_a_piece_goes_to_the_kernel_that_its_context_asks_for(ctx, pkg, dtype, heads, kv, dim, new, behind, many):
+    """Many rows of one sequence, or few whose keys are many, are those of the kernel for many rows, here with four wavefronts a workgroup; others stay with the kernel for few."""
+    pages, rng = filled(ctx, pkg, kv, dim, behind + new)
+    q = rng.standard_normal((new, heads, dim)).astype(dtype)
+    got = bits(pages.prompt_attention(q, [new]))
+    with ctx.options(HIPC_PROMPT_WAVES=4):
+        assert np.array_equal(got, bits(pages.prompt_attention(q, [new]))) == many
+    pages.free()

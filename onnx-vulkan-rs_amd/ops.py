@@ -435,7 +435,10 @@ class Rotary:
 
     def __call__(self, q, k, positions):
         """``q [rows, heads, dim]`` and ``k [rows, kv heads, dim]`` at ``positions [rows]``: both normed and turned."""
-        q, k, positions = np.ascontiguousarray(q), np.ascontiguousarray(k), np.ascontiguousarray(positions, np.int32)
+        q, k, positions = np.ascontiguousarray(q), np.ascontiguousarray(k), np.asarray(positions)
+        if positions.size and (positions.dtype.kind not in "iu" or positions.min() < -2 ** 31 or positions.max() >= 2 ** 31):
+            raise ValueError(f"Rotary: positions ({positions.dtype}) that are no whole numbers of 32 bits")
+        positions = np.ascontiguousarray(positions, np.int32)
         self.rows_match("Rotary", q, k)
         _rows_match("Rotary", (positions,), ((q.shape[0],),), np.int32)
         dQ, dK, dP = (self.ctx.upload(x) for x in (q, k, positions))

@@ -396,6 +396,8 @@ ROTARY_LINEAR, ROTARY_BASE, ROTARY_BY_PARTS = 1, 2, 3
 def rotary_frequencies(theta, rotary_dim, kind=None, factor=1.0, trained=0.0, slow=1.0, fast=32.0):
     """The frequencies of a rotation, ``[rotary_dim / 2]`` float32 on the host, stretched ``factor``-fold in one of the kinds above
     (``hipc_rotary_frequencies``)."""
+    if kind is None and (factor, trained) != (1.0, 0.0):
+        raise ValueError(f"rotary_frequencies: a factor of {factor} over {trained} positions and no kind")
     lib, out = load_library(), np.zeros(max(int(rotary_dim), 0) // 2, np.float32)
     scaling = None if kind is None else C.byref(RotaryScaling(kind, factor, trained, slow, fast))
     rc = lib.hipc_rotary_frequencies(theta, rotary_dim, scaling, out.ctypes.data)

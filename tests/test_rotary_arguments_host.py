@@ -14,3 +14,10 @@ def test_positions_that_32_bits_do_not_hold(pkg, positions):
     turn = pkg.ops.Rotary(Host(), 4, 2, 64, np.zeros(32, np.float32))
     with pytest.raises(ValueError, match="positions"):
         turn(np.zeros((3, 4, 64), np.float16), np.zeros((3, 2, 64), np.float16), positions)
+
+
+@pytest.mark.parametrize("given", [dict(factor=8.0), dict(trained=8192.0), dict(factor=8.0, trained=8192.0, slow=1.0, fast=4.0)], ids=str)
+def test_a_stretch_of_no_kind(pkg, given):
+    """(they were left out of account, and the frequencies those of no stretch)"""
+    with pytest.raises(ValueError, match="kind"):
+        pkg.ops.rotary_frequencies(1e4, 64, **given)

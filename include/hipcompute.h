@@ -423,7 +423,7 @@ typedef struct {
  *   BY_PARTS  with r turns over `trained` positions: pairs of fewer than `slow` turns as LINEAR, of more than `fast` as they were,
  *             between them both, weighed by (r - slow) / (fast - slow)
  * (What a model multiplies its cosines with goes to `amplitude`: 0.1 ln factor + 1 is usual with BY_PARTS.)
- * Host code only (no context): writes rotary_dim / 2 numbers; a failed call leaves its message in hipc_host_error. */
+ * Host code only (no context): writes rotary_dim / 2 numbers, or where one is past f32's writes none and is HIPC_ERR_INVALID; a failed call leaves its message in hipc_host_error. */
 #define HIPC_ROTARY_LINEAR 1
 #define HIPC_ROTARY_BASE 2
 #define HIPC_ROTARY_BY_PARTS 3

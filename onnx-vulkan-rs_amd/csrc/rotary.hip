@@ -375,7 +375,7 @@ int hipc_rotary_frequencies(double theta, int32_t rotary_dim, const hipc_rotary_
             return host_fail(HIPC_ERR_INVALID, "%s: %g positions, %g to %g turns", who, scaling->trained, scaling->slow, scaling->fast);
         if (scaling->kind == HIPC_ROTARY_BASE && rotary_dim > 2) theta *= std::pow((double)scaling->factor, d / (d - 2.0));
     }
-    for (int i = 0; i < rotary_dim / 2; i++) {
+    auto frequency = [&](int i) {
         double f = std::pow(theta, -2.0 * i / d);
         if (scaling && scaling->kind == HIPC_ROTARY_LINEAR) f /= scaling->factor;
         if (scaling && scaling->kind == HIPC_ROTARY_BY_PARTS) {
@@ -383,8 +383,11 @@ int hipc_rotary_frequencies(double theta, int32_t rotary_dim, const hipc_rotary_
             const double keep = std::min(std::max((turns - scaling->slow) / ((double)scaling->fast - scaling->slow), 0.0), 1.0);
             f = f / scaling->factor * (1.0 - keep) + f * keep;
         }
-        frequencies[i] = (float)f;
-    }
+        return (float)f;
+    };
+    for (int i = 0; i < rotary_dim / 2; i++)
+        if (!std::isfinite(frequency(i))) return host_fail(HIPC_ERR_INVALID, "%s: a base of %g makes frequency %d infinite", who, theta, i);
+    for (int i = 0; i < rotary_dim / 2; i++) frequencies[i] = frequency(i);
     return HIPC_OK;
 }
 

@@ -21,3 +21,15 @@ def test_a_stretch_of_no_kind(pkg, given):
     """(they were left out of account, and the frequencies those of no stretch)"""
     with pytest.raises(ValueError, match="kind"):
         pkg.ops.rotary_frequencies(1e4, 64, **given)
+
+
+@pytest.mark.parametrize("theta,dim,more", [(1e-45, 64, ()), (1e-300, 4, ()), (5e-324, 128, (1, 2.0))], ids=str)
+def test_bases_whose_frequencies_f32_does_not_hold(pkg, theta, dim, more):
+    """theta^(-2i / dim) past f32's numbers: an infinite frequency would make NaN of every row."""
+    with pytest.raises(pkg.HipComputeError) as e:
+        pkg.ops.rotary_frequencies(theta, dim, *more)
+    assert e.value.code == 1 and "hipc_rotary_frequencies" in e.value.message
+
+
+def test_bases_below_one(pkg):
+    assert np.allclose(pkg.ops.rotary_frequencies(0.25, 4), [1, 2], rtol=2 ** -23) and np.all(np.isfinite(pkg.ops.rotary_frequencies(1e-38, 64)))

@@ -422,7 +422,8 @@ typedef struct {
  *   BASE      theta times factor^(rotary_dim / (rotary_dim - 2)): the slowest pair as LINEAR has it, the fastest as it was
  *   BY_PARTS  with r turns over `trained` positions: pairs of fewer than `slow` turns as LINEAR, of more than `fast` as they were,
  *             between them both, weighed by (r - slow) / (fast - slow)
- * (What a model multiplies its cosines with goes to `amplitude`: 0.1 ln factor + 1 is usual with BY_PARTS.)
+ * (What a model multiplies its cosines with goes to `amplitude`. Models that multiply with 0.1 ln factor + 1 commonly weigh the pairs between the two bounds by the pair's
+ * index, not by its turns as BY_PARTS does: other middle frequencies, which a program for such a model forms itself.)
  * Host code only (no context): writes rotary_dim / 2 numbers, or where one is past f32's writes none and is HIPC_ERR_INVALID; a failed call leaves its message in hipc_host_error. */
 #define HIPC_ROTARY_LINEAR 1
 #define HIPC_ROTARY_BASE 2

@@ -303,6 +303,12 @@ int rotary_rows(hipc_ctx *ctx, const char *who, const char *what, const RotaryAr
     return HIPC_OK;
 }
 
+// rows that are turned where they lie stay there
+int rotary_in_place(hipc_ctx *ctx, const char *who, const char *what, const RotaryArgs &a, int heads, const void *p, int64_t stride, const void *out, int64_t out_stride) {
+    HIPC_REQUIRE(ctx, heads == 0 || p != out || stride == out_stride || a.rows <= 1, "%s: %s where it lies, rows %lld apart and then %lld", who, what, (long long)stride, (long long)out_stride);
+    return HIPC_OK;
+}
+
 template <typename T, bool STORE>
 int rotary_launch(hipc_ctx *ctx, const char *who, RotaryArgs a, bool near) {
     const int64_t strides[5] = {a.q_stride, a.k_stride, a.v_stride, a.q_out_stride, a.k_out_stride};
@@ -404,6 +410,8 @@ int hipc_rotary(hipc_ctx *ctx, const hipc_rotary_heads *heads, int dtype, const 
         if (int rc = rotary_rows(ctx, who, "K", a, a.n_kv, size, K, k_stride)) return rc;
         if (int rc = rotary_rows(ctx, who, "Q_out", a, a.n_q, size, Q_out, q_out_stride)) return rc;
         if (int rc = rotary_rows(ctx, who, "K_out", a, a.n_kv, size, K_out, k_out_stride)) return rc;
+        if (int rc = rotary_in_place(ctx, who, "Q", a, a.n_q, Q, q_stride, Q_out, q_out_stride)) return rc;
+        if (int rc = rotary_in_place(ctx, who, "K", a, a.n_kv, K, k_stride, K_out, k_out_stride)) return rc;
         a.positions = static_cast<const int *>(positions);
         a.q = Q, a.k = K, a.q_out = Q_out, a.k_out = K_out, a.q_stride = q_stride, a.k_stride = k_stride, a.q_out_stride = q_out_stride, a.k_out_stride = k_out_stride;
         return dtype == HIPC_F16 ? rotary_launch<_Float16, false>(ctx, who, a, heads->interleaved) : rotary_launch<float, false>(ctx, who, a, heads->interleaved);
@@ -426,6 +434,7 @@ int hipc_kv4_append_rotary(hipc_ctx *ctx, const hipc_kv4_cache *cache, const hip
         if (int rc = rotary_rows(ctx, who, "K", a, a.n_kv, size, K, k_stride)) return rc;
         if (int rc = rotary_rows(ctx, who, "V", a, a.n_kv, size, V, v_stride)) return rc;
         if (int rc = rotary_rows(ctx, who, "Q_out", a, a.n_q, size, Q_out, q_out_stride)) return rc;
+        if (int rc = rotary_in_place(ctx, who, "Q", a, a.n_q, Q, q_stride, Q_out, q_out_stride)) return rc;
         a.cache = *cache, a.starts = static_cast<const int *>(starts);
         a.q = Q, a.k = K, a.v = V, a.q_out = Q_out, a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.q_out_stride = q_out_stride;
         return dtype == HIPC_F16 ? rotary_launch<_Float16, true>(ctx, who, a, heads->interleaved) : rotary_launch<float, true>(ctx, who, a, heads->interleaved);

@@ -777,8 +777,9 @@ int hipc_kv4_prompt_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const 
         const bool many = ctx->tune.prompt_waves >= 4 || all > (dtype == HIPC_F16 ? 4096 : 6144) || (all > few && (total - cache->n_seqs + 1) * a.group > kKv4FewRows);
         // One sequence is one kernel's. So are several, where those that bring few rows cannot make the other kernel much longer: their key tiles, taken by as many workgroups
         // as run at once, are less than the launch that finds nothing to do, and none has many more than the tiles of a prompt of a thousand. us, two kernels / one: six
-        // prompts of up to 1024, 28 / 4 heads of 128 in f16, 40 / 38; pieces of 1000 that see 512 keys, 4 / 1 heads of 256, 33 / 31; a prompt of 500 beside seven tokens
-        // behind 1200, 32 / 8 heads of 128, 33 / 30; five of 700 beside three of 5 72 / 59; four pieces of 300 beside twenty tokens that see 512, 4 / 1 heads of 256, 45 / 47.
+        // prompts of up to 1024, 28 / 4 heads of 128 in f16, 46 / 44; pieces of 1000 that see 512 keys, 4 / 1 heads of 256, 33 / 31; a prompt of 500 beside seven tokens
+        // behind 1200, 32 / 8 heads of 128, 43 / 33; five of 700 beside three of 5 79 / 67; four pieces of 300 beside twenty tokens that see 512, 4 / 1 heads of 256, 46 / 33.
+        // (What sequences hold is known on the device only: the table's room stands for it.)
         const int64_t tiles = ceil_div(seen, cache->head_dim > 128 ? 32 : 64) + 1;
         const bool together = cache->n_seqs == 1 || (tiles <= 24 && seqs * cache->n_kv_heads * tiles <= 5 * (int64_t)ctx->cu_count);
         a.most = many ? (together ? 0 : kKv4FewRows) : 1 << 30;

@@ -6,7 +6,8 @@
 // The matrix cores bound it: of a key tile of 64 a wavefront's 32 rows of 128 channels take 48 products of 32x32x16 -- weights enter as two terms each -- beside some 290 vector
 // instructions, an exponential and some six others a score and a quarter of them to unpack codes. So codes become f16 once a workgroup, in LDS, not once a wavefront, and eight
 // wavefronts share them where there are rows for that. 2048 rows behind 30000 keys, 32 / 8 heads of 128 in f16: 1500 us, 0.69 PFLOP/s of the operation's, 1.04 of the products that it takes
-// (a product of 8192^3: 1.21). 500 rows behind 8000: 120 us. Short prompts are chains: 2.4 us a key tile, 5 to start.
+// (a product of 8192^3: 1.21); matrix cores busy 52 % of the cycles, vector instructions 51 %, LDS 44 %, half of that bank conflicts (Kv4TileReads). 500 rows behind 8000: 120 us.
+// Short prompts are chains: 2.4 us a key tile, 5 to start; a chain is cut only where query tiles are fewer than half of the workgroups that run at once.
 #include <algorithm>
 #include <type_traits>
 
@@ -157,8 +158,9 @@ struct TileRow {
     }
 };
 
-// Where a lane reads operands in key tiles of KT rows of PITCH halfs in LDS. 16-byte chunks of a row lie at chunk ^ f(row), so that the rows a read takes at a time lie in
-// different banks.
+// Where a lane reads operands in key tiles of KT rows of PITCH halfs in LDS. 16-byte chunks of a row lie at chunk ^ f(row), three bits of it, so that rows of 128 bytes that a read
+// takes at a time lie in different banks. In longer rows three bits leave a read in one 128-byte half of its rows: it has half of the banks, and takes twice as long as it would with all
+// (2048 rows behind 30000 keys, 128 channels: 1.6e8 of LDS's 3.2e8 cycles are conflicts).
 template <int KT, int PITCH>
 struct Kv4TileReads {
     uint32_t k_at[4], v_at[2];
@@ -633,8 +635,8 @@ int kv4_tiles(hipc_ctx *ctx, const Kv4Tiles &a, int dtype, size_t part_bytes) {
     auto launch = [&](auto width) -> int {
         constexpr int HD = decltype(width)::value;
         // Eight wavefronts unpack a key tile once for twice as many rows as four and are half as many workgroups. us, four / eight: 2048 rows behind 30000 keys, 32 / 8 heads of 128 in
-        // f16 1360 / 1207; 500 behind 8000 beside single tokens 148 / 139; prompts of up to 1024, 28 / 4 heads, 44 / 47; pieces of 1000 that see 512 keys, 4 / 1 heads of 256,
-        // 33 / 40. How long sequences are is known on the device only: the table's room stands for it.
+        // f16 1606 / 1505; 500 behind 8000 beside single tokens 160 / 155; prompts of up to 1024, 28 / 4 heads, 44 / 52; pieces of 1000 that see 512 keys, 4 / 1 heads of 256,
+        // 31 / 38. How long sequences are is known on the device only: the table's room stands for it (a prompt of 1000, 28 / 4 heads of 128: 35.5, with a table of 32768 positions 39.7).
         const int64_t units = ceil_div((int64_t)a.total * a.group, HD > 128 ? 128 : 256) * a.cache.n_kv_heads;
         const int64_t room = a.cache.table_width * a.cache.page_size, keys = a.window > 0 ? std::min<int64_t>(room, a.window) : room;
         int waves = units >= (int64_t)ctx->cu_count || (keys >= 4096 && 4 * units >= (int64_t)ctx->cu_count) ? 8 : 4;

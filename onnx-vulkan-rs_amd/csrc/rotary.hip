@@ -11,7 +11,8 @@
 //
 // Memory bounds it. A wavefront has a row, or some heads of one where rows are few or long, and takes 64 / L heads at a time, L lanes a head; a lane has
 // two vectors of V channels, half a rotation apart (the channels that turn with each other, or pairs that lie in one vector), the same channels of every head it sees, so that its
-// cosines and sines stay in registers. 8192 rows of 32 / 8 heads of 128: f16 33.1 to 34.7 us by card, 5.0 TB/s, f32 65.7, 5.1 (a 1 GiB copy: 4.96); 1500 of 16 / 16 heads of 96 in f32 8.0; 48 rows 4.
+// cosines and sines stay in registers. Graphs of launches, rows of several such calls in turn (1.2 GB) / of the same call again, which the last cache holds in part: 8192 rows of
+// 32 / 8 heads of 128 in f16, 168 MB, 38.1 / 29 us, 4.4 TB/s (a 1 GiB copy: 4.96), in f32 62.6 / 49, 5.4 TB/s; 1500 of 16 / 16 heads of 96 in f32 12.4 / 9.2; 48 rows 3.6. Figures below are of rows in turn.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -314,7 +315,7 @@ int rotary_launch(hipc_ctx *ctx, const char *who, RotaryArgs a, bool near) {
     const int64_t strides[5] = {a.q_stride, a.k_stride, a.v_stride, a.q_out_stride, a.k_out_stride};
     const void *rows[5] = {a.q, a.k, a.v, a.q_out, a.k_out};
     const int heads[5] = {a.n_q, a.n_kv, STORE ? a.n_kv : 0, a.n_q, STORE ? 0 : a.n_kv};
-    // vectors of 16 bytes where pairs and rows allow (of eight f32, two loads: 8192 rows of 32 / 8 heads of 128 69.7 us, of four 67.0), f16 ones of 8, or single values
+    // vectors of 16 bytes where pairs and rows allow (of eight f32, two loads: 8192 rows of 32 / 8 heads of 128 76.9 us, of four 62.6), f16 ones of 8, or single values
     auto fits = [&](int v) {
         const int64_t bytes = std::min<int64_t>(v * sizeof(T), 16);
         bool ok = a.dim % v == 0 && a.half % v == 0;
@@ -330,8 +331,8 @@ int rotary_launch(hipc_ctx *ctx, const char *who, RotaryArgs a, bool near) {
         const int together = 64 >> a.lg_lanes;
         const int64_t passes = ceil_div(a.n_q, together) + ceil_div(a.n_kv, together) + (STORE ? ceil_div((int64_t)a.n_kv * a.dim, 64 * N) : 0);
         if (passes == 0) return HIPC_OK;
-        // Rows that do not fill the device are shared by wavefronts, 32 a CU (storing 16): 1500 rows of 16 / 16 heads of 96 in f32 9.0 us, by eight a CU 13.2; stored, of 32 / 8 heads
-        // of 128 in f16, 13.3, and 15.3. So are long rows of f32, in pairs of passes, however many: 8192 of 32 / 8 heads of 128 65.7 us, a wavefront each 86.8 (f16 35 and 30).
+        // Rows that do not fill the device are shared by wavefronts, 32 a CU (storing 16): 1500 rows of 16 / 16 heads of 96 in f32, the same again, 9.0 us, by eight a CU 13.2; stored, of
+        // 32 / 8 heads of 128 in f16, 13.3, and 15.3. So are long rows of f32, in pairs of passes, however many: 8192 of 32 / 8 heads of 128 62.6 us, a wavefront each 84.9 (f16 37.8 and 38.1).
         a.chunks = (int)std::max<int64_t>(1, std::min(passes, (STORE ? 16 : 32) * (int64_t)ctx->cu_count / a.rows));
         if (sizeof(T) == 4 && passes > 8) a.chunks = std::max(a.chunks, (int)ceil_div(passes, 2));
         a.per = (int)ceil_div(passes, a.chunks), a.chunks = (int)ceil_div(passes, a.per);
@@ -341,7 +342,7 @@ int rotary_launch(hipc_ctx *ctx, const char *who, RotaryArgs a, bool near) {
             hipLaunchKernelGGL((rotary_kernel<T, V, decltype(neighbours)::value, STORE, decltype(past)::value>), (unsigned)groups, 256, 0, ctx->stream, a);
         };
         // Many rows -- more than the caches near the CUs hold -- leave past these where neighbouring lanes store side by side, whole lines: 8192 rows of 32 / 8 heads of 128 in f16
-        // 33.4 us (through the caches 40.3), in f32 86.8 (94.3); 48 rows 6.9 and 6.4.
+        // 38.1 us (through the caches 41.5), in f32 62.6 (69.4).
         constexpr bool LINES = sizeof(T) * V == 16;
         const bool past = LINES && a.half * sizeof(T) % 128 == 0 && (int64_t)a.rows * (a.n_q + (STORE ? 0 : a.n_kv)) * a.dim * (int64_t)sizeof(T) >= kRotaryCaches;
         auto kinds = [&](auto neighbours) {

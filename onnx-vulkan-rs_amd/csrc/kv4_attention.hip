@@ -768,11 +768,13 @@ int hipc_kv4_prompt_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const 
         //   4 / 1 heads of 256, f16    1024   21 / 26   36 / 38   58 / 57   84 / 78   159 / 145
         //                              1536   33 / 28   48 / 39   68 / 56  107 / 88   232 / 196
         // Up to 4096 rows this kernel has a workgroup for each 16 of them; the longer their keys, the sooner it costs more that every 16 rows unpack these by themselves. Of several
-        // sequences: two pieces of 60 behind 30000, 32 / 8 heads of 128 in f16 208 / 147, 100 rows beside 23 tokens, 28 / 4 heads, 235 / 213; but heads of 256, 8 of 40 behind 200 14 / 22.
+        // sequences later, since the kernels run in turn: two pieces of 50 behind 30000, 32 / 8 heads of 128 in f16, 216 / 142, behind 12000 101 / 91; 100 rows beside 20 tokens, 28 / 4 heads,
+        // 248 / 204, behind 12000 107 / 123; heads of 256, 8 of 40 behind 200 14 / 22.
         const int64_t seqs = std::min<int64_t>(cache->n_seqs, total), room = cache->table_width * cache->page_size;
         const int64_t seen = a.window > 0 ? std::min<int64_t>(room, (int64_t)a.window + a.sinks + kKv4FewRows) : room;
         const int64_t all = total * a.group * cache->n_kv_heads;
-        const double few = cache->head_dim > 128 ? (cache->n_seqs == 1 ? 1024. : 4096.) : 4096. * std::min(1., std::cbrt(5000. / (double)std::max<int64_t>(seen, 1)));
+        const bool one = cache->n_seqs == 1, wide = cache->head_dim > 128;
+        const double few = one && wide ? 1024. : !wide && seen > (one ? 5000 : 20000) ? 4096. * std::cbrt(5000. / (double)seen) : 4096.;
         // (only if one sequence can bring more than kKv4FewRows where the others bring one each: up to 4096, f32 6144, single tokens stay one launch)
         const bool many = ctx->tune.prompt_waves >= 4 || all > (dtype == HIPC_F16 ? 4096 : 6144) || (all > few && (total - cache->n_seqs + 1) * a.group > kKv4FewRows);
         // One sequence is one kernel's. So are several, where those that bring few rows cannot make the other kernel much longer: their key tiles, taken by as many workgroups

@@ -46,3 +46,20 @@ def test_a_piece_goes_to_the_kernel_that_its_context_asks_for(ctx, pkg, dtype, h
     with ctx.options(HIPC_PROMPT_WAVES=4):
         assert np.array_equal(got, bits(pages.prompt_attention(q, [new]))) == many
     pages.free()
+
+
+@pytest.mark.parametrize("behind,many", [(12000, False), (30000, True)], ids=str)
+def test_a_piece_beside_single_tokens_goes_there_later(ctx, pkg, behind, many):
+    """100 rows of one sequence and a token of each of five, which hold the same pages: the kernels run in turn, which pays behind 30000 keys and not behind 12000."""
+    page, length = 64, behind + 100
+    width, rng = -(-length // page), np.random.default_rng(behind)
+    pages = pkg.ops.Kv4Pages(ctx, width, page, 8, 128, np.tile(np.arange(width), (6, 1)))
+    pages.set_lengths([length] + [behind] * 5)
+    k, v = (rng.standard_normal((length, 8, 128)).astype(np.float16) for _ in range(2))
+    pages.append(k, v, [length, 0, 0, 0, 0, 0])
+    q = rng.standard_normal((105, 32, 128)).astype(np.float16)
+    got = bits(pages.prompt_attention(q, [100, 1, 1, 1, 1, 1]))
+    with ctx.options(HIPC_PROMPT_WAVES=4):
+        forced = bits(pages.prompt_attention(q, [100, 1, 1, 1, 1, 1]))
+    assert np.array_equal(got[:100], forced[:100]) == many
+    pages.free()

@@ -759,15 +759,15 @@ int hipc_kv4_prompt_attention(hipc_ctx *ctx, const hipc_kv4_cache *cache, const 
         if (int rc = kv4_attend_scratch(ctx, &a)) return rc;
         // Who brings how many is known on the device. While all rows together are few enough for the workgroups of this file's kernel it takes them all; beyond, both
         // kernels are launched, sequences of more than kKv4FewRows rows are the other one's, and each leaves the other's alone (nothing to do takes one 4.5 us). One
-        // sequence, this kernel / the other, in us (by rows of all its heads; behind 200, 1000, 4000, 10000, 30000 keys):
-        //   32 / 8 heads of 128, f16   2048   14 / 18   20 / 29   30 / 43   54 / 64   129 / 127
-        //                              3072   17 / 18   24 / 29   45 / 54   87 / 81   223 / 134      (f32 19 / 24   26 / 33   49 / 59   93 / 90   227 / 153)
-        //                              4096   18 / 20   24 / 29   48 / 58   90 / 85   232 / 144      (f32 19 / 24   27 / 34   52 / 66   97 / 95   240 / 168)
-        //                              6144   31 / 22   41 / 30   77 / 59  142 / 86   356 / 183      (f32 33 / 26   43 / 34   79 / 68  152 / 100  370 / 218)
-        //   14 / 2 heads of 64, f16    3584   13 / 19   18 / 23   32 / 35   59 / 59   141 / 94
-        //   4 / 1 heads of 256, f16    1024   21 / 26   36 / 38   58 / 57   84 / 78   159 / 145
-        //                              1536   33 / 28   48 / 39   68 / 56  107 / 88   232 / 196
-        // Up to 4096 rows this kernel has a workgroup for each 16 of them; the longer their keys, the sooner it costs more that every 16 rows unpack these by themselves. Of several
+        // sequence, this kernel / the other, in us (tokens; behind 200, 1000, 4000, 10000, 30000 keys):
+        //   32 / 8 heads of 128, f16     64   14 / 18   20 / 29   30 / 43   54 / 64   129 / 127
+        //                                96   17 / 18   24 / 29   45 / 54   87 / 81   223 / 134      (f32 19 / 24   26 / 33   49 / 59   93 / 90   227 / 153)
+        //                               128   18 / 20   24 / 29   48 / 58   90 / 85   232 / 144      (f32 19 / 24   27 / 34   52 / 66   97 / 95   240 / 168)
+        //                               192   31 / 22   41 / 30   77 / 59  142 / 86   356 / 183      (f32 33 / 26   43 / 34   79 / 68  152 / 100  370 / 218)
+        //   14 / 2 heads of 64, f16     256   13 / 19   18 / 23   32 / 35   59 / 59   141 / 94
+        //   4 / 1 heads of 256, f16     256   21 / 26   36 / 38   58 / 57   84 / 78   159 / 145
+        //                               384   33 / 28   48 / 39   68 / 56  107 / 88   232 / 196
+        // Up to 4096 rows of all heads this kernel has a workgroup for each 16 of them; the longer their keys, the sooner it costs more that every 16 rows unpack these by themselves. Of several
         // sequences later, since the kernels run in turn: two pieces of 50 behind 30000, 32 / 8 heads of 128 in f16, 216 / 142, behind 12000 101 / 91; 100 rows beside 20 tokens, 28 / 4 heads,
         // 248 / 204, behind 12000 107 / 123; heads of 256, 8 of 40 behind 200 14 / 22.
         const int64_t seqs = std::min<int64_t>(cache->n_seqs, total), room = cache->table_width * cache->page_size;
